@@ -115,6 +115,13 @@ PROTOTYPES = {
     "amoe_ffn_fwd": (C.c_int, [P, P, SZ, P, P]),
     "amoe_ffn_bwd": (C.c_int, [P, P, SZ, P, P]),
     "amoe_ffn_stage_name": (C.c_char_p, [I32, I32]),
+    "amoe_rotary": (C.c_int, [P, P]),
+    "amoe_rotary_args_bytes": (SZ, []),
+    "amoe_attention_fwd_workspace": (SZ, [P]),
+    "amoe_attention_fwd": (C.c_int, [P, P, SZ, P]),
+    "amoe_attention_bwd_workspace": (SZ, [P]),
+    "amoe_attention_bwd": (C.c_int, [P, P, SZ, P]),
+    "amoe_attn_args_bytes": (SZ, []),
     "amoe_select_workspace": (SZ, [I64, I32]),
     "amoe_select_fwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, SZ, P]),
     "amoe_select_bwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, P]),
@@ -133,6 +140,18 @@ FFN_ARGS = struct.Struct("<"
                          "6qq3d"       # dy grad_x grad_keys grad_values grad_gate grad_ir, gradient_relative, 3 scalars
                          "q")          # stage_events
 
+# amoe_rotary_args and amoe_attn_args, likewise
+ROTARY_ARGS = struct.Struct("<"
+                            "9qd"         # dtype B S q_heads k_heads d R interleaved inverse, size
+                            "q2q3q"       # turns, positions positions_are_i64, 2 strides start
+                            "4q4q4q4q")   # q, k, q_out, k_out with 3 strides each
+ATTN_ARGS = struct.Struct("<"
+                          "8qd"           # dtype B S T H G d causal, scale
+                          "4q4q4q"        # q, k, v with 3 strides each
+                          "2q2q"          # lengths lengths_is_i64, starts starts_is_i64
+                          "2q"            # out lse
+                          "4q3q")         # go with 3 strides, dq dk dv
+
 
 @functools.lru_cache(maxsize=256)
 def bounds_array(bounds):
@@ -148,8 +167,9 @@ def bind(path: str) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    if lib.amoe_ffn_args_bytes() != FFN_ARGS.size:
-        raise RuntimeError(f"{path}: amoe_ffn_args has another layout than this package packs")
+    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS)):
+        if getattr(lib, f"amoe_{name}_args_bytes")() != layout.size:
+            raise RuntimeError(f"{path}: amoe_{name}_args has another layout than this package packs")
     return lib
 
 

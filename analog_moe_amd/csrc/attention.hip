@@ -1,0 +1,152 @@
+// Entry points of attention: argument checks, the choice of the kernel, the workspace.
+#include "attn_host.h"
+
+using namespace amoe;
+
+namespace {
+
+int check_operand(const void* p, const int64_t* st, int64_t rows, int64_t heads, int64_t d, size_t es) {
+  if (rows == 0 || heads == 0) return AMOE_OK;
+  if (!p) return AMOE_ENULL;
+  if (!aligned(p, es)) return AMOE_EALIGN;
+  for (int i = 0; i < 3; i++)
+    if (st[i] < 0 || st[i] > (INT64_C(1) << 40)) return AMOE_EINVAL;
+  return d < 1 ? AMOE_EINVAL : AMOE_OK;
+}
+
+// 1: rows start on 16 bytes; 2: and a tile's rows can be addressed by 32-bit offsets into a resource that ends with them
+int operand_vec(const void* p, const int64_t* st, int64_t rows, int64_t d, size_t es) {
+  const int64_t c = 16 / (int64_t)es;
+  if (!aligned(p, 16) || st[0] % c || st[1] % c || st[2] % c) return 0;
+  if (rows > 1 && (st[1] < d || st[1] * (int64_t)es > (INT64_C(1) << 24))) return 1;
+  return 2;
+}
+
+int check_sizes(const amoe_attn_args* a) {
+  if (!a) return AMOE_ENULL;
+  if (a->dtype != AMOE_F32 && a->dtype != AMOE_BF16 && a->dtype != AMOE_F16) return AMOE_EINVAL;
+  if (a->B < 0 || a->S < 0 || a->T < 0 || a->H < 1 || a->G < 1 || a->d < 1) return AMOE_EINVAL;
+  if (a->H % a->G) return AMOE_ESHAPE;
+  if (!(a->scale > 0) || !(a->scale < 3.4e38)) return AMOE_EINVAL;
+  if (a->d > kAttnMaxHead || a->S > kAttnMaxRows || a->T > kAttnMaxRows) return AMOE_EUNSUPPORTED;
+  // workgroup and row numbers stay in 31 bits
+  const int64_t limit = INT64_C(1) << 31;
+  if (a->B > limit || a->H > limit || (a->S > 0 && a->H / a->G > limit / a->S - 64)) return AMOE_EUNSUPPORTED;
+  const int64_t tiles = (a->S > a->T ? a->S : a->T) / 32 + 1;
+  if (a->B > 0 && a->H > limit / tiles / a->B) return AMOE_EUNSUPPORTED;
+  return AMOE_OK;
+}
+
+// Parts of the key axis for the kernel of few rows; 0: the kernel of many rows.
+int attn_splits(const amoe_attn_args* a) {
+  const int64_t rows = a->H / a->G * a->S, cus = num_compute_units();
+  const int64_t many = a->B * a->H * ((a->S + kAttnRows - 1) / kAttnRows);
+  if (rows > 32 && (many * 2 > cus || a->T < 1024)) return 0;
+  const int64_t groups = a->B * a->G * ((rows + 31) / 32);
+  int64_t n = (2 * cus + groups - 1) / groups;
+  const int64_t most = (a->T + 127) / 128;
+  if (n > most) n = most;
+  return (int)(n < 1 ? 1 : n);
+}
+
+void fill(AttnParams& p, const amoe_attn_args* a) {
+  p.q = {a->q, a->q_sb, a->q_ss, a->q_sh};
+  p.k = {a->k, a->k_sb, a->k_ss, a->k_sh};
+  p.v = {a->v, a->v_sb, a->v_ss, a->v_sh};
+  p.lengths = a->lengths; p.lengths_i64 = (int)a->lengths_is_i64;
+  p.starts = a->starts; p.starts_i64 = (int)a->starts_is_i64;
+  p.B = (int)a->B; p.S = (int)a->S; p.T = (int)a->T; p.H = (int)a->H; p.G = (int)a->G; p.R = (int)(a->H / a->G);
+  p.d = (int)a->d; p.causal = a->causal != 0;
+  p.c = (float)(a->scale * 1.4426950408889634074);
+  p.scale = (float)a->scale;
+  p.lse = a->lse;
+  const size_t es = esize((int)a->dtype);
+  int vec = operand_vec(a->q, &a->q_sb, a->S, a->d, es);
+  if (a->T > 0) {
+    const int vk = operand_vec(a->k, &a->k_sb, a->T, a->d, es), vv = operand_vec(a->v, &a->v_sb, a->T, a->d, es);
+    vec = vk < vec ? vk : vec;
+    vec = vv < vec ? vv : vec;
+  }
+  p.vec = vec;
+}
+
+int check_inputs(const amoe_attn_args* a) {
+  const size_t es = esize((int)a->dtype);
+  if (int rc = check_operand(a->q, &a->q_sb, a->S, a->H, a->d, es)) return rc;
+  if (int rc = check_operand(a->k, &a->k_sb, a->T, a->G, a->d, es)) return rc;
+  if (int rc = check_operand(a->v, &a->v_sb, a->T, a->G, a->d, es)) return rc;
+  if (!aligned(a->lengths, a->lengths_is_i64 ? 8 : 4) || !aligned(a->starts, a->starts_is_i64 ? 8 : 4)) return AMOE_EALIGN;
+  return aligned(a->lse, 4) ? AMOE_OK : AMOE_EALIGN;
+}
+
+}  // namespace
+
+extern "C" size_t amoe_attn_args_bytes(void) { return sizeof(amoe_attn_args); }
+
+extern "C" size_t amoe_attention_fwd_workspace(const amoe_attn_args* a) {
+  if (check_sizes(a) || a->B == 0 || a->S == 0) return 0;
+  const int n = attn_splits(a);
+  return n > 1 ? (size_t)n * (size_t)(a->B * a->H * a->S) * (size_t)(a->d + 2) * 4 : 0;
+}
+
+extern "C" int amoe_attention_fwd(const amoe_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_sizes(a)) return rc;
+  if (a->B == 0 || a->S == 0) return AMOE_OK;
+  if (int rc = check_inputs(a)) return rc;
+  const size_t es = esize((int)a->dtype);
+  if (!a->out) return AMOE_ENULL;
+  if (!aligned(a->out, es)) return AMOE_EALIGN;
+  AttnParams p{};
+  fill(p, a);
+  p.out = a->out;
+  if (!aligned(a->out, 16) && p.vec == 2) p.vec = 1;
+  p.splits = attn_splits(a);
+  if (p.splits > 1) {
+    const size_t need = amoe_attention_fwd_workspace(a);
+    if (!workspace) return AMOE_ENULL;
+    if (workspace_bytes < need) return AMOE_EWORKSPACE;
+    if (!aligned(workspace, 16)) return AMOE_EALIGN;
+    // (the rows first: their 16-byte stores)
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + (size_t)p.splits * (size_t)(a->B * a->H * a->S) * (size_t)a->d;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return a->dtype == AMOE_F32   ? launch_attn_fwd_f32(p, st)
+         : a->dtype == AMOE_F16 ? launch_attn_fwd_f16(p, st)
+                                : launch_attn_fwd_bf16(p, st);
+}
+
+extern "C" size_t amoe_attention_bwd_workspace(const amoe_attn_args* a) {
+  if (check_sizes(a)) return 0;
+  return (size_t)(a->B * a->H * a->S) * 4;
+}
+
+extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_sizes(a)) return rc;
+  if (a->B == 0 || (a->S == 0 && a->T == 0)) return AMOE_OK;
+  if (int rc = check_inputs(a)) return rc;
+  const size_t es = esize((int)a->dtype);
+  if (int rc = check_operand(a->go, &a->go_sb, a->S, a->H, a->d, es)) return rc;
+  if ((a->S > 0 && (!a->out || !a->lse || !a->dq || !workspace)) || !a->dk != !a->dv) return AMOE_ENULL;
+  if (!aligned(a->out, es) || !aligned(a->dq, es) || !aligned(a->dk, es) || !aligned(a->dv, es)) return AMOE_EALIGN;
+  if (workspace_bytes < amoe_attention_bwd_workspace(a)) return AMOE_EWORKSPACE;
+  if (!aligned(workspace, 4)) return AMOE_EALIGN;
+  AttnParams p{};
+  fill(p, a);
+  p.go = {a->go, a->go_sb, a->go_ss, a->go_sh};
+  if (a->S > 0) {
+    const int vg = operand_vec(a->go, &a->go_sb, a->S, a->d, es);
+    p.vec = vg < p.vec ? vg : p.vec;
+  }
+  const bool whole = aligned(a->out, 16) && aligned(a->dq, 16) && aligned(a->dk, 16) && aligned(a->dv, 16);
+  if (!whole) p.vec = 0;
+  // (rows of `out` are d elements apart: with another d their starts are not on 16 bytes)
+  if ((a->d * es) % 16) p.vec = 0;
+  p.o = a->out;
+  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  p.delta = static_cast<float*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return a->dtype == AMOE_F32   ? launch_attn_bwd_f32(p, st)
+         : a->dtype == AMOE_F16 ? launch_attn_bwd_f16(p, st)
+                                : launch_attn_bwd_bf16(p, st);
+}

@@ -1,0 +1,285 @@
+// Attention forward: out = softmax(scale * q k^T + mask) v in one pass over the keys, with the running maximum and sum of every
+// row; a row that sees no key gives zeros.
+#pragma once
+#include "attn_tile.h"
+
+namespace amoe {
+
+// A row's scores are kept as s * c in the exponent of 2.  fp16 probabilities are kept 2^15 times as large (so that what is
+// 2^-29 of a row's largest is still a normal number; at 1 times, a long row's tail below 2^-14 would lose bits that its sum
+// counts): the sum carries the same factor and the quotient none.
+template <typename T> inline constexpr float kProbShift = kIsF16<T> ? 15.f : 0.f;
+
+// State of a wave's 32 queries (a lane and its partner l ^ 32 hold one): output columns, running maximum, running sum of
+// this lane's keys.
+template <typename T, int DP> struct AttnState {
+  f32x16 o[DP / 32];
+  float m, l;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < DP / 32; t++) o[t] = f32x16_zero();
+    m = -INFINITY;
+    l = 0.f;
+  }
+};
+
+// NB blocks of 32 keys from key0 on against the wave's queries: s[n] are their scores, `seen` the number of keys the lane's
+// query sees (from key 0), v the tile whose first row is key0.
+template <typename T, int DP, int NB>
+__device__ __forceinline__ void attn_step(AttnState<T, DP>& st, f32x16 (&s)[NB], const T* v, int key0, int seen, bool mask, float c) {
+  const int h = lane_id() >> 5;
+  float mx = st.m;
+  if (mask) {
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (key0 + 32 * n + 8 * (i / 4) + 4 * h + i % 4 >= seen) s[n][i] = -INFINITY;
+  }
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[n][i]);
+  mx = attn_pair_max(mx);
+  // what was summed so far, in units of the new maximum; once the maxima have settled nothing changes for a whole wave
+  if (wave_ballot(mx > st.m) != 0) {
+    const float f = mx > st.m ? fast_exp2((st.m - mx) * c) : 1.f;
+    st.l *= f;
+#pragma unroll
+    for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) st.o[t][i] *= f;
+    st.m = mx;
+  }
+  const float base = kProbShift<T> - (mx == -INFINITY ? 0.f : mx * c);
+  float sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      float pr[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        pr[j] = fast_exp2(fmaf(s[n][8 * w + j], c, base));
+        sum += pr[j];
+      }
+      const attn_frag<T> b = attn_pack<T>(pr);
+#pragma unroll
+      for (int t = 0; t < DP / 32; t++) st.o[t] = attn_mma<T>(AttnTile<T, DP>::col_frag(v, 32 * n + 16 * w, t), b, st.o[t]);
+    }
+  st.l += sum;
+}
+
+// Many rows: a workgroup has 128 queries of one head, 32 per wave, and walks the keys in tiles of kKeys that go through
+// registers into LDS, two tiles by turns with one barrier each.
+template <typename T> inline constexpr int kAttnKeys = sizeof(T) == 4 ? 32 : 64;
+
+template <typename T, int DP, bool EDGE>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_rows_kernel(AttnParams p) {
+  using Tile = AttnTile<T, DP>;
+  constexpr int BN = kAttnKeys<T>, NB = BN / 32, NK = DP / 16;
+  __shared__ __align__(16) T lds_k[2][BN * DP];
+  __shared__ __align__(16) T lds_v[2][BN * DP];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
+  // workgroups with one head next to each other's on an XCD (ids go round the eight); the longest rows first
+  const int BH = p.B * p.H, bh = (int)(blockIdx.x % (unsigned)BH), tile = (p.S + kAttnRows - 1) / kAttnRows - 1 - (int)(blockIdx.x / (unsigned)BH);
+  const int b = bh / p.H, hd = bh - b * p.H, g = hd / p.R;
+  const int length = attn_length(p, b), start = attn_start(p, b);
+  const int w0 = tile * kAttnRows + wave * 32, i = w0 + (lane & 31);
+  const int last = p.S - 1 < tile * kAttnRows + kAttnRows - 1 ? p.S - 1 : tile * kAttnRows + kAttnRows - 1;
+  const int group_sees = attn_seen(p, length, start, last);
+  const int wave_last = p.S - 1 < w0 + 31 ? p.S - 1 : w0 + 31;
+  const int wave_sees = w0 < p.S ? attn_seen(p, length, start, wave_last) : 0;
+  const int wave_all = w0 < p.S ? attn_seen(p, length, start, w0) : 0;         // keys that every row of the wave sees
+  const int seen = attn_seen(p, length, start, i < p.S ? i : p.S - 1);
+
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+  AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
+  sk.init(tid, p.k.ss, p.d);
+  sv.init(tid, p.v.ss, p.d);
+  const int n_tiles = (group_sees + BN - 1) / BN;
+  if (n_tiles > 0) {
+    sk.load(tid, kb, p.k.ss, 0, group_sees, p.d, p.vec);
+    sv.load(tid, vb, p.v.ss, 0, group_sees, p.d, p.vec);
+  }
+  attn_frag<T> q[NK];
+  const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
+#pragma unroll
+  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, i < p.S, p.vec);
+
+  AttnState<T, DP> st;
+  st.clear();
+  if (n_tiles > 0) {
+    sk.store(tid, lds_k[0]);
+    sv.store(tid, lds_v[0]);
+  }
+  for (int t = 0; t < n_tiles; t++) {
+    const int key0 = t * BN;
+    __syncthreads();       // tile t is there, and nobody reads the other one any more
+    if (t + 1 < n_tiles) {
+      sk.load(tid, kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
+      sv.load(tid, vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
+    }
+    if (key0 < wave_sees) {
+      f32x16 s[NB];
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        s[n] = f32x16_zero();
+#pragma unroll
+        for (int kk = 0; kk < NK; kk++) s[n] = attn_mma<T>(Tile::row_frag(lds_k[t & 1], 32 * n, kk), q[kk], s[n]);
+      }
+      attn_step<T, DP, NB>(st, s, lds_v[t & 1], key0, seen, key0 + BN > wave_all, p.c);
+    }
+    if (t + 1 < n_tiles) {
+      sk.store(tid, lds_k[(t + 1) & 1]);
+      sv.store(tid, lds_v[(t + 1) & 1]);
+    }
+  }
+  const float l = attn_pair_sum(st.l), inv = l == 0.f ? 0.f : 1.f / l;
+  if (i < p.S) {
+    const int64_t row = ((int64_t)b * p.S + i) * p.H + hd;
+    attn_store_col<T, DP, EDGE>(static_cast<T*>(p.out) + row * p.d, st.o, inv, p.d);
+    if (p.lse && h == 0) p.lse[(int64_t)bh * p.S + i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
+  }
+}
+
+// Few rows: the R * S rows that share a key head, 32 per workgroup, and one of `splits` parts of the keys they see; every
+// wave takes every fourth block of 32 keys of the part.  K goes from global memory into the operands, V through a tile of the
+// wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.
+template <typename T, int DP, bool EDGE>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_split_kernel(AttnParams p) {
+  constexpr int NK = DP / 16, kRowF = DP + 4;     // floats between joined rows
+  constexpr int kTileBytes = 4 * 32 * DP * (int)sizeof(T), kJoinBytes = 4 * 32 * kRowF * 4;
+  __shared__ __align__(16) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
+  __shared__ float lds_m[4][32], lds_l[4][32];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
+  const int rows = p.R * p.S, row_tiles = (rows + 31) / 32;
+  int id = (int)blockIdx.x;
+  const int bg = id % (p.B * p.G);
+  id /= p.B * p.G;
+  const int split = id % p.splits, r0 = (id / p.splits) * 32;
+  const int b = bg / p.G, g = bg - b * p.G;
+  const int length = attn_length(p, b), start = attn_start(p, b);
+  // row r is query r % S of the group's head r / S
+  const int r = r0 + (lane & 31), rr = r < rows ? r : rows - 1, hd = g * p.R + rr / p.S, i = rr % p.S;
+  const int seen = attn_seen(p, length, start, i);
+  // keys that any row of the tile sees: with one head's rows in order it is the last row's, else the last query's
+  const int r_last = r0 + 31 < rows ? r0 + 31 : rows - 1;
+  const int tile_sees = attn_seen(p, length, start, r0 / p.S == r_last / p.S ? r_last % p.S : p.S - 1);
+  const int per = ((tile_sees + p.splits - 1) / p.splits + 127) / 128 * 128;
+  const int64_t lo64 = (int64_t)split * per;
+  const int key_lo = lo64 < tile_sees ? (int)lo64 : tile_sees, key_hi = tile_sees - key_lo < per ? tile_sees : key_lo + per;
+
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+  T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
+  attn_frag<T> q[NK], kf[NK];
+  const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
+  AttnStage<T, DP, 32, 64, EDGE> sv;
+  sv.init(lane, p.v.ss, p.d);
+  const auto fetch = [&](int key0) {
+    const int key = key0 + (lane & 31);
+    const T* krow = kb + (int64_t)key * p.k.ss;
+#pragma unroll
+    for (int kk = 0; kk < NK; kk++) kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, key < key_hi, p.vec);
+    sv.load(lane, vb, p.v.ss, key0, key_hi, p.d, p.vec);
+  };
+  int key0 = key_lo + 32 * wave;
+  if (key0 < key_hi) fetch(key0);
+#pragma unroll
+  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, r < rows, p.vec);
+  AttnState<T, DP> st;
+  st.clear();
+  for (; key0 < key_hi; key0 += 128) {
+    f32x16 s[1] = {f32x16_zero()};
+#pragma unroll
+    for (int kk = 0; kk < NK; kk++) s[0] = attn_mma<T>(kf[kk], q[kk], s[0]);
+    wave_sync();           // the tile's last reads are done
+    sv.store(lane, tile);
+    wave_sync();
+    if (key0 + 128 < key_hi) fetch(key0 + 128);
+    attn_step<T, DP, 1>(st, s, tile, key0, seen < key_hi ? seen : key_hi, true, p.c);
+  }
+
+  // the four waves' rows in units of the largest maximum
+  const float l = attn_pair_sum(st.l);
+  if (h == 0) {
+    lds_m[wave][lane] = st.m;
+    lds_l[wave][lane] = l;
+  }
+  __syncthreads();
+  float m = lds_m[0][lane & 31];
+  for (int w = 1; w < 4; w++) m = fmaxf(m, lds_m[w][lane & 31]);
+  const float f = st.m == -INFINITY ? 0.f : fast_exp2((st.m - m) * p.c);
+  float* mine = reinterpret_cast<float*>(lds) + (wave * 32 + (lane & 31)) * kRowF;
+#pragma unroll
+  for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      f32x4 o = {st.o[t][4 * u] * f, st.o[t][4 * u + 1] * f, st.o[t][4 * u + 2] * f, st.o[t][4 * u + 3] * f};
+      *reinterpret_cast<f32x4*>(mine + 32 * t + 8 * u + 4 * h) = o;
+    }
+  __syncthreads();
+  constexpr int kPer = 32 * DP / 4 / kAttnThreads;     // four elements each
+#pragma unroll
+  for (int u = 0; u < kPer; u++) {
+    const int idx = tid + u * kAttnThreads, row = idx / (DP / 4), e = idx % (DP / 4) * 4;
+    if (r0 + row >= rows || e >= p.d) continue;
+    float mr = lds_m[0][row], lr = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 1; w < 4; w++) mr = fmaxf(mr, lds_m[w][row]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float mw = lds_m[w][row];
+      lr += lds_l[w][row] * (mw == -INFINITY ? 0.f : fast_exp2((mw - mr) * p.c));
+      const f32x4 o = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * 32 + row) * kRowF + e);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] += o[j];
+    }
+    const int head = g * p.R + (r0 + row) / p.S, query = (r0 + row) % p.S;
+    const int64_t at = ((int64_t)b * p.H + head) * p.S + query;
+    if (p.splits > 1) {
+      const int64_t part = (int64_t)split * p.B * p.H * p.S + at;
+      store4<float>(p.part_o + part * p.d + e, v, EDGE ? p.d - e : 4, !EDGE);
+      if (e == 0) {
+        p.part_ml[2 * part] = mr;
+        p.part_ml[2 * part + 1] = lr;
+      }
+    } else {
+      const float inv = lr == 0.f ? 0.f : 1.f / lr;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] *= inv;
+      T* out = static_cast<T*>(p.out) + (((int64_t)b * p.S + query) * p.H + head) * p.d + e;
+      store4<T>(out, v, EDGE ? p.d - e : 4, !EDGE);
+      if (p.lse && e == 0) p.lse[at] = lr == 0.f ? INFINITY : mr * p.c + fast_log2(lr) - kProbShift<T>;
+    }
+  }
+}
+
+// The parts of a row joined: sums in units of the largest maximum, in the order of the parts.  One wave per row.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams p) {
+  const int64_t n = (int64_t)p.B * p.H * p.S, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = lane_id();
+  if (at >= n) return;
+  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_ml[2 * (s * n + at)]);
+  for (int s = 0; s < p.splits; s++) {
+    const float ms = p.part_ml[2 * (s * n + at)];
+    const float f = ms == -INFINITY ? 0.f : fast_exp2((ms - m) * p.c);
+    l += p.part_ml[2 * (s * n + at) + 1] * f;
+    const float* po = p.part_o + (s * n + at) * p.d;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (lane + 64 * j < p.d) o[j] += po[lane + 64 * j] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t bh = at / p.S, i = at - bh * p.S, b = bh / p.H, hd = bh - b * p.H;
+  T* out = static_cast<T*>(p.out) + ((b * p.S + i) * p.H + hd) * p.d;
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (lane + 64 * j < p.d) out[lane + 64 * j] = Elem<T>::cvt(o[j] * inv);
+  if (p.lse && lane == 0) p.lse[at] = l == 0.f ? INFINITY : m * p.c + fast_log2(l) - kProbShift<T>;
+}
+
+}  // namespace amoe

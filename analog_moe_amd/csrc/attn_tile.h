@@ -1,0 +1,239 @@
+// What the attention kernels share: the arguments, the tiles in LDS, the operands of the matrix instructions.
+//
+// All kernels work on 32 x 32 blocks of scores whose COLUMNS belong to lanes: the forward pass and the gradient of q form
+// K Q^T (a lane owns one query), the gradients of k and v form Q K^T (a lane owns one key).  Lane l then holds rows
+// 8 * (i / 4) + 4 * (l / 32) + i % 4, i = 0 .. 15, of column l % 32, so that the sums of a softmax are sums over registers
+// and one exchange with lane l ^ 32, and what is made of the scores is an operand of the next product where it lies: the
+// contraction of that product may run over the rows in any order, so the other operand is read in the order of the registers.
+#pragma once
+#include "common.h"
+
+namespace amoe {
+
+constexpr int kAttnThreads = 256;    // 4 waves
+constexpr int kAttnRows = 128;       // queries (keys, for their gradients) of a workgroup, 32 per wave
+constexpr int kAttnMaxHead = 128;    // elements of a head, at most
+constexpr int64_t kAttnMaxRows = 1 << 28;   // queries and keys of a sequence, at most
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnOperand {                 // [B, rows, heads, d] with these strides (elements), the last one 1
+  const void* p;
+  int64_t sb, ss, sh;
+};
+
+struct AttnParams {
+  AttnOperand q, k, v, go;           // go: gradient of the output
+  void* out;                         // [B, S, H, d]
+  const void* o;                     // the same, read by the backward pass
+  float* lse;                        // [B, H, S]: log2 of the sum of 2^(score * c); +inf where a row sees nothing.  May be null
+  float* delta;                      // [B, H, S]: sum over d of out * gradient of out
+  void *dq, *dk, *dv;                // [B, S, H, d], [B, T, G, d]
+  const void *lengths, *starts;      // [B] int32 / int64 or null
+  int lengths_i64, starts_i64;
+  int B, S, T, H, G, R, d, causal;   // G key heads, R = H / G query heads share one
+  int vec;                           // every operand in whole aligned 16-byte chunks with offsets that fit 32 bits
+  float c;                           // scale * log2(e)
+  float scale;
+  int splits;                        // forward of few rows: parts of the key axis
+  float *part_o, *part_ml;           // [splits][B * H * S][d], [splits][B * H * S][2]
+};
+
+// keys that sequence b holds
+__device__ __forceinline__ int attn_length(const AttnParams& p, int b) {
+  if (!p.lengths) return p.T;
+  const int64_t n = p.lengths_i64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
+  return (int)(n < 0 ? 0 : (n > p.T ? p.T : n));
+}
+// position of its first query; kept within +-2^29 (there are at most 2^28 queries and keys, so that no answer changes): sums
+// with row numbers stay in 32 bits
+__device__ __forceinline__ int attn_start(const AttnParams& p, int b) {
+  int64_t n = (int64_t)p.T - p.S;
+  if (p.starts) n = p.starts_i64 ? static_cast<const int64_t*>(p.starts)[b] : static_cast<const int32_t*>(p.starts)[b];
+  constexpr int64_t lim = 1 << 29;
+  return (int)(n < -lim ? -lim : (n > lim ? lim : n));
+}
+// keys [0, n) are what query i sees
+__device__ __forceinline__ int attn_seen(const AttnParams& p, int length, int start, int i) {
+  if (!p.causal) return length;
+  const int n = start + i + 1;
+  return n < 0 ? 0 : (n < length ? n : length);
+}
+
+// ---- operands -----------------------------------------------------------------------------------
+// 16 steps of a contraction for one matrix operand: lane l holds 8 of them (which 8 depends on l / 32) of row or column
+// l % 32.  16-bit types: one matrix instruction; fp32: eight, each of which takes element j of both halves of the wave.
+template <typename T> struct AttnFrag { typedef u32x4 type; };
+struct F32x8 { float v[8]; };
+template <> struct AttnFrag<float> { typedef F32x8 type; };
+template <typename T> using attn_frag = typename AttnFrag<T>::type;
+
+template <typename T>
+__device__ __forceinline__ f32x16 attn_mma(const attn_frag<T>& a, const attn_frag<T>& b, f32x16 c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c = mfma_32x32x2_f32(a.v[j], b.v[j], c);
+    return c;
+  } else {
+    return mfma_32x32x16<T>(a, b, c);
+  }
+}
+// eight values rounded to T (nearest, ties to even): for 16-bit types the matrix unit takes nothing wider.  A probability
+// or a score's gradient is off by 2^-9 (bf16) or 2^-12 (fp16) of itself at most, as much as a rounded output, and the errors
+// of a sum's terms are independent of each other.
+template <typename T>
+__device__ __forceinline__ attn_frag<T> attn_pack(const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    F32x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; j++) r.v[j] = v[j];
+    return r;
+  } else {
+    return raw_pack<T>(v);
+  }
+}
+
+// ---- tiles in LDS ---------------------------------------------------------------------------------
+// Rows of DP elements in 16-byte chunks; chunk c of row r lies at chunk c ^ swizzle(r) of the row.  Both ways a tile is
+// read touch every bank once: 16 rows at one chunk (operands whose rows are the tile's), and 4 rows at 4 adjacent chunks
+// (the transposing read).  Which bits of r go where depends on how many of the 64 banks a row moves on by.
+template <typename T, int DP> struct AttnTile {
+  static constexpr int kRowChunks = DP * (int)sizeof(T) / 16;
+  static constexpr int kChunk = 16 / (int)sizeof(T);
+  static constexpr int kRowWords = DP * (int)sizeof(T) / 4;
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (kRowWords % 64 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (kRowWords % 64 == 32) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  }
+  // element offset of chunk c of row r
+  static __device__ __forceinline__ int at(int r, int c) { return (r * kRowChunks + (c ^ swizzle(r))) * kChunk; }
+
+  // steps 16 * kk .. + 15 of the head axis, rows r0 + l % 32
+  static __device__ __forceinline__ attn_frag<T> row_frag(const T* tile, int r0, int kk) {
+    const int l = lane_id(), r = r0 + (l & 31), h = l >> 5;
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h + 1));
+      return F32x8{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+    } else {
+      return *reinterpret_cast<const u32x4*>(tile + at(r, 2 * kk + h));
+    }
+  }
+  // rows r0 .. r0 + 15 as the steps, in the order of a score block's registers, of head elements 32 * dt + l % 32
+  static __device__ __forceinline__ attn_frag<T> col_frag(const T* tile, int r0, int dt) {
+    const int l = lane_id(), h = l >> 5;
+    if constexpr (sizeof(T) == 4) {
+      const int d = 32 * dt + (l & 31);
+      F32x8 f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) f.v[j] = tile[at(r0 + 8 * (j / 4) + 4 * h + j % 4, d / 4) + d % 4];
+      return f;
+    } else {
+      const int r = r0 + 4 * h + ((l & 15) >> 2), d = 32 * dt + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+      const u32x2 lo = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(tile + at(r, d / 8) + d % 8));
+      const u32x2 hi = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(tile + at(r + 8, d / 8) + d % 8));
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  }
+};
+
+// Rows [row0, row0 + ROWS) of one head on their way from global memory through registers to a tile, by NT threads.  Rows at
+// or past row_end and elements at or past d read as zero and are not touched in memory.  EDGE: any strides and alignment.
+template <typename T, int DP, int ROWS, int NT, bool EDGE>
+struct AttnStage {
+  using Tile = AttnTile<T, DP>;
+  static constexpr int kN = ROWS * Tile::kRowChunks / NT;
+  static_assert(ROWS * Tile::kRowChunks % NT == 0, "whole chunks per thread");
+  Raw r[kN];
+  uint32_t off[EDGE ? 1 : kN];
+
+  __device__ __forceinline__ void init(int tid, int64_t stride, int d) {
+    if constexpr (!EDGE) {
+#pragma unroll
+      for (int i = 0; i < kN; i++) {
+        const int idx = tid + i * NT, row = idx / Tile::kRowChunks, ch = idx % Tile::kRowChunks;
+        // (an offset past every resource: reads zero)
+        off[i] = ch * Tile::kChunk < d ? (uint32_t)(row * stride * (int64_t)sizeof(T)) + (uint32_t)ch * 16u : 0xfffffff0u;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(int tid, const T* base, int64_t stride, int row0, int row_end, int d, bool vec) {
+    const T* p = base + (int64_t)row0 * stride;
+    const int rows = row_end - row0 < ROWS ? row_end - row0 : ROWS;
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int i = 0; i < kN; i++) {
+        const int idx = tid + i * NT, row = idx / Tile::kRowChunks, ch = idx % Tile::kRowChunks;
+        r[i] = raw_zero();
+        if (row < rows) r[i] = raw_load<T>(p + row * stride + ch * Tile::kChunk, d - ch * Tile::kChunk, vec);
+      }
+    } else {
+      const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d) * (uint32_t)sizeof(T) : 0u;
+      const BufRsrc rs = make_rsrc_sized(const_cast<T*>(rows > 0 ? p : base), bytes);
+#pragma unroll
+      for (int i = 0; i < kN; i++) r[i] = buffer_load_b128(rs, off[i], 0);
+    }
+  }
+  __device__ __forceinline__ void store(int tid, T* tile) const {
+#pragma unroll
+    for (int i = 0; i < kN; i++) {
+      const int idx = tid + i * NT;
+      *reinterpret_cast<Raw*>(tile + Tile::at(idx / Tile::kRowChunks, idx % Tile::kRowChunks)) = r[i];
+    }
+  }
+};
+
+// One row's operand, steps 16 * kk .., straight from global memory; ok: the row exists.
+template <typename T, bool EDGE>
+__device__ __forceinline__ attn_frag<T> attn_global_frag(const T* row, int kk, int d, bool ok, bool vec) {
+  const int h = lane_id() >> 5, e = 16 * kk + 8 * h;
+  const bool v = EDGE ? vec : true;
+  constexpr int C = Elem<T>::kChunk;
+  if constexpr (sizeof(T) == 4) {
+    Raw a = raw_zero(), b = raw_zero();
+    if (ok && e < d) a = raw_load<T>(row + e, EDGE ? d - e : C, v);
+    if (ok && e + 4 < d) b = raw_load<T>(row + e + 4, EDGE ? d - e - 4 : C, v);
+    return F32x8{{as_f32(a[0]), as_f32(a[1]), as_f32(a[2]), as_f32(a[3]), as_f32(b[0]), as_f32(b[1]), as_f32(b[2]), as_f32(b[3])}};
+  } else {
+    Raw a = raw_zero();
+    if (ok && e < d) a = raw_load<T>(row + e, EDGE ? d - e : C, v);
+    return a;
+  }
+}
+
+// the larger (the sum) of a lane's and its partner's in the other half of the wave
+__device__ __forceinline__ float attn_pair_max(float v) {
+  uint32_t a = as_u32(v), b = a;
+  swap_half_waves(a, b);
+  return fmaxf(as_f32(a), as_f32(b));
+}
+__device__ __forceinline__ float attn_pair_sum(float v) {
+  uint32_t a = as_u32(v), b = a;
+  swap_half_waves(a, b);
+  return as_f32(a) + as_f32(b);
+}
+
+// A lane's column of a [head elements][32] product: rows 8 * g + 4 * (l / 32) .. + 3 of every 32 are adjacent in memory.
+template <typename T, int DP, bool EDGE>
+__device__ __forceinline__ void attn_store_col(T* row, const f32x16* acc, float factor, int d) {
+  const int h = lane_id() >> 5;
+  const bool vec = (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int e = 32 * dt + 8 * g + 4 * h;
+      if (e >= d) continue;
+      const float v[4] = {acc[dt][4 * g] * factor, acc[dt][4 * g + 1] * factor, acc[dt][4 * g + 2] * factor, acc[dt][4 * g + 3] * factor};
+      store4<T>(row + e, v, EDGE ? d - e : 4, EDGE ? vec : true);
+    }
+}
+
+__device__ __forceinline__ f32x16 f32x16_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; i++) z[i] = 0.f;
+  return z;
+}
+
+}  // namespace amoe

@@ -14,8 +14,10 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 struct BufRsrc { const unsigned char* base; uint32_t bytes; };
 inline BufRsrc make_rsrc(const void* base) { return BufRsrc{static_cast<const unsigned char*>(base), 0xffffffffu}; }
 inline BufRsrc make_rsrc_sized(void* base, uint32_t bytes) { return BufRsrc{static_cast<const unsigned char*>(base), bytes}; }
+// out-of-range loads of a sized resource read zeros
 inline u32x4 buffer_load_b128(BufRsrc r, uint32_t lane_off, uint32_t uniform_off) {
-  u32x4 v;
+  u32x4 v{0u, 0u, 0u, 0u};
+  if (r.bytes != 0xffffffffu && (uint64_t)lane_off + uniform_off + 16 > r.bytes) return v;
   std::memcpy(&v, r.base + (size_t)lane_off + (size_t)uniform_off, 16);
   return v;
 }
@@ -211,6 +213,11 @@ inline float fast_sin_rev(float x) { return sinf(6.283185307179586f * x); }
 inline float fast_cos_rev(float x) { return cosf(6.283185307179586f * x); }
 inline int wave_uniform(int v) { return v; }
 inline float fast_log2(float x) { return log2f(x); }
+inline float fast_exp2(float x) { return exp2f(x); }
+inline void sincos_half_turns(float x, float* s, float* c) {
+  *s = (float)std::sin(3.14159265358979323846 * x);
+  *c = (float)std::cos(3.14159265358979323846 * x);
+}
 inline float fast_sqrt(float x) { return sqrtf(x); }
 inline uint32_t umulhi32(uint32_t a, uint32_t b) { return (uint32_t)(((uint64_t)a * b) >> 32); }
 

@@ -75,7 +75,7 @@ __device__ __forceinline__ u32x2 buffer_load_b64(BufRsrc r, uint32_t lane_off, u
   return __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, uniform_off, 0);
 }
 // Resource over [base, base + bytes): an access at a byte offset >= bytes is out of range; out-of-range stores are
-// dropped by the hardware, which makes a store conditional without a branch around it.
+// dropped by the hardware, which makes a store conditional without a branch around it, and out-of-range loads read zeros.
 __device__ __forceinline__ BufRsrc make_rsrc_sized(void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)bytes, 0x00020000);
 }
@@ -141,6 +141,10 @@ __device__ __forceinline__ float fast_sin_rev(float x) { return __builtin_amdgcn
 __device__ __forceinline__ float fast_cos_rev(float x) { return __builtin_amdgcn_cosf(x); }
 // log2 of a normal positive number (no denormal handling)
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
+// 2^x; a result below the normal numbers is zero
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// sin and cos of pi * x, to the last bit or two
+__device__ __forceinline__ void sincos_half_turns(float x, float* s, float* c) { ::sincospif(x, s, c); }
 __device__ __forceinline__ float fast_sqrt(float x) { return __builtin_amdgcn_sqrtf(x); }
 __device__ __forceinline__ uint32_t umulhi32(uint32_t a, uint32_t b) { return __umulhi(a, b); }
 

@@ -15,6 +15,7 @@ so every group of calls the Python layer makes is one opaque operator with a fak
   amoe::cvmm_forward        everything CVMM.forward launches  (cvmm.py:701-769)
   amoe::cvmm_backward       everything CVMM.backward launches (cvmm.py:772-897)
   amoe::ffn_fwd / ffn_bwd   the fused expert feed-forward, with its autograd formula registered
+  amoe::attention_fwd / attention_bwd, amoe::rotary   the decoder's attention and rotary positions, likewise
 
 Operators return an empty tensor where the Python interface returns ``None``.
 """
@@ -25,7 +26,7 @@ from typing import List, Optional
 import torch
 from torch import Tensor
 
-from . import ffn, ops
+from . import attention, ffn, ops, rotary
 
 _EMPTY_SHAPE = (0,)
 
@@ -359,3 +360,79 @@ def _ffn_autograd(ctx, dy, *_unused):
 
 
 ffn_fwd.register_autograd(_ffn_autograd, setup_context=_ffn_setup_context)
+
+
+# --------------------------------------------------------------------------- attention and rotary positions
+@torch.library.custom_op(
+    "amoe::attention_fwd", mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor? lengths, Tensor? starts, bool causal, float? scale, bool want_lse)"
+           " -> (Tensor, Tensor)")
+def attention_fwd(q, k, v, lengths, starts, causal, scale, want_lse):
+    """(out [B, S, H, d], lse [B, H, S] or empty)."""
+    out, lse = attention.attention_forward(q, k, v, lengths, starts, causal, scale, want_lse)
+    return out, torch.empty(_EMPTY_SHAPE, dtype=torch.float32, device=q.device) if lse is None else lse
+
+
+@attention_fwd.register_fake
+def _(q, k, v, lengths, starts, causal, scale, want_lse):
+    B, S, H, d = q.shape
+    return q.new_empty((B, S, H, d)), torch.empty((B, H, S) if want_lse else _EMPTY_SHAPE, dtype=torch.float32, device=q.device)
+
+
+@torch.library.custom_op(
+    "amoe::attention_bwd", mutates_args=(),
+    schema="(Tensor go, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor? lengths, Tensor? starts, bool causal, "
+           "float? scale) -> (Tensor, Tensor, Tensor)")
+def attention_bwd(go, q, k, v, out, lse, lengths, starts, causal, scale):
+    return attention.attention_backward(go, q, k, v, out, lse, lengths, starts, causal, scale)
+
+
+@attention_bwd.register_fake
+def _(go, q, k, v, out, lse, lengths, starts, causal, scale):
+    return q.new_empty(tuple(q.shape)), k.new_empty(tuple(k.shape)), v.new_empty(tuple(v.shape))
+
+
+def _attention_setup_context(ctx, inputs, output):
+    q, k, v, lengths, starts, causal, scale, want_lse = inputs
+    ctx.save_for_backward(q, k, v, lengths, starts, *output)
+    ctx.args = (causal, scale)
+    ctx.has_lse = want_lse
+    ctx.set_materialize_grads(False)
+
+
+def _attention_autograd(ctx, go, _grad_lse):
+    if go is None:
+        return (None,) * 8
+    if not ctx.has_lse:
+        raise RuntimeError("amoe::attention_fwd was called without want_lse: there is nothing to go back from")
+    q, k, v, lengths, starts, out, lse = ctx.saved_tensors
+    return (*torch.ops.amoe.attention_bwd(go, q, k, v, out, lse, lengths, starts, *ctx.args),) + (None,) * 5
+
+
+attention_fwd.register_autograd(_attention_autograd, setup_context=_attention_setup_context)
+
+
+@torch.library.custom_op(
+    "amoe::rotary", mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor turns, Tensor? positions, int start, bool interleaved, float size, bool inverse)"
+           " -> (Tensor, Tensor)")
+def rotary_op(q, k, turns, positions, start, interleaved, size, inverse):
+    return rotary.rotate(q, k, turns, positions, start, interleaved, size, inverse)
+
+
+@rotary_op.register_fake
+def _(q, k, turns, positions, start, interleaved, size, inverse):
+    return q.new_empty(tuple(q.shape)), k.new_empty(tuple(k.shape))
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    _, _, turns, positions, *ctx.args, ctx.inverse = inputs
+    ctx.save_for_backward(turns, positions)
+
+
+def _rotary_autograd(ctx, gq, gk):
+    turns, positions = ctx.saved_tensors
+    return (*torch.ops.amoe.rotary(gq, gk, turns, positions, *ctx.args, not ctx.inverse),) + (None,) * 6
+
+
+rotary_op.register_autograd(_rotary_autograd, setup_context=_rotary_setup_context)

@@ -6,6 +6,7 @@ There is no CPU path and no fallback: the library must have been built
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -54,6 +55,16 @@ def side_stream(device: torch.device) -> "torch.cuda.Stream":
 def _side(t: torch.Tensor):
     """Handle of the device's extra stream (None where there are no streams)."""
     return side_stream(t.device).cuda_stream if t.is_cuda else None
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """A context in which t's device is the current one: launches go to the streams of the current device."""
+    if not t.is_cuda or t.device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(t.device)
 
 
 def unwatched() -> bool:

@@ -1,0 +1,148 @@
+"""Rotary positions of the decoder's queries and keys on the HIP kernel (``amoe_rotary``).
+
+Pair i of a head turns by position * theta_i, theta_i = base^(-2 i / dim).  The pairs are (i, i + dim / 2), or (2 i, 2 i + 1) when
+interleaved; elements behind the first ``dim`` of a head stay.  For contexts past the trained one the angles are scaled:
+
+  "linear"  theta / factor: positions squeezed into the trained range;
+  "base"    base * factor^(dim / (dim - 2)): the slowest pair is stretched by ``factor``, the fastest keeps its angle;
+  "parts"   pairs that turn 32 times or more within ``trained_context`` keep their angle, those that turn once or less are
+            stretched by ``factor``, those between in proportion; turned values grow by 1 + 0.1 ln(factor).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
+
+from . import _abi, ops, raw
+
+SCALINGS = ("none", "linear", "base", "parts")
+
+
+def _angles(dim: int, base: float, scaling: str, factor: float, trained_context: Optional[int]):
+    """Radians per position of every pair."""
+    if scaling == "base" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    theta = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear":
+        theta = [t / factor for t in theta]
+    elif scaling == "parts":
+        keep = [min(1.0, max(0.0, (trained_context * t / (2 * math.pi) - 1) / 31)) for t in theta]
+        theta = [t * (w + (1 - w) / factor) for t, w in zip(theta, keep)]
+    return theta
+
+
+def _turns(theta) -> Tensor:
+    """Revolutions per position times 2^64, as the int64 with those bits: what the kernel multiplies positions by, exactly."""
+    words = [round(t / (2 * math.pi) * 2 ** 64) % 2 ** 64 for t in theta]
+    return torch.tensor([w - 2 ** 64 if w >= 2 ** 63 else w for w in words], dtype=torch.int64)
+
+
+def _rows(t: Tensor) -> Tensor:
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def rotate(q: Tensor, k: Tensor, turns: Tensor, positions: Optional[Tensor] = None, start: int = 0, interleaved: bool = False,
+           size: float = 1.0, inverse: bool = False, out: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor]:
+    """q [B, S, H, d] and k [B, S, G, d] turned by their positions (``amoe_rotary``), into new tensors or into ``out``, whose
+    strides are free but for adjacent head elements: q and k themselves, or the next rows of a cache.  turns: int64
+    [dim / 2], as ``Rotary`` holds it; inverse: the other way round."""
+    ops._need_gpu(q, k, turns, positions, *(out or ()))
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [batch, tokens, heads, head size]")
+    B, S, H, d = q.shape
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
+    code = raw.dtype_code(q)
+    if k.dtype != q.dtype:
+        raise TypeError("q and k must share one dtype")
+    if turns.dtype != torch.int64 or turns.dim() != 1 or not turns.is_contiguous():
+        raise TypeError("turns must be a contiguous int64 vector")
+    R = 2 * turns.numel()
+    if not 2 <= R <= d:
+        raise ValueError(f"{R} turning elements do not fit heads of {d}")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64, not {positions.dtype}")
+        if positions.shape not in ((S,), (B, S)):
+            raise ValueError(f"positions must be [{S}] or [{B}, {S}], not {tuple(positions.shape)}")
+        if start:
+            raise ValueError("positions or start, not both")
+    if any(t is not None and t.device != q.device for t in (k, turns, positions, *(out or ()))):
+        raise ValueError("all tensors must be on one device")
+    q, k = _rows(q), _rows(k)
+    if out is None:
+        out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    else:
+        for t, o in zip((q, k), out):
+            if o.shape != t.shape or o.dtype != t.dtype or (o.stride(3) != 1 and d > 1):
+                raise ValueError("out must have the shapes and dtype of q and k, with adjacent head elements")
+    args = _abi.ROTARY_ARGS.pack(
+        code, B, S, H, k.shape[2], d, R, interleaved, inverse, size, turns.data_ptr(),
+        0 if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64,
+        *((0, 0) if positions is None else (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()), start,
+        *(w for t in (q, k, *out) for w in (t.data_ptr(), *t.stride()[:3])))
+    lib = ops.get_lib()
+    with ops.device_of(q):
+        rc = lib.amoe_rotary(args, ops._stream(q))
+    _abi.check(lib, rc, "amoe_rotary")
+    return out
+
+
+class RotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, turns, positions, start, interleaved, size):
+        ctx.save_for_backward(turns, positions)
+        ctx.args = (start, interleaved, size)
+        return rotate(q, k, turns, positions, start, interleaved, size)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        turns, positions = ctx.saved_tensors
+        dq, dk = rotate(gq, gk, turns, positions, *ctx.args, inverse=True)
+        return dq, dk, None, None, None, None, None
+
+
+class Rotary(nn.Module):
+    """``rotary(q, k, positions=None, start=0) -> (q, k)`` turned.  positions: int32 / int64 [S] or [B, S], any value; without
+    them token s stands at start + s.  The table is an int64 buffer, so that ``.to(torch.bfloat16)`` of a model leaves the
+    angles as they are.  ``out``: tensors to write to instead (without gradients only)."""
+
+    def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 trained_context: Optional[int] = None):
+        super().__init__()
+        if dim < 2 or dim % 2 or dim > 2048:
+            raise ValueError(f"the turning part of a head has 2 to 2048 elements, an even number, not {dim}")
+        if scaling not in SCALINGS:
+            raise ValueError(f"scaling must be one of {SCALINGS}, not {scaling!r}")
+        if not base >= 1.0 or not factor >= 1.0 or math.isinf(base) or math.isinf(factor):
+            raise ValueError("base and factor must be finite and at least 1")
+        if scaling == "parts" and (trained_context is None or trained_context < 1):
+            raise ValueError("scaling by parts needs the trained context")
+        self.dim, self.interleaved = dim, interleaved
+        self.size = 1.0 + 0.1 * math.log(factor) if scaling == "parts" else 1.0
+        self.register_buffer("turns", _turns(_angles(dim, base, scaling, factor, trained_context)), persistent=False)
+
+    def forward(self, q: Tensor, k: Tensor, positions: Optional[Tensor] = None, start: int = 0,
+                out: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor]:
+        args = (q, k, self.turns, positions, start, self.interleaved, self.size)
+        grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)
+        if out is not None:
+            if grad or any(t.requires_grad for t in out):
+                raise RuntimeError("out is for calls without gradients")
+            return rotate(*args, out=out)
+        if torch.compiler.is_compiling():
+            return torch.ops.amoe.rotary(*args, False)
+        if not grad and ops.unwatched():
+            return rotate(*args)
+        return RotaryFunction.apply(*args)
+
+    def extra_repr(self) -> str:
+        return f"dim={self.dim}, interleaved={self.interleaved}"
+
+
+from . import library  # noqa: E402,F401  (registers the operators that traced calls go through; it imports this module)

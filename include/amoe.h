@@ -448,6 +448,56 @@ int amoe_ffn_bwd(const amoe_ffn_args* args, void* workspace, size_t workspace_by
 const char* amoe_ffn_stage_name(int32_t backward, int32_t i);
 size_t amoe_ffn_args_bytes(void);
 
+/* ---------------------------------------------------------------------------------------
+ * The decoder's attention (the reference's decoder is the third-party sigma_moe model, example_aihwkit.py:6, 86-100; nothing
+ * of the reference's own is replaced here).  Every field of the argument structures is 8 bytes wide.
+ *
+ * amoe_rotary turns the first R elements of every head of q [B, S, q_heads, d] and k [B, S, k_heads, d] by their token's
+ * position: pair i = (i, i + R / 2), or (2i, 2i + 1) with `interleaved`, by positions * turns[i] / 2^64 revolutions, times
+ * `size`; elements R .. d - 1 are copied.  `inverse` turns the other way, which is the gradient.  Last strides are 1; outputs
+ * may be the inputs themselves, or views of a cache.  q_heads or k_heads may be 0. */
+typedef struct amoe_rotary_args {
+  int64_t dtype, B, S, q_heads, k_heads, d, R, interleaved, inverse;
+  double size;
+  const int64_t* turns;                                         /* [R / 2] */
+  const void* positions;  int64_t positions_are_i64;            /* int32 / int64 [B, S], or NULL: start + s */
+  int64_t pos_sb, pos_ss, start;
+  const void* q;  int64_t q_sb, q_ss, q_sh;
+  const void* k;  int64_t k_sb, k_ss, k_sh;
+  void* q_out;  int64_t q_out_sb, q_out_ss, q_out_sh;
+  void* k_out;  int64_t k_out_sb, k_out_ss, k_out_sh;
+} amoe_rotary_args;
+int amoe_rotary(const amoe_rotary_args* args, void* stream);
+size_t amoe_rotary_args_bytes(void);
+
+/* out = softmax(scale * q k^T + mask) v for q [B, S, H, d] and k, v [B, T, G, d], H a multiple of G: head h reads key head
+ * h / (H / G).  Sequence b holds the keys [0, lengths[b]) (NULL: T; values outside [0, T] are taken as the nearer end); keys
+ * behind them are not read.  With `causal` query i stands at position starts[b] + i (NULL: T - S + i) and sees the keys up to
+ * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; last strides are 1.
+ * Few rows over many keys are worked on in parts of the key axis, whose results pass through the workspace.
+ * The backward call recomputes the probabilities from lse (log2 of a row's sum, made by the forward call; NULL there: not
+ * wanted) and reads out; its workspace holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold are zero.
+ * Neither call uses atomics: equal inputs give equal bits. */
+typedef struct amoe_attn_args {
+  int64_t dtype, B, S, T, H, G, d, causal;
+  double scale;
+  const void* q;  int64_t q_sb, q_ss, q_sh;
+  const void* k;  int64_t k_sb, k_ss, k_sh;
+  const void* v;  int64_t v_sb, v_ss, v_sh;
+  const void* lengths;  int64_t lengths_is_i64;                 /* [B] int32 / int64 */
+  const void* starts;  int64_t starts_is_i64;
+  void* out;                                                    /* [B, S, H, d] */
+  float* lse;                                                   /* [B, H, S] */
+  /* backward only */
+  const void* go;  int64_t go_sb, go_ss, go_sh;                 /* gradient of out */
+  void* dq;  void* dk;  void* dv;                               /* [B, S, H, d], [B, T, G, d] */
+} amoe_attn_args;
+size_t amoe_attention_fwd_workspace(const amoe_attn_args* args);
+int amoe_attention_fwd(const amoe_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t amoe_attention_bwd_workspace(const amoe_attn_args* args);
+int amoe_attention_bwd(const amoe_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t amoe_attn_args_bytes(void);
+
 #ifdef __cplusplus
 }
 #endif
