@@ -86,7 +86,7 @@ extern "C" size_t amoe_attn_args_bytes(void) { return sizeof(amoe_attn_args); }
 extern "C" size_t amoe_attention_fwd_workspace(const amoe_attn_args* a) {
   if (check_sizes(a) || a->B == 0 || a->S == 0) return 0;
   const int n = attn_splits(a);
-  return n > 1 ? (size_t)n * (size_t)(a->B * a->H * a->S) * (size_t)(a->d + 2) * 4 : 0;
+  return n > 1 ? (size_t)n * (size_t)(a->B * a->H * a->S) * (size_t)((a->d + 3) / 4 * 4 + 2) * 4 : 0;
 }
 
 extern "C" int amoe_attention_fwd(const amoe_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -108,7 +108,7 @@ extern "C" int amoe_attention_fwd(const amoe_attn_args* a, void* workspace, size
     if (!aligned(workspace, 16)) return AMOE_EALIGN;
     // (the rows first: their 16-byte stores)
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = p.part_o + (size_t)p.splits * (size_t)(a->B * a->H * a->S) * (size_t)a->d;
+    p.part_ml = p.part_o + (size_t)p.splits * (size_t)(a->B * a->H * a->S) * (size_t)((a->d + 3) / 4 * 4);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a->dtype == AMOE_F32   ? launch_attn_fwd_f32(p, st)

@@ -19,7 +19,7 @@ template <typename T, int DP> struct AttnGrad {
     for (int t = 0; t < DP / 32; t++) acc[t] = f32x16_zero();
     scale = kIsF16<T> ? 0x1p100f : 1.f;
   }
-  __device__ __forceinline__ void fit(float (&ds)[16]) {
+  template <class V> __device__ __forceinline__ void fit(V& ds) {       // 16 values
     if constexpr (kIsF16<T>) {
       float a = 0.f;
 #pragma unroll
@@ -41,6 +41,18 @@ template <typename T, int DP> struct AttnGrad {
     }
   }
 };
+
+// a block's 16 values of a lane as two operands
+template <typename T, class V>
+__device__ __forceinline__ void attn_pack_block(const V& v, attn_frag<T> (&f)[2]) {
+#pragma unroll
+  for (int w = 0; w < 2; w++) {
+    float half[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) half[j] = v[8 * w + j];
+    f[w] = attn_pack<T>(half);
+  }
+}
 
 // dq: 128 queries of one head per workgroup, 32 per wave, keys in tiles as in the forward pass.  Also leaves delta.
 template <typename T, int DP, bool EDGE>
@@ -66,10 +78,11 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
   AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
   sk.init(tid, p.k.ss, p.d);
   sv.init(tid, p.v.ss, p.d);
+  typename Tile::Lane at;
   const int n_tiles = (group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, kb, p.k.ss, 0, group_sees, p.d, p.vec);
-    sv.load(tid, vb, p.v.ss, 0, group_sees, p.d, p.vec);
+    sk.load(tid, lds_k[0], kb, p.k.ss, 0, group_sees, p.d, p.vec);
+    sv.load(tid, lds_v[0], vb, p.v.ss, 0, group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK], go[NK];
   const int64_t row = ((int64_t)b * p.S + i) * p.H + hd;
@@ -105,38 +118,47 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
   }
   for (int t = 0; t < n_tiles; t++) {
     const int key0 = t * BN;
+    sk.finish();
     __syncthreads();
     if (t + 1 < n_tiles) {
-      sk.load(tid, kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
-      sv.load(tid, vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
+      sk.load(tid, lds_k[(t + 1) & 1], kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
+      sv.load(tid, lds_v[(t + 1) & 1], vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
     }
     if (key0 < wave_sees) {
       const T *kt = lds_k[t & 1], *vt = lds_v[t & 1];
       const bool mask = key0 + BN > wave_all;
+      // per 32 keys: 2 * NK products for the scores and dP by turns, 2 * DP / 32 with dS
+      constexpr int NU = DP / 32, NS = 2 * NK, NF = NS + 2 * NU;
+      const auto load = [&](int x) -> attn_frag<T> {
+        const int n = x / NF, e = x % NF;
+        return e < NS ? Tile::row_frag(e & 1 ? vt : kt, at, 32 * n, e / 2) : Tile::col_frag(kt, at, 32 * n + 16 * ((e - NS) / NU), (e - NS) % NU);
+      };
+      at.hide();
+      AttnRun<T, NB * NF, sizeof(T) == 2 && DP == 128 ? 4 : kAttnAhead<T>> run;      // (more do not fit the registers)
+      run.begin(load);
 #pragma unroll
       for (int n = 0; n < NB; n++) {
         f32x16 s = f32x16_zero(), dp = f32x16_zero();
-#pragma unroll
-        for (int kk = 0; kk < NK; kk++) {
-          s = attn_mma<T>(Tile::row_frag(kt, 32 * n, kk), q[kk], s);
-          dp = attn_mma<T>(Tile::row_frag(vt, 32 * n, kk), go[kk], dp);
-        }
+        run.steps(n * NF, n * NF + NS, load, [&](int x, const attn_frag<T>& a) {
+          const int e = x % NF;
+          if (e & 1) dp = attn_mma<T>(a, go[e / 2], dp);
+          else s = attn_mma<T>(a, q[e / 2], s);
+        });
         float ds[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          ds[e] = fast_exp2(fmaf(s[e], p.c, -lse)) * (dp[e] - delta);
-          if (mask && key0 + 32 * n + 8 * (e / 4) + 4 * h + e % 4 >= seen) ds[e] = 0.f;
+        for (int e = 0; e < 16; e++) ds[e] = fast_exp2(fmaf(s[e], p.c, -lse)) * (dp[e] - delta);
+        if (mask) {
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (key0 + 32 * n + 8 * (e / 4) + 4 * h + e % 4 >= seen) ds[e] = 0.f;
         }
         dq.fit(ds);
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          float half[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) half[j] = ds[8 * w + j];
-          const attn_frag<T> bf = attn_pack<T>(half);
-#pragma unroll
-          for (int u = 0; u < DP / 32; u++) dq.acc[u] = attn_mma<T>(Tile::col_frag(kt, 32 * n + 16 * w, u), bf, dq.acc[u]);
-        }
+        attn_frag<T> df[2];
+        attn_pack_block<T>(ds, df);
+        run.steps(n * NF + NS, n * NF + NF, load, [&](int x, const attn_frag<T>& a) {
+          const int e = x % NF - NS;
+          dq.acc[e % NU] = attn_mma<T>(a, df[e / NU], dq.acc[e % NU]);
+        });
       }
     }
     if (t + 1 < n_tiles) {
@@ -147,117 +169,172 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
   if (i < p.S) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, p.scale / dq.scale, p.d);
 }
 
-// dk, dv: 128 keys of one key head per workgroup, 32 per wave with their k and v as operands in registers; the queries of all
-// heads that share them pass in tiles.
-template <typename T, int DP, bool EDGE>
-__global__ __launch_bounds__(kAttnThreads, 1) void attn_bwd_kv_kernel(AttnParams p) {
+// dk, dv: KW waves hold 32 keys each of one key head, k and v as operands in registers, in QW copies; the queries of all heads
+// that share them pass in tiles of 32 * QW, 32 for each copy, and the copies' sums are added at the end, in order.  Every wave
+// reads what the other keys' waves read (a product of 32 x 32 takes as long as the LDS reads of its operands do); more copies
+// make shorter loops of the same work where there are few keys, and finer workgroups where causal rows differ in length.
+template <typename T, int DP, bool EDGE> struct AttnKvShape {
+  static constexpr bool kBig = sizeof(T) * DP > 256 || EDGE;       // fp32 heads past 64: 512 registers a wave, 4 waves
+  static constexpr int KW = 2, QW = sizeof(T) == 2 && DP == 128 && !EDGE ? 4 : 2;
+  // 16-bit heads past 96: dk, dv and k fill the registers, v is read from LDS for every product
+  static constexpr bool kVInLds = sizeof(T) == 2 && DP == 128 && !EDGE;
+  static constexpr int kThreads = 64 * KW * QW, kWavesPerSimd = kBig ? 1 : 2;
+};
+template <typename T, int DP, bool EDGE, class Shape = AttnKvShape<T, DP, EDGE>>
+__global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void attn_bwd_kv_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
-  constexpr int BM = kAttnKeys<T>, NB = BM / 32, NK = DP / 16;
-  __shared__ __align__(16) T lds_q[2][BM * DP];
-  __shared__ __align__(16) T lds_g[2][BM * DP];
+  constexpr int KW = Shape::KW, QW = Shape::QW, NT = Shape::kThreads, BM = 32 * QW, NK = DP / 16, NU = DP / 32;
+  constexpr int kTileElems = BM * DP, kTileBytes = 4 * kTileElems * (int)sizeof(T), kSumBytes = KW * (QW - 1) * NU * 16 * 64 * 4;
+  __shared__ __align__(1024) char lds[kTileBytes > kSumBytes ? kTileBytes : kSumBytes];
+  __shared__ __align__(1024) T lds_v[Shape::kVInLds ? 32 * KW * DP : 8];
   __shared__ __align__(16) float lds_lse[2][BM], lds_delta[2][BM];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
+  T* const lds_t = reinterpret_cast<T*>(lds);       // q by turns, then the output's gradient
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), kw = wave % KW, qw = wave / KW, h = lane >> 5;
   const int BG = p.B * p.G, bg = (int)(blockIdx.x % (unsigned)BG), tile = (int)(blockIdx.x / (unsigned)BG);
   const int b = bg / p.G, g = bg - b * p.G;
   const int length = attn_length(p, b), start = attn_start(p, b);
-  const int group0 = tile * kAttnRows, w0 = group0 + wave * 32, key = w0 + (lane & 31);
+  const int group0 = tile * 32 * KW, w0 = group0 + kw * 32, key = w0 + (lane & 31);
   const bool held = key < length;
-  const T* krow = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh + (int64_t)key * p.k.ss;
-  const T* vrow = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh + (int64_t)key * p.v.ss;
-  attn_frag<T> kf[NK], vf[NK];
-#pragma unroll
-  for (int kk = 0; kk < NK; kk++) {
-    kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, held, p.vec);
-    vf[kk] = attn_global_frag<T, EDGE>(vrow, kk, p.d, held, p.vec);
-  }
   // queries from q_first on see the first key of the group; tiles of every head in turn
   int q_first = 0;
   if (p.causal && group0 > start) q_first = group0 - start < p.S ? group0 - start : p.S;
   if (group0 >= length) q_first = p.S;
   const int tile0 = q_first / BM, per_head = (p.S + BM - 1) / BM - tile0, n_tiles = q_first < p.S ? per_head * p.R : 0;
 
-  AttnStage<T, DP, BM, kAttnThreads, EDGE> sq, sg;
+  AttnStage<T, DP, BM, NT, EDGE> sq, sg;
   sq.init(tid, p.q.ss, p.d);
   sg.init(tid, p.go.ss, p.d);
   float stat = 0.f;                                   // threads 0 .. BM - 1: lse, the next BM: delta
   const auto fetch = [&](int t) {
-    const int hd = g * p.R + t / per_head, q0 = (tile0 + t % per_head) * BM;
-    sq.load(tid, static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh, p.q.ss, q0, p.S, p.d, p.vec);
-    sg.load(tid, static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh, p.go.ss, q0, p.S, p.d, p.vec);
+    const int hd = g * p.R + t / per_head, q0 = (tile0 + t % per_head) * BM, buf = t & 1;
+    sq.load(tid, lds_t + buf * kTileElems, static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh, p.q.ss, q0, p.S, p.d, p.vec);
+    sg.load(tid, lds_t + (2 + buf) * kTileElems, static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh, p.go.ss, q0, p.S, p.d, p.vec);
     if (tid < 2 * BM) {
       const int qi = q0 + (tid < BM ? tid : tid - BM);
-      const int64_t at = ((int64_t)b * p.H + hd) * p.S + qi;
-      stat = qi < p.S ? (tid < BM ? p.lse[at] : p.delta[at]) : (tid < BM ? INFINITY : 0.f);
+      const int64_t row = ((int64_t)b * p.H + hd) * p.S + qi;
+      stat = qi < p.S ? (tid < BM ? p.lse[row] : p.delta[row]) : (tid < BM ? INFINITY : 0.f);
     }
   };
   const auto put = [&](int buf) {
-    sq.store(tid, lds_q[buf]);
-    sg.store(tid, lds_g[buf]);
+    sq.store(tid, lds_t + buf * kTileElems);
+    sg.store(tid, lds_t + (2 + buf) * kTileElems);
     if (tid < BM) lds_lse[buf][tid] = stat;
     else if (tid < 2 * BM) lds_delta[buf][tid - BM] = stat;
   };
+  if (n_tiles > 0) fetch(0);
+  const T* krow = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh + (int64_t)key * p.k.ss;
+  const T* vrow = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh + (int64_t)key * p.v.ss;
+  attn_frag<T> kf[NK], vf[Shape::kVInLds ? 1 : NK];
+#pragma unroll
+  for (int kk = 0; kk < NK; kk++) {
+    kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, held, p.vec);
+    if constexpr (!Shape::kVInLds) vf[kk] = attn_global_frag<T, EDGE>(vrow, kk, p.d, held, p.vec);
+  }
+  if constexpr (Shape::kVInLds) {
+    AttnStage<T, DP, 32 * KW, NT, EDGE> sv;
+    sv.init(tid, p.v.ss, p.d);
+    sv.load(tid, lds_v, static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, group0 < length ? group0 : 0,
+            group0 < length ? length : 0, p.d, p.vec);
+  }
   AttnGrad<T, DP> dk, dv;
   dk.clear();
   dv.clear();
-  if (n_tiles > 0) {
-    fetch(0);
-    put(0);
-  }
+  typename Tile::Lane at;
+  if (n_tiles > 0) put(0);
   for (int t = 0; t < n_tiles; t++) {
-    const int q0 = (tile0 + t % per_head) * BM, buf = t & 1;
+    const int q0 = (tile0 + t % per_head) * BM + 32 * qw, buf = t & 1;
+    sq.finish();
     __syncthreads();
     if (t + 1 < n_tiles) fetch(t + 1);
-    // the wave's keys are seen by some query of the tile, and whether by every one
-    if (w0 < length && (!p.causal || start + q0 + BM > w0)) {
-      const T *qt = lds_q[buf], *gt = lds_g[buf];
+    // the wave's keys are seen by some query of its block, and whether by every one
+    if (w0 < length && q0 < p.S && (!p.causal || start + q0 + 32 > w0)) {
+      const T *qt = lds_t + buf * kTileElems + 32 * qw * DP, *gt = lds_t + (2 + buf) * kTileElems + 32 * qw * DP;
       const bool mask = w0 + 32 > length || (p.causal && start + q0 < w0 + 31);
+      // 2 * NK products for the scores and dP by turns, 4 * DP / 32 with P and dS by turns
+      constexpr int kPer = Shape::kVInLds ? 3 : 2, NS = kPer * NK, NF = NS + 4 * NU;      // operands a score product and a dP product read
+      const auto load = [&](int e) -> attn_frag<T> {
+        if (e < NS) return e % kPer == 2 ? Tile::row_frag(lds_v, at, 32 * kw, e / kPer) : Tile::row_frag(e % kPer ? gt : qt, at, 0, e / kPer);
+        const int r = e - NS;
+        return Tile::col_frag(r & 1 ? qt : gt, at, 16 * (r / (2 * NU)), r / 2 % NU);
+      };
+      at.hide();
+      AttnRun<T, NF, sizeof(T) == 2 && DP == 128 ? 4 : kAttnAhead<T>> run;      // (more do not fit the registers)
+      run.begin(load);
+      f32x16 s = f32x16_zero(), dp = f32x16_zero();
+      attn_frag<T> gf;
+      run.steps(0, NS, load, [&](int e, const attn_frag<T>& a) {
+        if (e % kPer == 0) s = attn_mma<T>(a, kf[e / kPer], s);
+        else if (e % kPer == 2) dp = attn_mma<T>(gf, a, dp);
+        else if (Shape::kVInLds) gf = a;
+        else dp = attn_mma<T>(a, vf[e / kPer], dp);
+      });
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-        f32x16 s = f32x16_zero(), dp = f32x16_zero();
+      for (int u = 0; u < 4; u++) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&lds_lse[buf][32 * qw + 8 * u + 4 * h]);
+        const f32x4 del = *reinterpret_cast<const f32x4*>(&lds_delta[buf][32 * qw + 8 * u + 4 * h]);
 #pragma unroll
-        for (int kk = 0; kk < NK; kk++) {
-          s = attn_mma<T>(Tile::row_frag(qt, 32 * n, kk), kf[kk], s);
-          dp = attn_mma<T>(Tile::row_frag(gt, 32 * n, kk), vf[kk], dp);
-        }
-        float pr[16], ds[16];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const f32x4 lse = *reinterpret_cast<const f32x4*>(&lds_lse[buf][32 * n + 8 * u + 4 * h]);
-          const f32x4 del = *reinterpret_cast<const f32x4*>(&lds_delta[buf][32 * n + 8 * u + 4 * h]);
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const int e = 4 * u + j;
-            // (2^15 times P for fp16, as in the forward pass)
-            pr[e] = fast_exp2(fmaf(s[e], p.c, kProbShift<T> - lse[j]));
-            ds[e] = pr[e] * (dp[e] - del[j]);
-            if (mask && (!held || (p.causal && key > start + q0 + 32 * n + 8 * u + 4 * h + j))) pr[e] = ds[e] = 0.f;
-          }
-        }
-        dk.fit(ds);
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          float a[8], c[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            a[j] = pr[8 * w + j];
-            c[j] = ds[8 * w + j];
-          }
-          const attn_frag<T> pf = attn_pack<T>(a), df = attn_pack<T>(c);
-#pragma unroll
-          for (int u = 0; u < DP / 32; u++) {
-            dv.acc[u] = attn_mma<T>(Tile::col_frag(gt, 32 * n + 16 * w, u), pf, dv.acc[u]);
-            dk.acc[u] = attn_mma<T>(Tile::col_frag(qt, 32 * n + 16 * w, u), df, dk.acc[u]);
-          }
+        for (int j = 0; j < 4; j++) {
+          const int e = 4 * u + j;
+          // (2^15 times P for fp16, as in the forward pass)
+          s[e] = fast_exp2(fmaf(s[e], p.c, kProbShift<T> - lse[j]));
+          dp[e] = s[e] * (dp[e] - del[j]);
         }
       }
+      if (mask) {
+        // queries of the block before this one do not see the key
+        const int hides = held ? (p.causal ? key - start - q0 - 4 * h : -32) : 32;
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          if (8 * (e / 4) + e % 4 < hides) s[e] = dp[e] = 0.f;
+      }
+      dk.fit(dp);
+      attn_frag<T> pf[2], df[2];
+      attn_pack_block<T>(s, pf);
+      attn_pack_block<T>(dp, df);
+      run.steps(NS, NF, load, [&](int e, const attn_frag<T>& a) {
+        const int r = e - NS, w = r / (2 * NU), u = r / 2 % NU;
+        if (r & 1) dk.acc[u] = attn_mma<T>(a, df[w], dk.acc[u]);
+        else dv.acc[u] = attn_mma<T>(a, pf[w], dv.acc[u]);
+      });
     }
     if (t + 1 < n_tiles) put(buf ^ 1);
   }
-  if (key < p.T) {
-    const int64_t row = (((int64_t)b * p.T + key) * p.G + g) * p.d;
-    constexpr float kUnshift = kIsF16<T> ? 0x1p-15f : 1.f;
-    attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dv) + row, dv.acc, kUnshift, p.d);
-    attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dk) + row, dk.acc, p.scale * kUnshift / dk.scale, p.d);
+  // the copies' sums, in the layout of the registers: dv, then dk
+  constexpr float kUnshift = kIsF16<T> ? 0x1p-15f : 1.f;
+  const int64_t row = (((int64_t)b * p.T + key) * p.G + g) * p.d;
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+    f32x16* acc = which ? dk.acc : dv.acc;
+    const float factor = which ? p.scale * kUnshift / dk.scale : kUnshift;
+    __syncthreads();
+    if (qw > 0) {
+#pragma unroll
+      for (int t = 0; t < NU; t++)
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          sums[((((qw - 1) * KW + kw) * NU + t) * 4 + u) * 64 + lane] =
+              f32x4{acc[t][4 * u] * factor, acc[t][4 * u + 1] * factor, acc[t][4 * u + 2] * factor, acc[t][4 * u + 3] * factor};
+    }
+    __syncthreads();
+    if (qw == 0 && key < p.T) {
+#pragma unroll
+      for (int t = 0; t < NU; t++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          f32x4 v = f32x4{acc[t][4 * u] * factor, acc[t][4 * u + 1] * factor, acc[t][4 * u + 2] * factor, acc[t][4 * u + 3] * factor};
+#pragma unroll
+          for (int c = 0; c < QW - 1; c++) {
+            const f32x4 o = sums[(((c * KW + kw) * NU + t) * 4 + u) * 64 + lane];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += o[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[t][4 * u + j] = v[j];
+          sched_fence();          // (all the reads at once do not fit the registers)
+        }
+      attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d);
+    }
   }
 }
 

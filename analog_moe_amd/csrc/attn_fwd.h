@@ -23,10 +23,11 @@ template <typename T, int DP> struct AttnState {
   }
 };
 
-// NB blocks of 32 keys from key0 on against the wave's queries: s[n] are their scores, `seen` the number of keys the lane's
-// query sees (from key 0), v the tile whose first row is key0.
+// The scores s of NB blocks of 32 keys from key0 on become probabilities, as operands pr of the product with v; `seen` is the
+// number of keys the lane's query sees (from key 0).
 template <typename T, int DP, int NB>
-__device__ __forceinline__ void attn_step(AttnState<T, DP>& st, f32x16 (&s)[NB], const T* v, int key0, int seen, bool mask, float c) {
+__device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[NB], attn_frag<T> (&pr)[2 * NB], int key0, int seen,
+                                             bool mask, float c) {
   const int h = lane_id() >> 5;
   float mx = st.m;
   if (mask) {
@@ -57,15 +58,13 @@ __device__ __forceinline__ void attn_step(AttnState<T, DP>& st, f32x16 (&s)[NB],
   for (int n = 0; n < NB; n++)
 #pragma unroll
     for (int w = 0; w < 2; w++) {
-      float pr[8];
+      float e[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        pr[j] = fast_exp2(fmaf(s[n][8 * w + j], c, base));
-        sum += pr[j];
+        e[j] = fast_exp2(fmaf(s[n][8 * w + j], c, base));
+        sum += e[j];
       }
-      const attn_frag<T> b = attn_pack<T>(pr);
-#pragma unroll
-      for (int t = 0; t < DP / 32; t++) st.o[t] = attn_mma<T>(AttnTile<T, DP>::col_frag(v, 32 * n + 16 * w, t), b, st.o[t]);
+      pr[2 * n + w] = attn_pack<T>(e);
     }
   st.l += sum;
 }
@@ -98,10 +97,11 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
   sk.init(tid, p.k.ss, p.d);
   sv.init(tid, p.v.ss, p.d);
+  typename Tile::Lane at;
   const int n_tiles = (group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, kb, p.k.ss, 0, group_sees, p.d, p.vec);
-    sv.load(tid, vb, p.v.ss, 0, group_sees, p.d, p.vec);
+    sk.load(tid, lds_k[0], kb, p.k.ss, 0, group_sees, p.d, p.vec);
+    sv.load(tid, lds_v[0], vb, p.v.ss, 0, group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK];
   const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
@@ -116,20 +116,30 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   }
   for (int t = 0; t < n_tiles; t++) {
     const int key0 = t * BN;
+    sk.finish();
     __syncthreads();       // tile t is there, and nobody reads the other one any more
     if (t + 1 < n_tiles) {
-      sk.load(tid, kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
-      sv.load(tid, vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
+      sk.load(tid, lds_k[(t + 1) & 1], kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
+      sv.load(tid, lds_v[(t + 1) & 1], vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
     }
     if (key0 < wave_sees) {
+      // NB * NK products for the scores, 2 * NB * DP / 32 with the probabilities
+      constexpr int NS = NB * NK, NU = DP / 32;
+      const T *kt = lds_k[t & 1], *vt = lds_v[t & 1];
+      const auto load = [&](int e) -> attn_frag<T> {
+        return e < NS ? Tile::row_frag(kt, at, 32 * (e % NB), e / NB) : Tile::col_frag(vt, at, 16 * ((e - NS) / NU), (e - NS) % NU);
+      };
+      at.hide();
+      AttnRun<T, NS + 2 * NB * NU> run;
+      run.begin(load);
       f32x16 s[NB];
+      attn_frag<T> pr[2 * NB];
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-        s[n] = f32x16_zero();
-#pragma unroll
-        for (int kk = 0; kk < NK; kk++) s[n] = attn_mma<T>(Tile::row_frag(lds_k[t & 1], 32 * n, kk), q[kk], s[n]);
-      }
-      attn_step<T, DP, NB>(st, s, lds_v[t & 1], key0, seen, key0 + BN > wave_all, p.c);
+      for (int n = 0; n < NB; n++) s[n] = f32x16_zero();
+      run.steps(0, NS, load, [&](int e, const attn_frag<T>& a) { s[e % NB] = attn_mma<T>(a, q[e / NB], s[e % NB]); });
+      attn_softmax<T, DP, NB>(st, s, pr, key0, seen, key0 + BN > wave_all, p.c);
+      run.steps(NS, NS + 2 * NB * NU, load,
+                [&](int e, const attn_frag<T>& a) { st.o[(e - NS) % NU] = attn_mma<T>(a, pr[(e - NS) / NU], st.o[(e - NS) % NU]); });
     }
     if (t + 1 < n_tiles) {
       sk.store(tid, lds_k[(t + 1) & 1]);
@@ -149,6 +159,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 // wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.
 template <typename T, int DP, bool EDGE>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_split_kernel(AttnParams p) {
+  using Tile = AttnTile<T, DP>;
   constexpr int NK = DP / 16, kRowF = DP + 4;     // floats between joined rows
   constexpr int kTileBytes = 4 * 32 * DP * (int)sizeof(T), kJoinBytes = 4 * 32 * kRowF * 4;
   __shared__ __align__(16) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
@@ -176,14 +187,15 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
   attn_frag<T> q[NK], kf[NK];
   const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
-  AttnStage<T, DP, 32, 64, EDGE> sv;
+  AttnStage<T, DP, 32, 64, EDGE, true> sv;
   sv.init(lane, p.v.ss, p.d);
+  typename Tile::Lane at;
   const auto fetch = [&](int key0) {
     const int key = key0 + (lane & 31);
     const T* krow = kb + (int64_t)key * p.k.ss;
 #pragma unroll
     for (int kk = 0; kk < NK; kk++) kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, key < key_hi, p.vec);
-    sv.load(lane, vb, p.v.ss, key0, key_hi, p.d, p.vec);
+    sv.load(lane, nullptr, vb, p.v.ss, key0, key_hi, p.d, p.vec);
   };
   int key0 = key_lo + 32 * wave;
   if (key0 < key_hi) fetch(key0);
@@ -199,7 +211,12 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
     sv.store(lane, tile);
     wave_sync();
     if (key0 + 128 < key_hi) fetch(key0 + 128);
-    attn_step<T, DP, 1>(st, s, tile, key0, seen < key_hi ? seen : key_hi, true, p.c);
+    attn_frag<T> pr[2];
+    attn_softmax<T, DP, 1>(st, s, pr, key0, seen < key_hi ? seen : key_hi, true, p.c);
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+      for (int u = 0; u < DP / 32; u++) st.o[u] = attn_mma<T>(Tile::col_frag(tile, at, 16 * w, u), pr[w], st.o[u]);
   }
 
   // the four waves' rows in units of the largest maximum
@@ -237,10 +254,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
       for (int j = 0; j < 4; j++) v[j] += o[j];
     }
     const int head = g * p.R + (r0 + row) / p.S, query = (r0 + row) % p.S;
-    const int64_t at = ((int64_t)b * p.H + head) * p.S + query;
+    const int64_t where = ((int64_t)b * p.H + head) * p.S + query;
     if (p.splits > 1) {
-      const int64_t part = (int64_t)split * p.B * p.H * p.S + at;
-      store4<float>(p.part_o + part * p.d + e, v, EDGE ? p.d - e : 4, !EDGE);
+      const int64_t part = (int64_t)split * p.B * p.H * p.S + where;
+      store4<float>(p.part_o + part * ((p.d + 3) & ~3) + e, v, 4, true);
       if (e == 0) {
         p.part_ml[2 * part] = mr;
         p.part_ml[2 * part + 1] = lr;
@@ -251,35 +268,62 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
       for (int j = 0; j < 4; j++) v[j] *= inv;
       T* out = static_cast<T*>(p.out) + (((int64_t)b * p.S + query) * p.H + head) * p.d + e;
       store4<T>(out, v, EDGE ? p.d - e : 4, !EDGE);
-      if (p.lse && e == 0) p.lse[at] = lr == 0.f ? INFINITY : mr * p.c + fast_log2(lr) - kProbShift<T>;
+      if (p.lse && e == 0) p.lse[where] = lr == 0.f ? INFINITY : mr * p.c + fast_log2(lr) - kProbShift<T>;
     }
   }
 }
 
-// The parts of a row joined: sums in units of the largest maximum, in the order of the parts.  One wave per row.
+// The parts of a row joined, a workgroup per row: sums in units of the largest maximum, eight runs of parts side by side and
+// then those in order.
+constexpr int kAttnMaxSplits = 1024;
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams p) {
-  const int64_t n = (int64_t)p.B * p.H * p.S, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = lane_id();
-  if (at >= n) return;
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_ml[2 * (s * n + at)]);
-  for (int s = 0; s < p.splits; s++) {
+  __shared__ float lds_f[kAttnMaxSplits], lds_red[8];
+  __shared__ __align__(16) f32x4 lds_o[8][32];
+  const int64_t n = (int64_t)p.B * p.H * p.S, at = blockIdx.x;
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, row_units = (p.d + 3) / 4;
+  float m = -INFINITY;
+  for (int s = tid; s < p.splits; s += kAttnThreads) m = fmaxf(m, p.part_ml[2 * (s * n + at)]);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, wave_shfl_xor(m, x));
+  if (lane == 0) lds_red[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(lds_red[0], lds_red[1]), fmaxf(lds_red[2], lds_red[3]));
+  float l = 0.f;
+  for (int s = tid; s < p.splits; s += kAttnThreads) {
     const float ms = p.part_ml[2 * (s * n + at)];
     const float f = ms == -INFINITY ? 0.f : fast_exp2((ms - m) * p.c);
+    lds_f[s] = f;
     l += p.part_ml[2 * (s * n + at) + 1] * f;
-    const float* po = p.part_o + (s * n + at) * p.d;
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-      if (lane + 64 * j < p.d) o[j] += po[lane + 64 * j] * f;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += wave_shfl_xor(l, x);
+  if (lane == 0) lds_red[4 + wave] = l;
+  __syncthreads();
+  l = (lds_red[4] + lds_red[5]) + (lds_red[6] + lds_red[7]);
+  const int unit = tid & 31, run = tid >> 5;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (unit < row_units) {
+    const f32x4* po = reinterpret_cast<const f32x4*>(p.part_o) + at * row_units + unit;
+#pragma unroll 8
+    for (int s = run; s < p.splits; s += 8) {
+      const f32x4 v = po[s * n * row_units];
+      const float f = lds_f[s];
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = fmaf(v[j], f, o[j]);
+    }
+  }
+  lds_o[run][unit] = o;
+  __syncthreads();
   const int64_t bh = at / p.S, i = at - bh * p.S, b = bh / p.H, hd = bh - b * p.H;
   T* out = static_cast<T*>(p.out) + ((b * p.S + i) * p.H + hd) * p.d;
+  if (tid < p.d) {
+    float v = 0.f;
 #pragma unroll
-  for (int j = 0; j < 2; j++)
-    if (lane + 64 * j < p.d) out[lane + 64 * j] = Elem<T>::cvt(o[j] * inv);
-  if (p.lse && lane == 0) p.lse[at] = l == 0.f ? INFINITY : m * p.c + fast_log2(l) - kProbShift<T>;
+    for (int r = 0; r < 8; r++) v += lds_o[r][tid >> 2][tid & 3];
+    out[tid] = Elem<T>::cvt(v * (l == 0.f ? 0.f : 1.f / l));
+  }
+  if (p.lse && tid == 0) p.lse[at] = l == 0.f ? INFINITY : m * p.c + fast_log2(l) - kProbShift<T>;
 }
 
 }  // namespace amoe

@@ -35,7 +35,7 @@ struct AttnParams {
   float c;                           // scale * log2(e)
   float scale;
   int splits;                        // forward of few rows: parts of the key axis
-  float *part_o, *part_ml;           // [splits][B * H * S][d], [splits][B * H * S][2]
+  float *part_o, *part_ml;           // [splits][B * H * S][d rounded up to 4], [splits][B * H * S][2]
 };
 
 // keys that sequence b holds
@@ -108,56 +108,110 @@ template <typename T, int DP> struct AttnTile {
   // element offset of chunk c of row r
   static __device__ __forceinline__ int at(int r, int c) { return (r * kRowChunks + (c ^ swizzle(r))) * kChunk; }
 
-  // steps 16 * kk .. + 15 of the head axis, rows r0 + l % 32
-  static __device__ __forceinline__ attn_frag<T> row_frag(const T* tile, int r0, int kk) {
-    const int l = lane_id(), r = r0 + (l & 31), h = l >> 5;
+  // Byte offsets of a lane's reads in a tile, but for what a constant of the read adds or flips: the swizzle only sees the
+  // low four bits of a row, and rows start on a power of two or 64 bytes, so that steps along the head are flipped bits.  (Kept
+  // apart they would be 16 registers; a loop makes them anew by hide().)
+  struct Lane {
+    int row, col;
+    __device__ __forceinline__ Lane() {
+      const int l = lane_id(), h = l >> 5;
+      row = at(l & 31, h) * (int)sizeof(T);
+      const int r = 4 * h + ((l & 15) >> 2), d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
+      col = (at(r, d / 8) + d % 8) * (int)sizeof(T);
+    }
+    __device__ __forceinline__ void hide() {
+      opaque(row);
+      opaque(col);
+    }
+  };
+  static constexpr int kRowBytes = DP * (int)sizeof(T);
+  static constexpr bool kPow2 = kRowWords % 32 == 0;
+
+  // steps 16 * kk .. + 15 of the head axis, rows r0 + l % 32 (r0 a multiple of 16, as below)
+  static __device__ __forceinline__ attn_frag<T> row_frag(const T* tile, const Lane& lane, int r0, int kk) {
     if constexpr (sizeof(T) == 4) {
+      const int l = lane_id(), r = r0 + (l & 31), h = l >> 5;
       const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h));
       const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h + 1));
       return F32x8{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
     } else {
-      return *reinterpret_cast<const u32x4*>(tile + at(r, 2 * kk + h));
+      const char* p = reinterpret_cast<const char*>(tile) + r0 * kRowBytes;
+      if constexpr (kPow2) return *reinterpret_cast<const u32x4*>(p + (lane.row ^ (kk << 5)));
+      else return *reinterpret_cast<const u32x4*>(p + (lane.row ^ ((kk & 1) << 5)) + (kk >> 1) * 64);
     }
   }
   // rows r0 .. r0 + 15 as the steps, in the order of a score block's registers, of head elements 32 * dt + l % 32
-  static __device__ __forceinline__ attn_frag<T> col_frag(const T* tile, int r0, int dt) {
-    const int l = lane_id(), h = l >> 5;
+  static __device__ __forceinline__ attn_frag<T> col_frag(const T* tile, const Lane& lane, int r0, int dt) {
     if constexpr (sizeof(T) == 4) {
-      const int d = 32 * dt + (l & 31);
+      const int l = lane_id(), h = l >> 5, d = 32 * dt + (l & 31);
       F32x8 f;
 #pragma unroll
       for (int j = 0; j < 8; j++) f.v[j] = tile[at(r0 + 8 * (j / 4) + 4 * h + j % 4, d / 4) + d % 4];
       return f;
     } else {
-      const int r = r0 + 4 * h + ((l & 15) >> 2), d = 32 * dt + 16 * ((l >> 4) & 1) + 4 * (l & 3);
-      const u32x2 lo = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(tile + at(r, d / 8) + d % 8));
-      const u32x2 hi = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(tile + at(r + 8, d / 8) + d % 8));
-      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      const char* p = reinterpret_cast<const char*>(tile) + r0 * kRowBytes;
+      u32x2 half[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {                        // rows 4 h .. + 3, and the same 8 on
+        const int o = kPow2 ? lane.col ^ (dt << 6) ^ (u << 5) : (lane.col ^ (u << 5)) + dt * 64;
+        half[u] = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(p + o + 8 * u * kRowBytes));
+      }
+      return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
     }
   }
 };
 
-// Rows [row0, row0 + ROWS) of one head on their way from global memory through registers to a tile, by NT threads.  Rows at
-// or past row_end and elements at or past d read as zero and are not touched in memory.  EDGE: any strides and alignment.
-template <typename T, int DP, int ROWS, int NT, bool EDGE>
+// A run of matrix products whose first operands come from LDS, with kAttnAhead of them on their way: a read takes as long as
+// three or four products, and left to itself the compiler has one in flight (of this kernel family's first form, which waited
+// for every operand, the backward pass ran at 36 % of the matrix rate, now at the figures beside the kernels).  Nothing is
+// moved across a step.  fp32 products take eight instructions each: two ahead do.
+template <typename T> inline constexpr int kAttnAhead = sizeof(T) == 4 ? 2 : 6;
+template <typename T, int N, int AHEAD = kAttnAhead<T>> struct AttnRun {
+  static constexpr int D = AHEAD < N ? AHEAD : N;
+  attn_frag<T> f[D];
+  template <class Load>
+  __device__ __forceinline__ void begin(Load load) {
+#pragma unroll
+    for (int i = 0; i < D; i++) f[i] = load(i);
+    sched_fence();
+  }
+  // steps lo .. hi - 1: use(i, operand i), and operand i + D is asked for
+  template <class Load, class Use>
+  __device__ __forceinline__ void steps(int lo, int hi, Load load, Use use) {
+#pragma unroll
+    for (int i = lo; i < hi; i++) {
+      use(i, f[i % D]);
+      if (i + D < N) f[i % D] = load(i + D);
+      sched_fence();
+    }
+  }
+};
+
+// Rows [row0, row0 + ROWS) of one head on their way from global memory to a tile, by NT threads.  Rows at or past row_end and
+// elements at or past d are zeros in the tile and are not touched in memory.  THROUGH_REGS: load() leaves them in registers and
+// store() puts them into the tile; else load() sends them straight there, in the order of the tile's slots (which saves 16 to 32
+// registers that the products need), to be there after finish() and a barrier.  EDGE: any strides and alignment, through registers.
+template <typename T, int DP, int ROWS, int NT, bool EDGE, bool THROUGH_REGS = EDGE>
 struct AttnStage {
   using Tile = AttnTile<T, DP>;
   static constexpr int kN = ROWS * Tile::kRowChunks / NT;
   static_assert(ROWS * Tile::kRowChunks % NT == 0, "whole chunks per thread");
-  Raw r[kN];
+  static_assert(!EDGE || THROUGH_REGS, "edges go through registers");
+  Raw r[THROUGH_REGS ? kN : 1];
   uint32_t off[EDGE ? 1 : kN];
 
   __device__ __forceinline__ void init(int tid, int64_t stride, int d) {
     if constexpr (!EDGE) {
 #pragma unroll
       for (int i = 0; i < kN; i++) {
-        const int idx = tid + i * NT, row = idx / Tile::kRowChunks, ch = idx % Tile::kRowChunks;
+        const int idx = tid + i * NT, row = idx / Tile::kRowChunks, slot = idx % Tile::kRowChunks;
+        const int ch = THROUGH_REGS ? slot : slot ^ Tile::swizzle(row);
         // (an offset past every resource: reads zero)
         off[i] = ch * Tile::kChunk < d ? (uint32_t)(row * stride * (int64_t)sizeof(T)) + (uint32_t)ch * 16u : 0xfffffff0u;
       }
     }
   }
-  __device__ __forceinline__ void load(int tid, const T* base, int64_t stride, int row0, int row_end, int d, bool vec) {
+  __device__ __forceinline__ void load(int tid, T* tile, const T* base, int64_t stride, int row0, int row_end, int d, bool vec) {
     const T* p = base + (int64_t)row0 * stride;
     const int rows = row_end - row0 < ROWS ? row_end - row0 : ROWS;
     if constexpr (EDGE) {
@@ -170,16 +224,25 @@ struct AttnStage {
     } else {
       const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d) * (uint32_t)sizeof(T) : 0u;
       const BufRsrc rs = make_rsrc_sized(const_cast<T*>(rows > 0 ? p : base), bytes);
+      char* to = reinterpret_cast<char*>(tile) + wave_uniform(tid >> 6) * 1024;
 #pragma unroll
-      for (int i = 0; i < kN; i++) r[i] = buffer_load_b128(rs, off[i], 0);
+      for (int i = 0; i < kN; i++) {
+        if constexpr (THROUGH_REGS) r[i] = buffer_load_b128(rs, off[i], 0);
+        else buffer_to_lds_b128(rs, to + i * NT * 16, off[i]);
+      }
     }
   }
   __device__ __forceinline__ void store(int tid, T* tile) const {
+    if constexpr (THROUGH_REGS) {
 #pragma unroll
-    for (int i = 0; i < kN; i++) {
-      const int idx = tid + i * NT;
-      *reinterpret_cast<Raw*>(tile + Tile::at(idx / Tile::kRowChunks, idx % Tile::kRowChunks)) = r[i];
+      for (int i = 0; i < kN; i++) {
+        const int idx = tid + i * NT;
+        *reinterpret_cast<Raw*>(tile + Tile::at(idx / Tile::kRowChunks, idx % Tile::kRowChunks)) = r[i];
+      }
     }
+  }
+  __device__ __forceinline__ void finish() const {
+    if constexpr (!THROUGH_REGS) lds_dma_wait();
   }
 };
 

@@ -21,6 +21,11 @@ inline u32x4 buffer_load_b128(BufRsrc r, uint32_t lane_off, uint32_t uniform_off
   std::memcpy(&v, r.base + (size_t)lane_off + (size_t)uniform_off, 16);
   return v;
 }
+inline void buffer_to_lds_b128(BufRsrc r, void* lds, uint32_t lane_off) {
+  const u32x4 v = buffer_load_b128(r, lane_off, 0);
+  std::memcpy(static_cast<char*>(lds) + 16 * (threadIdx.x & 63), &v, 16);
+}
+inline void lds_dma_wait() {}
 inline uint32_t buffer_load_b32(BufRsrc r, uint32_t lane_off, uint32_t uniform_off = 0) {
   uint32_t v;
   std::memcpy(&v, r.base + (size_t)lane_off + (size_t)uniform_off, 4);
@@ -39,6 +44,7 @@ inline uint32_t pack_high_halves(uint32_t hi, uint32_t lo) { return (hi & 0xffff
 inline uint32_t pack_low_halves(uint32_t hi, uint32_t lo) { return (hi << 16) | (lo & 0xffffu); }
 // scheduling fences mean nothing to a host compiler
 inline void sched_fence() {}
+inline void opaque(int&) {}
 
 inline int lane_id() { return threadIdx.x & 63; }
 

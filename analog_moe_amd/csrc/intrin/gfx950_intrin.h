@@ -74,6 +74,12 @@ __device__ __forceinline__ uint32_t buffer_load_b32(BufRsrc r, uint32_t lane_off
 __device__ __forceinline__ u32x2 buffer_load_b64(BufRsrc r, uint32_t lane_off, uint32_t uniform_off) {
   return __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, uniform_off, 0);
 }
+// 16 bytes per lane from memory straight to LDS, lane l's to lds + 16 * l (lds the same for the whole wave); zeros for lanes out
+// of range.  They are there after lds_dma_wait() and, for other waves, the barrier behind it.
+__device__ __forceinline__ void buffer_to_lds_b128(BufRsrc r, void* lds, uint32_t lane_off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, lane_off, 0, 0, 0);
+}
+__device__ __forceinline__ void lds_dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
 // Resource over [base, base + bytes): an access at a byte offset >= bytes is out of range; out-of-range stores are
 // dropped by the hardware, which makes a store conditional without a branch around it, and out-of-range loads read zeros.
 __device__ __forceinline__ BufRsrc make_rsrc_sized(void* base, uint32_t bytes) {
@@ -86,6 +92,8 @@ __device__ __forceinline__ void buffer_store_b128_nt(BufRsrc r, u32x4 v, uint32_
 
 // Nothing is scheduled across this point (the compiler otherwise re-orders a software pipeline to save registers).
 __device__ __forceinline__ void sched_fence() { __builtin_amdgcn_sched_barrier(0); }
+// v becomes something the compiler knows nothing about: what is made of it inside a loop is not kept in registers across it
+__device__ __forceinline__ void opaque(int& v) { asm volatile("" : "+v"(v)); }
 
 // the high halves of two words as one word: hi's in the upper half, lo's in the lower (one byte permute)
 __device__ __forceinline__ uint32_t pack_high_halves(uint32_t hi, uint32_t lo) {

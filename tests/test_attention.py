@@ -119,10 +119,10 @@ def lib_last(lib):
     return lib.amoe_emu_last_kernel()
 
 
-def test_what_lies_behind_the_keys_is_not_read(emu_ops):
-    for d in (64, 13):
-        q, k, v, go = inputs(2, 6, 50, 2, 1, d, "bf16")
-        lengths, starts = marks([19, 33]), marks([13, 27])
+def behind_the_keys(device, sizes):
+    for d in sizes:
+        q, k, v, go = (t.to(device) for t in inputs(2, 6, 50, 2, 1, d, "bf16"))
+        lengths, starts = marks([19, 33]).to(device), marks([13, 27]).to(device)
         want, _ = A.attention_forward(q, k, v, lengths, starts, want_lse=True)
         k, v = k.clone(), v.clone()
         for b, n in enumerate((19, 33)):
@@ -132,6 +132,20 @@ def test_what_lies_behind_the_keys_is_not_read(emu_ops):
         dq, dk, dv = A.attention_backward(go, q, k, v, out, lse, lengths, starts)
         assert all(torch.isfinite(t).all() for t in (dq, dk, dv))
         assert not dk[0, 19:].any() and not dv[1, 33:].any()
+
+
+def test_what_lies_behind_the_keys_is_not_read(emu_ops):
+    behind_the_keys("cpu", (64, 13))
+
+
+@pytest.mark.gpu
+def test_gpu_what_lies_behind_the_keys_is_not_read():
+    # (not a number everywhere first: nothing that a workgroup finds in its LDS may get into results either)
+    nan = torch.full((64, 256, 8, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
+    for d in (128, 96, 80, 64, 48, 13):
+        out, lse = A.attention_forward(nan, nan, nan, want_lse=True)
+        A.attention_backward(nan, nan, nan, nan, out, lse)
+        behind_the_keys("cuda", (d,))
 
 
 def test_marks_outside_the_tensors(emu_ops):
