@@ -11,7 +11,6 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _abi, ops, raw
 
@@ -23,119 +22,139 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _marks(t: Optional[Tensor], B: int, like: Tensor, name: str) -> Optional[Tensor]:
-    if t is None:
-        return None
+def _marks(t: Tensor, B: int, device: torch.device, name: str) -> Tensor:
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
     if t.shape != (B,):
         raise ValueError(f"{name} must hold one value per sequence, [{B}], not {tuple(t.shape)}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, q on {like.device}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, q on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _check(q: Tensor, k: Tensor, v: Tensor) -> None:
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError("q, k and v must be [batch, tokens, heads, head size]")
-    raw.dtype_code(q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError("q, k and v must share one dtype")
-    if k.device != q.device or v.device != q.device:
-        raise ValueError("q, k and v must be on one device")
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"{q.shape[2]} query heads cannot share {k.shape[2]} key heads evenly")
-    if not 1 <= q.shape[3] <= MAX_HEAD:
-        raise ValueError(f"heads have 1 to {MAX_HEAD} elements, not {q.shape[3]}")
+class _Call:
+    """One call's operands, checked, as the library takes them.  (Made for every call: kept lean.)"""
+    __slots__ = ("q", "k", "v", "lengths", "starts", "head", "middle", "shape", "kv_shape")
 
+    def __init__(self, q, k, v, lengths, starts, causal, scale):
+        ops._need_gpu(q, k, v, lengths, starts)
+        shape, kv = q.shape, k.shape
+        if len(shape) != 4 or len(kv) != 4:
+            raise ValueError("q, k and v must be [batch, tokens, heads, head size]")
+        B, S, H, d = shape
+        T, G = kv[1], kv[2]
+        dtype, device = q.dtype, q.device
+        code = raw.code_of(dtype)
+        if k.dtype != dtype or v.dtype != dtype:
+            raise TypeError("q, k and v must share one dtype")
+        if k.device != device or v.device != device:
+            raise ValueError("q, k and v must be on one device")
+        if kv != v.shape or kv[0] != B or kv[3] != d:
+            raise ValueError(f"q {tuple(shape)}, k {tuple(kv)} and v {tuple(v.shape)} do not match")
+        if G == 0 or H == 0 or H % G:
+            raise ValueError(f"{H} query heads cannot share {G} key heads evenly")
+        if not 1 <= d <= MAX_HEAD:
+            raise ValueError(f"heads have 1 to {MAX_HEAD} elements, not {d}")
+        if scale is None:
+            scale = 1.0 / math.sqrt(d)
+        elif not 0.0 < scale < 3.4e38:
+            raise ValueError(f"scale must be positive and finite, not {scale}")
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        n = m = n64 = m64 = 0
+        if lengths is not None:
+            lengths = _marks(lengths, B, device, "lengths")
+            n, n64 = lengths.data_ptr(), lengths.dtype == torch.int64
+        if starts is not None:
+            starts = _marks(starts, B, device, "starts")
+            m, m64 = starts.data_ptr(), starts.dtype == torch.int64
+        self.q, self.k, self.v, self.lengths, self.starts, self.shape, self.kv_shape = q, k, v, lengths, starts, shape, kv
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        self.head = (code, B, S, T, H, G, d, causal, scale, q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
+                     v.data_ptr(), vs[0], vs[1], vs[2], n, n64, m, m64)
 
-def _scale(scale: Optional[float], d: int) -> float:
-    if scale is None:
-        return 1.0 / math.sqrt(d)
-    if not 0.0 < scale < 3.4e38:
-        raise ValueError(f"scale must be positive and finite, not {scale}")
-    return float(scale)
+    def pack(self, out: Tensor, lse: Optional[Tensor], go: Optional[Tensor] = None, grads=(0, 0, 0)) -> bytes:
+        gp, gs = (0, (0, 0, 0)) if go is None else (go.data_ptr(), go.stride())
+        return _abi.ATTN_ARGS.pack(*self.head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), gp, gs[0], gs[1], gs[2], *grads)
 
+    def forward(self, want_lse: bool):
+        q, lib = self.q, ops.get_lib()
+        out = q.new_empty(self.shape)
+        B, S, H, _ = self.shape
+        lse = q.new_empty((B, H, S), dtype=torch.float32) if want_lse else None
+        args = self.pack(out, lse)
+        with ops.device_of(q):
+            need = lib.amoe_attention_fwd_workspace(args)
+            ws = q.new_empty(need, dtype=torch.uint8) if need else None
+            rc = lib.amoe_attention_fwd(args, None if ws is None else ws.data_ptr(), need, ops._stream(q))
+        if rc:
+            _abi.check(lib, rc, "amoe_attention_fwd")
+        return out, lse
 
-def _pack(q, k, v, lengths, starts, causal, scale, out, lse, go=None, grads=(0, 0, 0)) -> bytes:
-    B, S, H, d = q.shape
-    return _abi.ATTN_ARGS.pack(
-        raw.dtype_code(q), B, S, k.shape[1], H, k.shape[2], d, causal, scale,
-        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-        0 if lengths is None else lengths.data_ptr(), lengths is not None and lengths.dtype == torch.int64,
-        0 if starts is None else starts.data_ptr(), starts is not None and starts.dtype == torch.int64,
-        out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        *((0, 0, 0, 0) if go is None else (go.data_ptr(), *go.stride()[:3])), *grads)
+    def backward(self, go: Tensor, out: Tensor, lse: Tensor, want_kv: bool):
+        q, lib, go = self.q, ops.get_lib(), _rows(go)
+        dq = q.new_empty(self.shape)
+        dk = dv = None
+        if want_kv:
+            dk, dv = q.new_empty(self.kv_shape), q.new_empty(self.kv_shape)
+            args = self.pack(out, lse, go, (dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
+        else:
+            args = self.pack(out, lse, go, (dq.data_ptr(), 0, 0))
+        with ops.device_of(q):
+            ws = q.new_empty(max(lib.amoe_attention_bwd_workspace(args), 4), dtype=torch.uint8)
+            rc = lib.amoe_attention_bwd(args, ws.data_ptr(), ws.numel(), ops._stream(q))
+        if rc:
+            _abi.check(lib, rc, "amoe_attention_bwd")
+        return dq, dk, dv
 
 
 def attention_forward(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor] = None, starts: Optional[Tensor] = None,
                       causal: bool = True, scale: Optional[float] = None,
                       want_lse: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
     """(out [B, S, H, d], lse [B, H, S] fp32 or None): ``amoe_attention_fwd``.  lse is what ``attention_backward`` reads."""
-    ops._need_gpu(q, k, v, lengths, starts)
-    _check(q, k, v)
-    scale = _scale(scale, q.shape[3])
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    B, S, H, d = q.shape
-    lengths, starts = _marks(lengths, B, q, "lengths"), _marks(starts, B, q, "starts")
-    lib = ops.get_lib()
-    out = torch.empty((B, S, H, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if want_lse else None
-    args = _pack(q, k, v, lengths, starts, causal, scale, out, lse)
-    with ops.device_of(q):
-        need = lib.amoe_attention_fwd_workspace(args)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        rc = lib.amoe_attention_fwd(args, None if ws is None else ws.data_ptr(), need, ops._stream(q))
-    _abi.check(lib, rc, "amoe_attention_fwd")
-    return out, lse
+    return _Call(q, k, v, lengths, starts, causal, scale).forward(want_lse)
 
 
 def attention_backward(go: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, lengths: Optional[Tensor] = None,
                        starts: Optional[Tensor] = None, causal: bool = True, scale: Optional[float] = None,
                        want_kv: bool = True) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     """(dq, dk, dv) of ``attention_forward``'s arguments and results (``amoe_attention_bwd``); without want_kv only dq."""
-    ops._need_gpu(go, q, k, v, out, lse, lengths, starts)
-    _check(q, k, v)
-    scale = _scale(scale, q.shape[3])
-    if go.shape != q.shape or out.shape != q.shape or go.dtype != q.dtype or out.dtype != q.dtype:
+    ops._need_gpu(go, out, lse)
+    call = _Call(q, k, v, lengths, starts, causal, scale)
+    B, S, H, _ = call.shape
+    if go.shape != call.shape or out.shape != call.shape or go.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError("out and its gradient must have q's shape and dtype")
-    B, S, H, d = q.shape
     if lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or any(t.device != q.device for t in (go, out, lse)):
         raise ValueError("lse must be fp32 [batch, heads, queries], and all tensors on one device")
-    q, k, v, go = _rows(q), _rows(k), _rows(v), _rows(go)
-    out, lse = out.contiguous(), lse.contiguous()
-    lengths, starts = _marks(lengths, B, q, "lengths"), _marks(starts, B, q, "starts")
-    lib = ops.get_lib()
-    dq = torch.empty((B, S, H, d), dtype=q.dtype, device=q.device)
-    dk = dv = None
-    if want_kv:
-        dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    args = _pack(q, k, v, lengths, starts, causal, scale, out, lse, go,
-                 (dq.data_ptr(), 0 if dk is None else dk.data_ptr(), 0 if dv is None else dv.data_ptr()))
-    with ops.device_of(q):
-        ws = torch.empty(max(lib.amoe_attention_bwd_workspace(args), 4), dtype=torch.uint8, device=q.device)
-        rc = lib.amoe_attention_bwd(args, ws.data_ptr(), ws.numel(), ops._stream(q))
-    _abi.check(lib, rc, "amoe_attention_bwd")
-    return dq, dk, dv
+    return call.backward(go, out.contiguous(), lse.contiguous(), want_kv)
 
 
 class Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, starts, causal, scale):
-        out, lse = attention_forward(q, k, v, lengths, starts, causal, scale, want_lse=True)
+        out, lse = _Call(q, k, v, lengths, starts, causal, scale).forward(True)
         ctx.save_for_backward(q, k, v, lengths, starts, out, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, go):
         q, k, v, lengths, starts, out, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = attention_backward(go, q, k, v, out, lse, lengths, starts, ctx.causal, ctx.scale, need[1] or need[2])
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+        # (what the forward pass left may come back through hooks in another layout)
+        if not out.is_contiguous() or not lse.is_contiguous():
+            out, lse = out.contiguous(), lse.contiguous()
+        dq, dk, dv = _Call(q, k, v, lengths, starts, ctx.causal, ctx.scale).backward(go, out, lse, need[1] or need[2])
+        grads = dq if need[0] else None, dk if need[1] else None, dv if need[2] else None
+        if torch.is_grad_enabled():
+            grads = once(grads, "attention")
+        return (*grads, None, None, None, None)
+
+
+def once(grads, what: str):
+    """Gradients of a backward pass that is itself differentiated (create_graph): going back through them is an error, not
+    a gradient that silently lacks a term."""
+    error = torch._C._functions.DelayedError(f"{what} is differentiable once: its backward pass has no derivative", 1)
+    return tuple(None if g is None else error(g.detach().requires_grad_()) for g in grads)
 
 
 def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Optional[float] = None,

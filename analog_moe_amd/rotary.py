@@ -15,7 +15,6 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import _abi, ops, raw
 
@@ -50,61 +49,75 @@ def rotate(q: Tensor, k: Tensor, turns: Tensor, positions: Optional[Tensor] = No
     """q [B, S, H, d] and k [B, S, G, d] turned by their positions (``amoe_rotary``), into new tensors or into ``out``, whose
     strides are free but for adjacent head elements: q and k themselves, or the next rows of a cache.  turns: int64
     [dim / 2], as ``Rotary`` holds it; inverse: the other way round."""
-    ops._need_gpu(q, k, turns, positions, *(out or ()))
-    if q.dim() != 4 or k.dim() != 4:
+    ops._need_gpu(q, k, turns, positions)
+    shape, kv = q.shape, k.shape
+    if len(shape) != 4 or len(kv) != 4:
         raise ValueError("q and k must be [batch, tokens, heads, head size]")
-    B, S, H, d = q.shape
-    if k.shape[:2] != q.shape[:2] or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
-    code = raw.dtype_code(q)
-    if k.dtype != q.dtype:
+    B, S, H, d = shape
+    if kv[0] != B or kv[1] != S or kv[3] != d:
+        raise ValueError(f"q {tuple(shape)} and k {tuple(kv)} do not match")
+    dtype, device = q.dtype, q.device
+    code = raw.code_of(dtype)
+    if k.dtype != dtype:
         raise TypeError("q and k must share one dtype")
     if turns.dtype != torch.int64 or turns.dim() != 1 or not turns.is_contiguous():
         raise TypeError("turns must be a contiguous int64 vector")
     R = 2 * turns.numel()
     if not 2 <= R <= d:
         raise ValueError(f"{R} turning elements do not fit heads of {d}")
+    if k.device != device or turns.device != device or (positions is not None and positions.device != device):
+        raise ValueError("all tensors must be on one device")
+    place, place64, pb, ps = 0, False, 0, 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, not {positions.dtype}")
-        if positions.shape not in ((S,), (B, S)):
-            raise ValueError(f"positions must be [{S}] or [{B}, {S}], not {tuple(positions.shape)}")
         if start:
             raise ValueError("positions or start, not both")
-    if any(t is not None and t.device != q.device for t in (k, turns, positions, *(out or ()))):
-        raise ValueError("all tensors must be on one device")
+        place, place64 = positions.data_ptr(), positions.dtype == torch.int64
+        if positions.shape == (B, S):
+            pb, ps = positions.stride()
+        elif positions.shape == (S,):
+            ps = positions.stride(0)
+        else:
+            raise ValueError(f"positions must be [{S}] or [{B}, {S}], not {tuple(positions.shape)}")
     q, k = _rows(q), _rows(k)
     if out is None:
-        out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+        oq, ok = q.new_empty(shape), k.new_empty(kv)
     else:
-        for t, o in zip((q, k), out):
-            if o.shape != t.shape or o.dtype != t.dtype or (o.stride(3) != 1 and d > 1):
-                raise ValueError("out must have the shapes and dtype of q and k, with adjacent head elements")
+        oq, ok = out
+        ops._need_gpu(oq, ok)
+        for t, o in ((q, oq), (k, ok)):
+            if o.shape != t.shape or o.dtype != dtype or o.device != device or (o.stride(3) != 1 and d > 1):
+                raise ValueError("out must have the shapes, dtype and device of q and k, with adjacent head elements")
+            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+                raise ValueError("out must have memory of its own for every element")
+    sq, sk, tq, tk = q.stride(), k.stride(), oq.stride(), ok.stride()
     args = _abi.ROTARY_ARGS.pack(
-        code, B, S, H, k.shape[2], d, R, interleaved, inverse, size, turns.data_ptr(),
-        0 if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64,
-        *((0, 0) if positions is None else (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()), start,
-        *(w for t in (q, k, *out) for w in (t.data_ptr(), *t.stride()[:3])))
+        code, B, S, H, kv[2], d, R, interleaved, inverse, size, turns.data_ptr(), place, place64, pb, ps, start,
+        q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+        oq.data_ptr(), tq[0], tq[1], tq[2], ok.data_ptr(), tk[0], tk[1], tk[2])
     lib = ops.get_lib()
     with ops.device_of(q):
         rc = lib.amoe_rotary(args, ops._stream(q))
-    _abi.check(lib, rc, "amoe_rotary")
-    return out
+    if rc:
+        _abi.check(lib, rc, "amoe_rotary")
+    return oq, ok
 
 
 class RotaryFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, turns, positions, start, interleaved, size):
-        ctx.save_for_backward(turns, positions)
-        ctx.args = (start, interleaved, size)
-        return rotate(q, k, turns, positions, start, interleaved, size)
+    """The gradient of a turn is the turn the other way round, itself differentiable in the same way."""
 
     @staticmethod
-    @once_differentiable
+    def forward(ctx, q, k, turns, positions, start, interleaved, size, inverse):
+        ctx.save_for_backward(turns, positions)
+        ctx.args = (start, interleaved, size, not inverse)
+        return rotate(q, k, turns, positions, start, interleaved, size, inverse)
+
+    @staticmethod
     def backward(ctx, gq, gk):
         turns, positions = ctx.saved_tensors
-        dq, dk = rotate(gq, gk, turns, positions, *ctx.args, inverse=True)
-        return dq, dk, None, None, None, None, None
+        f = RotaryFunction.apply if torch.is_grad_enabled() else rotate
+        return (*f(gq, gk, turns, positions, *ctx.args), None, None, None, None, None, None)
 
 
 class Rotary(nn.Module):
@@ -139,7 +152,7 @@ class Rotary(nn.Module):
             return torch.ops.amoe.rotary(*args, False)
         if not grad and ops.unwatched():
             return rotate(*args)
-        return RotaryFunction.apply(*args)
+        return RotaryFunction.apply(*args, False)
 
     def extra_repr(self) -> str:
         return f"dim={self.dim}, interleaved={self.interleaved}"

@@ -102,7 +102,7 @@ def test_few_rows_in_parts(emu_ops, monkeypatch):
     """Rows over a long axis are worked on in parts, joined by a second kernel; also where a part holds no key."""
     q, k, v, _ = inputs(1, 1, 700, 2, 1, 64, "bf16", seed=3)
     lib = emu_ops.get_lib()
-    args = A._pack(q, k, v, None, None, True, 0.125, q, None)
+    args = A._Call(q, k, v, None, None, True, 0.125).pack(q, None)
     assert lib.amoe_attention_fwd_workspace(args) == 6 * 2 * 66 * 4
     for n in (700, 130, 128, 1, 0):
         kw = dict(lengths=marks([n]), starts=marks([n - 1], torch.int64))
@@ -192,7 +192,7 @@ def test_library_refuses_what_it_cannot_address(emu_ops):
     lib = emu_ops.get_lib()
     q, k, v, go = inputs(1, 2, 3, 2, 1, 32, "f32")
     out, lse = torch.empty_like(q), torch.empty(1, 2, 2)
-    good = list(_abi.ATTN_ARGS.unpack(A._pack(q, k, v, None, None, True, 0.5, out, lse, go, (1 << 20,) * 3)))
+    good = list(_abi.ATTN_ARGS.unpack(A._Call(q, k, v, None, None, True, 0.5).pack(out, lse, go, (1 << 20,) * 3)))
 
     def fwd(**change):
         a = list(good)
@@ -222,8 +222,10 @@ def test_autograd(emu_ops):
     compare(torch.autograd.grad(out, v, go), want[3:], bounds[3:], "values only")
     # a gradient of stride zero, and of the gradient: refused
     (g,) = torch.autograd.grad(A.attention(q, k, v).sum(), q, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    compare((g.detach(),), O.attention(q.detach(), k.detach(), v.detach(), torch.ones_like(go))[0][1:2],
+            O.attention(q.detach(), k.detach(), v.detach(), torch.ones_like(go))[1][1:2], "ones")
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g.sum() + q.sum()).backward()
     with torch.no_grad():
         assert torch.equal(A.attention(q, k, v), A.attention_forward(q, k, v)[0])
 

@@ -142,9 +142,11 @@ def test_gradient(emu_ops):
         assert abs(a - b) < 40 * 2.0 ** -24 * (x.abs().double().sum() * g.abs().max())
     (only,) = torch.autograd.grad(r(q, k.detach(), start=3)[0].sum(), q)
     assert torch.equal(only, R.rotate(torch.ones_like(q), k, r.turns, None, 3, False, r.size, True)[0])
-    (g2,) = torch.autograd.grad(r(q, k)[0].sum(), q, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g2.sum().backward()
+    # differentiable as often as wanted: the gradient is linear in gq, its derivative the turn itself
+    gq, gk = gq.requires_grad_(), gk.requires_grad_()
+    dq, _ = torch.autograd.grad(r(q, k, start=3), (q, k), (gq, gk), create_graph=True)
+    (back,) = torch.autograd.grad(dq, gq, q.detach())
+    assert torch.equal(back, R.rotate(q, k, r.turns, None, 3, False, r.size)[0])
     with pytest.raises(RuntimeError):
         r(q, k, out=(torch.empty_like(q), torch.empty_like(k)))
 
@@ -160,7 +162,8 @@ def test_refusals(emu_ops):
     for bad in (lambda: R.rotate(q[0], k, t), lambda: R.rotate(q, k[:, :2], t), lambda: R.rotate(q, k[..., :4], t),
                 lambda: R.rotate(q, k, R.Rotary(10).turns), lambda: R.rotate(q, k, t[:0]), lambda: R.rotate(q, k, t, at[:2]),
                 lambda: R.rotate(q, k, t, at, 1), lambda: R.rotate(q, k, t, at[None]),
-                lambda: R.rotate(q, k, t, out=(q[:1], k)), lambda: R.rotate(q, k, t, out=(q.half(), k))):
+                lambda: R.rotate(q, k, t, out=(q[:1], k)), lambda: R.rotate(q, k, t, out=(q.half(), k)),
+                lambda: R.rotate(q, k, t, out=(q[:, :, :1].expand_as(q), k))):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: R.rotate(q.double(), k.double(), t), lambda: R.rotate(q, k.half(), t), lambda: R.rotate(q, k, t.float()),
