@@ -43,10 +43,16 @@ int attn_splits(const amoe_attn_args* a) {
   const int64_t many = a->B * a->H * ((a->S + kAttnRows - 1) / kAttnRows);
   if (rows > 32 && (many * 2 > cus || a->T < 1024)) return 0;
   const int64_t groups = a->B * a->G * ((rows + 31) / 32);
-  int64_t n = (2 * cus + groups - 1) / groups;
-  const int64_t most = (a->T + 127) / 128;
-  if (n > most) n = most;
-  return (int)(n < 1 ? 1 : n);
+  // parts of 512 keys or more, up to eight workgroups per CU (sequences differ in length, and the last round of workgroups
+  // is then short); where that leaves CUs without work, parts of down to 128 keys for two
+  const auto parts = [&](int64_t per_cu, int64_t keys) {
+    const int64_t n = (per_cu * cus + groups - 1) / groups, most = (a->T + keys - 1) / keys;
+    return n < most ? n : most;
+  };
+  int64_t n = parts(8, 512);
+  const int64_t few = parts(2, 128);
+  if (few > n) n = few;
+  return (int)(n < 1 ? 1 : n > kAttnMaxSplits ? kAttnMaxSplits : n);
 }
 
 void fill(AttnParams& p, const amoe_attn_args* a) {

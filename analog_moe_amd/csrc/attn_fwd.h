@@ -275,7 +275,6 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 
 // The parts of a row joined, a workgroup per row: sums in units of the largest maximum, eight runs of parts side by side and
 // then those in order.
-constexpr int kAttnMaxSplits = 1024;
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams p) {
   __shared__ float lds_f[kAttnMaxSplits], lds_red[8];

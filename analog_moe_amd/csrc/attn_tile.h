@@ -13,6 +13,7 @@ namespace amoe {
 constexpr int kAttnThreads = 256;    // 4 waves
 constexpr int kAttnRows = 128;       // queries (keys, for their gradients) of a workgroup, 32 per wave
 constexpr int kAttnMaxHead = 128;    // elements of a head, at most
+constexpr int kAttnMaxSplits = 1024;        // parts of the key axis
 constexpr int64_t kAttnMaxRows = 1 << 28;   // queries and keys of a sequence, at most
 constexpr float kLog2e = 1.4426950408889634f;
 
