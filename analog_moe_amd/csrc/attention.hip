@@ -40,7 +40,7 @@ int check_sizes(const amoe_attn_args* a) {
 // Parts of the key axis for the kernel of few rows; 0: the kernel of many rows.
 int attn_splits(const amoe_attn_args* a) {
   const int64_t rows = a->H / a->G * a->S, cus = num_compute_units();
-  const int64_t many = a->B * a->H * ((a->S + kAttnRows - 1) / kAttnRows);
+  const int64_t many = a->B * a->H * ((a->S + 127) / 128);
   if (rows > 32 && (many * 2 > cus || a->T < 1024)) return 0;
   const int64_t groups = a->B * a->G * ((rows + 31) / 32);
   // parts of 512 keys or more, up to eight workgroups per CU (sequences differ in length, and the last round of workgroups

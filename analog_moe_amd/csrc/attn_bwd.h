@@ -54,47 +54,41 @@ __device__ __forceinline__ void attn_pack_block(const V& v, attn_frag<T> (&f)[2]
   }
 }
 
-// dq: 128 queries of one head per workgroup, 32 per wave, keys in tiles as in the forward pass.  Also leaves delta.
-template <typename T, int DP, bool EDGE>
-__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q_kernel(AttnParams p) {
+// dq: 32 * RW queries of one head per workgroup, keys in tiles as in the forward pass.  Also leaves delta.
+template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
+__global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd_q_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
-  constexpr int BN = kAttnKeys<T>, NB = BN / 32, NK = DP / 16;
-  __shared__ __align__(16) T lds_k[2][BN * DP];
-  __shared__ __align__(16) T lds_v[2][BN * DP];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
-  const int BH = p.B * p.H, bh = (int)(blockIdx.x % (unsigned)BH), tile = (p.S + kAttnRows - 1) / kAttnRows - 1 - (int)(blockIdx.x / (unsigned)BH);
-  const int b = bh / p.H, hd = bh - b * p.H, g = hd / p.R;
-  const int length = attn_length(p, b), start = attn_start(p, b);
-  const int w0 = tile * kAttnRows + wave * 32, i = w0 + (lane & 31);
-  const int last = p.S - 1 < tile * kAttnRows + kAttnRows - 1 ? p.S - 1 : tile * kAttnRows + kAttnRows - 1;
-  const int group_sees = attn_seen(p, length, start, last);
-  const int wave_last = p.S - 1 < w0 + 31 ? p.S - 1 : w0 + 31;
-  const int wave_sees = w0 < p.S ? attn_seen(p, length, start, wave_last) : 0;
-  const int wave_all = w0 < p.S ? attn_seen(p, length, start, w0) : 0;
-  const int seen = attn_seen(p, length, start, i < p.S ? i : p.S - 1);
+  constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
+  constexpr int kElems = BN * DP, kTileBytes = 4 * kElems * (int)sizeof(T), kJoinBytes = (KG - 1) * RW * DP * 32 * 4;
+  __shared__ __align__(1024) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
+  T* const lds_k = reinterpret_cast<T*>(lds);
+  T* const lds_v = lds_k + 2 * kElems;
+  const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5;
+  const AttnRowsOf w = attn_rows_of<Shape>(p);
 
-  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
-  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+  const T* kb = static_cast<const T*>(p.k.p) + w.b * p.k.sb + w.g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + w.b * p.v.sb + w.g * p.v.sh;
   AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
   sk.init(tid, p.k.ss, p.d);
   sv.init(tid, p.v.ss, p.d);
   typename Tile::Lane at;
-  const int n_tiles = (group_sees + BN - 1) / BN;
+  const int n_tiles = (w.group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, lds_k[0], kb, p.k.ss, 0, group_sees, p.d, p.vec);
-    sv.load(tid, lds_v[0], vb, p.v.ss, 0, group_sees, p.d, p.vec);
+    sk.load(tid, lds_k, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
+    sv.load(tid, lds_v, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK], go[NK];
-  const int64_t row = ((int64_t)b * p.S + i) * p.H + hd;
-  const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
-  const T* grow = static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh + (int64_t)i * p.go.ss;
+  const bool real = w.i < p.S;
+  const int64_t row = ((int64_t)w.b * p.S + w.i) * p.H + w.hd, stat = (int64_t)w.bh * p.S + w.i;
+  const T* qrow = static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh + (int64_t)w.i * p.q.ss;
+  const T* grow = static_cast<const T*>(p.go.p) + w.b * p.go.sb + w.hd * p.go.sh + (int64_t)w.i * p.go.ss;
   const T* orow = static_cast<const T*>(p.o) + row * p.d;
   float delta = 0.f;
 #pragma unroll
   for (int kk = 0; kk < NK; kk++) {
-    q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, i < p.S, p.vec);
-    go[kk] = attn_global_frag<T, EDGE>(grow, kk, p.d, i < p.S, p.vec);
-    const attn_frag<T> o = attn_global_frag<T, EDGE>(orow, kk, p.d, i < p.S, p.vec);
+    q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, real, p.vec);
+    go[kk] = attn_global_frag<T, EDGE>(grow, kk, p.d, real, p.vec);
+    const attn_frag<T> o = attn_global_frag<T, EDGE>(orow, kk, p.d, real, p.vec);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int j = 0; j < 8; j++) delta = fmaf(o.v[j], go[kk].v[j], delta);
@@ -107,26 +101,27 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
     }
   }
   delta = attn_pair_sum(delta);
-  const float lse = i < p.S ? p.lse[(int64_t)bh * p.S + i] : INFINITY;
-  if (i < p.S && h == 0) p.delta[(int64_t)bh * p.S + i] = delta;
+  const float lse = real ? p.lse[stat] : INFINITY;
+  if (real && h == 0 && w.kg == 0) p.delta[stat] = delta;
 
   AttnGrad<T, DP> dq;
   dq.clear();
   if (n_tiles > 0) {
-    sk.store(tid, lds_k[0]);
-    sv.store(tid, lds_v[0]);
+    sk.store(tid, lds_k);
+    sv.store(tid, lds_v);
   }
   for (int t = 0; t < n_tiles; t++) {
-    const int key0 = t * BN;
+    const int cur = (t & 1) * kElems, next = kElems - cur;
     sk.finish();
     __syncthreads();
     if (t + 1 < n_tiles) {
-      sk.load(tid, lds_k[(t + 1) & 1], kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
-      sv.load(tid, lds_v[(t + 1) & 1], vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
+      sk.load(tid, lds_k + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sv.load(tid, lds_v + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
     }
-    if (key0 < wave_sees) {
-      const T *kt = lds_k[t & 1], *vt = lds_v[t & 1];
-      const bool mask = key0 + BN > wave_all;
+    const int key0 = t * BN + 32 * NB * w.kg;
+    if (key0 < w.wave_sees) {
+      const T *kt = lds_k + cur + 32 * NB * w.kg * DP, *vt = lds_v + cur + 32 * NB * w.kg * DP;
+      const bool mask = key0 + 32 * NB > w.wave_all;
       // per 32 keys: 2 * NK products for the scores and dP by turns, 2 * DP / 32 with dS
       constexpr int NU = DP / 32, NS = 2 * NK, NF = NS + 2 * NU;
       const auto load = [&](int x) -> attn_frag<T> {
@@ -150,7 +145,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
         if (mask) {
 #pragma unroll
           for (int e = 0; e < 16; e++)
-            if (key0 + 32 * n + 8 * (e / 4) + 4 * h + e % 4 >= seen) ds[e] = 0.f;
+            if (key0 + 32 * n + 8 * (e / 4) + 4 * h + e % 4 >= w.seen) ds[e] = 0.f;
         }
         dq.fit(ds);
         attn_frag<T> df[2];
@@ -162,25 +157,42 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_bwd
       }
     }
     if (t + 1 < n_tiles) {
-      sk.store(tid, lds_k[(t + 1) & 1]);
-      sv.store(tid, lds_v[(t + 1) & 1]);
+      sk.store(tid, lds_k + next);
+      sv.store(tid, lds_v + next);
     }
   }
-  if (i < p.S) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, p.scale / dq.scale, p.d);
+  float factor = p.scale / dq.scale;
+  if constexpr (KG > 1) {
+    __syncthreads();
+    f32x4* join = reinterpret_cast<f32x4*>(lds);
+    if (w.kg > 0) attn_put_acc<DP>(join, (w.kg - 1) * RW + w.rw, dq.acc, factor);
+    __syncthreads();
+    if (w.kg == 0) {
+#pragma unroll
+      for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) dq.acc[t][e] *= factor;
+#pragma unroll
+      for (int c = 1; c < KG; c++) attn_add_acc<DP>(join, (c - 1) * RW + w.rw, dq.acc, 1.f);
+      factor = 1.f;
+    }
+  }
+  if (w.kg == 0 && real) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, factor, p.d);
 }
 
 // dk, dv: KW waves hold 32 keys each of one key head, k and v as operands in registers, in QW copies; the queries of all heads
 // that share them pass in tiles of 32 * QW, 32 for each copy, and the copies' sums are added at the end, in order.  Every wave
 // reads what the other keys' waves read (a product of 32 x 32 takes as long as the LDS reads of its operands do); more copies
 // make shorter loops of the same work where there are few keys, and finer workgroups where causal rows differ in length.
-template <typename T, int DP, bool EDGE> struct AttnKvShape {
-  static constexpr bool kBig = sizeof(T) * DP > 256 || EDGE;       // fp32 heads past 64: 512 registers a wave, 4 waves
-  static constexpr int KW = 2, QW = sizeof(T) == 2 && DP == 128 && !EDGE ? 4 : 2;
+template <typename T, int DP, bool EDGE, int QW_> struct AttnKvShape {
+  static constexpr int KW = 2, QW = QW_, kThreads = 64 * KW * QW;
+  static constexpr int kWavesPerSimd = sizeof(T) * DP > 256 || EDGE ? 1 : 2;       // fp32 heads past 64: 512 registers a wave
   // 16-bit heads past 96: dk, dv and k fill the registers, v is read from LDS for every product
   static constexpr bool kVInLds = sizeof(T) == 2 && DP == 128 && !EDGE;
-  static constexpr int kThreads = 64 * KW * QW, kWavesPerSimd = kBig ? 1 : 2;
+  // two copies have room for two workgroups on a CU; four are one
+  static constexpr bool kFits = 128 * QW * DP * (int)sizeof(T) <= (QW == 2 && !EDGE && sizeof(T) == 2 ? 48 : 128) << 10;
 };
-template <typename T, int DP, bool EDGE, class Shape = AttnKvShape<T, DP, EDGE>>
+template <typename T, int DP, bool EDGE, int QW_, class Shape = AttnKvShape<T, DP, EDGE, QW_>>
 __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void attn_bwd_kv_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
   constexpr int KW = Shape::KW, QW = Shape::QW, NT = Shape::kThreads, BM = 32 * QW, NK = DP / 16, NU = DP / 32;
@@ -305,35 +317,19 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   f32x4* const sums = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
   for (int which = 0; which < 2; which++) {
-    f32x16* acc = which ? dk.acc : dv.acc;
+    f32x16(&acc)[NU] = which ? dk.acc : dv.acc;
     const float factor = which ? p.scale * kUnshift / dk.scale : kUnshift;
     __syncthreads();
-    if (qw > 0) {
-#pragma unroll
-      for (int t = 0; t < NU; t++)
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-          sums[((((qw - 1) * KW + kw) * NU + t) * 4 + u) * 64 + lane] =
-              f32x4{acc[t][4 * u] * factor, acc[t][4 * u + 1] * factor, acc[t][4 * u + 2] * factor, acc[t][4 * u + 3] * factor};
-    }
+    if (qw > 0) attn_put_acc<DP>(sums, (qw - 1) * KW + kw, acc, factor);
     __syncthreads();
-    if (qw == 0 && key < p.T) {
+    if (qw == 0) {
 #pragma unroll
       for (int t = 0; t < NU; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-          f32x4 v = f32x4{acc[t][4 * u] * factor, acc[t][4 * u + 1] * factor, acc[t][4 * u + 2] * factor, acc[t][4 * u + 3] * factor};
+        for (int e = 0; e < 16; e++) acc[t][e] *= factor;
 #pragma unroll
-          for (int c = 0; c < QW - 1; c++) {
-            const f32x4 o = sums[(((c * KW + kw) * NU + t) * 4 + u) * 64 + lane];
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] += o[j];
-          }
-#pragma unroll
-          for (int j = 0; j < 4; j++) acc[t][4 * u + j] = v[j];
-          sched_fence();          // (all the reads at once do not fit the registers)
-        }
-      attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d);
+      for (int c = 0; c < QW - 1; c++) attn_add_acc<DP>(sums, c * KW + kw, acc, 1.f);
+      if (key < p.T) attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d);
     }
   }
 }

@@ -69,63 +69,114 @@ __device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[N
   st.l += sum;
 }
 
-// Many rows: a workgroup has 128 queries of one head, 32 per wave, and walks the keys in tiles of kKeys that go through
-// registers into LDS, two tiles by turns with one barrier each.
-template <typename T> inline constexpr int kAttnKeys = sizeof(T) == 4 ? 32 : 64;
-
-template <typename T, int DP, bool EDGE>
-__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_rows_kernel(AttnParams p) {
-  using Tile = AttnTile<T, DP>;
-  constexpr int BN = kAttnKeys<T>, NB = BN / 32, NK = DP / 16;
-  __shared__ __align__(16) T lds_k[2][BN * DP];
-  __shared__ __align__(16) T lds_v[2][BN * DP];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
+// What the waves of a workgroup work on, for the kernels whose lanes own queries.
+struct AttnRowsOf {
+  int b, hd, g, bh, i, rw, kg;
+  int length, start;
+  int group_sees;     // keys that the last query of the workgroup sees
+  int wave_sees;      // the last one of the wave
+  int wave_all;       // the first one of the wave
+  int seen;           // the lane's
+};
+template <class Shape>
+__device__ __forceinline__ AttnRowsOf attn_rows_of(const AttnParams& p) {
+  AttnRowsOf w;
+  const int wave = wave_uniform(threadIdx.x >> 6);
+  w.rw = wave % Shape::RW;
+  w.kg = wave / Shape::RW;
   // workgroups with one head next to each other's on an XCD (ids go round the eight); the longest rows first
-  const int BH = p.B * p.H, bh = (int)(blockIdx.x % (unsigned)BH), tile = (p.S + kAttnRows - 1) / kAttnRows - 1 - (int)(blockIdx.x / (unsigned)BH);
-  const int b = bh / p.H, hd = bh - b * p.H, g = hd / p.R;
-  const int length = attn_length(p, b), start = attn_start(p, b);
-  const int w0 = tile * kAttnRows + wave * 32, i = w0 + (lane & 31);
-  const int last = p.S - 1 < tile * kAttnRows + kAttnRows - 1 ? p.S - 1 : tile * kAttnRows + kAttnRows - 1;
-  const int group_sees = attn_seen(p, length, start, last);
-  const int wave_last = p.S - 1 < w0 + 31 ? p.S - 1 : w0 + 31;
-  const int wave_sees = w0 < p.S ? attn_seen(p, length, start, wave_last) : 0;
-  const int wave_all = w0 < p.S ? attn_seen(p, length, start, w0) : 0;         // keys that every row of the wave sees
-  const int seen = attn_seen(p, length, start, i < p.S ? i : p.S - 1);
+  const int BH = p.B * p.H;
+  w.bh = (int)(blockIdx.x % (unsigned)BH);
+  const int row0 = ((p.S + Shape::kRows - 1) / Shape::kRows - 1 - (int)(blockIdx.x / (unsigned)BH)) * Shape::kRows;
+  w.b = w.bh / p.H;
+  w.hd = w.bh - w.b * p.H;
+  w.g = w.hd / p.R;
+  w.length = attn_length(p, w.b);
+  w.start = attn_start(p, w.b);
+  const int w0 = row0 + w.rw * 32, end = p.S - 1;
+  w.i = w0 + (lane_id() & 31);
+  const int group_last = row0 + Shape::kRows - 1, wave_last = w0 + 31;
+  w.group_sees = attn_seen(p, w.length, w.start, group_last < end ? group_last : end);
+  w.wave_sees = w0 <= end ? attn_seen(p, w.length, w.start, wave_last < end ? wave_last : end) : 0;
+  w.wave_all = w0 <= end ? attn_seen(p, w.length, w.start, w0) : 0;
+  w.seen = attn_seen(p, w.length, w.start, w.i < end ? w.i : end);
+  return w;
+}
+// a wave's accumulators to and from LDS, 16 bytes per lane and access: slot `copy` of as many as there are
+template <int DP>
+__device__ __forceinline__ void attn_put_acc(f32x4* lds, int copy, const f32x16 (&acc)[DP / 32], float factor) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      lds[((copy * (DP / 32) + t) * 4 + u) * 64 + lane] =
+          f32x4{acc[t][4 * u] * factor, acc[t][4 * u + 1] * factor, acc[t][4 * u + 2] * factor, acc[t][4 * u + 3] * factor};
+}
+template <int DP>
+__device__ __forceinline__ void attn_add_acc(const f32x4* lds, int copy, f32x16 (&acc)[DP / 32], float factor) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int t = 0; t < DP / 32; t++) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const f32x4 o = lds[((copy * (DP / 32) + t) * 4 + u) * 64 + lane];
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[t][4 * u + j] = fmaf(o[j], factor, acc[t][4 * u + j]);
+    }
+    sched_fence();          // (all the reads at once do not fit the registers)
+  }
+}
 
-  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
-  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+// Many rows: a workgroup has 32 * RW queries of one head and walks the keys in tiles that go straight from memory into LDS, two
+// tiles by turns with one barrier each.
+template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
+__global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd_rows_kernel(AttnParams p) {
+  using Tile = AttnTile<T, DP>;
+  constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
+  constexpr int kElems = BN * DP, kTileBytes = 4 * kElems * (int)sizeof(T), kJoinBytes = (KG - 1) * RW * DP * 32 * 4;
+  __shared__ __align__(1024) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
+  __shared__ float lds_ml[KG][RW][2][64];
+  T* const lds_k = reinterpret_cast<T*>(lds);
+  T* const lds_v = lds_k + 2 * kElems;
+  const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5;
+  const AttnRowsOf w = attn_rows_of<Shape>(p);
+
+  const T* kb = static_cast<const T*>(p.k.p) + w.b * p.k.sb + w.g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + w.b * p.v.sb + w.g * p.v.sh;
   AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
   sk.init(tid, p.k.ss, p.d);
   sv.init(tid, p.v.ss, p.d);
   typename Tile::Lane at;
-  const int n_tiles = (group_sees + BN - 1) / BN;
+  const int n_tiles = (w.group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, lds_k[0], kb, p.k.ss, 0, group_sees, p.d, p.vec);
-    sv.load(tid, lds_v[0], vb, p.v.ss, 0, group_sees, p.d, p.vec);
+    sk.load(tid, lds_k, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
+    sv.load(tid, lds_v, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK];
-  const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
+  const T* qrow = static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh + (int64_t)w.i * p.q.ss;
 #pragma unroll
-  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, i < p.S, p.vec);
+  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, w.i < p.S, p.vec);
 
   AttnState<T, DP> st;
   st.clear();
   if (n_tiles > 0) {
-    sk.store(tid, lds_k[0]);
-    sv.store(tid, lds_v[0]);
+    sk.store(tid, lds_k);
+    sv.store(tid, lds_v);
   }
   for (int t = 0; t < n_tiles; t++) {
-    const int key0 = t * BN;
+    const int cur = (t & 1) * kElems, next = kElems - cur;
     sk.finish();
     __syncthreads();       // tile t is there, and nobody reads the other one any more
     if (t + 1 < n_tiles) {
-      sk.load(tid, lds_k[(t + 1) & 1], kb, p.k.ss, key0 + BN, group_sees, p.d, p.vec);
-      sv.load(tid, lds_v[(t + 1) & 1], vb, p.v.ss, key0 + BN, group_sees, p.d, p.vec);
+      sk.load(tid, lds_k + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sv.load(tid, lds_v + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
     }
-    if (key0 < wave_sees) {
+    const int key0 = t * BN + 32 * NB * w.kg;
+    if (key0 < w.wave_sees) {
       // NB * NK products for the scores, 2 * NB * DP / 32 with the probabilities
       constexpr int NS = NB * NK, NU = DP / 32;
-      const T *kt = lds_k[t & 1], *vt = lds_v[t & 1];
+      const T *kt = lds_k + cur + 32 * NB * w.kg * DP, *vt = lds_v + cur + 32 * NB * w.kg * DP;
       const auto load = [&](int e) -> attn_frag<T> {
         return e < NS ? Tile::row_frag(kt, at, 32 * (e % NB), e / NB) : Tile::col_frag(vt, at, 16 * ((e - NS) / NU), (e - NS) % NU);
       };
@@ -137,20 +188,48 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 #pragma unroll
       for (int n = 0; n < NB; n++) s[n] = f32x16_zero();
       run.steps(0, NS, load, [&](int e, const attn_frag<T>& a) { s[e % NB] = attn_mma<T>(a, q[e / NB], s[e % NB]); });
-      attn_softmax<T, DP, NB>(st, s, pr, key0, seen, key0 + BN > wave_all, p.c);
+      attn_softmax<T, DP, NB>(st, s, pr, key0, w.seen, key0 + 32 * NB > w.wave_all, p.c);
       run.steps(NS, NS + 2 * NB * NU, load,
                 [&](int e, const attn_frag<T>& a) { st.o[(e - NS) % NU] = attn_mma<T>(a, pr[(e - NS) / NU], st.o[(e - NS) % NU]); });
     }
     if (t + 1 < n_tiles) {
-      sk.store(tid, lds_k[(t + 1) & 1]);
-      sv.store(tid, lds_v[(t + 1) & 1]);
+      sk.store(tid, lds_k + next);
+      sv.store(tid, lds_v + next);
     }
   }
-  const float l = attn_pair_sum(st.l), inv = l == 0.f ? 0.f : 1.f / l;
-  if (i < p.S) {
-    const int64_t row = ((int64_t)b * p.S + i) * p.H + hd;
+  float l = attn_pair_sum(st.l);
+  if constexpr (KG > 1) {
+    // the copies in units of the largest maximum; the first one takes the sums
+    __syncthreads();
+    f32x4* join = reinterpret_cast<f32x4*>(lds);
+    lds_ml[w.kg][w.rw][0][lane] = st.m;
+    lds_ml[w.kg][w.rw][1][lane] = l;
+    if (w.kg > 0) attn_put_acc<DP>(join, (w.kg - 1) * RW + w.rw, st.o, 1.f);
+    __syncthreads();
+    if (w.kg == 0) {
+      float m = st.m;
+#pragma unroll
+      for (int c = 1; c < KG; c++) m = fmaxf(m, lds_ml[c][w.rw][0][lane]);
+      const float own = st.m == -INFINITY ? 0.f : fast_exp2((st.m - m) * p.c);
+      l *= own;
+#pragma unroll
+      for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) st.o[t][e] *= own;
+#pragma unroll
+      for (int c = 1; c < KG; c++) {
+        const float mc = lds_ml[c][w.rw][0][lane], f = mc == -INFINITY ? 0.f : fast_exp2((mc - m) * p.c);
+        l = fmaf(lds_ml[c][w.rw][1][lane], f, l);
+        attn_add_acc<DP>(join, (c - 1) * RW + w.rw, st.o, f);
+      }
+      st.m = m;
+    }
+  }
+  if (w.kg == 0 && w.i < p.S) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t row = ((int64_t)w.b * p.S + w.i) * p.H + w.hd;
     attn_store_col<T, DP, EDGE>(static_cast<T*>(p.out) + row * p.d, st.o, inv, p.d);
-    if (p.lse && h == 0) p.lse[(int64_t)bh * p.S + i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
+    if (p.lse && h == 0) p.lse[(int64_t)w.bh * p.S + w.i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
   }
 }
 

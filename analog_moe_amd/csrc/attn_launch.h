@@ -15,6 +15,44 @@ namespace amoe {
     else LAUNCH(TYPE, 128, false);                                       \
   } while (0)
 
+// Waves over the rows of a workgroup (AttnShape) by how many workgroups there are: four where two can be on every CU, else two,
+// and one where those would not give every CU a workgroup; the tiles' room allowing.  Measured, forward pass: 256 workgroups of
+// 128 rows (2 sequences of 1024, 16 heads of 64, fp32) 88 us, 512 of 64 66 us, 1024 of 32 78 us; 256 of 128 (2 x 1003 queries over
+// 5003 keys, 16 heads of 128, bf16) 98 us, 512 of 64 90 us; 8 of 128 (2 x 100, 4 heads of 32, fp32) 14 us, 16 of 64 10 us, 32 of 32
+// 8 us; 2048 of 128 (16 x 1024, 16 heads of 64, bf16) 65 us, 4096 of 64 77 us.
+template <template <int> class Launch, bool FITS2, bool FITS1>
+int launch_attn_rows(const AttnParams& p, hipStream_t st) {
+  const int64_t heads = (int64_t)p.B * p.H, want = 2 * num_compute_units();
+  if constexpr (FITS2) {
+    if (heads * ((p.S + 127) / 128) < want) {
+      if constexpr (FITS1) {
+        if (heads * ((p.S + 63) / 64) < want / 2) return Launch<1>::run(p, st);
+      }
+      return Launch<2>::run(p, st);
+    }
+  }
+  return Launch<4>::run(p, st);
+}
+
+template <typename T, int DP, bool EDGE> struct AttnFwdRows {
+  template <int RW> struct Launch {
+    static int run(const AttnParams& p, hipStream_t st) {
+      const dim3 grid((unsigned)((int64_t)p.B * p.H * ((p.S + 32 * RW - 1) / (32 * RW))));
+      hipLaunchKernelGGL((&attn_fwd_rows_kernel<T, DP, EDGE, RW>), grid, dim3(kAttnThreads), 0, st, p);
+      return launch_rc();
+    }
+  };
+};
+template <typename T, int DP, bool EDGE> struct AttnBwdRows {
+  template <int RW> struct Launch {
+    static int run(const AttnParams& p, hipStream_t st) {
+      const dim3 grid((unsigned)((int64_t)p.B * p.H * ((p.S + 32 * RW - 1) / (32 * RW))));
+      hipLaunchKernelGGL((&attn_bwd_q_kernel<T, DP, EDGE, RW>), grid, dim3(kAttnThreads), 0, st, p);
+      return launch_rc();
+    }
+  };
+};
+
 template <typename T>
 int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
   if (p.splits > 0) {
@@ -28,32 +66,52 @@ int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
     }
     return launch_rc();
   }
-  const dim3 grid((unsigned)((int64_t)p.B * p.H * ((p.S + kAttnRows - 1) / kAttnRows)));
-#define AMOE_LAUNCH(TYPE, DP, EDGE) hipLaunchKernelGGL((&attn_fwd_rows_kernel<TYPE, DP, EDGE>), grid, dim3(kAttnThreads), 0, st, p)
+  int rc = AMOE_OK;
+#define AMOE_LAUNCH(TYPE, DP, EDGE)                                                                             \
+  rc = launch_attn_rows<AttnFwdRows<TYPE, DP, EDGE>::template Launch, !EDGE && AttnShape<TYPE, DP, EDGE, 2>::kFits, \
+                        !EDGE && AttnShape<TYPE, DP, EDGE, 1>::kFits>(p, st)
   AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
 #undef AMOE_LAUNCH
+  return rc;
+}
+
+// Copies of the waves over the queries: two where there are two workgroups for every CU, else four.  Measured: 324 workgroups
+// (6 padded sequences of 1717, 2 key heads of 80, fp16) 146 us with two, 105 us with four; 512 (2 x 1024, 16 heads of 64, fp32) 116
+// and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 139 and 206 us.
+template <typename T, int DP, bool EDGE, int QW>
+int launch_attn_kv_of(const AttnParams& p, int64_t groups, hipStream_t st) {
+  hipLaunchKernelGGL((&attn_bwd_kv_kernel<T, DP, EDGE, QW>), dim3((unsigned)groups), dim3(AttnKvShape<T, DP, EDGE, QW>::kThreads), 0, st, p);
   return launch_rc();
+}
+template <typename T, int DP, bool EDGE>
+int launch_attn_kv(const AttnParams& p, hipStream_t st) {
+  constexpr bool kTwo = AttnKvShape<T, DP, EDGE, 2>::kFits, kFour = !EDGE && AttnKvShape<T, DP, EDGE, 4>::kFits;
+  static_assert(kTwo || kFour, "one of them");
+  const int64_t groups = (int64_t)p.B * p.G * ((p.T + 63) / 64);
+  if constexpr (kFour) {
+    if (!kTwo || groups <= 2 * num_compute_units()) return launch_attn_kv_of<T, DP, EDGE, 4>(p, groups, st);
+  }
+  if constexpr (kTwo) return launch_attn_kv_of<T, DP, EDGE, 2>(p, groups, st);
+  return AMOE_EUNSUPPORTED;
 }
 
 template <typename T>
 int launch_attn_bwd(const AttnParams& p, hipStream_t st) {
+  int rc = AMOE_OK;
   if (p.S > 0) {
-    const dim3 grid((unsigned)((int64_t)p.B * p.H * ((p.S + kAttnRows - 1) / kAttnRows)));
-#define AMOE_LAUNCH(TYPE, DP, EDGE) hipLaunchKernelGGL((&attn_bwd_q_kernel<TYPE, DP, EDGE>), grid, dim3(kAttnThreads), 0, st, p)
+#define AMOE_LAUNCH(TYPE, DP, EDGE)                                                                             \
+  rc = launch_attn_rows<AttnBwdRows<TYPE, DP, EDGE>::template Launch, !EDGE && AttnShape<TYPE, DP, EDGE, 2>::kFits, \
+                        !EDGE && AttnShape<TYPE, DP, EDGE, 1>::kFits>(p, st)
     AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);          // (leaves delta for the next)
 #undef AMOE_LAUNCH
+    if (rc) return rc;
   }
   if (p.T > 0 && p.dk) {
-#define AMOE_LAUNCH(TYPE, DP, EDGE)                                                                             \
-  do {                                                                                                          \
-    using Shape = AttnKvShape<TYPE, DP, EDGE>;                                                                  \
-    const dim3 grid((unsigned)((int64_t)p.B * p.G * ((p.T + 32 * Shape::KW - 1) / (32 * Shape::KW))));          \
-    hipLaunchKernelGGL((&attn_bwd_kv_kernel<TYPE, DP, EDGE>), grid, dim3(Shape::kThreads), 0, st, p); \
-  } while (0)
+#define AMOE_LAUNCH(TYPE, DP, EDGE) rc = launch_attn_kv<TYPE, DP, EDGE>(p, st)
     AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
 #undef AMOE_LAUNCH
   }
-  return launch_rc();
+  return rc;
 }
 
 }  // namespace amoe

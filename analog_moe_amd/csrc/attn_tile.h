@@ -11,7 +11,6 @@
 namespace amoe {
 
 constexpr int kAttnThreads = 256;    // 4 waves
-constexpr int kAttnRows = 128;       // queries (keys, for their gradients) of a workgroup, 32 per wave
 constexpr int kAttnMaxHead = 128;    // elements of a head, at most
 constexpr int kAttnMaxSplits = 1024;        // parts of the key axis
 constexpr int64_t kAttnMaxRows = 1 << 28;   // queries and keys of a sequence, at most
@@ -160,6 +159,18 @@ template <typename T, int DP> struct AttnTile {
       return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
     }
   }
+};
+
+// A workgroup's waves over rows and keys: RW waves have 32 queries each, in KG copies that take every KG-th block of 32 keys and
+// are joined at the end.  Copies make more and shorter workgroups of the same work, for launches that would leave CUs idle, at
+// the price of reading the keys for fewer rows at a time.  kBlocks blocks of keys per copy and tile: two, where the tiles of 16-bit
+// elements leave room for two workgroups on a CU; fp32 tiles are twice as large.
+template <typename T, int DP, bool EDGE, int RW_> struct AttnShape {
+  static constexpr int RW = RW_, KG = 4 / RW, kRows = 32 * RW;
+  static constexpr int kBlocks = KG == 1 && sizeof(T) == 2 ? 2 : 1, kKeys = 32 * KG * kBlocks;
+  static constexpr int kWavesPerSimd = sizeof(T) == 4 && (DP > 64 || EDGE) ? 1 : 2;
+  // what fits the 160 KB of a CU
+  static constexpr bool kFits = 4 * kKeys * DP * (int)sizeof(T) <= 128 << 10;
 };
 
 // A run of matrix products whose first operands come from LDS, with kAttnAhead of them on their way: a read takes as long as
