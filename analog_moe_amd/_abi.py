@@ -149,7 +149,7 @@ ATTN_ARGS = struct.Struct("<"
                           "8qd"           # dtype B S T H G d causal, scale
                           "4q4q4q"        # q, k, v with 3 strides each
                           "2q2q"          # lengths lengths_is_i64, starts starts_is_i64
-                          "2q"            # out lse
+                          "3q"            # out lse rest
                           "4q3q")         # go with 3 strides, dq dk dv
 
 

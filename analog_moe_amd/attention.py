@@ -72,33 +72,37 @@ class _Call:
         self.head = (code, B, S, T, H, G, d, causal, scale, q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
                      v.data_ptr(), vs[0], vs[1], vs[2], n, n64, m, m64)
 
-    def pack(self, out: Tensor, lse: Optional[Tensor], go: Optional[Tensor] = None, grads=(0, 0, 0)) -> bytes:
+    def pack(self, out: Tensor, lse: Optional[Tensor], rest: Optional[Tensor], go: Optional[Tensor] = None, grads=(0, 0, 0)) -> bytes:
         gp, gs = (0, (0, 0, 0)) if go is None else (go.data_ptr(), go.stride())
-        return _abi.ATTN_ARGS.pack(*self.head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), gp, gs[0], gs[1], gs[2], *grads)
+        return _abi.ATTN_ARGS.pack(*self.head, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                   0 if rest is None else rest.data_ptr(), gp, gs[0], gs[1], gs[2], *grads)
 
     def forward(self, want_lse: bool):
         q, lib = self.q, ops.get_lib()
         out = q.new_empty(self.shape)
-        B, S, H, _ = self.shape
-        lse = q.new_empty((B, H, S), dtype=torch.float32) if want_lse else None
-        args = self.pack(out, lse)
+        lse = rest = None
+        if want_lse:
+            B, S, H, _ = self.shape
+            lse = q.new_empty((B, H, S), dtype=torch.float32)
+            rest = None if q.dtype == torch.float32 else q.new_empty(self.shape)
+        args = self.pack(out, lse, rest)
         with ops.device_of(q):
             need = lib.amoe_attention_fwd_workspace(args)
             ws = q.new_empty(need, dtype=torch.uint8) if need else None
             rc = lib.amoe_attention_fwd(args, None if ws is None else ws.data_ptr(), need, ops._stream(q))
         if rc:
             _abi.check(lib, rc, "amoe_attention_fwd")
-        return out, lse
+        return out, lse, rest
 
-    def backward(self, go: Tensor, out: Tensor, lse: Tensor, want_kv: bool):
+    def backward(self, go: Tensor, out: Tensor, lse: Tensor, rest: Optional[Tensor], want_kv: bool):
         q, lib, go = self.q, ops.get_lib(), _rows(go)
         dq = q.new_empty(self.shape)
         dk = dv = None
         if want_kv:
             dk, dv = q.new_empty(self.kv_shape), q.new_empty(self.kv_shape)
-            args = self.pack(out, lse, go, (dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
+            args = self.pack(out, lse, rest, go, (dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
         else:
-            args = self.pack(out, lse, go, (dq.data_ptr(), 0, 0))
+            args = self.pack(out, lse, rest, go, (dq.data_ptr(), 0, 0))
         with ops.device_of(q):
             ws = q.new_empty(max(lib.amoe_attention_bwd_workspace(args), 4), dtype=torch.uint8)
             rc = lib.amoe_attention_bwd(args, ws.data_ptr(), ws.numel(), ops._stream(q))
@@ -109,41 +113,45 @@ class _Call:
 
 def attention_forward(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor] = None, starts: Optional[Tensor] = None,
                       causal: bool = True, scale: Optional[float] = None,
-                      want_lse: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
-    """(out [B, S, H, d], lse [B, H, S] fp32 or None): ``amoe_attention_fwd``.  lse is what ``attention_backward`` reads."""
+                      want_lse: bool = False) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+    """(out [B, S, H, d], lse [B, H, S] fp32, rest like out): ``amoe_attention_fwd``.  With want_lse lse and, for 16-bit types,
+    rest (what the rounding of out took away) are there for ``attention_backward``, else None."""
     return _Call(q, k, v, lengths, starts, causal, scale).forward(want_lse)
 
 
-def attention_backward(go: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, lengths: Optional[Tensor] = None,
-                       starts: Optional[Tensor] = None, causal: bool = True, scale: Optional[float] = None,
-                       want_kv: bool = True) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+def attention_backward(go: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, rest: Optional[Tensor] = None,
+                       lengths: Optional[Tensor] = None, starts: Optional[Tensor] = None, causal: bool = True,
+                       scale: Optional[float] = None, want_kv: bool = True) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     """(dq, dk, dv) of ``attention_forward``'s arguments and results (``amoe_attention_bwd``); without want_kv only dq."""
-    ops._need_gpu(go, out, lse)
+    ops._need_gpu(go, out, lse, rest)
     call = _Call(q, k, v, lengths, starts, causal, scale)
     B, S, H, _ = call.shape
     if go.shape != call.shape or out.shape != call.shape or go.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError("out and its gradient must have q's shape and dtype")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or any(t.device != q.device for t in (go, out, lse)):
         raise ValueError("lse must be fp32 [batch, heads, queries], and all tensors on one device")
-    return call.backward(go, out.contiguous(), lse.contiguous(), want_kv)
+    if rest is not None:
+        if rest.shape != call.shape or rest.dtype != q.dtype or rest.device != q.device:
+            raise ValueError("rest must have out's shape, dtype and device")
+        rest = rest.contiguous()
+    return call.backward(go, out.contiguous(), lse.contiguous(), rest, want_kv)
 
 
 class Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, starts, causal, scale):
-        out, lse = _Call(q, k, v, lengths, starts, causal, scale).forward(True)
-        ctx.save_for_backward(q, k, v, lengths, starts, out, lse)
+        out, lse, rest = _Call(q, k, v, lengths, starts, causal, scale).forward(True)
+        ctx.save_for_backward(q, k, v, lengths, starts, out, lse, rest)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     def backward(ctx, go):
-        q, k, v, lengths, starts, out, lse = ctx.saved_tensors
+        q, k, v, lengths, starts, out, lse, rest = ctx.saved_tensors
         need = ctx.needs_input_grad
         # (what the forward pass left may come back through hooks in another layout)
-        if not out.is_contiguous() or not lse.is_contiguous():
-            out, lse = out.contiguous(), lse.contiguous()
-        dq, dk, dv = _Call(q, k, v, lengths, starts, ctx.causal, ctx.scale).backward(go, out, lse, need[1] or need[2])
+        out, lse, rest = (t if t is None or t.is_contiguous() else t.contiguous() for t in (out, lse, rest))
+        dq, dk, dv = _Call(q, k, v, lengths, starts, ctx.causal, ctx.scale).backward(go, out, lse, rest, need[1] or need[2])
         grads = dq if need[0] else None, dk if need[1] else None, dv if need[2] else None
         if torch.is_grad_enabled():
             grads = once(grads, "attention")

@@ -14,11 +14,14 @@ int check_operand(const void* p, const int64_t* st, int64_t rows, int64_t heads,
   return d < 1 ? AMOE_EINVAL : AMOE_OK;
 }
 
+// Rows further apart than this are not addressed by 32-bit offsets (128 of them must stay below 2^31).
+constexpr int64_t kAttnRowBytes = INT64_C(1) << 23;
+
 // 1: rows start on 16 bytes; 2: and a tile's rows can be addressed by 32-bit offsets into a resource that ends with them
 int operand_vec(const void* p, const int64_t* st, int64_t rows, int64_t d, size_t es) {
   const int64_t c = 16 / (int64_t)es;
   if (!aligned(p, 16) || st[0] % c || st[1] % c || st[2] % c) return 0;
-  if (rows > 1 && (st[1] < d || st[1] * (int64_t)es > (INT64_C(1) << 24))) return 1;
+  if (rows > 1 && (st[1] < d || st[1] * (int64_t)es > kAttnRowBytes)) return 1;
   return 2;
 }
 
@@ -105,7 +108,9 @@ extern "C" int amoe_attention_fwd(const amoe_attn_args* a, void* workspace, size
   AttnParams p{};
   fill(p, a);
   p.out = a->out;
-  if (!aligned(a->out, 16) && p.vec == 2) p.vec = 1;
+  p.rest = a->rest;
+  if (!aligned(a->rest, es)) return AMOE_EALIGN;
+  if ((!aligned(a->out, 16) || !aligned(a->rest, 16)) && p.vec == 2) p.vec = 1;
   p.splits = attn_splits(a);
   if (p.splits > 1) {
     const size_t need = amoe_attention_fwd_workspace(a);
@@ -134,7 +139,7 @@ extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size
   const size_t es = esize((int)a->dtype);
   if (int rc = check_operand(a->go, &a->go_sb, a->S, a->H, a->d, es)) return rc;
   if ((a->S > 0 && (!a->out || !a->lse || !a->dq || !workspace)) || !a->dk != !a->dv) return AMOE_ENULL;
-  if (!aligned(a->out, es) || !aligned(a->dq, es) || !aligned(a->dk, es) || !aligned(a->dv, es)) return AMOE_EALIGN;
+  if (!aligned(a->out, es) || !aligned(a->rest, es) || !aligned(a->dq, es) || !aligned(a->dk, es) || !aligned(a->dv, es)) return AMOE_EALIGN;
   if (workspace_bytes < amoe_attention_bwd_workspace(a)) return AMOE_EWORKSPACE;
   if (!aligned(workspace, 4)) return AMOE_EALIGN;
   AttnParams p{};
@@ -144,11 +149,13 @@ extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size
     const int vg = operand_vec(a->go, &a->go_sb, a->S, a->d, es);
     p.vec = vg < p.vec ? vg : p.vec;
   }
-  const bool whole = aligned(a->out, 16) && aligned(a->dq, 16) && aligned(a->dk, 16) && aligned(a->dv, 16);
+  const bool whole = aligned(a->out, 16) && aligned(a->rest, 16) && aligned(a->dq, 16) && aligned(a->dk, 16) && aligned(a->dv, 16);
   if (!whole) p.vec = 0;
   // (rows of `out` are d elements apart: with another d their starts are not on 16 bytes)
   if ((a->d * es) % 16) p.vec = 0;
+  if (a->S > 1 && a->H * a->d * (int64_t)es > kAttnRowBytes && p.vec == 2) p.vec = 1;
   p.o = a->out;
+  p.rest = a->rest;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   p.delta = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);

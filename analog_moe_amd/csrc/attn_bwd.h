@@ -80,24 +80,26 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
   attn_frag<T> q[NK], go[NK];
   const bool real = w.i < p.S;
   const int64_t row = ((int64_t)w.b * p.S + w.i) * p.H + w.hd, stat = (int64_t)w.bh * p.S + w.i;
-  const T* qrow = static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh + (int64_t)w.i * p.q.ss;
-  const T* grow = static_cast<const T*>(p.go.p) + w.b * p.go.sb + w.hd * p.go.sh + (int64_t)w.i * p.go.ss;
-  const T* orow = static_cast<const T*>(p.o) + row * p.d;
+  attn_frag<T> o[NK], rest[NK];
+  const int64_t out0 = ((int64_t)w.b * p.S * p.H + w.hd) * p.d, out_stride = (int64_t)p.H * p.d;
+  attn_row_frags<T, DP, EDGE>(q, static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh, p.q.ss, w.w0, p.S, p.d, p.vec);
+  attn_row_frags<T, DP, EDGE>(go, static_cast<const T*>(p.go.p) + w.b * p.go.sb + w.hd * p.go.sh, p.go.ss, w.w0, p.S, p.d, p.vec);
+  attn_row_frags<T, DP, EDGE>(o, static_cast<const T*>(p.o) + out0, out_stride, w.w0, p.S, p.d, p.vec);
+  if constexpr (sizeof(T) == 2)
+    attn_row_frags<T, DP, EDGE>(rest, static_cast<const T*>(p.rest ? p.rest : p.o) + out0, out_stride, w.w0, p.rest ? p.S : 0, p.d, p.vec);
   float delta = 0.f;
 #pragma unroll
   for (int kk = 0; kk < NK; kk++) {
-    q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, real, p.vec);
-    go[kk] = attn_global_frag<T, EDGE>(grow, kk, p.d, real, p.vec);
-    const attn_frag<T> o = attn_global_frag<T, EDGE>(orow, kk, p.d, real, p.vec);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) delta = fmaf(o.v[j], go[kk].v[j], delta);
+      for (int j = 0; j < 8; j++) delta = fmaf(o[kk].v[j], go[kk].v[j], delta);
     } else {
-      float ov[8], gv[8];
-      raw_unpack<T>(o, ov);
+      float ov[8], gv[8], rv[8];
+      raw_unpack<T>(o[kk], ov);
       raw_unpack<T>(go[kk], gv);
+      raw_unpack<T>(rest[kk], rv);
 #pragma unroll
-      for (int j = 0; j < 8; j++) delta = fmaf(ov[j], gv[j], delta);
+      for (int j = 0; j < 8; j++) delta = fmaf(ov[j] + rv[j], gv[j], delta);
     }
   }
   delta = attn_pair_sum(delta);
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
       factor = 1.f;
     }
   }
-  if (w.kg == 0 && real) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, factor, p.d);
+  if (w.kg == 0) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, factor, p.d, real);
 }
 
 // dk, dv: KW waves hold 32 keys each of one key head, k and v as operands in registers, in QW copies; the queries of all heads
@@ -234,14 +236,10 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
     else if (tid < 2 * BM) lds_delta[buf][tid - BM] = stat;
   };
   if (n_tiles > 0) fetch(0);
-  const T* krow = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh + (int64_t)key * p.k.ss;
-  const T* vrow = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh + (int64_t)key * p.v.ss;
-  attn_frag<T> kf[NK], vf[Shape::kVInLds ? 1 : NK];
-#pragma unroll
-  for (int kk = 0; kk < NK; kk++) {
-    kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, held, p.vec);
-    if constexpr (!Shape::kVInLds) vf[kk] = attn_global_frag<T, EDGE>(vrow, kk, p.d, held, p.vec);
-  }
+  attn_frag<T> kf[NK], vf[NK];
+  attn_row_frags<T, DP, EDGE>(kf, static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh, p.k.ss, w0 < length ? w0 : 0, w0 < length ? length : 0, p.d, p.vec);
+  if constexpr (!Shape::kVInLds)
+    attn_row_frags<T, DP, EDGE>(vf, static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, w0 < length ? w0 : 0, w0 < length ? length : 0, p.d, p.vec);
   if constexpr (Shape::kVInLds) {
     AttnStage<T, DP, 32 * KW, NT, EDGE> sv;
     sv.init(tid, p.v.ss, p.d);
@@ -329,7 +327,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
         for (int e = 0; e < 16; e++) acc[t][e] *= factor;
 #pragma unroll
       for (int c = 0; c < QW - 1; c++) attn_add_acc<DP>(sums, c * KW + kw, acc, 1.f);
-      if (key < p.T) attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d);
+      attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d, key < p.T);
     }
   }
 }

@@ -71,7 +71,7 @@ __device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[N
 
 // What the waves of a workgroup work on, for the kernels whose lanes own queries.
 struct AttnRowsOf {
-  int b, hd, g, bh, i, rw, kg;
+  int b, hd, g, bh, w0, i, rw, kg;   // w0: the wave's first query, i: the lane's
   int length, start;
   int group_sees;     // keys that the last query of the workgroup sees
   int wave_sees;      // the last one of the wave
@@ -94,6 +94,7 @@ __device__ __forceinline__ AttnRowsOf attn_rows_of(const AttnParams& p) {
   w.length = attn_length(p, w.b);
   w.start = attn_start(p, w.b);
   const int w0 = row0 + w.rw * 32, end = p.S - 1;
+  w.w0 = w0;
   w.i = w0 + (lane_id() & 31);
   const int group_last = row0 + Shape::kRows - 1, wave_last = w0 + 31;
   w.group_sees = attn_seen(p, w.length, w.start, group_last < end ? group_last : end);
@@ -154,9 +155,7 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
     sv.load(tid, lds_v, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK];
-  const T* qrow = static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh + (int64_t)w.i * p.q.ss;
-#pragma unroll
-  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, w.i < p.S, p.vec);
+  attn_row_frags<T, DP, EDGE>(q, static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh, p.q.ss, w.w0, p.S, p.d, p.vec);
 
   AttnState<T, DP> st;
   st.clear();
@@ -225,11 +224,13 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
       st.m = m;
     }
   }
-  if (w.kg == 0 && w.i < p.S) {
+  if (w.kg == 0) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool real = w.i < p.S;
     const int64_t row = ((int64_t)w.b * p.S + w.i) * p.H + w.hd;
-    attn_store_col<T, DP, EDGE>(static_cast<T*>(p.out) + row * p.d, st.o, inv, p.d);
-    if (p.lse && h == 0) p.lse[(int64_t)w.bh * p.S + w.i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
+    attn_store_col<T, DP, EDGE>(static_cast<T*>(p.out) + row * p.d, st.o, inv, p.d, real);
+    if (p.rest) attn_store_col<T, DP, EDGE, true>(static_cast<T*>(p.rest) + row * p.d, st.o, inv, p.d, real);
+    if (p.lse && real && h == 0) p.lse[(int64_t)w.bh * p.S + w.i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
   }
 }
 
@@ -270,10 +271,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   sv.init(lane, p.v.ss, p.d);
   typename Tile::Lane at;
   const auto fetch = [&](int key0) {
-    const int key = key0 + (lane & 31);
-    const T* krow = kb + (int64_t)key * p.k.ss;
-#pragma unroll
-    for (int kk = 0; kk < NK; kk++) kf[kk] = attn_global_frag<T, EDGE>(krow, kk, p.d, key < key_hi, p.vec);
+    attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, key0, key_hi, p.d, p.vec);
     sv.load(lane, nullptr, vb, p.v.ss, key0, key_hi, p.d, p.vec);
   };
   int key0 = key_lo + 32 * wave;
@@ -345,8 +343,12 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
       const float inv = lr == 0.f ? 0.f : 1.f / lr;
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] *= inv;
-      T* out = static_cast<T*>(p.out) + (((int64_t)b * p.S + query) * p.H + head) * p.d + e;
-      store4<T>(out, v, EDGE ? p.d - e : 4, !EDGE);
+      const int64_t to = (((int64_t)b * p.S + query) * p.H + head) * p.d + e;
+      store4<T>(static_cast<T*>(p.out) + to, v, EDGE ? p.d - e : 4, !EDGE);
+      if (p.rest) {
+        const float rest[4] = {attn_rest<T>(v[0]), attn_rest<T>(v[1]), attn_rest<T>(v[2]), attn_rest<T>(v[3])};
+        store4<T>(static_cast<T*>(p.rest) + to, rest, EDGE ? p.d - e : 4, !EDGE);
+      }
       if (p.lse && e == 0) p.lse[where] = lr == 0.f ? INFINITY : mr * p.c + fast_log2(lr) - kProbShift<T>;
     }
   }
@@ -394,12 +396,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams p) {
   lds_o[run][unit] = o;
   __syncthreads();
   const int64_t bh = at / p.S, i = at - bh * p.S, b = bh / p.H, hd = bh - b * p.H;
-  T* out = static_cast<T*>(p.out) + ((b * p.S + i) * p.H + hd) * p.d;
+  const int64_t to = ((b * p.S + i) * p.H + hd) * p.d;
   if (tid < p.d) {
     float v = 0.f;
 #pragma unroll
     for (int r = 0; r < 8; r++) v += lds_o[r][tid >> 2][tid & 3];
-    out[tid] = Elem<T>::cvt(v * (l == 0.f ? 0.f : 1.f / l));
+    v *= l == 0.f ? 0.f : 1.f / l;
+    static_cast<T*>(p.out)[to + tid] = Elem<T>::cvt(v);
+    if (p.rest) static_cast<T*>(p.rest)[to + tid] = Elem<T>::cvt(attn_rest<T>(v));
   }
   if (p.lse && tid == 0) p.lse[at] = l == 0.f ? INFINITY : m * p.c + fast_log2(l) - kProbShift<T>;
 }

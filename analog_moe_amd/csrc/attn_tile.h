@@ -25,6 +25,7 @@ struct AttnParams {
   AttnOperand q, k, v, go;           // go: gradient of the output
   void* out;                         // [B, S, H, d]
   const void* o;                     // the same, read by the backward pass
+  void* rest;                        // [B, S, H, d]: out before its rounding less out, of the same type; written and read.  May be null
   float* lse;                        // [B, H, S]: log2 of the sum of 2^(score * c); +inf where a row sees nothing.  May be null
   float* delta;                      // [B, H, S]: sum over d of out * gradient of out
   void *dq, *dk, *dv;                // [B, S, H, d], [B, T, G, d]
@@ -276,6 +277,37 @@ __device__ __forceinline__ attn_frag<T> attn_global_frag(const T* row, int kk, i
   }
 }
 
+// The operands of rows row0 + l % 32, the whole head, straight from global memory; rows at or past row_end and elements past d are
+// zeros.  (Without edges one resource that ends with the rows does that, and no load waits for a branch.)
+template <typename T, int DP, bool EDGE>
+__device__ __forceinline__ void attn_row_frags(attn_frag<T> (&f)[DP / 16], const T* base, int64_t stride, int row0, int row_end, int d, bool vec) {
+  const int l = lane_id(), h = l >> 5;
+  const T* p = base + (int64_t)row0 * stride;
+  if constexpr (EDGE) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; kk++)
+      f[kk] = attn_global_frag<T, EDGE>(p + (l & 31) * stride, kk, d, row0 + (l & 31) < row_end, vec);
+  } else {
+    const int rows = row_end - row0 < 32 ? row_end - row0 : 32;
+    const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d) * (uint32_t)sizeof(T) : 0u;
+    const BufRsrc rs = make_rsrc_sized(const_cast<T*>(rows > 0 ? p : base), bytes);
+    const uint32_t at = (uint32_t)((l & 31) * stride + 8 * h) * (uint32_t)sizeof(T);
+    // (no more rows than there are: an offset past the end reads zero, but must not wrap round)
+    const bool ok = (l & 31) < rows;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; kk++) {
+      const uint32_t off = ok && 16 * kk + 8 * h < d ? at + 16u * kk * (uint32_t)sizeof(T) : 0xfffffff0u;
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t off2 = ok && 16 * kk + 8 * h + 4 < d ? off + 16u : 0xfffffff0u;
+        const Raw a = buffer_load_b128(rs, off, 0), b = buffer_load_b128(rs, off2, 0);
+        f[kk] = F32x8{{as_f32(a[0]), as_f32(a[1]), as_f32(a[2]), as_f32(a[3]), as_f32(b[0]), as_f32(b[1]), as_f32(b[2]), as_f32(b[3])}};
+      } else {
+        f[kk] = buffer_load_b128(rs, off, 0);
+      }
+    }
+  }
+}
+
 // the larger (the sum) of a lane's and its partner's in the other half of the wave
 __device__ __forceinline__ float attn_pair_max(float v) {
   uint32_t a = as_u32(v), b = a;
@@ -288,20 +320,45 @@ __device__ __forceinline__ float attn_pair_sum(float v) {
   return as_f32(a) + as_f32(b);
 }
 
-// A lane's column of a [head elements][32] product: rows 8 * g + 4 * (l / 32) .. + 3 of every 32 are adjacent in memory.
-template <typename T, int DP, bool EDGE>
-__device__ __forceinline__ void attn_store_col(T* row, const f32x16* acc, float factor, int d) {
+template <typename T>
+__device__ __forceinline__ float attn_rest(float v) { return v - Elem<T>::to_f32(Elem<T>::cvt(v)); }
+
+// A lane's column of a [head elements][32] product times factor, to its row in memory (ok: it has one).  It holds 4 adjacent
+// elements of every 8, its partner l ^ 32 the other 4; 16-bit elements change places so that each stores 8 at a time.  The whole
+// wave calls this.  REST: what the rounding to T takes away, instead.
+template <typename T, int DP, bool EDGE, bool REST = false>
+__device__ __forceinline__ void attn_store_col(T* row, const f32x16* acc, float factor, int d, bool ok) {
   const int h = lane_id() >> 5;
-  const bool vec = (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
+  const auto value = [&](int t, int i) {
+    const float v = acc[t][i] * factor;
+    return REST ? attn_rest<T>(v) : v;
+  };
+  if constexpr (EDGE || sizeof(T) == 4) {
+    const bool vec = !EDGE || (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; dt++)
+    for (int t = 0; t < DP / 32; t++)
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int e = 32 * dt + 8 * g + 4 * h;
-      if (e >= d) continue;
-      const float v[4] = {acc[dt][4 * g] * factor, acc[dt][4 * g + 1] * factor, acc[dt][4 * g + 2] * factor, acc[dt][4 * g + 3] * factor};
-      store4<T>(row + e, v, EDGE ? d - e : 4, EDGE ? vec : true);
-    }
+      for (int g = 0; g < 4; g++) {
+        const int e = 32 * t + 8 * g + 4 * h;
+        if (!ok || e >= d) continue;
+        const float v[4] = {value(t, 4 * g), value(t, 4 * g + 1), value(t, 4 * g + 2), value(t, 4 * g + 3)};
+        store4<T>(row + e, v, EDGE ? d - e : 4, vec);
+      }
+  } else {
+#pragma unroll
+    for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        const float v[8] = {value(t, 4 * g),     value(t, 4 * g + 1), value(t, 4 * g + 2), value(t, 4 * g + 3),
+                            value(t, 4 * g + 4), value(t, 4 * g + 5), value(t, 4 * g + 6), value(t, 4 * g + 7)};
+        const Raw r = raw_pack<T>(v);
+        uint32_t a0 = r[0], a1 = r[1], b0 = r[2], b1 = r[3];
+        swap_half_waves(a0, b0);
+        swap_half_waves(a1, b1);
+        const int e = 32 * t + 8 * (g + h);
+        if (ok && e < d) *reinterpret_cast<Raw*>(row + e) = Raw{a0, a1, b0, b1};
+      }
+  }
 }
 
 __device__ __forceinline__ f32x16 f32x16_zero() {

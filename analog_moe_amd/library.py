@@ -366,29 +366,31 @@ ffn_fwd.register_autograd(_ffn_autograd, setup_context=_ffn_setup_context)
 @torch.library.custom_op(
     "amoe::attention_fwd", mutates_args=(),
     schema="(Tensor q, Tensor k, Tensor v, Tensor? lengths, Tensor? starts, bool causal, float? scale, bool want_lse)"
-           " -> (Tensor, Tensor)")
+           " -> (Tensor, Tensor, Tensor)")
 def attention_fwd(q, k, v, lengths, starts, causal, scale, want_lse):
-    """(out [B, S, H, d], lse [B, H, S] or empty)."""
-    out, lse = attention.attention_forward(q, k, v, lengths, starts, causal, scale, want_lse)
-    return out, torch.empty(_EMPTY_SHAPE, dtype=torch.float32, device=q.device) if lse is None else lse
+    """(out [B, S, H, d], lse [B, H, S] or empty, rest like out or empty)."""
+    out, lse, rest = attention.attention_forward(q, k, v, lengths, starts, causal, scale, want_lse)
+    return (out, torch.empty(_EMPTY_SHAPE, dtype=torch.float32, device=q.device) if lse is None else lse,
+            q.new_empty(_EMPTY_SHAPE) if rest is None else rest)
 
 
 @attention_fwd.register_fake
 def _(q, k, v, lengths, starts, causal, scale, want_lse):
     B, S, H, d = q.shape
-    return q.new_empty((B, S, H, d)), torch.empty((B, H, S) if want_lse else _EMPTY_SHAPE, dtype=torch.float32, device=q.device)
+    return (q.new_empty((B, S, H, d)), torch.empty((B, H, S) if want_lse else _EMPTY_SHAPE, dtype=torch.float32, device=q.device),
+            q.new_empty((B, S, H, d) if want_lse and q.dtype != torch.float32 else _EMPTY_SHAPE))
 
 
 @torch.library.custom_op(
     "amoe::attention_bwd", mutates_args=(),
-    schema="(Tensor go, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor? lengths, Tensor? starts, bool causal, "
-           "float? scale) -> (Tensor, Tensor, Tensor)")
-def attention_bwd(go, q, k, v, out, lse, lengths, starts, causal, scale):
-    return attention.attention_backward(go, q, k, v, out, lse, lengths, starts, causal, scale)
+    schema="(Tensor go, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor rest, Tensor? lengths, Tensor? starts, "
+           "bool causal, float? scale) -> (Tensor, Tensor, Tensor)")
+def attention_bwd(go, q, k, v, out, lse, rest, lengths, starts, causal, scale):
+    return attention.attention_backward(go, q, k, v, out, lse, rest if rest.shape == out.shape else None, lengths, starts, causal, scale)
 
 
 @attention_bwd.register_fake
-def _(go, q, k, v, out, lse, lengths, starts, causal, scale):
+def _(go, q, k, v, out, lse, rest, lengths, starts, causal, scale):
     return q.new_empty(tuple(q.shape)), k.new_empty(tuple(k.shape)), v.new_empty(tuple(v.shape))
 
 
@@ -400,13 +402,13 @@ def _attention_setup_context(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _attention_autograd(ctx, go, _grad_lse):
+def _attention_autograd(ctx, go, _grad_lse, _grad_rest):
     if go is None:
         return (None,) * 8
     if not ctx.has_lse:
         raise RuntimeError("amoe::attention_fwd was called without want_lse: there is nothing to go back from")
-    q, k, v, lengths, starts, out, lse = ctx.saved_tensors
-    return (*torch.ops.amoe.attention_bwd(go, q, k, v, out, lse, lengths, starts, *ctx.args),) + (None,) * 5
+    q, k, v, lengths, starts, out, lse, rest = ctx.saved_tensors
+    return (*torch.ops.amoe.attention_bwd(go, q, k, v, out, lse, rest, lengths, starts, *ctx.args),) + (None,) * 5
 
 
 attention_fwd.register_autograd(_attention_autograd, setup_context=_attention_setup_context)

@@ -476,7 +476,8 @@ size_t amoe_rotary_args_bytes(void);
  * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; last strides are 1.
  * Few rows over many keys are worked on in parts of the key axis, whose results pass through the workspace.
  * The backward call recomputes the probabilities from lse (log2 of a row's sum, made by the forward call; NULL there: not
- * wanted) and reads out; its workspace holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold are zero.
+ * wanted) and reads out and, unless it is NULL, rest: the sums of out times its gradient are then as good as those of an output
+ * that was not rounded, which takes a third of their error from dq and dk of 16-bit types (fp32 needs none); its workspace holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold are zero.
  * Neither call uses atomics: equal inputs give equal bits. */
 typedef struct amoe_attn_args {
   int64_t dtype, B, S, T, H, G, d, causal;
@@ -488,6 +489,7 @@ typedef struct amoe_attn_args {
   const void* starts;  int64_t starts_is_i64;
   void* out;                                                    /* [B, S, H, d] */
   float* lse;                                                   /* [B, H, S] */
+  void* rest;                                                   /* [B, S, H, d] what out's rounding took, or NULL */
   /* backward only */
   const void* go;  int64_t go_sb, go_ss, go_sh;                 /* gradient of out */
   void* dq;  void* dk;  void* dv;                               /* [B, S, H, d], [B, T, G, d] */

@@ -46,12 +46,14 @@ def check(q, k, v, go, lengths=None, starts=None, causal=True, scale=None, devic
     want, bounds = O.attention(q, k, v, go, **kw)
     to = lambda t: None if t is None else t if device == "cpu" else _on_gpu(t)          # noqa: E731
     q, k, v, go, lengths, starts = map(to, (q, k, v, go, lengths, starts))
-    out, lse = A.attention_forward(q, k, v, lengths, starts, causal, scale, want_lse=True)
-    plain, none = A.attention_forward(q, k, v, lengths, starts, causal, scale)
-    assert none is None and torch.equal(plain, out)
-    grads = A.attention_backward(go, q, k, v, out, lse, lengths, starts, causal, scale)
+    out, lse, rest = A.attention_forward(q, k, v, lengths, starts, causal, scale, want_lse=True)
+    plain, *none = A.attention_forward(q, k, v, lengths, starts, causal, scale)
+    assert none == [None, None] and torch.equal(plain, out)
+    assert rest is None if q.dtype == torch.float32 else (rest.abs() <= out.abs() * torch.finfo(q.dtype).eps + torch.finfo(q.dtype).tiny).all()
+    compare((out, *A.attention_backward(go, q, k, v, out, lse, None, lengths, starts, causal, scale)), want, bounds, kw)
+    grads = A.attention_backward(go, q, k, v, out, lse, rest, lengths, starts, causal, scale)
     compare((out, *grads), want, bounds, kw)
-    again = A.attention_backward(go, q, k, v, out, lse, lengths, starts, causal, scale)
+    again = A.attention_backward(go, q, k, v, out, lse, rest, lengths, starts, causal, scale)
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
     seen = O.visible(q.shape[0], q.shape[1], k.shape[1], causal, None if lengths is None else lengths.cpu(),
                      None if starts is None else starts.cpu()).any(-1)
@@ -102,12 +104,12 @@ def test_few_rows_in_parts(emu_ops, monkeypatch):
     """Rows over a long axis are worked on in parts, joined by a second kernel; also where a part holds no key."""
     q, k, v, _ = inputs(1, 1, 700, 2, 1, 64, "bf16", seed=3)
     lib = emu_ops.get_lib()
-    args = A._Call(q, k, v, None, None, True, 0.125).pack(q, None)
+    args = A._Call(q, k, v, None, None, True, 0.125).pack(q, None, None)
     assert lib.amoe_attention_fwd_workspace(args) == 6 * 2 * 66 * 4
     for n in (700, 130, 128, 1, 0):
         kw = dict(lengths=marks([n]), starts=marks([n - 1], torch.int64))
         (want,), (bound,) = O.attention(q, k, v, **kw)
-        out, lse = A.attention_forward(q, k, v, **kw, want_lse=True)
+        out, lse, _ = A.attention_forward(q, k, v, **kw, want_lse=True)
         assert b"attn_join" in lib_last(lib)
         compare((out,), (want,), (bound,), n)
         assert torch.isinf(lse).all() == (n == 0)
@@ -123,13 +125,13 @@ def behind_the_keys(device, sizes):
     for d in sizes:
         q, k, v, go = (t.to(device) for t in inputs(2, 6, 50, 2, 1, d, "bf16"))
         lengths, starts = marks([19, 33]).to(device), marks([13, 27]).to(device)
-        want, _ = A.attention_forward(q, k, v, lengths, starts, want_lse=True)
+        want = A.attention_forward(q, k, v, lengths, starts)[0]
         k, v = k.clone(), v.clone()
         for b, n in enumerate((19, 33)):
             k[b, n:], v[b, n:] = float("nan"), float("inf")
-        out, lse = A.attention_forward(q, k, v, lengths, starts, want_lse=True)
+        out, lse, rest = A.attention_forward(q, k, v, lengths, starts, want_lse=True)
         assert torch.equal(out, want)
-        dq, dk, dv = A.attention_backward(go, q, k, v, out, lse, lengths, starts)
+        dq, dk, dv = A.attention_backward(go, q, k, v, out, lse, rest, lengths, starts)
         assert all(torch.isfinite(t).all() for t in (dq, dk, dv))
         assert not dk[0, 19:].any() and not dv[1, 33:].any()
 
@@ -143,8 +145,8 @@ def test_gpu_what_lies_behind_the_keys_is_not_read():
     # (not a number everywhere first: nothing that a workgroup finds in its LDS may get into results either)
     nan = torch.full((64, 256, 8, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
     for d in (128, 96, 80, 64, 48, 13):
-        out, lse = A.attention_forward(nan, nan, nan, want_lse=True)
-        A.attention_backward(nan, nan, nan, nan, out, lse)
+        out, lse, rest = A.attention_forward(nan, nan, nan, want_lse=True)
+        A.attention_backward(nan, nan, nan, nan, out, lse, rest)
         behind_the_keys("cuda", (d,))
 
 
@@ -178,10 +180,10 @@ def test_refusals(emu_ops):
     for bad in (lambda: f(q.double(), k, v), lambda: f(q, k.bfloat16(), v), lambda: f(q, k, v, torch.tensor([1.0, 2.0]))):
         with pytest.raises(TypeError):
             bad()
-    out, lse = f(q, k, v, want_lse=True)
+    out, lse, _ = f(q, k, v, want_lse=True)
     b = A.attention_backward
     for bad in (lambda: b(go[:, :3], q, k, v, out, lse), lambda: b(go, q, k, v, out, lse[:, :, :3]), lambda: b(go.half(), q, k, v, out, lse),
-                lambda: b(go, q, k, v, out, lse.half())):
+                lambda: b(go, q, k, v, out, lse.half()), lambda: b(go, q, k, v, out, lse, out[:1])):
         with pytest.raises(ValueError):
             bad()
 
@@ -192,7 +194,7 @@ def test_library_refuses_what_it_cannot_address(emu_ops):
     lib = emu_ops.get_lib()
     q, k, v, go = inputs(1, 2, 3, 2, 1, 32, "f32")
     out, lse = torch.empty_like(q), torch.empty(1, 2, 2)
-    good = list(_abi.ATTN_ARGS.unpack(A._Call(q, k, v, None, None, True, 0.5).pack(out, lse, go, (1 << 20,) * 3)))
+    good = list(_abi.ATTN_ARGS.unpack(A._Call(q, k, v, None, None, True, 0.5).pack(out, lse, None, go, (1 << 20,) * 3)))
 
     def fwd(**change):
         a = list(good)
@@ -233,8 +235,7 @@ def test_autograd(emu_ops):
 def test_gradients_are_differences(emu_ops):
     """dq, dk and dv against central differences of the loss sum(out * go): step h, error h^2 * third derivative + 2^-24 / h."""
     q, k, v, go = inputs(1, 5, 7, 2, 1, 16, "f32", seed=11)
-    out, lse = A.attention_forward(q, k, v, want_lse=True)
-    grads = A.attention_backward(go, q, k, v, out, lse)
+    grads = A.attention_backward(go, q, k, v, *A.attention_forward(q, k, v, want_lse=True))
     h = 2.0 ** -7
     loss = lambda a: (A.attention_forward(*a)[0].double() * go.double()).sum().item()          # noqa: E731
     for n, index in ((0, (0, 3, 1, 2)), (0, (0, 0, 0, 0)), (1, (0, 2, 0, 5)), (1, (0, 6, 0, 1)), (2, (0, 1, 0, 9)), (2, (0, 4, 0, 0))):
@@ -315,8 +316,8 @@ def test_gpu_stream_and_graph():
     side = torch.cuda.Stream()
 
     def work():
-        out, lse = A.attention_forward(q2, k2, v2, want_lse=True)
-        return (A.attention_forward(q, k, v, lengths, lengths - 1)[0], out, *A.attention_backward(go2, q2, k2, v2, out, lse))
+        left = A.attention_forward(q2, k2, v2, want_lse=True)
+        return (A.attention_forward(q, k, v, lengths, lengths - 1)[0], left[0], *A.attention_backward(go2, q2, k2, v2, *left))
     want = [t.clone() for t in work()]
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
