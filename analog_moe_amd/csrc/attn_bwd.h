@@ -8,6 +8,9 @@
 
 namespace amoe {
 
+// fp16 probabilities as operands, 2^15 times as large: no more than 2^15, and 2^-29 is still a normal number.
+template <typename T> inline constexpr float kGradShift = kIsF16<T> ? 15.f : 0.f;
+
 // dS as matrix operands.  fp16 has no range for it: a gradient's size is the caller's, and where many keys share a row dS is
 // tiny against what it sums up to.  So every column (a lane's query or key) carries a power of two that keeps its largest
 // entry within fp16; it only falls, and the sums so far fall with it.  bf16 and fp32 need none.
@@ -285,8 +288,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int e = 4 * u + j;
-          // (2^15 times P for fp16, as in the forward pass)
-          s[e] = fast_exp2(fmaf(s[e], p.c, kProbShift<T> - lse[j]));
+          s[e] = fast_exp2(fmaf(s[e], p.c, kGradShift<T> - lse[j]));
           dp[e] = s[e] * (dp[e] - del[j]);
         }
       }

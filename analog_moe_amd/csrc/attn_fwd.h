@@ -5,10 +5,14 @@
 
 namespace amoe {
 
-// A row's scores are kept as s * c in the exponent of 2.  fp16 probabilities are kept 2^15 times as large (so that what is
-// 2^-29 of a row's largest is still a normal number; at 1 times, a long row's tail below 2^-14 would lose bits that its sum
-// counts): the sum carries the same factor and the quotient none.
-template <typename T> inline constexpr float kProbShift = kIsF16<T> ? 15.f : 0.f;
+// A row's scores are kept as s * c in the exponent of 2.  The maximum that is taken out of them lags behind: it follows only when
+// a larger one leaves it by more than 2^kMaxLag, which after a row's first keys it hardly ever does (following at every step
+// costs a multiplication of the whole output state: 8192 queries of 16 heads of 128, bf16, 350 us, so 309 us); sums in fp32 and
+// bf16 operands have the range for that.  fp16 probabilities are kept 2^7 times as large, which with the lag stays below 2^16:
+// what is 2^-21 of a row's largest is still a normal number, where at 1 times a long row's tail below 2^-14 would lose bits
+// that its sum counts.  The sum carries the same factor and the quotient none.
+constexpr float kMaxLag = 8.f;
+template <typename T> inline constexpr float kProbShift = kIsF16<T> ? 7.f : 0.f;
 
 // State of a wave's 32 queries (a lane and its partner l ^ 32 hold one): output columns, running maximum, running sum of
 // this lane's keys.
@@ -42,17 +46,18 @@ __device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[N
 #pragma unroll
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[n][i]);
   mx = attn_pair_max(mx);
-  // what was summed so far, in units of the new maximum; once the maxima have settled nothing changes for a whole wave
-  if (wave_ballot(mx > st.m) != 0) {
-    const float f = mx > st.m ? fast_exp2((st.m - mx) * c) : 1.f;
+  // what was summed so far, in units of the new maximum
+  const bool follow = (mx - st.m) * c > kMaxLag;             // (the first keys: from -inf)
+  if (wave_ballot(follow) != 0) {
+    const float f = follow ? fast_exp2((st.m - mx) * c) : 1.f;
     st.l *= f;
 #pragma unroll
     for (int t = 0; t < DP / 32; t++)
 #pragma unroll
       for (int i = 0; i < 16; i++) st.o[t][i] *= f;
-    st.m = mx;
+    st.m = follow ? mx : st.m;
   }
-  const float base = kProbShift<T> - (mx == -INFINITY ? 0.f : mx * c);
+  const float base = kProbShift<T> - (st.m == -INFINITY ? 0.f : st.m * c);
   float sum = 0.f;
 #pragma unroll
   for (int n = 0; n < NB; n++)
