@@ -18,10 +18,10 @@ int check_operand(const void* p, const int64_t* st, int64_t rows, int64_t heads,
 constexpr int64_t kAttnRowBytes = INT64_C(1) << 23;
 
 // 1: rows start on 16 bytes; 2: and a tile's rows can be addressed by 32-bit offsets into a resource that ends with them
-int operand_vec(const void* p, const int64_t* st, int64_t rows, int64_t d, size_t es) {
+int operand_vec(const AttnOperand& o, int64_t rows, int64_t d, size_t es) {
   const int64_t c = 16 / (int64_t)es;
-  if (!aligned(p, 16) || st[0] % c || st[1] % c || st[2] % c) return 0;
-  if (rows > 1 && (st[1] < d || st[1] * (int64_t)es > kAttnRowBytes)) return 1;
+  if (!aligned(o.p, 16) || o.sb % c || o.ss % c || o.sh % c) return 0;
+  if (rows > 1 && (o.ss < d || o.ss * (int64_t)es > kAttnRowBytes)) return 1;
   return 2;
 }
 
@@ -32,12 +32,11 @@ int check_sizes(const amoe_attn_args* a) {
   if (a->H % a->G) return AMOE_ESHAPE;
   if (!(a->scale > 0) || !(a->scale < 3.4e38)) return AMOE_EINVAL;
   if (a->d > kAttnMaxHead || a->S > kAttnMaxRows || a->T > kAttnMaxRows) return AMOE_EUNSUPPORTED;
-  // workgroup and row numbers stay in 31 bits
-  const int64_t limit = INT64_C(1) << 31;
-  if (a->B > limit || a->H > limit || (a->S > 0 && a->H / a->G > limit / a->S - 64)) return AMOE_EUNSUPPORTED;
-  const int64_t tiles = (a->S > a->T ? a->S : a->T) / 32 + 1;
-  if (a->B > 0 && a->H > limit / tiles / a->B) return AMOE_EUNSUPPORTED;
-  return AMOE_OK;
+  // threads of a launch are counted in 32 bits: 2^24 workgroups of 256 over the queries, 2^23 of 512 over the keys
+  const int64_t over = INT64_C(1) << 23;
+  if (a->B > over || a->H > over || a->B * a->H > over) return AMOE_EUNSUPPORTED;
+  if (a->B * a->H * ((a->S + 127) / 128) >= over || a->B * a->G * ((a->T + 63) / 64) >= over) return AMOE_EUNSUPPORTED;
+  return a->H / a->G * a->S > (INT64_C(1) << 30) ? AMOE_EUNSUPPORTED : AMOE_OK;
 }
 
 // Parts of the key axis for the kernel of few rows; 0: the kernel of many rows.
@@ -58,10 +57,15 @@ int attn_splits(const amoe_attn_args* a) {
   return (int)(n < 1 ? 1 : n > kAttnMaxSplits ? kAttnMaxSplits : n);
 }
 
+// (how far apart the one element of a dimension of size 1 is from the next says nothing)
+AttnOperand operand(const void* p, const int64_t* st, int64_t batch, int64_t rows, int64_t heads) {
+  return {p, batch == 1 ? 0 : st[0], rows == 1 ? 0 : st[1], heads == 1 ? 0 : st[2]};
+}
+
 void fill(AttnParams& p, const amoe_attn_args* a) {
-  p.q = {a->q, a->q_sb, a->q_ss, a->q_sh};
-  p.k = {a->k, a->k_sb, a->k_ss, a->k_sh};
-  p.v = {a->v, a->v_sb, a->v_ss, a->v_sh};
+  p.q = operand(a->q, &a->q_sb, a->B, a->S, a->H);
+  p.k = operand(a->k, &a->k_sb, a->B, a->T, a->G);
+  p.v = operand(a->v, &a->v_sb, a->B, a->T, a->G);
   p.lengths = a->lengths; p.lengths_i64 = (int)a->lengths_is_i64;
   p.starts = a->starts; p.starts_i64 = (int)a->starts_is_i64;
   p.B = (int)a->B; p.S = (int)a->S; p.T = (int)a->T; p.H = (int)a->H; p.G = (int)a->G; p.R = (int)(a->H / a->G);
@@ -70,9 +74,9 @@ void fill(AttnParams& p, const amoe_attn_args* a) {
   p.scale = (float)a->scale;
   p.lse = a->lse;
   const size_t es = esize((int)a->dtype);
-  int vec = operand_vec(a->q, &a->q_sb, a->S, a->d, es);
+  int vec = operand_vec(p.q, a->S, a->d, es);
   if (a->T > 0) {
-    const int vk = operand_vec(a->k, &a->k_sb, a->T, a->d, es), vv = operand_vec(a->v, &a->v_sb, a->T, a->d, es);
+    const int vk = operand_vec(p.k, a->T, a->d, es), vv = operand_vec(p.v, a->T, a->d, es);
     vec = vk < vec ? vk : vec;
     vec = vv < vec ? vv : vec;
   }
@@ -144,9 +148,9 @@ extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size
   if (!aligned(workspace, 4)) return AMOE_EALIGN;
   AttnParams p{};
   fill(p, a);
-  p.go = {a->go, a->go_sb, a->go_ss, a->go_sh};
+  p.go = operand(a->go, &a->go_sb, a->B, a->S, a->H);
   if (a->S > 0) {
-    const int vg = operand_vec(a->go, &a->go_sb, a->S, a->d, es);
+    const int vg = operand_vec(p.go, a->S, a->d, es);
     p.vec = vg < p.vec ? vg : p.vec;
   }
   const bool whole = aligned(a->out, 16) && aligned(a->rest, 16) && aligned(a->dq, 16) && aligned(a->dk, 16) && aligned(a->dv, 16);

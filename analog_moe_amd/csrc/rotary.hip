@@ -136,14 +136,19 @@ extern "C" int amoe_rotary(const amoe_rotary_args* a, void* stream) {
     const int64_t* is = i ? &a->k_sb : &a->q_sb;
     const int64_t* os = i ? &a->k_out_sb : &a->q_out_sb;
     const int64_t heads = i ? a->k_heads : a->q_heads;
-    p.part[i] = {in, out, is[0], is[1], is[2], os[0], os[1], os[2], (int)heads};
+    const int64_t size[3] = {a->B, a->S, heads};
+    int64_t st[2][3];
+    p.part[i].heads = (int)heads;
     if (!heads) continue;
     if (!aligned(in, es) || !aligned(out, es)) return AMOE_EALIGN;
     vec = vec && aligned(in, 16) && aligned(out, 16);
     for (int j = 0; j < 3; j++) {
       if (is[j] < 0 || os[j] < 0) return AMOE_EINVAL;
-      vec = vec && is[j] % c == 0 && os[j] % c == 0;
+      st[0][j] = size[j] == 1 ? 0 : is[j];
+      st[1][j] = size[j] == 1 ? 0 : os[j];
+      vec = vec && st[0][j] % c == 0 && st[1][j] % c == 0;
     }
+    p.part[i] = {in, out, st[0][0], st[0][1], st[0][2], st[1][0], st[1][1], st[1][2], (int)heads};
   }
   p.turns = a->turns;
   p.pos = a->positions; p.pos_sb = a->pos_sb; p.pos_ss = a->pos_ss; p.pos_start = a->start; p.pos_i64 = (int)a->positions_are_i64;
@@ -158,6 +163,7 @@ extern "C" int amoe_rotary(const amoe_rotary_args* a, void* stream) {
   if (n > spread) n = spread;
   if (n > most) n = most;
   p.tokens_per_group = (int)(n < 1 ? 1 : n);
+  if (p.tokens / p.tokens_per_group >= INT64_C(1) << 23) return AMOE_EUNSUPPORTED;      // (threads of a launch are counted in 32 bits)
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a->dtype == AMOE_F32   ? launch_rotary<float>(p, vec, st)
          : a->dtype == AMOE_F16 ? launch_rotary<f16_t>(p, vec, st)

@@ -455,7 +455,7 @@ size_t amoe_ffn_args_bytes(void);
  * amoe_rotary turns the first R elements of every head of q [B, S, q_heads, d] and k [B, S, k_heads, d] by their token's
  * position: pair i = (i, i + R / 2), or (2i, 2i + 1) with `interleaved`, by positions * turns[i] / 2^64 revolutions, times
  * `size`; elements R .. d - 1 are copied.  `inverse` turns the other way, which is the gradient.  Last strides are 1; outputs
- * may be the inputs themselves, or views of a cache.  q_heads or k_heads may be 0. */
+ * may be views of a cache, or the inputs themselves element for element (no other overlap).  q_heads or k_heads may be 0. */
 typedef struct amoe_rotary_args {
   int64_t dtype, B, S, q_heads, k_heads, d, R, interleaved, inverse;
   double size;
@@ -473,7 +473,8 @@ size_t amoe_rotary_args_bytes(void);
 /* out = softmax(scale * q k^T + mask) v for q [B, S, H, d] and k, v [B, T, G, d], H a multiple of G: head h reads key head
  * h / (H / G).  Sequence b holds the keys [0, lengths[b]) (NULL: T; values outside [0, T] are taken as the nearer end); keys
  * behind them are not read.  With `causal` query i stands at position starts[b] + i (NULL: T - S + i) and sees the keys up to
- * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; last strides are 1.
+ * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; H / G * S <= 2^30; fewer than 2^23 blocks of 128 queries and of 64 keys over all heads
+ * and sequences (AMOE_EUNSUPPORTED otherwise); last strides are 1.
  * Few rows over many keys are worked on in parts of the key axis, whose results pass through the workspace.
  * The backward call recomputes the probabilities from lse (log2 of a row's sum, made by the forward call; NULL there: not
  * wanted) and reads out and, unless it is NULL, rest: the sums of out times its gradient are then as good as those of an output

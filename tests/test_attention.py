@@ -160,6 +160,22 @@ def test_marks_outside_the_tensors(emu_ops):
     assert not A.attention_forward(q, k, v, None, marks([-big, -4], torch.int64))[0].any()
 
 
+def test_no_sequences_no_queries(emu_ops):
+    for B, S, T in ((0, 3, 4), (2, 0, 5), (0, 0, 0)):
+        q, k, v, go = inputs(B, S, T, 2, 1, 32, "bf16")
+        left = A.attention_forward(q, k, v, want_lse=True)
+        dq, dk, dv = A.attention_backward(go, q, k, v, *left)
+        assert left[0].shape == q.shape == dq.shape and dk.shape == k.shape and not dk.any() and not dv.any()
+
+
+def test_strides_of_single_elements(emu_ops):
+    """How far apart the only sequence, token or head is from the next says nothing."""
+    q, k, v, go = inputs(1, 1, 40, 1, 1, 64, "bf16")
+    want = A.attention_forward(q, k, v)[0]
+    odd = lambda t, st: torch.empty(0, dtype=t.dtype).set_(t.contiguous().untyped_storage(), 0, t.shape, st)          # noqa: E731
+    assert torch.equal(A.attention_forward(odd(q, (7, 3, 1, 1)), odd(k, (5, 64, 3, 1)), odd(v, (1, 64, 9, 1)))[0], want)
+
+
 def test_fp16_gradients_of_any_size(emu_ops):
     """The score gradients of fp16 tensors are held at a scale of their own: small and large gradients keep their accuracy."""
     for gain in (2.0 ** -9, 1.0, 2.0 ** 9):
@@ -206,7 +222,7 @@ def test_library_refuses_what_it_cannot_address(emu_ops):
     assert fwd(_9=0) == fwd(_13=0) == fwd(_17=0) == fwd(_25=0) == -2
     assert fwd(_4=3, _5=2) == -3
     assert fwd(_9=good[9] + 2) == fwd(_21=good[9] + 2) == fwd(_26=good[26] + 1) == -4
-    assert fwd(_6=129) == fwd(_2=2 ** 28 + 1) == fwd(_1=2 ** 31, _4=2 ** 20) == -6
+    assert fwd(_6=129) == fwd(_2=2 ** 28 + 1) == fwd(_1=2 ** 31, _4=2 ** 20) == fwd(_1=2 ** 22, _2=1000) == -6
     assert lib.amoe_attention_bwd(_abi.ATTN_ARGS.pack(*good), None, 0, None) == -2
     assert lib.amoe_attention_bwd(_abi.ATTN_ARGS.pack(*good), lse.data_ptr(), 4, None) == -5
     assert lib.amoe_attention_fwd(None, None, 0, None) == -2
@@ -230,6 +246,19 @@ def test_autograd(emu_ops):
         (g.sum() + q.sum()).backward()
     with torch.no_grad():
         assert torch.equal(A.attention(q, k, v), A.attention_forward(q, k, v)[0])
+
+
+def test_watched_calls(emu_ops):
+    """Forward-mode derivatives and function transforms are refused, a trace computes anew (as for the expert layer)."""
+    from torch.autograd import forward_ad
+    q, k, v, _ = inputs(1, 4, 4, 1, 1, 16, "f32")
+    with torch.no_grad(), forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        A.attention(forward_ad.make_dual(q, q), k, v)
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: A.attention(x, k, v))(q[None])
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda x: A.attention(x, k, v), (q,), check_trace=False)
+        assert torch.equal(traced(k), A.attention(k, k, v))
 
 
 def test_gradients_are_differences(emu_ops):

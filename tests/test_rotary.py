@@ -151,6 +151,16 @@ def test_gradient(emu_ops):
         r(q, k, out=(torch.empty_like(q), torch.empty_like(k)))
 
 
+def test_watched_calls(emu_ops):
+    from torch.autograd import forward_ad
+    q, k = inputs(1, 4, 1, 1, 16, "f32")
+    r = R.Rotary(16)
+    with torch.no_grad(), forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        r(forward_ad.make_dual(q, q), k)
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: r(x, k)[0])(q[None])
+
+
 def test_refusals(emu_ops):
     for bad in (dict(dim=0), dict(dim=3), dict(dim=2050), dict(dim=8, base=0.5), dict(dim=8, factor=0.5), dict(dim=8, base=float("inf")),
                 dict(dim=8, scaling="other"), dict(dim=8, scaling="parts"), dict(dim=8, factor=float("nan"))):
@@ -188,7 +198,7 @@ def test_library_refuses(emu_ops):
     assert call(_0=5) == call(_1=-1) == call(_6=7) == call(_6=10) == call(_6=0) == call(_17=-1) == -1
     assert call(_10=0) == call(_16=0) == call(_28=0) == -2
     assert call(_10=t.data_ptr() + 4) == call(_16=x.data_ptr() + 2) == call(_11=t.data_ptr() + 1) == -4
-    assert call(_5=4096, _6=4096) == call(_1=2 ** 30, _2=2 ** 20) == -6
+    assert call(_5=4096, _6=4096) == call(_1=2 ** 30, _2=2 ** 20) == call(_1=2 ** 30, _3=256) == -6
     assert lib.amoe_rotary(None, None) == -2
 
 
