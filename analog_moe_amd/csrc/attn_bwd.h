@@ -62,10 +62,10 @@ template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, 
 __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd_q_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
   constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
-  constexpr int kElems = BN * DP, kTileBytes = 4 * kElems * (int)sizeof(T), kJoinBytes = (KG - 1) * RW * DP * 32 * 4;
-  __shared__ __align__(1024) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
-  T* const lds_k = reinterpret_cast<T*>(lds);
-  T* const lds_v = lds_k + 2 * kElems;
+  constexpr int kElems = BN * DP, kTilesBytes = 2 * kElems * (int)sizeof(T);
+  static_assert((KG - 1) * RW * DP * 32 * 4 <= kTilesBytes, "the copies are joined in the keys' tiles");
+  __shared__ __align__(1024) char lds_k[kTilesBytes], lds_v[kTilesBytes];
+  T *const tk = reinterpret_cast<T*>(lds_k), *const tv = reinterpret_cast<T*>(lds_v);
   const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5;
   const AttnRowsOf w = attn_rows_of<Shape>(p);
 
@@ -77,8 +77,8 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
   typename Tile::Lane at;
   const int n_tiles = (w.group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, lds_k, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
-    sv.load(tid, lds_v, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
+    sk.load(tid, tk, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
+    sv.load(tid, tv, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK], go[NK];
   const bool real = w.i < p.S;
@@ -112,28 +112,27 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
   AttnGrad<T, DP> dq;
   dq.clear();
   if (n_tiles > 0) {
-    sk.store(tid, lds_k);
-    sv.store(tid, lds_v);
+    sk.store(tid, tk);
+    sv.store(tid, tv);
   }
   for (int t = 0; t < n_tiles; t++) {
     const int cur = (t & 1) * kElems, next = kElems - cur;
     sk.finish();
     __syncthreads();
     if (t + 1 < n_tiles) {
-      sk.load(tid, lds_k + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
-      sv.load(tid, lds_v + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sk.load(tid, tk + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sv.load(tid, tv + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
     }
     const int key0 = t * BN + 32 * NB * w.kg;
     if (key0 < w.wave_sees) {
-      const T *kt = lds_k + cur + 32 * NB * w.kg * DP, *vt = lds_v + cur + 32 * NB * w.kg * DP;
+      const typename Tile::Lane in = at.in(cur + 32 * NB * w.kg * DP);
       const bool mask = key0 + 32 * NB > w.wave_all;
       // per 32 keys: 2 * NK products for the scores and dP by turns, 2 * DP / 32 with dS
       constexpr int NU = DP / 32, NS = 2 * NK, NF = NS + 2 * NU;
       const auto load = [&](int x) -> attn_frag<T> {
         const int n = x / NF, e = x % NF;
-        return e < NS ? Tile::row_frag(e & 1 ? vt : kt, at, 32 * n, e / 2) : Tile::col_frag(kt, at, 32 * n + 16 * ((e - NS) / NU), (e - NS) % NU);
+        return e < NS ? Tile::row_frag(e & 1 ? lds_v : lds_k, in, 32 * n, e / 2) : Tile::col_frag(lds_k, in, 32 * n + 16 * ((e - NS) / NU), (e - NS) % NU);
       };
-      at.hide();
       AttnRun<T, NB * NF, sizeof(T) == 2 && DP == 128 ? 4 : kAttnAhead<T>> run;      // (more do not fit the registers)
       run.begin(load);
 #pragma unroll
@@ -162,14 +161,14 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
       }
     }
     if (t + 1 < n_tiles) {
-      sk.store(tid, lds_k + next);
-      sv.store(tid, lds_v + next);
+      sk.store(tid, tk + next);
+      sv.store(tid, tv + next);
     }
   }
   float factor = p.scale / dq.scale;
   if constexpr (KG > 1) {
     __syncthreads();
-    f32x4* join = reinterpret_cast<f32x4*>(lds);
+    f32x4* join = reinterpret_cast<f32x4*>(lds_k);
     if (w.kg > 0) attn_put_acc<DP>(join, (w.kg - 1) * RW + w.rw, dq.acc, factor);
     __syncthreads();
     if (w.kg == 0) {
@@ -201,11 +200,13 @@ template <typename T, int DP, bool EDGE, int QW_, class Shape = AttnKvShape<T, D
 __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void attn_bwd_kv_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
   constexpr int KW = Shape::KW, QW = Shape::QW, NT = Shape::kThreads, BM = 32 * QW, NK = DP / 16, NU = DP / 32;
-  constexpr int kTileElems = BM * DP, kTileBytes = 4 * kTileElems * (int)sizeof(T), kSumBytes = KW * (QW - 1) * NU * 16 * 64 * 4;
-  __shared__ __align__(1024) char lds[kTileBytes > kSumBytes ? kTileBytes : kSumBytes];
-  __shared__ __align__(1024) T lds_v[Shape::kVInLds ? 32 * KW * DP : 8];
+  constexpr int kTileElems = BM * DP, kTilesBytes = 2 * kTileElems * (int)sizeof(T);
+  constexpr int kSumsPer = kTilesBytes / (NU * 16 * 64 * 4);       // accumulators that fit a pair of tiles
+  static_assert(KW * (QW - 1) <= 2 * kSumsPer, "the copies' sums fit the tiles' room");
+  __shared__ __align__(1024) char lds_q[kTilesBytes], lds_g[kTilesBytes];
+  __shared__ __align__(1024) char lds_v[Shape::kVInLds ? 32 * KW * DP * (int)sizeof(T) : 16];
   __shared__ __align__(16) float lds_lse[2][BM], lds_delta[2][BM];
-  T* const lds_t = reinterpret_cast<T*>(lds);       // q by turns, then the output's gradient
+  T *const tq = reinterpret_cast<T*>(lds_q), *const tg = reinterpret_cast<T*>(lds_g);
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), kw = wave % KW, qw = wave / KW, h = lane >> 5;
   const int BG = p.B * p.G, bg = (int)(blockIdx.x % (unsigned)BG), tile = (int)(blockIdx.x / (unsigned)BG);
   const int b = bg / p.G, g = bg - b * p.G;
@@ -224,8 +225,8 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   float stat = 0.f;                                   // threads 0 .. BM - 1: lse, the next BM: delta
   const auto fetch = [&](int t) {
     const int hd = g * p.R + t / per_head, q0 = (tile0 + t % per_head) * BM, buf = t & 1;
-    sq.load(tid, lds_t + buf * kTileElems, static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh, p.q.ss, q0, p.S, p.d, p.vec);
-    sg.load(tid, lds_t + (2 + buf) * kTileElems, static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh, p.go.ss, q0, p.S, p.d, p.vec);
+    sq.load(tid, tq + buf * kTileElems, static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh, p.q.ss, q0, p.S, p.d, p.vec);
+    sg.load(tid, tg + buf * kTileElems, static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh, p.go.ss, q0, p.S, p.d, p.vec);
     if (tid < 2 * BM) {
       const int qi = q0 + (tid < BM ? tid : tid - BM);
       const int64_t row = ((int64_t)b * p.H + hd) * p.S + qi;
@@ -233,8 +234,8 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
     }
   };
   const auto put = [&](int buf) {
-    sq.store(tid, lds_t + buf * kTileElems);
-    sg.store(tid, lds_t + (2 + buf) * kTileElems);
+    sq.store(tid, tq + buf * kTileElems);
+    sg.store(tid, tg + buf * kTileElems);
     if (tid < BM) lds_lse[buf][tid] = stat;
     else if (tid < 2 * BM) lds_delta[buf][tid - BM] = stat;
   };
@@ -246,7 +247,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   if constexpr (Shape::kVInLds) {
     AttnStage<T, DP, 32 * KW, NT, EDGE> sv;
     sv.init(tid, p.v.ss, p.d);
-    sv.load(tid, lds_v, static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, group0 < length ? group0 : 0,
+    sv.load(tid, reinterpret_cast<T*>(lds_v), static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, group0 < length ? group0 : 0,
             group0 < length ? length : 0, p.d, p.vec);
   }
   AttnGrad<T, DP> dk, dv;
@@ -261,17 +262,16 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
     if (t + 1 < n_tiles) fetch(t + 1);
     // the wave's keys are seen by some query of its block, and whether by every one
     if (w0 < length && q0 < p.S && (!p.causal || start + q0 + 32 > w0)) {
-      const T *qt = lds_t + buf * kTileElems + 32 * qw * DP, *gt = lds_t + (2 + buf) * kTileElems + 32 * qw * DP;
+      const typename Tile::Lane in = at.in(buf * kTileElems + 32 * qw * DP);
       const bool mask = w0 + 32 > length || (p.causal && start + q0 < w0 + 31);
       // 2 * NK products for the scores and dP by turns, 4 * DP / 32 with P and dS by turns
       constexpr int kPer = Shape::kVInLds ? 3 : 2, NS = kPer * NK, NF = NS + 4 * NU;      // operands a score product and a dP product read
       const auto load = [&](int e) -> attn_frag<T> {
-        if (e < NS) return e % kPer == 2 ? Tile::row_frag(lds_v, at, 32 * kw, e / kPer) : Tile::row_frag(e % kPer ? gt : qt, at, 0, e / kPer);
+        if (e < NS) return e % kPer == 2 ? Tile::row_frag(lds_v, at, 32 * kw, e / kPer) : Tile::row_frag(e % kPer ? lds_g : lds_q, in, 0, e / kPer);
         const int r = e - NS;
-        return Tile::col_frag(r & 1 ? qt : gt, at, 16 * (r / (2 * NU)), r / 2 % NU);
+        return Tile::col_frag(r & 1 ? lds_q : lds_g, in, 16 * (r / (2 * NU)), r / 2 % NU);
       };
-      at.hide();
-      AttnRun<T, NF, sizeof(T) == 2 && DP == 128 ? 4 : kAttnAhead<T>> run;      // (more do not fit the registers)
+      AttnRun<T, NF, sizeof(T) == 2 && DP == 128 ? 3 : kAttnAhead<T>> run;      // (more do not fit the registers)
       run.begin(load);
       f32x16 s = f32x16_zero(), dp = f32x16_zero();
       attn_frag<T> gf;
@@ -314,13 +314,13 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   // the copies' sums, in the layout of the registers: dv, then dk
   constexpr float kUnshift = kIsF16<T> ? 0x1p-15f : 1.f;
   const int64_t row = (((int64_t)b * p.T + key) * p.G + g) * p.d;
-  f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+  const auto sums = [&](int slot) { return reinterpret_cast<f32x4*>(slot < kSumsPer ? lds_q : lds_g); };
 #pragma unroll
   for (int which = 0; which < 2; which++) {
     f32x16(&acc)[NU] = which ? dk.acc : dv.acc;
     const float factor = which ? p.scale * kUnshift / dk.scale : kUnshift;
     __syncthreads();
-    if (qw > 0) attn_put_acc<DP>(sums, (qw - 1) * KW + kw, acc, factor);
+    if (qw > 0) attn_put_acc<DP>(sums((qw - 1) * KW + kw), ((qw - 1) * KW + kw) % kSumsPer, acc, factor);
     __syncthreads();
     if (qw == 0) {
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[t][e] *= factor;
 #pragma unroll
-      for (int c = 0; c < QW - 1; c++) attn_add_acc<DP>(sums, c * KW + kw, acc, 1.f);
+      for (int c = 0; c < QW - 1; c++) attn_add_acc<DP>(sums(c * KW + kw), (c * KW + kw) % kSumsPer, acc, 1.f);
       attn_store_col<T, DP, EDGE>(static_cast<T*>(which ? p.dk : p.dv) + row, acc, 1.f, p.d, key < p.T);
     }
   }

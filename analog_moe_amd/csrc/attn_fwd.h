@@ -140,11 +140,12 @@ template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, 
 __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd_rows_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
   constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
-  constexpr int kElems = BN * DP, kTileBytes = 4 * kElems * (int)sizeof(T), kJoinBytes = (KG - 1) * RW * DP * 32 * 4;
-  __shared__ __align__(1024) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
+  constexpr int kElems = BN * DP, kTilesBytes = 2 * kElems * (int)sizeof(T);
+  static_assert((KG - 1) * RW * DP * 32 * 4 <= kTilesBytes, "the copies are joined in the keys' tiles");
+  // (arrays of their own for keys and values also where one would do: see AttnTile's reads)
+  __shared__ __align__(1024) char lds_k[kTilesBytes], lds_v[kTilesBytes];
   __shared__ float lds_ml[KG][RW][2][64];
-  T* const lds_k = reinterpret_cast<T*>(lds);
-  T* const lds_v = lds_k + 2 * kElems;
+  T *const tk = reinterpret_cast<T*>(lds_k), *const tv = reinterpret_cast<T*>(lds_v);
   const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5;
   const AttnRowsOf w = attn_rows_of<Shape>(p);
 
@@ -156,8 +157,8 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
   typename Tile::Lane at;
   const int n_tiles = (w.group_sees + BN - 1) / BN;
   if (n_tiles > 0) {
-    sk.load(tid, lds_k, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
-    sv.load(tid, lds_v, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
+    sk.load(tid, tk, kb, p.k.ss, 0, w.group_sees, p.d, p.vec);
+    sv.load(tid, tv, vb, p.v.ss, 0, w.group_sees, p.d, p.vec);
   }
   attn_frag<T> q[NK];
   attn_row_frags<T, DP, EDGE>(q, static_cast<const T*>(p.q.p) + w.b * p.q.sb + w.hd * p.q.sh, p.q.ss, w.w0, p.S, p.d, p.vec);
@@ -165,26 +166,25 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
   AttnState<T, DP> st;
   st.clear();
   if (n_tiles > 0) {
-    sk.store(tid, lds_k);
-    sv.store(tid, lds_v);
+    sk.store(tid, tk);
+    sv.store(tid, tv);
   }
   for (int t = 0; t < n_tiles; t++) {
     const int cur = (t & 1) * kElems, next = kElems - cur;
     sk.finish();
     __syncthreads();       // tile t is there, and nobody reads the other one any more
     if (t + 1 < n_tiles) {
-      sk.load(tid, lds_k + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
-      sv.load(tid, lds_v + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sk.load(tid, tk + next, kb, p.k.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
+      sv.load(tid, tv + next, vb, p.v.ss, (t + 1) * BN, w.group_sees, p.d, p.vec);
     }
     const int key0 = t * BN + 32 * NB * w.kg;
     if (key0 < w.wave_sees) {
       // NB * NK products for the scores, 2 * NB * DP / 32 with the probabilities
       constexpr int NS = NB * NK, NU = DP / 32;
-      const T *kt = lds_k + cur + 32 * NB * w.kg * DP, *vt = lds_v + cur + 32 * NB * w.kg * DP;
+      const typename Tile::Lane in = at.in(cur + 32 * NB * w.kg * DP);
       const auto load = [&](int e) -> attn_frag<T> {
-        return e < NS ? Tile::row_frag(kt, at, 32 * (e % NB), e / NB) : Tile::col_frag(vt, at, 16 * ((e - NS) / NU), (e - NS) % NU);
+        return e < NS ? Tile::row_frag(lds_k, in, 32 * (e % NB), e / NB) : Tile::col_frag(lds_v, in, 16 * ((e - NS) / NU), (e - NS) % NU);
       };
-      at.hide();
       AttnRun<T, NS + 2 * NB * NU> run;
       run.begin(load);
       f32x16 s[NB];
@@ -197,15 +197,15 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
                 [&](int e, const attn_frag<T>& a) { st.o[(e - NS) % NU] = attn_mma<T>(a, pr[(e - NS) / NU], st.o[(e - NS) % NU]); });
     }
     if (t + 1 < n_tiles) {
-      sk.store(tid, lds_k + next);
-      sv.store(tid, lds_v + next);
+      sk.store(tid, tk + next);
+      sv.store(tid, tv + next);
     }
   }
   float l = attn_pair_sum(st.l);
   if constexpr (KG > 1) {
     // the copies in units of the largest maximum; the first one takes the sums
     __syncthreads();
-    f32x4* join = reinterpret_cast<f32x4*>(lds);
+    f32x4* join = reinterpret_cast<f32x4*>(lds_k);
     lds_ml[w.kg][w.rw][0][lane] = st.m;
     lds_ml[w.kg][w.rw][1][lane] = l;
     if (w.kg > 0) attn_put_acc<DP>(join, (w.kg - 1) * RW + w.rw, st.o, 1.f);
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
   AttnStage<T, DP, 32, 64, EDGE, true> sv;
   sv.init(lane, p.v.ss, p.d);
-  typename Tile::Lane at;
+  const typename Tile::Lane at = typename Tile::Lane().in(wave * 32 * DP);
   const auto fetch = [&](int key0) {
     attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, key0, key_hi, p.d, p.vec);
     sv.load(lane, nullptr, vb, p.v.ss, key0, key_hi, p.d, p.vec);
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-      for (int u = 0; u < DP / 32; u++) st.o[u] = attn_mma<T>(Tile::col_frag(tile, at, 16 * w, u), pr[w], st.o[u]);
+      for (int u = 0; u < DP / 32; u++) st.o[u] = attn_mma<T>(Tile::col_frag(lds, at, 16 * w, u), pr[w], st.o[u]);
   }
 
   // the four waves' rows in units of the largest maximum

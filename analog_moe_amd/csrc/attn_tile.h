@@ -111,51 +111,59 @@ template <typename T, int DP> struct AttnTile {
 
   // Byte offsets of a lane's reads in a tile, but for what a constant of the read adds or flips: the swizzle only sees the
   // low four bits of a row, and rows start on a power of two or 64 bytes, so that steps along the head are flipped bits.  (Kept
-  // apart they would be 16 registers; a loop makes them anew by hide().)
+  // apart they would be 16 registers: in() makes them anew for every tile.)
   struct Lane {
-    int row, col;
+    int row, col, first = 0;
     __device__ __forceinline__ Lane() {
       const int l = lane_id(), h = l >> 5;
       row = at(l & 31, h) * (int)sizeof(T);
       const int r = 4 * h + ((l & 15) >> 2), d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
       col = (at(r, d / 8) + d % 8) * (int)sizeof(T);
     }
-    __device__ __forceinline__ void hide() {
-      opaque(row);
-      opaque(col);
+    // in the tile that begins at this element (a multiple of 256 bytes: no bit of it is flipped)
+    __device__ __forceinline__ Lane in(int tile) const {
+      Lane l = *this;
+      l.row += tile * (int)sizeof(T);
+      l.col += tile * (int)sizeof(T);
+      l.first += tile;
+      opaque(l.row);
+      opaque(l.col);
+      return l;
     }
   };
   static constexpr int kRowBytes = DP * (int)sizeof(T);
   static constexpr bool kPow2 = kRowWords % 32 == 0;
 
+  // Addresses are summed up before they meet the array of LDS that the tile lies in, and a kernel has more than one such array: the
+  // compiler then knows which array a read is of, and does not make it wait for the tiles on their way into LDS.
+  //
   // steps 16 * kk .. + 15 of the head axis, rows r0 + l % 32 (r0 a multiple of 16, as below)
-  static __device__ __forceinline__ attn_frag<T> row_frag(const T* tile, const Lane& lane, int r0, int kk) {
+  static __device__ __forceinline__ attn_frag<T> row_frag(const char* lds, const Lane& lane, int r0, int kk) {
     if constexpr (sizeof(T) == 4) {
       const int l = lane_id(), r = r0 + (l & 31), h = l >> 5;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h));
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + at(r, 4 * kk + 2 * h + 1));
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(lds + 4 * (lane.first + at(r, 4 * kk + 2 * h)));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(lds + 4 * (lane.first + at(r, 4 * kk + 2 * h + 1)));
       return F32x8{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
     } else {
-      const char* p = reinterpret_cast<const char*>(tile) + r0 * kRowBytes;
-      if constexpr (kPow2) return *reinterpret_cast<const u32x4*>(p + (lane.row ^ (kk << 5)));
-      else return *reinterpret_cast<const u32x4*>(p + (lane.row ^ ((kk & 1) << 5)) + (kk >> 1) * 64);
+      const int o = kPow2 ? lane.row ^ (kk << 5) : (lane.row ^ ((kk & 1) << 5)) + (kk >> 1) * 64;
+      return *reinterpret_cast<const u32x4*>(lds + (r0 * kRowBytes + o));
     }
   }
   // rows r0 .. r0 + 15 as the steps, in the order of a score block's registers, of head elements 32 * dt + l % 32
-  static __device__ __forceinline__ attn_frag<T> col_frag(const T* tile, const Lane& lane, int r0, int dt) {
+  static __device__ __forceinline__ attn_frag<T> col_frag(const char* lds, const Lane& lane, int r0, int dt) {
     if constexpr (sizeof(T) == 4) {
       const int l = lane_id(), h = l >> 5, d = 32 * dt + (l & 31);
       F32x8 f;
 #pragma unroll
-      for (int j = 0; j < 8; j++) f.v[j] = tile[at(r0 + 8 * (j / 4) + 4 * h + j % 4, d / 4) + d % 4];
+      for (int j = 0; j < 8; j++)
+        f.v[j] = *reinterpret_cast<const float*>(lds + 4 * (lane.first + at(r0 + 8 * (j / 4) + 4 * h + j % 4, d / 4) + d % 4));
       return f;
     } else {
-      const char* p = reinterpret_cast<const char*>(tile) + r0 * kRowBytes;
       u32x2 half[2];
 #pragma unroll
       for (int u = 0; u < 2; u++) {                        // rows 4 h .. + 3, and the same 8 on
         const int o = kPow2 ? lane.col ^ (dt << 6) ^ (u << 5) : (lane.col ^ (u << 5)) + dt * 64;
-        half[u] = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(p + o + 8 * u * kRowBytes));
+        half[u] = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(lds + (r0 * kRowBytes + o + 8 * u * kRowBytes)));
       }
       return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
     }

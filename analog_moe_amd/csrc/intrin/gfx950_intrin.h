@@ -75,9 +75,13 @@ __device__ __forceinline__ u32x2 buffer_load_b64(BufRsrc r, uint32_t lane_off, u
   return __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, uniform_off, 0);
 }
 // 16 bytes per lane from memory straight to LDS, lane l's to lds + 16 * l (lds the same for the whole wave); zeros for lanes out
-// of range.  They are there after lds_dma_wait() and, for other waves, the barrier behind it.
+// of range.  They are there after lds_dma_wait() and, for other waves, the barrier behind it; the compiler is not told which
+// array they go to, or it would have every read of that array wait for them.
 __device__ __forceinline__ void buffer_to_lds_b128(BufRsrc r, void* lds, uint32_t lane_off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, lane_off, 0, 0, 0);
+  typedef __attribute__((address_space(3))) void* LdsPtr;
+  uint32_t to = (uint32_t)(uintptr_t)(LdsPtr)lds;
+  asm volatile("" : "+s"(to));
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(uintptr_t)to, 16, lane_off, 0, 0, 0);
 }
 __device__ __forceinline__ void lds_dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
 // Resource over [base, base + bytes): an access at a byte offset >= bytes is out of range; out-of-range stores are
