@@ -55,49 +55,80 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
   const int pair_units = p.interleaved ? (V == 1 ? half : p.R / V) : half / V;
   const int units = pair_units + (p.d - p.R) / V, heads = p.part[0].heads + p.part[1].heads;
   const int per_token = units * heads;
-  for (int j = tid; j < tokens * per_token; j += 256) {
+  struct Item {
+    T* out;
+    const float *cs, *sn;
+    int u;
+    Raw a, c;
+    float x, y;
+  };
+  const auto fetch = [&](int j, Item& it) {
     const int t = j / per_token, hu = j - t * per_token, hd = hu / units, u = hu - hd * units;
     const int64_t token = token0 + t, b = token / p.S, s = token - b * p.S;
     const RotaryPart& part = p.part[hd < p.part[0].heads ? 0 : 1];
     const int head = hd < p.part[0].heads ? hd : hd - p.part[0].heads;
     const T* in = static_cast<const T*>(part.in) + b * part.in_sb + s * part.in_ss + head * part.in_sh;
-    T* out = static_cast<T*>(part.out) + b * part.out_sb + s * part.out_ss + head * part.out_sh;
-    const float *cs = lds_cos + t * half, *sn = lds_sin + t * half;
+    it.out = static_cast<T*>(part.out) + b * part.out_sb + s * part.out_ss + head * part.out_sh;
+    it.cs = lds_cos + t * half;
+    it.sn = lds_sin + t * half;
+    it.u = u;
+    if constexpr (V == 1) {
+      const int ea = u >= pair_units ? p.R + u - pair_units : p.interleaved ? 2 * u : u;
+      it.x = Elem<T>::load(in + ea);
+      it.y = u >= pair_units ? 0.f : Elem<T>::load(in + (p.interleaved ? 2 * u + 1 : u + half));
+    } else {
+      const int e = u >= pair_units ? p.R + (u - pair_units) * V : u * V;
+      it.a = *reinterpret_cast<const Raw*>(in + e);
+      if (u < pair_units && !p.interleaved) it.c = *reinterpret_cast<const Raw*>(in + half + e);
+    }
+  };
+  const auto finish = [&](const Item& it) {
+    const int u = it.u;
+    T* out = it.out;
     if constexpr (V == 1) {
       if (u >= pair_units) {
-        out[p.R + u - pair_units] = in[p.R + u - pair_units];
-        continue;
+        out[p.R + u - pair_units] = Elem<T>::cvt(it.x);
+        return;
       }
-      const int ea = p.interleaved ? 2 * u : u, eb = p.interleaved ? 2 * u + 1 : u + half;
-      const float a = Elem<T>::load(in + ea), c = Elem<T>::load(in + eb);
-      out[ea] = Elem<T>::cvt(a * cs[u] - c * sn[u]);
-      out[eb] = Elem<T>::cvt(c * cs[u] + a * sn[u]);
+      out[p.interleaved ? 2 * u : u] = Elem<T>::cvt(it.x * it.cs[u] - it.y * it.sn[u]);
+      out[p.interleaved ? 2 * u + 1 : u + half] = Elem<T>::cvt(it.y * it.cs[u] + it.x * it.sn[u]);
     } else if (u >= pair_units) {
-      const int e = p.R + (u - pair_units) * V;
-      *reinterpret_cast<Raw*>(out + e) = *reinterpret_cast<const Raw*>(in + e);
+      *reinterpret_cast<Raw*>(out + p.R + (u - pair_units) * V) = it.a;
     } else if (p.interleaved) {
       float v[V];
-      raw_unpack<T>(*reinterpret_cast<const Raw*>(in + u * V), v);
+      raw_unpack<T>(it.a, v);
 #pragma unroll
       for (int i = 0; i < V / 2; i++) {
-        const float a = v[2 * i], c = v[2 * i + 1], x = cs[u * (V / 2) + i], y = sn[u * (V / 2) + i];
+        const float a = v[2 * i], c = v[2 * i + 1], x = it.cs[u * (V / 2) + i], y = it.sn[u * (V / 2) + i];
         v[2 * i] = a * x - c * y;
         v[2 * i + 1] = c * x + a * y;
       }
       *reinterpret_cast<Raw*>(out + u * V) = raw_pack<T>(v);
     } else {
       float a[V], c[V];
-      raw_unpack<T>(*reinterpret_cast<const Raw*>(in + u * V), a);
-      raw_unpack<T>(*reinterpret_cast<const Raw*>(in + half + u * V), c);
+      raw_unpack<T>(it.a, a);
+      raw_unpack<T>(it.c, c);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float x = cs[u * V + i], y = sn[u * V + i], first = a[i];
+        const float x = it.cs[u * V + i], y = it.sn[u * V + i], first = a[i];
         a[i] = first * x - c[i] * y;
         c[i] = c[i] * x + first * y;
       }
       *reinterpret_cast<Raw*>(out + u * V) = raw_pack<T>(a);
       *reinterpret_cast<Raw*>(out + half + u * V) = raw_pack<T>(c);
     }
+  };
+  // (units are read and written by one thread each, so that outputs may be the inputs; four are on their way at once)
+  constexpr int kAhead = 4;
+  const int n = tokens * per_token;
+  for (int j0 = tid; j0 < n; j0 += kAhead * 256) {
+    Item it[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      if (j0 + k * 256 < n) fetch(j0 + k * 256, it[k]);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      if (j0 + k * 256 < n) finish(it[k]);
   }
 }
 
