@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
       out[p.interleaved ? 2 * u : u] = Elem<T>::cvt(it.x * it.cs[u] - it.y * it.sn[u]);
       out[p.interleaved ? 2 * u + 1 : u + half] = Elem<T>::cvt(it.y * it.cs[u] + it.x * it.sn[u]);
     } else if (u >= pair_units) {
-      *reinterpret_cast<Raw*>(out + p.R + (u - pair_units) * V) = it.a;
+      store_streaming(out + p.R + (u - pair_units) * V, it.a);
     } else if (p.interleaved) {
       float v[V];
       raw_unpack<T>(it.a, v);
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
         v[2 * i] = a * x - c * y;
         v[2 * i + 1] = c * x + a * y;
       }
-      *reinterpret_cast<Raw*>(out + u * V) = raw_pack<T>(v);
+      store_streaming(out + u * V, raw_pack<T>(v));
     } else {
       float a[V], c[V];
       raw_unpack<T>(it.a, a);
@@ -114,8 +114,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
         a[i] = first * x - c[i] * y;
         c[i] = c[i] * x + first * y;
       }
-      *reinterpret_cast<Raw*>(out + u * V) = raw_pack<T>(a);
-      *reinterpret_cast<Raw*>(out + half + u * V) = raw_pack<T>(c);
+      store_streaming(out + u * V, raw_pack<T>(a));
+      store_streaming(out + half + u * V, raw_pack<T>(c));
     }
   };
   // (units are read and written by one thread each, so that outputs may be the inputs; four are on their way at once)
