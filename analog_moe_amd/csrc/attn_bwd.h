@@ -186,20 +186,22 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
   if (w.kg == 0) attn_store_col<T, DP, EDGE>(static_cast<T*>(p.dq) + row * p.d, dq.acc, factor, p.d, real);
 }
 
-// dk, dv: KW waves hold 32 keys each of one key head, k and v as operands in registers, in QW copies; the queries of all heads
+// dk, dv: KW waves hold 32 keys each of one key head, k and v as operands in registers or LDS, in QW copies; the queries of all heads
 // that share them pass in tiles of 32 * QW, 32 for each copy, and the copies' sums are added at the end, in order.  Every wave
 // reads what the other keys' waves read; more copies make shorter loops of the same work where there are few keys, and finer
 // workgroups where causal rows differ in length.  Four products per block; heads of 128 are bound by registers (two waves on a
 // SIMD with every one of them used, and operands no more than three reads ahead), heads of 64 by the vector work.  8192 keys, 16
-// over 4 heads of 128, bf16, causal: 650 us, 850 TFLOP/s; 16 x 1024, 16 heads of 64: 125 to 140 us.  Measured and not kept there: the
-// exponentials between the products of one wave (900 us), two workgroups of four waves on a CU (1000 us), three waves on a SIMD
-// with some registers in memory (heads of 64: 170 us), the queries from the other end (no difference).
+// over 4 heads of 128, bf16, causal: 650 us, 850 TFLOP/s; 16 x 1024, 16 heads of 64: 100 us.  Measured and not kept there: the
+// exponentials between the products of one wave (900 us), two workgroups of four waves on a CU (1000 us), the queries from the other end (no difference).
 template <typename T, int DP, bool EDGE, int QW_> struct AttnKvShape {
   static constexpr int KW = 2, QW = QW_, kThreads = 64 * KW * QW;
-  static constexpr int kWavesPerSimd = sizeof(T) * DP > 256 || EDGE ? 1 : 2;       // fp32 heads past 64: 512 registers a wave
-  // 16-bit heads past 96: dk, dv and k fill the registers, v is read from LDS for every product
-  static constexpr bool kVInLds = sizeof(T) == 2 && DP == 128 && !EDGE;
-  // two copies have room for two workgroups on a CU; four are one
+  // k and v read from LDS for every product, for the registers that makes free.  16-bit heads past 96: v only, with dk, dv and k
+  // the registers are full (both do not fit LDS).  Heads of 64, two copies: both, for a third workgroup on the CU (16 x 1024, 16 heads
+  // of 64, bf16: 123 us with two; with three 100 us, or 115 with k in registers and 4 of them in memory).
+  static constexpr bool kVInLds = sizeof(T) == 2 && !EDGE && (DP == 128 || (DP == 64 && QW == 2)), kKInLds = kVInLds && DP == 64;
+  static constexpr int kWavesPerSimd = sizeof(T) * DP > 256 || EDGE ? 1 : kKInLds ? 3 : 2;       // fp32 heads past 64: 512 registers a wave
+  static constexpr int kAhead = kKInLds ? 4 : kVInLds ? 3 : kAttnAhead<T>;                       // (more do not fit the registers)
+  // two copies have room for two workgroups on a CU or three; four are one
   static constexpr bool kFits = 128 * QW * DP * (int)sizeof(T) <= (QW == 2 && !EDGE && sizeof(T) == 2 ? 48 : 128) << 10;
 };
 template <typename T, int DP, bool EDGE, int QW_, class Shape = AttnKvShape<T, DP, EDGE, QW_>>
@@ -210,7 +212,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   constexpr int kSumsPer = kTilesBytes / (NU * 16 * 64 * 4);       // accumulators that fit a pair of tiles
   static_assert(KW * (QW - 1) <= 2 * kSumsPer, "the copies' sums fit the tiles' room");
   __shared__ __align__(1024) char lds_q[kTilesBytes], lds_g[kTilesBytes];
-  __shared__ __align__(1024) char lds_v[Shape::kVInLds ? 32 * KW * DP * (int)sizeof(T) : 16];
+  __shared__ __align__(1024) char lds_k[Shape::kKInLds ? 32 * KW * DP * (int)sizeof(T) : 16], lds_v[Shape::kVInLds ? 32 * KW * DP * (int)sizeof(T) : 16];
   __shared__ __align__(16) float lds_lse[2][BM], lds_delta[2][BM];
   T *const tq = reinterpret_cast<T*>(lds_q), *const tg = reinterpret_cast<T*>(lds_g);
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), kw = wave % KW, qw = wave / KW, h = lane >> 5;
@@ -247,14 +249,20 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   };
   if (n_tiles > 0) fetch(0);
   attn_frag<T> kf[NK], vf[NK];
-  attn_row_frags<T, DP, EDGE>(kf, static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh, p.k.ss, w0 < length ? w0 : 0, w0 < length ? length : 0, p.d, p.vec);
-  if constexpr (!Shape::kVInLds)
-    attn_row_frags<T, DP, EDGE>(vf, static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, w0 < length ? w0 : 0, w0 < length ? length : 0, p.d, p.vec);
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+  const int wave0 = w0 < length ? w0 : 0, wave_end = w0 < length ? length : 0;
+  if constexpr (!Shape::kKInLds) attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, wave0, wave_end, p.d, p.vec);
+  if constexpr (!Shape::kVInLds) attn_row_frags<T, DP, EDGE>(vf, vb, p.v.ss, wave0, wave_end, p.d, p.vec);
   if constexpr (Shape::kVInLds) {
-    AttnStage<T, DP, 32 * KW, NT, EDGE> sv;
-    sv.init(tid, p.v.ss, p.d);
-    sv.load(tid, reinterpret_cast<T*>(lds_v), static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh, p.v.ss, group0 < length ? group0 : 0,
-            group0 < length ? length : 0, p.d, p.vec);
+    const int all0 = group0 < length ? group0 : 0, all_end = group0 < length ? length : 0;
+    AttnStage<T, DP, 32 * KW, NT, EDGE> st;
+    if constexpr (Shape::kKInLds) {
+      st.init(tid, p.k.ss, p.d);
+      st.load(tid, reinterpret_cast<T*>(lds_k), kb, p.k.ss, all0, all_end, p.d, p.vec);
+    }
+    st.init(tid, p.v.ss, p.d);
+    st.load(tid, reinterpret_cast<T*>(lds_v), vb, p.v.ss, all0, all_end, p.d, p.vec);
   }
   AttnGrad<T, DP> dk, dv;
   dk.clear();
@@ -270,22 +278,35 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
     if (w0 < length && q0 < p.S && (!p.causal || start + q0 + 32 > w0)) {
       const typename Tile::Lane in = at.in(buf * kTileElems + 32 * qw * DP);
       const bool mask = w0 + 32 > length || (p.causal && start + q0 < w0 + 31);
-      // 2 * NK products for the scores and dP by turns, 4 * DP / 32 with P and dS by turns
-      constexpr int kPer = Shape::kVInLds ? 3 : 2, NS = kPer * NK, NF = NS + 4 * NU;      // operands a score product and a dP product read
+      // 2 * NK products for the scores and dP by turns, 4 * DP / 32 with P and dS by turns; for the former are read, step by step
+      // of the head, q, k if it is in LDS, go, v if it is
+      constexpr int kG = Shape::kKInLds ? 2 : 1, kPer = kG + (Shape::kVInLds ? 2 : 1), NS = kPer * NK, NF = NS + 4 * NU;
       const auto load = [&](int e) -> attn_frag<T> {
-        if (e < NS) return e % kPer == 2 ? Tile::row_frag(lds_v, at, 32 * kw, e / kPer) : Tile::row_frag(e % kPer ? lds_g : lds_q, in, 0, e / kPer);
+        if (e < NS) {
+          const int kk = e / kPer, which = e % kPer;
+          if (which == 0 || which == kG) return Tile::row_frag(which ? lds_g : lds_q, in, 0, kk);
+          return Tile::row_frag(which < kG ? lds_k : lds_v, at, 32 * kw, kk);
+        }
         const int r = e - NS;
         return Tile::col_frag(r & 1 ? lds_q : lds_g, in, 16 * (r / (2 * NU)), r / 2 % NU);
       };
-      AttnRun<T, NF, sizeof(T) == 2 && DP == 128 ? 3 : kAttnAhead<T>> run;      // (more do not fit the registers)
+      AttnRun<T, NF, Shape::kAhead> run;
       run.begin(load);
       f32x16 s = f32x16_zero(), dp = f32x16_zero();
-      attn_frag<T> gf;
+      attn_frag<T> rows;                            // of q or go, for the product with what is read next
       run.steps(0, NS, load, [&](int e, const attn_frag<T>& a) {
-        if (e % kPer == 0) s = attn_mma<T>(a, kf[e / kPer], s);
-        else if (e % kPer == 2) dp = attn_mma<T>(gf, a, dp);
-        else if (Shape::kVInLds) gf = a;
-        else dp = attn_mma<T>(a, vf[e / kPer], dp);
+        const int kk = e / kPer, which = e % kPer;
+        if (which == 0) {
+          if constexpr (Shape::kKInLds) rows = a;
+          else s = attn_mma<T>(a, kf[kk], s);
+        } else if (which < kG) {
+          s = attn_mma<T>(rows, a, s);
+        } else if (which == kG) {
+          if constexpr (Shape::kVInLds) rows = a;
+          else dp = attn_mma<T>(a, vf[kk], dp);
+        } else {
+          dp = attn_mma<T>(rows, a, dp);
+        }
       });
 #pragma unroll
       for (int u = 0; u < 4; u++) {

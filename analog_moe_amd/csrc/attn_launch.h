@@ -77,7 +77,7 @@ int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
 
 // Copies of the waves over the queries: two where there are two workgroups for every CU, else four.  Measured: 324 workgroups
 // (6 padded sequences of 1717, 2 key heads of 80, fp16) 146 us with two, 105 us with four; 512 (2 x 1024, 16 heads of 64, fp32) 116
-// and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 139 and 206 us.
+// and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 100 and 206 us.
 template <typename T, int DP, bool EDGE, int QW>
 int launch_attn_kv_of(const AttnParams& p, int64_t groups, hipStream_t st) {
   hipLaunchKernelGGL((&attn_bwd_kv_kernel<T, DP, EDGE, QW>), dim3((unsigned)groups), dim3(AttnKvShape<T, DP, EDGE, QW>::kThreads), 0, st, p);
