@@ -140,8 +140,12 @@ __device__ __forceinline__ void attn_add_acc(const f32x4* lds, int copy, f32x16 
 // 32 queries only, as 64 would leave one wave on a SIMD with nobody to fill its waits.  8192 queries, 16 over 4 heads of 128,
 // bf16, causal: 298 us, 920 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 64 us, half
 // of it the time that q, k, v and the two results take to pass through memory.
+// Heads past 96 take one block of keys at a time, and with operands no more than four reads ahead three workgroups fit a CU (8192
+// queries as above: two blocks and two workgroups 312 us, one and three 294 us in turns on one card).
+template <typename T, int DP, bool EDGE, int RW>
+inline constexpr bool kAttnThree = sizeof(T) == 2 && DP == 128 && !EDGE && RW == 4;
 template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
-__global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd_rows_kernel(AttnParams p) {
+__global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Shape::kWavesPerSimd)) void attn_fwd_rows_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
   constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
   constexpr int kElems = BN * DP, kTilesBytes = 2 * kElems * (int)sizeof(T);
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_fwd
       const auto load = [&](int e) -> attn_frag<T> {
         return e < NS ? Tile::row_frag(lds_k, in, 32 * (e % NB), e / NB) : Tile::col_frag(lds_v, in, 16 * ((e - NS) / NU), (e - NS) % NU);
       };
-      AttnRun<T, NS + 2 * NB * NU> run;
+      AttnRun<T, NS + 2 * NB * NU, kAttnThree<T, DP, EDGE, RW> ? 4 : kAttnAhead<T>> run;
       run.begin(load);
       f32x16 s[NB];
       attn_frag<T> pr[2 * NB];

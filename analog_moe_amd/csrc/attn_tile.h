@@ -172,11 +172,11 @@ template <typename T, int DP> struct AttnTile {
 
 // A workgroup's waves over rows and keys: RW waves have 32 queries each, in KG copies that take every KG-th block of 32 keys and
 // are joined at the end.  Copies make more and shorter workgroups of the same work, for launches that would leave CUs idle, at
-// the price of reading the keys for fewer rows at a time.  kBlocks blocks of keys per copy and tile: two, where the tiles of 16-bit
-// elements leave room for two workgroups on a CU; fp32 tiles are twice as large.
+// the price of reading the keys for fewer rows at a time.  kBlocks blocks of keys per copy and tile: two, where the tiles and the
+// registers of two blocks leave room for three workgroups on a CU: 16-bit heads up to 96.
 template <typename T, int DP, bool EDGE, int RW_> struct AttnShape {
   static constexpr int RW = RW_, KG = 4 / RW, kRows = 32 * RW;
-  static constexpr int kBlocks = KG == 1 && sizeof(T) == 2 ? 2 : 1, kKeys = 32 * KG * kBlocks;
+  static constexpr int kBlocks = KG == 1 && sizeof(T) == 2 && DP < 128 ? 2 : 1, kKeys = 32 * KG * kBlocks;
   static constexpr int kWavesPerSimd = sizeof(T) == 4 && (DP > 64 || EDGE) ? 1 : 2;
   // what fits the 160 KB of a CU
   static constexpr bool kFits = 4 * kKeys * DP * (int)sizeof(T) <= 128 << 10;
