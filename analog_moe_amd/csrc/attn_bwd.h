@@ -192,7 +192,8 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
 // workgroups where causal rows differ in length.  Four products per block; heads of 128 are bound by registers (two waves on a
 // SIMD with every one of them used, and operands no more than three reads ahead), heads of 64 by the vector work.  8192 keys, 16
 // over 4 heads of 128, bf16, causal: 650 us, 850 TFLOP/s; 16 x 1024, 16 heads of 64: 100 us.  Measured and not kept there: the
-// exponentials between the products of one wave (900 us), two workgroups of four waves on a CU (1000 us), the queries from the other end (no difference).
+// exponentials between the products of one wave (900 us), two workgroups of four waves on a CU (1000 us), the queries from the
+// other end (no difference).
 template <typename T, int DP, bool EDGE, int QW_> struct AttnKvShape {
   static constexpr int KW = 2, QW = QW_, kThreads = 64 * KW * QW;
   // k and v read from LDS for every product, for the registers that makes free.  16-bit heads past 96: v only, with dk, dv and k

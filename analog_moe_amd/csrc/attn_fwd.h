@@ -138,7 +138,7 @@ __device__ __forceinline__ void attn_add_acc(const f32x4* lds, int copy, f32x16 
 // tiles by turns with one barrier each.  Two products of 32 x 32 x d per block of 32 keys on the matrix unit, 16 exponentials and
 // about 55 other vector instructions a lane between them, which are the longer part for heads of 64; operands of one wave's
 // 32 queries only, as 64 would leave one wave on a SIMD with nobody to fill its waits.  8192 queries, 16 over 4 heads of 128,
-// bf16, causal: 298 us, 920 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 64 us, half
+// bf16, causal: 283 us, 970 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 64 us, half
 // of it the time that q, k, v and the two results take to pass through memory.
 // Heads past 96 take one block of keys at a time, and with operands no more than four reads ahead three workgroups fit a CU (8192
 // queries as above: two blocks and two workgroups 312 us, one and three 294 us in turns on one card).
