@@ -473,12 +473,15 @@ size_t amoe_rotary_args_bytes(void);
 /* out = softmax(scale * q k^T + mask) v for q [B, S, H, d] and k, v [B, T, G, d], H a multiple of G: head h reads key head
  * h / (H / G).  Sequence b holds the keys [0, lengths[b]) (NULL: T; values outside [0, T] are taken as the nearer end); keys
  * behind them are not read.  With `causal` query i stands at position starts[b] + i (NULL: T - S + i) and sees the keys up to
- * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; H / G * S <= 2^30; fewer than 2^23 blocks of 128 queries and of 64 keys over all heads
- * and sequences (AMOE_EUNSUPPORTED otherwise); last strides are 1.
+ * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; H / G * S <= 2^30;
+ * fewer than 2^23 blocks of 128 queries and of 64 keys over all heads and sequences (AMOE_EUNSUPPORTED otherwise); last
+ * strides are 1.  An infinity or NaN in a key that a sequence holds may reach all its rows: zero times it is formed.
  * Few rows over many keys are worked on in parts of the key axis, whose results pass through the workspace.
  * The backward call recomputes the probabilities from lse (log2 of a row's sum, made by the forward call; NULL there: not
  * wanted) and reads out and, unless it is NULL, rest: the sums of out times its gradient are then as good as those of an output
- * that was not rounded, which takes a third of their error from dq and dk of 16-bit types (fp32 needs none); its workspace holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold are zero.
+ * that was not rounded, which takes a third of their error from dq and dk of 16-bit types (fp32 needs none); its workspace
+ * holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold
+ * are zero.
  * Neither call uses atomics: equal inputs give equal bits. */
 typedef struct amoe_attn_args {
   int64_t dtype, B, S, T, H, G, d, causal;
