@@ -14,6 +14,19 @@ namespace amoe {
 constexpr float kMaxLag = 8.f;
 template <typename T> inline constexpr float kProbShift = kIsF16<T> ? 7.f : 0.f;
 
+// A row's maximum is taken out within one multiply-add, s * c - rounded(m * c): all its terms are off by the same factor, which the
+// quotient does not see, as long as half a step of m * c is small against the range that the terms have.  Maxima further out
+// (2^16: half a step is 2^-8) are subtracted before the multiplication, where the largest score's difference is exactly 0.
+constexpr float kFarMax = 65536.f;
+constexpr float kMaxFloat = 3.402823466e38f;
+
+// log2 of a row's sum: m * c, finite also where the product is not, and the logarithm of the sum l of 2^(shift + (s - m) c)
+template <typename T>
+__device__ __forceinline__ float attn_lse(float m, float l, float c) {
+  if (l == 0.f) return INFINITY;
+  return fminf(fmaxf(m * c, -kMaxFloat), kMaxFloat) + (fast_log2(l) - kProbShift<T>);
+}
+
 // State of a wave's 32 queries (a lane and its partner l ^ 32 hold one): output columns, running maximum, running sum of
 // this lane's keys.
 template <typename T, int DP> struct AttnState {
@@ -57,7 +70,17 @@ __device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[N
       for (int i = 0; i < 16; i++) st.o[t][i] *= f;
     st.m = follow ? mx : st.m;
   }
-  const float base = kProbShift<T> - (st.m == -INFINITY ? 0.f : st.m * c);
+  const float taken = st.m == -INFINITY ? 0.f : st.m;
+  float base = taken * c;
+  const bool far = fabsf(base) > kFarMax;
+  if (wave_ballot(far) != 0) {
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[n][i] -= far ? taken : 0.f;
+    base = far ? 0.f : base;
+  }
+  base = kProbShift<T> - base;
   float sum = 0.f;
 #pragma unroll
   for (int n = 0; n < NB; n++)
@@ -243,7 +266,7 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
     const int64_t row = ((int64_t)w.b * p.S + w.i) * p.H + w.hd;
     attn_store_col<T, DP, EDGE>(static_cast<T*>(p.out) + row * p.d, st.o, inv, p.d, real);
     if (p.rest) attn_store_col<T, DP, EDGE, true>(static_cast<T*>(p.rest) + row * p.d, st.o, inv, p.d, real);
-    if (p.lse && real && h == 0) p.lse[(int64_t)w.bh * p.S + w.i] = l == 0.f ? INFINITY : st.m * p.c + fast_log2(l) - kProbShift<T>;
+    if (p.lse && real && h == 0) p.lse[(int64_t)w.bh * p.S + w.i] = attn_lse<T>(st.m, l, p.c);
   }
 }
 
@@ -365,7 +388,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
         const float rest[4] = {attn_rest<T>(v[0]), attn_rest<T>(v[1]), attn_rest<T>(v[2]), attn_rest<T>(v[3])};
         store4<T>(static_cast<T*>(p.rest) + to, rest, EDGE ? p.d - e : 4, !EDGE);
       }
-      if (p.lse && e == 0) p.lse[where] = lr == 0.f ? INFINITY : mr * p.c + fast_log2(lr) - kProbShift<T>;
+      if (p.lse && e == 0) p.lse[where] = attn_lse<T>(mr, lr, p.c);
     }
   }
 }
@@ -421,7 +444,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams p) {
     static_cast<T*>(p.out)[to + tid] = Elem<T>::cvt(v);
     if (p.rest) static_cast<T*>(p.rest)[to + tid] = Elem<T>::cvt(attn_rest<T>(v));
   }
-  if (p.lse && tid == 0) p.lse[at] = l == 0.f ? INFINITY : m * p.c + fast_log2(l) - kProbShift<T>;
+  if (p.lse && tid == 0) p.lse[at] = attn_lse<T>(m, l, p.c);
 }
 
 }  // namespace amoe

@@ -1,0 +1,71 @@
+"""Attention where its numbers leave the ordinary range: the kernels' source on the CPU, and the built library on the GPU."""
+import math
+
+import pytest
+import torch
+
+from analog_moe_amd import attention as A
+from tests.test_attention import DT, inputs
+from tests.test_emu_kernels import emu_ops  # noqa: F401
+
+
+def one_hot(q, k, causal, scale):
+    """[B, H, S] the key with a row's largest score, and whether it takes the whole row: the others then have less than 2^-127 of
+    it, whatever the roundings of a score (d + 8 of 2^-24 of sum|q k|, of both of them) may do."""
+    B, S, H, d = q.shape
+    T, G = k.shape[1:3]
+    Q, K = q.double().transpose(1, 2), k.double().transpose(1, 2).repeat_interleave(H // G, 1)
+    s = Q @ K.transpose(2, 3) * scale
+    size = Q.abs() @ K.abs().transpose(2, 3) * scale
+    if causal:
+        hidden = torch.arange(T) > torch.arange(S)[:, None] + T - S
+        s, size = s.masked_fill(hidden, -math.inf), size.masked_fill(hidden, 0.0)
+    two, top = s.topk(2, dim=-1)
+    return top[..., 0], two[..., 0] - two[..., 1] > 2 * (d + 8) * 2.0 ** -24 * size.amax(-1) + 127 * math.log(2)
+
+
+FAR = {
+    # B, S, T, H, G, d, dtype, size of q and k, scale, causal
+    "rows_f32": (1, 128, 128, 2, 1, 64, "f32", 1e5, None, True),
+    "rows_bf16": (1, 128, 128, 2, 2, 64, "bf16", 1e5, None, False),
+    "rows_bf16_128": (1, 70, 300, 2, 1, 128, "bf16", 1e6, None, True),
+    "rows_f16": (1, 96, 200, 2, 1, 80, "f16", 1e4, None, True),
+    "edges_f32": (1, 40, 90, 1, 1, 13, "f32", 1e9, None, True),
+    "scale_f32": (1, 40, 90, 1, 1, 64, "f32", 1.0, 1e30, True),
+    "step_f32": (2, 1, 300, 4, 2, 64, "f32", 1e7, None, True),
+    "step_f16": (1, 2, 700, 4, 1, 96, "f16", 1e4, 1.0, True),
+    "step_bf16": (1, 1, 500, 2, 1, 128, "bf16", 1e10, None, True),
+}
+
+
+def far_inputs(name):
+    *sizes, dtype, size, scale, causal = FAR[name]
+    q, k, v, go = inputs(*sizes, dtype, seed=len(name))
+    q, k = ((t.float() * size).to(DT[dtype]) for t in (q, k))
+    return q, k, v, go, causal, 1 / math.sqrt(sizes[5]) if scale is None else scale
+
+
+def check_far_forward(name, device="cpu"):
+    q, k, v, _, causal, scale = far_inputs(name)
+    top, sure = one_hot(q, k, causal, scale)
+    assert sure.double().mean() > 0.9
+    out = A.attention_forward(*(t.to(device) for t in (q, k, v)), causal=causal, scale=scale)[0].cpu().double().transpose(1, 2)
+    V = v.double().transpose(1, 2).repeat_interleave(q.shape[2] // k.shape[2], 1)
+    want = V.gather(2, top[..., None].expand(-1, -1, -1, v.shape[3]))
+    assert torch.isfinite(out).all()
+    # the one probability, its sum and their quotient: 4 roundings of fp32 (others add nothing), and one to the type
+    bound = (4 * 2.0 ** -24 + torch.finfo(q.dtype).eps / 2) * want.abs()
+    assert ((out - want).abs() <= bound)[sure].all()
+    assert (out.abs().amax(-1) > 0).all()                # no row is lost, whatever its scores
+
+
+@pytest.mark.parametrize("name", list(FAR))
+def test_far_scores(emu_ops, name):
+    """Scores of any finite size: the largest one's probability is 1, however far it is from zero."""
+    check_far_forward(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(FAR))
+def test_gpu_far_scores(name):
+    check_far_forward(name, "cuda")
