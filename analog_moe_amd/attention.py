@@ -57,8 +57,8 @@ class _Call:
             raise ValueError(f"heads have 1 to {MAX_HEAD} elements, not {d}")
         if scale is None:
             scale = 1.0 / math.sqrt(d)
-        elif not 0.0 < scale < 3.4e38:
-            raise ValueError(f"scale must be positive and finite, not {scale}")
+        elif not 2.0 ** -126 <= scale <= 2.0 ** 127:
+            raise ValueError(f"scale must be from 2^-126 to 2^127, not {scale}")
         q, k, v = _rows(q), _rows(k), _rows(v)
         n = m = n64 = m64 = 0
         if lengths is not None:
@@ -173,8 +173,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
 
     lengths [B] (int32 / int64): sequence b holds the keys [0, lengths[b]); those behind are not read, whatever lies there.
     causal: query i stands at position starts[b] + i (starts None: T - S + i, the last S of T) and sees keys up to its own
-    position.  scale: 1 / sqrt(d) unless given.  A query that sees no key gives zeros and zero gradients; so do keys that a
-    sequence does not hold.  k and v may be a cache with room behind what it holds; a single query per sequence over a long
+    position.  scale: 1 / sqrt(d) unless given, from 2^-126 to 2^127.  A query that sees no key gives zeros and zero gradients;
+    so do keys that a sequence does not hold.  k and v may be a cache with room behind what it holds; a single query per sequence over a long
     one is split along the keys.  Differentiable once in q, k and v; equal inputs give equal bits in both directions.
 
     An element that is infinite or not a number in a key or value that the sequence holds, in a query or in its gradient, may

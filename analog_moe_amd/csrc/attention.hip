@@ -30,7 +30,8 @@ int check_sizes(const amoe_attn_args* a) {
   if (a->dtype != AMOE_F32 && a->dtype != AMOE_BF16 && a->dtype != AMOE_F16) return AMOE_EINVAL;
   if (a->B < 0 || a->S < 0 || a->T < 0 || a->H < 1 || a->G < 1 || a->d < 1) return AMOE_EINVAL;
   if (a->H % a->G) return AMOE_ESHAPE;
-  if (!(a->scale > 0) || !(a->scale < 3.4e38)) return AMOE_EINVAL;
+  // (what the kernels take are the floats scale and scale * log2(e): normal ones, or masked scores meet 0 or infinity)
+  if (!(a->scale >= 0x1p-126) || !(a->scale <= 0x1p127)) return AMOE_EINVAL;
   if (a->d > kAttnMaxHead || a->S > kAttnMaxRows || a->T > kAttnMaxRows) return AMOE_EUNSUPPORTED;
   // threads of a launch are counted in 32 bits: 2^24 workgroups of 256 over the queries, 2^23 of 512 over the keys
   const int64_t over = INT64_C(1) << 23;

@@ -473,7 +473,8 @@ size_t amoe_rotary_args_bytes(void);
 /* out = softmax(scale * q k^T + mask) v for q [B, S, H, d] and k, v [B, T, G, d], H a multiple of G: head h reads key head
  * h / (H / G).  Sequence b holds the keys [0, lengths[b]) (NULL: T; values outside [0, T] are taken as the nearer end); keys
  * behind them are not read.  With `causal` query i stands at position starts[b] + i (NULL: T - S + i) and sees the keys up to
- * its own position.  A query that sees no key gives zeros, and zero gradients.  d <= 128; S, T <= 2^28; H / G * S <= 2^30;
+ * its own position.  A query that sees no key gives zeros, and zero gradients.  Scores and the scale, which is
+ * 2^-126 to 2^127, may be of any size that keeps them finite.  d <= 128; S, T <= 2^28; H / G * S <= 2^30;
  * fewer than 2^23 blocks of 128 queries and of 64 keys over all heads and sequences (AMOE_EUNSUPPORTED otherwise); last
  * strides are 1.  An infinity or NaN in a key that a sequence holds may reach all its rows: zero times it is formed.
  * Few rows over many keys are worked on in parts of the key axis, whose results pass through the workspace.

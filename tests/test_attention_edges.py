@@ -69,3 +69,27 @@ def test_far_scores(emu_ops, name):
 @pytest.mark.parametrize("name", list(FAR))
 def test_gpu_far_scores(name):
     check_far_forward(name, "cuda")
+
+
+def test_scales_that_leave_the_kernels_numbers(emu_ops):
+    """The kernels take scale and scale * log2(e) as normal floats: what is none of those is refused, the last ones that are work."""
+    q, k, v, _ = inputs(1, 40, 40, 1, 1, 64, "f32")
+    for scale in (1e-50, 1e-46, 2.0 ** -127, 1.8e38, 3e38, 1e300, -1.0):
+        with pytest.raises(ValueError):
+            A.attention_forward(q, k, v, scale=scale)
+    lib = emu_ops.get_lib()
+    out = torch.empty_like(q)
+    for scale, code in ((1e-46, -1), (2.0 ** -127, -1), (2.0 ** -126, 0), (2.0 ** 127, 0), (3e38, -1)):
+        call = A._Call(q, k, v, None, None, True, 0.5)
+        call.head = (*call.head[:8], scale, *call.head[9:])
+        assert lib.amoe_attention_fwd(call.pack(out, None, None), None, 0, None) == code, scale
+    # scores of no size at all: the mean of what a row sees (40 terms, their sum, a quotient: 42 roundings)
+    out = A.attention_forward(q, k, v, scale=2.0 ** -126)[0].double()
+    n = torch.arange(1, 41)[:, None, None]
+    assert ((out - v.double().cumsum(1) / n).abs() <= 48 * 2.0 ** -24 * v.double().abs().cumsum(1) / n).all()
+    # and of the largest: scores have to stay finite themselves
+    q, k = q * 2.0 ** -20, k * 2.0 ** -20
+    top, sure = one_hot(q, k, True, 2.0 ** 127)
+    out = A.attention_forward(q, k, v, scale=2.0 ** 127)[0].transpose(1, 2)
+    want = v.transpose(1, 2).gather(2, top[..., None].expand(-1, -1, -1, 64))
+    assert sure.all() and ((out - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
