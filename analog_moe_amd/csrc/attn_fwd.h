@@ -14,10 +14,12 @@ namespace amoe {
 constexpr float kMaxLag = 8.f;
 template <typename T> inline constexpr float kProbShift = kIsF16<T> ? 7.f : 0.f;
 
-// A row's maximum is taken out within one multiply-add, s * c - rounded(m * c): all its terms are off by the same factor, which the
-// quotient does not see, as long as half a step of m * c is small against the range that the terms have.  Maxima further out
-// (2^16: half a step is 2^-8) are subtracted before the multiplication, where the largest score's difference is exactly 0.
-constexpr float kFarMax = 65536.f;
+// A row's maximum is taken out within one multiply-add, s * c - rounded(m * c), so that all terms are off by the same factor, two to
+// the rounding of m * c.  The quotient does not see it, but what is joined does: terms from before the maximum moved on, and those
+// of other waves and parts, have factors of their own.  Maxima further from zero than this (half a step of it: 2^-18 in fp32,
+// which the scores' own rounding is as large as; 2^-15 for 16-bit types, against 2^-9 or 2^-12 of a probability's rounding) are
+// subtracted before the multiplication, where the largest score's difference is exactly 0.
+template <typename T> inline constexpr float kFar = sizeof(T) == 4 ? 128.f : 1024.f;
 constexpr float kMaxFloat = 3.402823466e38f;
 
 // log2 of a row's sum: m * c, finite also where the product is not, and the logarithm of the sum l of 2^(shift + (s - m) c)
@@ -72,7 +74,7 @@ __device__ __forceinline__ void attn_softmax(AttnState<T, DP>& st, f32x16 (&s)[N
   }
   const float taken = st.m == -INFINITY ? 0.f : st.m;
   float base = taken * c;
-  const bool far = fabsf(base) > kFarMax;
+  const bool far = fabsf(base) > kFar<T>;
   if (wave_ballot(far) != 0) {
 #pragma unroll
     for (int n = 0; n < NB; n++)

@@ -17,7 +17,7 @@ def visible(B, S, T, causal, lengths, starts):
     return seen & (key <= at[..., None]) if causal else seen
 
 
-def attention(q, k, v, go=None, causal=True, scale=None, lengths=None, starts=None):
+def attention(q, k, v, go=None, causal=True, scale=None, lengths=None, starts=None, exact_scores=False):
     """(out, dq, dk, dv, bounds): results in fp64 and, for tensors of q's type, how far each element may be off.
 
     With u half a step of the type (0 inside fp32 kernels, whose probabilities are not rounded again) and e = 2^-24:
@@ -25,7 +25,11 @@ def attention(q, k, v, go=None, causal=True, scale=None, lengths=None, starts=No
     exponent and logarithm relative to itself; sums over n terms by n e of the sum of their absolute values; probabilities and
     score gradients are rounded to the type before the second product, results at the end; the backward pass reads the
     rounded output.  The hardware's 2^x gives 0 for what is below the normal numbers, so that a probability is off by
-    2^-126 in absolute terms too, and what is made of it by that times what multiplies it."""
+    2^-126 in absolute terms too, and what is made of it by that times what multiplies it.
+
+    exact_scores: q k, and its distance from a row's largest, are numbers that fp32 holds.  A probability is then off by the
+    rounding of that distance x times the scale times log2(e), twice (the factor's own and the product's), and by the 16 e of
+    exponent and logarithm; the row's sum by what its terms are off on average."""
     B, S, H, d = q.shape
     T, G = k.shape[1], k.shape[2]
     scale = 1 / math.sqrt(d) if scale is None else scale
@@ -47,8 +51,11 @@ def attention(q, k, v, go=None, causal=True, scale=None, lengths=None, starts=No
     size = (Q.abs() @ K.abs().transpose(2, 3) * scale).masked_fill(~seen, 0.0)
     off = size.amax(-1, keepdim=True) if T else torch.zeros(B, H, S, 1)
     ep = 2 * ((d + 8) * e * off + 16 * e + 4 * e * top.abs())            # relative, of a probability
+    if exact_scores:
+        ep = 2 * e * torch.where(seen, top - s, 0.0) + 16 * e
+        ep = ep + (p * ep).sum(-1, keepdim=True)
     lost = 2.0 ** -126 * seen.double()
-    b_out = p @ V.abs() * (ep + T * e + inner) + lost @ V.abs() + u * out.abs() + tiny
+    b_out = (p * (ep + T * e + inner)) @ V.abs() + lost @ V.abs() + u * out.abs() + tiny
 
     def last(x):
         return x.transpose(1, 2)

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from analog_moe_amd import attention as A
-from tests.test_attention import DT, inputs
+from oracle import attention_oracle as O
+from tests.test_attention import DT, compare, inputs
 from tests.test_emu_kernels import emu_ops  # noqa: F401
 
 
@@ -93,3 +94,45 @@ def test_scales_that_leave_the_kernels_numbers(emu_ops):
     out = A.attention_forward(q, k, v, scale=2.0 ** 127)[0].transpose(1, 2)
     want = v.transpose(1, 2).gather(2, top[..., None].expand(-1, -1, -1, 64))
     assert sure.all() and ((out - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
+
+
+SHIFTED = {
+    # S, T, H, G, d, dtype, how far all scores of a row are from zero: 15 * size^2
+    "f32": (70, 140, 2, 1, 16, "f32", 32),
+    "f32_split": (2, 300, 2, 2, 16, "f32", 100),
+    "f32_128": (40, 70, 1, 1, 128, "f32", 64),
+    "bf16": (70, 140, 2, 1, 16, "bf16", 256),
+    "bf16_128": (33, 130, 2, 1, 128, "bf16", 256),
+    "f16": (70, 140, 2, 1, 16, "f16", 256),
+    "f16_96": (20, 90, 1, 1, 96, "f16", 512),
+    "odd_bf16": (40, 66, 1, 1, 17, "bf16", 256),
+}
+
+
+def check_shifted(name, device="cpu"):
+    S, T, H, G, d, dtype, size = SHIFTED[name]
+    _, _, v, go = inputs(1, S, T, H, G, d, dtype, seed=len(name))
+    q, k = torch.zeros(1, S, H, d), torch.zeros(1, T, G, d)
+    q[..., :15] = k[..., :15] = size
+    q[:, 1::3, :, :15] = 0.0                              # (every third row is near, among those that are far)
+    q[..., 15] = (-1.0) ** torch.arange(S)[:, None]
+    k[..., 15] = torch.randint(0, 8, (1, T, G), generator=torch.Generator().manual_seed(0)).float()
+    q, k = q.to(DT[dtype]), k.to(DT[dtype])
+    for kw in ({}, dict(lengths=torch.tensor([T - 1]), starts=torch.tensor([-1]))):
+        want, bounds = O.attention(q, k, v, go, scale=1.0, exact_scores=True, **kw)
+        on = [t.to(device) for t in (q, k, v, go)]
+        how = dict(scale=1.0, **{n: t.to(device) for n, t in kw.items()})
+        out = A.attention_forward(*on[:3], **how)[0]
+        compare((out,), want, bounds, name)
+
+
+@pytest.mark.parametrize("name", list(SHIFTED))
+def test_rows_far_from_zero(emu_ops, name):
+    """Scores that differ by some units, all of them far from zero: as exact as their differences are."""
+    check_shifted(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(SHIFTED))
+def test_gpu_rows_far_from_zero(name):
+    check_shifted(name, "cuda")
