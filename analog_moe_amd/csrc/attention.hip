@@ -134,7 +134,7 @@ extern "C" int amoe_attention_fwd(const amoe_attn_args* a, void* workspace, size
 
 extern "C" size_t amoe_attention_bwd_workspace(const amoe_attn_args* a) {
   if (check_sizes(a)) return 0;
-  return (size_t)(a->B * a->H * a->S) * 4;
+  return (size_t)(a->B * a->H * a->S) * 3 * 4;
 }
 
 extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -162,7 +162,7 @@ extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size
   p.o = a->out;
   p.rest = a->rest;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
-  p.delta = static_cast<float*>(workspace);
+  p.rows = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a->dtype == AMOE_F32   ? launch_attn_bwd_f32(p, st)
          : a->dtype == AMOE_F16 ? launch_attn_bwd_f16(p, st)

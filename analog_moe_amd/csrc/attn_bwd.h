@@ -11,6 +11,44 @@ namespace amoe {
 // fp16 probabilities as operands, 2^15 times as large: no more than 2^15, and 2^-29 is still a normal number.
 template <typename T> inline constexpr float kGradShift = kIsF16<T> ? 15.f : 0.f;
 
+// A log-sum is rounded to a float, and so are all probabilities of its row off by up to half a step of it.  Rows whose log-sum is
+// further from zero than kFar get theirs from a maximum and a sum made again: P = 2^((s - top) c - norm), with the maximum taken
+// out before the multiplication and norm the logarithm of the sum.  Other rows: top 0, norm lse.
+__device__ __forceinline__ bool attn_is_far(float lse, float limit) { return fabsf(lse) > limit && fabsf(lse) <= kMaxFloat; }
+// (a score made in another kernel may not be above the maximum either)
+__device__ __forceinline__ float attn_below(float s, float top) { return fminf(s - top, 0.f); }
+
+// top and norm of a wave's far rows, whose queries q holds: the keys they see once more, from memory
+template <typename T, int DP, bool EDGE>
+__device__ __forceinline__ void attn_far_rows(const AttnParams& p, const attn_frag<T> (&q)[DP / 16], const T* kb, int wave_sees, int seen,
+                                              bool far, float& top, float& norm) {
+  const int h = lane_id() >> 5;
+  float m = -INFINITY, l = 0.f;
+  for (int key0 = 0; key0 < wave_sees; key0 += 32) {
+    attn_frag<T> kf[DP / 16];
+    attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, key0, wave_sees, p.d, p.vec);
+    f32x16 s = f32x16_zero();
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; kk++) s = attn_mma<T>(kf[kk], q[kk], s);
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      if (key0 + 8 * (i / 4) + 4 * h + i % 4 >= seen) s[i] = -INFINITY;
+      mx = fmaxf(mx, s[i]);
+    }
+    mx = attn_pair_max(mx);
+    if (mx > m) l *= fast_exp2((m - mx) * p.c);
+    m = mx;
+#pragma unroll
+    for (int i = 0; i < 16; i++) l += fast_exp2((s[i] - m) * p.c);
+  }
+  l = attn_pair_sum(l);
+  if (far) {
+    top = m;
+    norm = fast_log2(l);
+  }
+}
+
 // dS as matrix operands.  fp16 has no range for it: a gradient's size is the caller's, and where many keys share a row dS is
 // tiny against what it sums up to.  So every column (a lane's query or key) carries a power of two that keeps its largest
 // entry within fp16; it only falls, and the sums so far fall with it.  bf16 and fp32 need none.
@@ -58,7 +96,7 @@ __device__ __forceinline__ void attn_pack_block(const V& v, attn_frag<T> (&f)[2]
 }
 
 // dq: 32 * RW queries of one head per workgroup, keys in tiles as in the forward pass; three products per block.  Also leaves
-// delta.  Bound as the forward pass is: 8192 queries, 16 over 4 heads of 128, bf16, causal: 394 us, 1050 TFLOP/s; 16 x 1024, 16
+// norm, delta and top of every row.  Bound as the forward pass is: 8192 queries, 16 over 4 heads of 128, bf16, causal: 394 us, 1050 TFLOP/s; 16 x 1024, 16
 // heads of 64: 78 us.
 template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
 __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd_q_kernel(AttnParams p) {
@@ -108,8 +146,15 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
     }
   }
   delta = attn_pair_sum(delta);
-  const float lse = real ? p.lse[stat] : INFINITY;
-  if (real && h == 0 && w.kg == 0) p.delta[stat] = delta;
+  float norm = real ? p.lse[stat] : INFINITY, top = 0.f;
+  const bool far = attn_is_far(norm, kFar<T>), any_far = wave_ballot(far) != 0;
+  if (any_far) attn_far_rows<T, DP, EDGE>(p, q, kb, w.wave_sees, w.seen, far, top, norm);
+  if (real && h == 0 && w.kg == 0) {
+    const int64_t n = (int64_t)p.B * p.H * p.S;
+    p.rows[stat] = norm;
+    p.rows[n + stat] = delta;
+    p.rows[2 * n + stat] = top;
+  }
 
   AttnGrad<T, DP> dq;
   dq.clear();
@@ -145,9 +190,13 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
           if (e & 1) dp = attn_mma<T>(a, go[e / 2], dp);
           else s = attn_mma<T>(a, q[e / 2], s);
         });
+        if (any_far) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[e] = far ? attn_below(s[e], top) : s[e];
+        }
         float ds[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) ds[e] = fast_exp2(fmaf(s[e], p.c, -lse)) * (dp[e] - delta);
+        for (int e = 0; e < 16; e++) ds[e] = fast_exp2(fmaf(s[e], p.c, -norm)) * (dp[e] - delta);
         if (mask) {
 #pragma unroll
           for (int e = 0; e < 16; e++)
@@ -214,7 +263,8 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   static_assert(KW * (QW - 1) <= 2 * kSumsPer, "the copies' sums fit the tiles' room");
   __shared__ __align__(1024) char lds_q[kTilesBytes], lds_g[kTilesBytes];
   __shared__ __align__(1024) char lds_k[Shape::kKInLds ? 32 * KW * DP * (int)sizeof(T) : 16], lds_v[Shape::kVInLds ? 32 * KW * DP * (int)sizeof(T) : 16];
-  __shared__ __align__(16) float lds_lse[2][BM], lds_delta[2][BM];
+  __shared__ __align__(16) float lds_rows[3][2][BM];              // norm, delta, top
+  __shared__ int lds_far[2][QW];                                  // a block of 32 queries has one with a top
   T *const tq = reinterpret_cast<T*>(lds_q), *const tg = reinterpret_cast<T*>(lds_g);
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), kw = wave % KW, qw = wave / KW, h = lane >> 5;
   const int BG = p.B * p.G, bg = (int)(blockIdx.x % (unsigned)BG), tile = (int)(blockIdx.x / (unsigned)BG);
@@ -231,22 +281,27 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   AttnStage<T, DP, BM, NT, EDGE> sq, sg;
   sq.init(tid, p.q.ss, p.d);
   sg.init(tid, p.go.ss, p.d);
-  float stat = 0.f;                                   // threads 0 .. BM - 1: lse, the next BM: delta
+  static_assert(3 * BM <= NT && BM % 64 == 0, "a thread for each, whole waves");
+  const int part = tid / BM;                          // threads 0 .. BM - 1: norm, the next BM: delta, the next: top
+  float stat = 0.f;
   const auto fetch = [&](int t) {
     const int hd = g * p.R + t / per_head, q0 = (tile0 + t % per_head) * BM, buf = t & 1;
     sq.load(tid, tq + buf * kTileElems, static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh, p.q.ss, q0, p.S, p.d, p.vec);
     sg.load(tid, tg + buf * kTileElems, static_cast<const T*>(p.go.p) + b * p.go.sb + hd * p.go.sh, p.go.ss, q0, p.S, p.d, p.vec);
-    if (tid < 2 * BM) {
-      const int qi = q0 + (tid < BM ? tid : tid - BM);
-      const int64_t row = ((int64_t)b * p.H + hd) * p.S + qi;
-      stat = qi < p.S ? (tid < BM ? p.lse[row] : p.delta[row]) : (tid < BM ? INFINITY : 0.f);
+    if (part < 3) {
+      const int qi = q0 + tid % BM;
+      const int64_t row = (((int64_t)part * p.B + b) * p.H + hd) * p.S + qi;
+      stat = qi < p.S ? p.rows[row] : part == 0 ? INFINITY : 0.f;
     }
   };
   const auto put = [&](int buf) {
     sq.store(tid, tq + buf * kTileElems);
     sg.store(tid, tg + buf * kTileElems);
-    if (tid < BM) lds_lse[buf][tid] = stat;
-    else if (tid < 2 * BM) lds_delta[buf][tid - BM] = stat;
+    if (part < 3) lds_rows[part][buf][tid % BM] = stat;
+    if (part == 2) {
+      const uint64_t tops = wave_ballot(stat != 0.f);
+      if (lane % 32 == 0) lds_far[buf][tid % BM / 32] = (uint32_t)(tops >> lane) != 0;
+    }
   };
   if (n_tiles > 0) fetch(0);
   attn_frag<T> kf[NK], vf[NK];
@@ -309,14 +364,22 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
           dp = attn_mma<T>(rows, a, dp);
         }
       });
+      if (wave_uniform(lds_far[buf][qw]) != 0) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const f32x4 top = *reinterpret_cast<const f32x4*>(&lds_rows[2][buf][32 * qw + 8 * u + 4 * h]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[4 * u + j] = top[j] != 0.f ? attn_below(s[4 * u + j], top[j]) : s[4 * u + j];
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&lds_lse[buf][32 * qw + 8 * u + 4 * h]);
-        const f32x4 del = *reinterpret_cast<const f32x4*>(&lds_delta[buf][32 * qw + 8 * u + 4 * h]);
+        const f32x4 norm = *reinterpret_cast<const f32x4*>(&lds_rows[0][buf][32 * qw + 8 * u + 4 * h]);
+        const f32x4 del = *reinterpret_cast<const f32x4*>(&lds_rows[1][buf][32 * qw + 8 * u + 4 * h]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int e = 4 * u + j;
-          s[e] = fast_exp2(fmaf(s[e], p.c, kGradShift<T> - lse[j]));
+          s[e] = fast_exp2(fmaf(s[e], p.c, kGradShift<T> - norm[j]));
           dp[e] = s[e] * (dp[e] - del[j]);
         }
       }

@@ -102,7 +102,7 @@ int launch_attn_bwd(const AttnParams& p, hipStream_t st) {
 #define AMOE_LAUNCH(TYPE, DP, EDGE)                                                                             \
   rc = launch_attn_rows<AttnBwdRows<TYPE, DP, EDGE>::template Launch, !EDGE && AttnShape<TYPE, DP, EDGE, 2>::kFits, \
                         !EDGE && AttnShape<TYPE, DP, EDGE, 1>::kFits>(p, st)
-    AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);          // (leaves delta for the next)
+    AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);          // (leaves rows for the next)
 #undef AMOE_LAUNCH
     if (rc) return rc;
   }

@@ -27,7 +27,8 @@ struct AttnParams {
   const void* o;                     // the same, read by the backward pass
   void* rest;                        // [B, S, H, d]: out before its rounding less out, of the same type; written and read.  May be null
   float* lse;                        // [B, H, S]: log2 of the sum of 2^(score * c); +inf where a row sees nothing.  May be null
-  float* delta;                      // [B, H, S]: sum over d of out * gradient of out
+  float* rows;                       // 3 x [B, H, S], what dk and dv need of a row: norm and top (attn_far_rows), and between them
+                                     // delta, the sum over d of out * gradient of out
   void *dq, *dk, *dv;                // [B, S, H, d], [B, T, G, d]
   const void *lengths, *starts;      // [B] int32 / int64 or null
   int lengths_i64, starts_i64;

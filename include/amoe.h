@@ -481,7 +481,7 @@ size_t amoe_rotary_args_bytes(void);
  * The backward call recomputes the probabilities from lse (log2 of a row's sum, made by the forward call; NULL there: not
  * wanted) and reads out and, unless it is NULL, rest: the sums of out times its gradient are then as good as those of an output
  * that was not rounded, which takes a third of their error from dq and dk of 16-bit types (fp32 needs none); its workspace
- * holds one fp32 value per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold
+ * holds three fp32 values per row.  dk and dv may both be NULL (not wanted).  Gradients of keys that a sequence does not hold
  * are zero.
  * Neither call uses atomics: equal inputs give equal bits. */
 typedef struct amoe_attn_args {

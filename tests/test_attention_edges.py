@@ -96,6 +96,44 @@ def test_scales_that_leave_the_kernels_numbers(emu_ops):
     assert sure.all() and ((out - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
 
 
+def check_far_backward(name, device="cpu"):
+    q, k, v, go, causal, scale = far_inputs(name)
+    B, S, H, d = q.shape
+    T, G = k.shape[1:3]
+    top, sure = one_hot(q, k, causal, scale)
+    Q, K, V = (t.double().transpose(1, 2).repeat_interleave(H // t.shape[2], 1) for t in (q, k, v))
+    for held in (go, torch.where(sure.transpose(1, 2)[..., None], go, torch.zeros_like(go))):
+        args = [t.to(device) for t in (held, q, k, v)]
+        left = A.attention_forward(*args[1:], causal=causal, scale=scale, want_lse=True)
+        grads = A.attention_backward(*args, *left, causal=causal, scale=scale)
+        assert all(torch.isfinite(t).all() for t in grads)
+    dq, dk, dv = (t.cpu().double().transpose(1, 2) for t in grads)
+    # a row that one key takes hands its gradient to that key's value, and to q and k nothing: what dP - delta leaves there is
+    # two sums of d products, 2 (d + 2) roundings, and their rounding to the type
+    u, e, tiny = torch.finfo(q.dtype).eps / 2, 2.0 ** -24, torch.finfo(q.dtype).smallest_normal
+    g = held.double().transpose(1, 2)
+    at = top[..., None].expand(-1, -1, -1, d)
+    ds = (2 * (d + 2) * e * (g.abs() * V.abs().gather(2, at)).sum(-1, keepdim=True) + tiny) * (1 + 2 * u)
+
+    def to_keys(x):
+        return torch.zeros(B, H, T, d, dtype=torch.float64).scatter_add_(2, at, x).reshape(B, G, H // G, T, d).sum(2)
+    want, size = to_keys(g), to_keys(g.abs())
+    assert ((dv - want).abs() <= u * want.abs() + (S * H // G + 8) * e * size + tiny).all()
+    assert (dq.abs() <= 1.01 * scale * ds * K.abs().gather(2, at) + tiny).all()
+    assert (dk.abs() <= 1.01 * scale * to_keys(ds * Q.abs()) + tiny).all()
+
+
+@pytest.mark.parametrize("name", list(FAR))
+def test_far_gradients(emu_ops, name):
+    check_far_backward(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(FAR))
+def test_gpu_far_gradients(name):
+    check_far_backward(name, "cuda")
+
+
 SHIFTED = {
     # S, T, H, G, d, dtype, how far all scores of a row are from zero: 15 * size^2
     "f32": (70, 140, 2, 1, 16, "f32", 32),
@@ -122,8 +160,8 @@ def check_shifted(name, device="cpu"):
         want, bounds = O.attention(q, k, v, go, scale=1.0, exact_scores=True, **kw)
         on = [t.to(device) for t in (q, k, v, go)]
         how = dict(scale=1.0, **{n: t.to(device) for n, t in kw.items()})
-        out = A.attention_forward(*on[:3], **how)[0]
-        compare((out,), want, bounds, name)
+        out, lse, rest = A.attention_forward(*on[:3], want_lse=True, **how)
+        compare((out, *A.attention_backward(on[3], *on[:3], out, lse, rest, **how)), want, bounds, name)
 
 
 @pytest.mark.parametrize("name", list(SHIFTED))
