@@ -94,6 +94,19 @@ __device__ __forceinline__ attn_frag<T> attn_pack(const float (&v)[8]) {
   }
 }
 
+// c plus the eight values as the matrix unit sees them, after their rounding
+template <typename T>
+__device__ __forceinline__ float attn_add_packed(const attn_frag<T>& f, float c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c += f.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = kIsF16<T> ? add_f16x2(f[j], c) : add_bf16x2(f[j], c);
+  }
+  return c;
+}
+
 // ---- tiles in LDS ---------------------------------------------------------------------------------
 // Rows of DP elements in 16-byte chunks; chunk c of row r lies at chunk c ^ swizzle(r) of the row.  Both ways a tile is
 // read touch every bank once: 16 rows at one chunk (operands whose rows are the tile's), and 4 rows at 4 adjacent chunks

@@ -174,3 +174,54 @@ def test_rows_far_from_zero(emu_ops, name):
 @pytest.mark.parametrize("name", list(SHIFTED))
 def test_gpu_rows_far_from_zero(name):
     check_shifted(name, "cuda")
+
+
+EQUAL_VALUES = {
+    # B, S, T, H, G, d, dtype, size of q
+    "rows_bf16": (1, 70, 140, 2, 1, 64, "bf16", 1.0),
+    "rows_f16": (2, 70, 140, 2, 1, 64, "f16", 1.0),
+    "rows_f32": (1, 40, 90, 2, 1, 64, "f32", 1.0),
+    "peaked_bf16_128": (1, 40, 300, 2, 2, 128, "bf16", 20.0),
+    "peaked_f16_80": (1, 33, 200, 2, 1, 80, "f16", 20.0),
+    "far_bf16": (1, 40, 140, 1, 1, 64, "bf16", 2000.0),
+    "edges_bf16": (1, 40, 90, 1, 1, 13, "bf16", 3.0),
+    "step_bf16": (2, 1, 700, 4, 2, 64, "bf16", 1.0),
+    "step_f16": (1, 2, 500, 4, 1, 96, "f16", 5.0),
+}
+
+
+def check_equal_values(name, device="cpu"):
+    *sizes, dtype, size = EQUAL_VALUES[name]
+    B, S, T, H, G, d = sizes
+    q, k, v, go = inputs(*sizes, dtype, seed=3)
+    q = (q.float() * size).to(q.dtype)
+    v = v[:, :1].expand(B, T, G, d)
+    on = [t.to(device) for t in (q, k, v, go)]
+    out, lse, rest = A.attention_forward(*on[:3], want_lse=True)
+    want = v[:, :1].repeat_interleave(H // G, 2).expand(B, S, H, d)
+    e = 2.0 ** -24
+    # two sums of T terms, in other orders, and half a step of the subnormal numbers where rest is one
+    off = 2 * (T + 4) * e * want.double().abs() + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2
+    have = out.cpu().double() + (0 if rest is None else rest.cpu().double())
+    assert ((have - want.double()).abs() <= off).all()
+    if dtype != "f32":
+        assert torch.equal(out.cpu(), want)                               # (what is off by less than half a step rounds back)
+    # dP is the same for all keys and delta that number: what is left of dS are the roundings of d products, twice, and out's
+    dq = A.attention_backward(on[3], *on[:3], out, lse, rest)[0].cpu().double()
+    g = go.double().abs()
+    ds = (g * (2 * (d + 2) * e * want.double().abs() + 2 * off)).sum(-1, keepdim=True) + torch.finfo(q.dtype).smallest_normal
+    big = k.double().abs().amax(1, keepdim=True).repeat_interleave(H // G, 2)
+    assert (dq.abs() <= 1.01 / math.sqrt(d) * ds * big + torch.finfo(q.dtype).smallest_normal).all()
+
+
+@pytest.mark.parametrize("name", list(EQUAL_VALUES))
+def test_equal_values(emu_ops, name):
+    """Whatever the probabilities are rounded to, the sum that divides them counts the same numbers: a mean of equal values is
+    that value, and q has no gradient."""
+    check_equal_values(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(EQUAL_VALUES))
+def test_gpu_equal_values(name):
+    check_equal_values(name, "cuda")
