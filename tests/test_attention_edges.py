@@ -225,3 +225,50 @@ def test_equal_values(emu_ops, name):
 @pytest.mark.parametrize("name", list(EQUAL_VALUES))
 def test_gpu_equal_values(name):
     check_equal_values(name, "cuda")
+
+
+def check_rest(dtype, S, d, device="cpu"):
+    """Queries of zeros: a row is the mean of the values it sees, its probabilities are exact (the maximum is 0, each 2^0, the sum
+    a whole number), so that nothing but the output's rounding is off by more than some 2^-24."""
+    q, _, v, go = inputs(1, S, S, 2, 1, d, dtype, seed=4)
+    q = torch.zeros_like(q)
+    k = torch.ones(1, S, 1, d, dtype=q.dtype)
+    # values next to each other: what rounding takes from their mean is as large as what they differ by
+    v = (1.0 + (v.float() * 4).round() * torch.finfo(q.dtype).eps).to(q.dtype)
+    on = [t.to(device) for t in (q, k, v, go)]
+    out, lse, rest = A.attention_forward(*on[:3], want_lse=True)
+    u, e = torch.finfo(q.dtype).eps / 2, 2.0 ** -24
+    n = torch.arange(1, S + 1)[:, None, None].double()
+    V = v.double()
+    mean, size = V.cumsum(1) / n, V.abs().cumsum(1) / n
+    # a sum of n terms, a quotient, a product; then rest, itself rounded (or half a step of the subnormal numbers)
+    off = (S + 4) * e * size
+    left = (mean - out.cpu().double()).abs()
+    small = torch.finfo(q.dtype).smallest_normal * u
+    b_rest = off + u * (left + off) + small
+    assert ((out.cpu().double() + rest.cpu().double() - mean).abs() <= b_rest).all()
+    assert rest.abs().max() > 0.2 * u                                     # (there is something to keep)
+    # dq = scale * sum of P (dP - delta) over keys of ones.  The formula has 0; P = 1 / n by 2^-lse is off by 8 e, the sum of
+    # what P's error multiplies by |dP - delta| at most; dS is rounded to the type; delta is off by b_rest and 2 d roundings
+    dq = A.attention_backward(on[3], *on[:3], out, lse, rest)[0].cpu().double()
+    g = go.double()
+    dP = (g.transpose(1, 2) @ V.transpose(1, 2).transpose(2, 3)).masked_fill(torch.ones(S, S).triu(1).bool(), 0.0)     # [1, 2, S, S]
+    delta = (g * mean).sum(-1).transpose(1, 2)[..., None]
+    ds = (dP - delta).abs().masked_fill(torch.ones(S, S).triu(1).bool(), 0.0).sum(-1) / n[:, 0, 0]
+    b_delta = ((g.abs() * (b_rest + 2 * (d + 2) * e * size)).sum(-1)).transpose(1, 2)
+    bound = (ds * (u + (8 + S) * e) + b_delta).transpose(1, 2)[..., None] / math.sqrt(d) * 1.01 + torch.finfo(q.dtype).smallest_normal
+    assert (dq.abs() <= bound).all(), (dq.abs() / bound).max()
+    for wrong in (None, -rest):                                           # (the bound tells rest from none, and from its opposite)
+        dq = A.attention_backward(on[3], *on[:3], out, lse, wrong)[0].cpu().double()
+        assert (dq.abs() > bound).any()
+
+
+@pytest.mark.parametrize("dtype, S, d", [("bf16", 90, 64), ("f16", 70, 64), ("bf16", 40, 128), ("bf16", 35, 13)])
+def test_rest(emu_ops, dtype, S, d):
+    check_rest(dtype, S, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, S, d", [("bf16", 300, 64), ("f16", 300, 96), ("bf16", 200, 128), ("bf16", 200, 13)])
+def test_gpu_rest(dtype, S, d):
+    check_rest(dtype, S, d, "cuda")
