@@ -101,6 +101,9 @@ def rotate(q: Tensor, k: Tensor, turns: Tensor, positions: Optional[Tensor] = No
         rc = lib.amoe_rotary(args, ops._stream(q))
     if rc:
         _abi.check(lib, rc, "amoe_rotary")
+    if out is not None:
+        # (a backward pass that saved them is to notice; inference tensors have no versions)
+        torch.autograd.graph.increment_version([t for t in out if not t.is_inference()])
     return oq, ok
 
 
