@@ -15,7 +15,7 @@ so every group of calls the Python layer makes is one opaque operator with a fak
   amoe::cvmm_forward        everything CVMM.forward launches  (cvmm.py:701-769)
   amoe::cvmm_backward       everything CVMM.backward launches (cvmm.py:772-897)
   amoe::ffn_fwd / ffn_bwd   the fused expert feed-forward, with its autograd formula registered
-  amoe::attention_fwd / attention_bwd, amoe::rotary   the decoder's attention and rotary positions, likewise
+  amoe::attention_fwd / attention_bwd, amoe::rotary / rotary_into   the decoder's attention and rotary positions, likewise
 
 Operators return an empty tensor where the Python interface returns ``None``.
 """
@@ -438,3 +438,17 @@ def _rotary_autograd(ctx, gq, gk):
 
 
 rotary_op.register_autograd(_rotary_autograd, setup_context=_rotary_setup_context)
+
+
+@torch.library.custom_op(
+    "amoe::rotary_into", mutates_args=("q_out", "k_out"),
+    schema="(Tensor q, Tensor k, Tensor(a!) q_out, Tensor(b!) k_out, Tensor turns, Tensor? positions, int start, bool interleaved, "
+           "float size) -> ()")
+def rotary_into(q, k, q_out, k_out, turns, positions, start, interleaved, size):
+    """amoe::rotary into q_out and k_out, which may be q and k; without gradients."""
+    rotary.rotate(q, k, turns, positions, start, interleaved, size, out=(q_out, k_out))
+
+
+@rotary_into.register_fake
+def _(q, k, q_out, k_out, turns, positions, start, interleaved, size):
+    return None

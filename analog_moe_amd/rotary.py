@@ -123,6 +123,15 @@ class RotaryFunction(torch.autograd.Function):
         return (*f(gq, gk, turns, positions, *ctx.args), None, None, None, None, None, None)
 
 
+class RotaryInto(torch.autograd.Function):
+    """``rotate`` into tensors that are there, for whom something watches: no derivative of either mode."""
+
+    @staticmethod
+    def forward(ctx, q, k, oq, ok, turns, positions, start, interleaved, size):
+        ctx.mark_dirty(oq, ok)
+        return rotate(q, k, turns, positions, start, interleaved, size, out=(oq, ok))
+
+
 class Rotary(nn.Module):
     """``rotary(q, k, positions=None, start=0) -> (q, k)`` turned.  positions: int32 / int64 [S] or [B, S], any value; without
     them token s stands at start + s.  The table is an int64 buffer, so that ``.to(torch.bfloat16)`` of a model leaves the
@@ -150,7 +159,10 @@ class Rotary(nn.Module):
         if out is not None:
             if grad or any(t.requires_grad for t in out):
                 raise RuntimeError("out is for calls without gradients")
-            return rotate(*args, out=out)
+            if torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None:
+                torch.ops.amoe.rotary_into(q, k, *out, *args[2:])
+                return out
+            return rotate(*args, out=out) if ops.unwatched() else RotaryInto.apply(q, k, *out, *args[2:])
         if torch.compiler.is_compiling():
             return torch.ops.amoe.rotary(*args, False)
         if not grad and ops.unwatched():

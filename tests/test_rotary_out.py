@@ -28,3 +28,58 @@ def test_what_was_saved_and_is_overwritten_is_noticed(emu_ops):
         want = r(a, b)
         r(a, b, out=(a, b))
         assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+def test_watched_calls(emu_ops):
+    """With out= as without: forward-mode derivatives and function transforms are refused, modes and traces work."""
+    q, k = inputs(1, 4, 1, 1, 16, "f32")
+    r = R.Rotary(16)
+    want = r(q, k)
+    new = lambda: (torch.zeros_like(q), torch.zeros_like(k))          # noqa: E731
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            r(forward_ad.make_dual(q, q), k, out=new())
+        out = new()
+        r(q, k, out=out)                                              # (nothing here has a tangent)
+        assert all(map(torch.equal, out, want))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: r(x, k, out=new())[0])(q[None])
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    out = new()
+    with Mode():
+        got = r(q, k, out=out)
+    assert all(map(torch.equal, out, want)) and all(map(torch.equal, got, want))
+    out = new()
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda x: r(x, k, out=out)[0] + 0, (q,), check_trace=False)
+        before = out[0]._version
+        assert torch.equal(traced(k), r(k, k)[0]) and out[0]._version > before
+
+
+def check_compiled(device):
+    """A compiled call writes where it is told, in place and into a cache too, and what follows it sees that."""
+    q, k = (t.to(device) for t in inputs(2, 3, 2, 1, 64, "bf16"))
+    r = R.Rotary(64).to(device)
+    cache = torch.zeros(2, 10, 1, 64, dtype=torch.bfloat16, device=device)
+
+    def step(q, k, cache):
+        turned, _ = r(q, k, start=4, out=(q, cache[:, 4:7]))
+        return turned * 2, cache.sum()
+    with torch.no_grad():
+        want = r(q, k, start=4)
+        torch._dynamo.reset()
+        doubled, total = torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, cache)
+    assert torch.equal(q, want[0]) and torch.equal(cache[:, 4:7], want[1]) and torch.equal(doubled, want[0] * 2)
+    assert not cache[:, :4].any() and not cache[:, 7:].any() and torch.equal(total, cache.sum())
+
+
+def test_compiled(emu_ops):
+    check_compiled("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_compiled():
+    check_compiled("cuda")
