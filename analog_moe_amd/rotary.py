@@ -44,11 +44,48 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+def _dims(t: Tensor):
+    """(stride, size) of the dimensions in which t has more than one element, the widest stride first."""
+    return sorted(((st, n) for n, st in zip(t.shape, t.stride()) if n > 1), reverse=True)
+
+
+def _reach(dims) -> int:
+    return 1 + sum(st * (n - 1) for st, n in dims)
+
+
+def _apart(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors of one type share no element, as far as their strides show it: one lies behind the other, or both
+    stay within their own part of every period of some stride that all wider ones are multiples of."""
+    x, y = _dims(a), _dims(b)
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if off >= _reach(x) or -off >= _reach(y):
+        return True
+    for m, _ in {*x, *y}:
+        if m and not any(st % m for st, _ in (*x, *y) if st >= m):
+            at = off % m
+            if _reach([d for d in x if d[0] < m]) <= at and at + _reach([d for d in y if d[0] < m]) <= m:
+                return True
+    return False
+
+
+def _check_out(q: Tensor, k: Tensor, oq: Tensor, ok: Tensor) -> None:
+    if oq.numel() + ok.numel() == 0:
+        return
+    for o in (oq, ok):
+        dims = _dims(o)
+        if any(st < _reach(dims[i + 1:]) for i, (st, _) in enumerate(dims)):
+            raise ValueError("out must have memory of its own for every element")
+    for o, t, own in ((oq, q, True), (ok, k, True), (oq, k, False), (ok, q, False), (oq, ok, False)):
+        in_place = own and o.data_ptr() == t.data_ptr() and all(n == 1 or a == b for n, a, b in zip(o.shape, o.stride(), t.stride()))
+        if o.numel() and t.numel() and not in_place and not _apart(o, t):
+            raise ValueError("out must be the inputs element for element, or have memory apart from them and from each other")
+
+
 def rotate(q: Tensor, k: Tensor, turns: Tensor, positions: Optional[Tensor] = None, start: int = 0, interleaved: bool = False,
            size: float = 1.0, inverse: bool = False, out: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor]:
     """q [B, S, H, d] and k [B, S, G, d] turned by their positions (``amoe_rotary``), into new tensors or into ``out``, whose
-    strides are free but for adjacent head elements: q and k themselves, or the next rows of a cache.  turns: int64
-    [dim / 2], as ``Rotary`` holds it; inverse: the other way round."""
+    strides are free but for adjacent head elements: q and k themselves, or memory apart from them, such as the rows of a cache
+    at which all its sequences go on.  turns: int64 [dim / 2], as ``Rotary`` holds it; inverse: the other way round."""
     ops._need_gpu(q, k, turns, positions)
     shape, kv = q.shape, k.shape
     if len(shape) != 4 or len(kv) != 4:
@@ -89,8 +126,7 @@ def rotate(q: Tensor, k: Tensor, turns: Tensor, positions: Optional[Tensor] = No
         for t, o in ((q, oq), (k, ok)):
             if o.shape != t.shape or o.dtype != dtype or o.device != device or (o.stride(3) != 1 and d > 1):
                 raise ValueError("out must have the shapes, dtype and device of q and k, with adjacent head elements")
-            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
-                raise ValueError("out must have memory of its own for every element")
+        _check_out(q, k, oq, ok)
     sq, sk, tq, tk = q.stride(), k.stride(), oq.stride(), ok.stride()
     args = _abi.ROTARY_ARGS.pack(
         code, B, S, H, kv[2], d, R, interleaved, inverse, size, turns.data_ptr(), place, place64, pb, ps, start,

@@ -83,3 +83,48 @@ def test_compiled(emu_ops):
 @pytest.mark.gpu
 def test_gpu_compiled():
     check_compiled("cuda")
+
+
+def test_outputs_that_overlap_are_refused(emu_ops):
+    """out's elements are memory of their own: of each other, of the other output, of both inputs unless they are the input."""
+    r = R.Rotary(8)
+    q, k = inputs(2, 4, 2, 1, 8, "f32")
+    room = torch.randn(2, 6, 3, 8, generator=torch.Generator().manual_seed(1))
+    a, b = room[:, 1:5, :2], room[:, 1:5, 2:]                     # packed heads
+    flat = torch.zeros(400)
+    for bad in (lambda: r(room[:, :4, :2], k, out=(a, k)),                                   # a token further on
+                lambda: r(a, k, out=(room[:, 1:5, 1:], torch.empty_like(k))),                # a head further on
+                lambda: r(q, b, out=(a, room[:, 1:5, 1:2])),                                 # one in the other
+                lambda: r(q, k, out=(torch.empty_like(q), q[:, :, :1])),                     # k's in q
+                lambda: r(q, room[:, :4, :1], out=(a, k)),                                   # q's in k, shifted
+                lambda: r(k, k, out=(k, torch.empty_like(k))),                               # q is k, and one of them written to
+                lambda: r(q, k, out=(q[:, :, :1].expand_as(q), k)),
+                lambda: r(q, k, out=(flat.as_strided((2, 4, 2, 8), (64, 8, 8, 1)), k)),      # tokens in heads
+                lambda: r(q, k, out=(flat.as_strided((2, 4, 2, 8), (30, 16, 8, 1)), k)),     # sequences in tokens
+                lambda: r(q, k, out=(flat.as_strided((2, 4, 2, 8), (60, 15, 7, 1)), k))):    # heads in heads
+        keep = [t.clone() for t in (q, k, room, flat)]
+        with pytest.raises(ValueError, match="memory"):
+            bad()
+        assert all(map(torch.equal, (q, k, room, flat), keep))
+    # what is not overlapping: in place in packed heads, heads first, tokens that alternate, the next tokens of one buffer
+    for B, S, make in ((2, 4, lambda n: n(2, 4, 3, 8)), (2, 4, lambda n: n(2, 3, 4, 8).transpose(1, 2)), (4, 2, lambda n: n(2, 4, 3, 8).transpose(0, 1)),
+                       (1, 1, lambda n: n(1, 1, 3, 8))):
+        w = make(lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(2)))
+        x, y = w[:, :, :2], w[:, :, 2:]
+        want = r(x, y)
+        got = r(x, y, out=(x, y))
+        assert all(map(torch.equal, got, want)) and torch.equal(w, torch.cat(want, 2))
+    w = torch.randn(2, 8, 3, 8, generator=torch.Generator().manual_seed(3))
+    even, odd = w[:, ::2], w[:, 1::2]
+    want = r(even[:, :, :2], even[:, :, 2:])
+    r(even[:, :, :2], even[:, :, 2:], out=(odd[:, :, :2], odd[:, :, 2:]))
+    assert torch.equal(odd, torch.cat(want, 2))
+    want = r(w[:, :3, :2], w[:, :3, 2:])
+    r(w[:, :3, :2], w[:, :3, 2:], out=(w[:, 4:7, :2], w[:, 4:7, 2:]))
+    assert torch.equal(w[:, 4:7], torch.cat(want, 2))
+    one = torch.randn(1, 1, 2, 8, generator=torch.Generator().manual_seed(4))
+    want = r(one, one[:, :, :0])
+    r(one, one[:, :, :0], out=(one.as_strided(one.shape, (5, 3, 8, 1)), one[:, :, :0]))      # (strides of single elements)
+    assert torch.equal(one, want[0])
+    none = r(q[:, :0], k[:, :0], out=(q[:, :0], q[:, :0, :1]))
+    assert none[0].shape == (2, 0, 2, 8)
