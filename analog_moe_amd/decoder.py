@@ -73,10 +73,12 @@ class RotarySelfAttention(nn.Module):
         if cache is not None:
             at = (torch.arange(B, device=x.device)[:, None], positions)
             keys, values = cache.keys[layer], cache.values[layer]
-            keys.index_put_(at, k)
-            values.index_put_(at, v)
+            keys.index_put_(at, k.to(keys.dtype))
+            values.index_put_(at, v.to(values.dtype))
             k, v, starts = keys[:, :cache.most + S], values[:, :cache.most + S], cache.held
-        return self.proj(attention(q, k, v, lengths=lengths, starts=starts).reshape(B, S, D))
+        # (a cache of another type than q's: attention in the cache's)
+        out = attention(q.to(k.dtype), k, v, lengths=lengths, starts=starts).to(q.dtype)
+        return self.proj(out.reshape(B, S, D))
 
 
 class DecoderBlock(nn.Module):
@@ -113,12 +115,15 @@ class SigmaMoEDecoder(nn.Module):
         self.head = nn.Linear(d_model, vocab_size, bias=False)
 
     def new_cache(self, batch: int, room: int) -> KVCache:
-        """An empty cache for ``batch`` sequences of up to ``room`` tokens, of the model's type and device."""
+        """An empty cache for ``batch`` sequences of up to ``room`` tokens, of the model's device and type (under autocast: of the
+        type that it makes keys and values in)."""
         if self.pos is not None:
             raise ValueError("a cache goes with rotary positions")
         attn, like = self.blocks[0].attn, self.head.weight
         shape = (len(self.blocks), batch, room, attn.kv_heads, attn.head)
-        keys, values = (torch.empty(shape, dtype=like.dtype, device=like.device) for _ in range(2))
+        kind = like.device.type
+        dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else like.dtype
+        keys, values = (torch.empty(shape, dtype=dtype, device=like.device) for _ in range(2))
         return KVCache(keys, values, torch.zeros(batch, dtype=torch.int64, device=like.device))
 
     def forward(self, ids: Tensor, labels: Optional[Tensor] = None, reg_weight: float = 0.0,
