@@ -41,7 +41,18 @@ class CausalSelfAttention(nn.Module):
 @dataclass
 class KVCache:
     """Keys (turned) and values of every layer with room for ``keys.shape[2]`` tokens a sequence.  held: int64 [batch], the
-    tokens that each sequence holds; most: no sequence holds more."""
+    tokens that each sequence holds; most: no sequence holds more.
+
+    A step of single tokens captured into a graph keeps the tensors and the number it was captured with: set ``most`` to the room
+    less one before, so that it reads keys up to the end, and advance the tensor that ``held`` was before the call, in place and
+    within the capture:
+
+        held, cache.most = cache.held, cache.keys.shape[2] - 1
+        with torch.cuda.graph(graph):
+            logits, _ = model(token, cache=cache)
+            held.add_(1)
+
+    and replay no further than the room (past it the positions are an assertion on the device)."""
     keys: Tensor                                 # [layers, batch, room, key heads, head size]
     values: Tensor
     held: Tensor
