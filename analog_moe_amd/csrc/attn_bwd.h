@@ -311,14 +311,17 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   if constexpr (!Shape::kKInLds) attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, wave0, wave_end, p.d, p.vec);
   if constexpr (!Shape::kVInLds) attn_row_frags<T, DP, EDGE>(vf, vb, p.v.ss, wave0, wave_end, p.d, p.vec);
   if constexpr (Shape::kVInLds) {
-    const int all0 = group0 < length ? group0 : 0, all_end = group0 < length ? length : 0;
-    AttnStage<T, DP, 32 * KW, NT, EDGE> st;
-    if constexpr (Shape::kKInLds) {
-      st.init(tid, p.k.ss, p.d);
-      st.load(tid, reinterpret_cast<T*>(lds_k), kb, p.k.ss, all0, all_end, p.d, p.vec);
+    // (only for tiles that come after: what is on its way into LDS is waited for there, and would else outlive the workgroup)
+    if (n_tiles > 0) {
+      const int all0 = group0 < length ? group0 : 0, all_end = group0 < length ? length : 0;
+      AttnStage<T, DP, 32 * KW, NT, EDGE> st;
+      if constexpr (Shape::kKInLds) {
+        st.init(tid, p.k.ss, p.d);
+        st.load(tid, reinterpret_cast<T*>(lds_k), kb, p.k.ss, all0, all_end, p.d, p.vec);
+      }
+      st.init(tid, p.v.ss, p.d);
+      st.load(tid, reinterpret_cast<T*>(lds_v), vb, p.v.ss, all0, all_end, p.d, p.vec);
     }
-    st.init(tid, p.v.ss, p.d);
-    st.load(tid, reinterpret_cast<T*>(lds_v), vb, p.v.ss, all0, all_end, p.d, p.vec);
   }
   AttnGrad<T, DP> dk, dv;
   dk.clear();

@@ -272,3 +272,27 @@ def test_rest(emu_ops, dtype, S, d):
 @pytest.mark.parametrize("dtype, S, d", [("bf16", 300, 64), ("f16", 300, 96), ("bf16", 200, 128), ("bf16", 200, 13)])
 def test_gpu_rest(dtype, S, d):
     check_rest(dtype, S, d, "cuda")
+
+
+def check_keys_that_no_query_sees(d, T, device="cpu"):
+    """Zeros, beside gradients of keys that are seen; the workgroups of the former have nothing to wait for."""
+    q, k, v, go = inputs(2, 40, T, 2, 1, d, "bf16")
+    starts = torch.tensor([30, 0])
+    want, bounds = O.attention(q, k, v, go, starts=starts)
+    on, starts = [t.to(device) for t in (q, k, v, go)], starts.to(device)
+    out, lse, rest = A.attention_forward(*on[:3], None, starts, want_lse=True)
+    grads = A.attention_backward(on[3], *on[:3], out, lse, rest, None, starts)
+    compare((out, *grads), want, bounds, d)
+    for g in grads[1:]:
+        assert g[0, :70].any(-1).all() and not g[0, 70:].any() and g[1, :40].any(-1).all() and not g[1, 40:].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_that_no_query_sees(emu_ops, d):
+    check_keys_that_no_query_sees(d, 200)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d, T", [(64, 200), (64, 20000), (128, 5000)])
+def test_gpu_keys_that_no_query_sees(d, T):
+    check_keys_that_no_query_sees(d, T, "cuda")
