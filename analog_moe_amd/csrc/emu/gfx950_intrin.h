@@ -22,10 +22,16 @@ inline u32x4 buffer_load_b128(BufRsrc r, uint32_t lane_off, uint32_t uniform_off
   return v;
 }
 inline void buffer_to_lds_b128(BufRsrc r, void* lds, uint32_t lane_off) {
-  const u32x4 v = buffer_load_b128(r, lane_off, 0);
-  std::memcpy(static_cast<char*>(lds) + 16 * (threadIdx.x & 63), &v, 16);
+  const bool in = r.bytes == 0xffffffffu || (uint64_t)lane_off + 16 <= r.bytes;
+  emu_lds_copies.push_back({in ? r.base + (size_t)lane_off : nullptr, static_cast<char*>(lds) + 16 * (threadIdx.x & 63)});
 }
-inline void lds_dma_wait() {}
+inline void lds_dma_wait() {
+  for (const EmuLdsCopy& c : emu_lds_copies) {
+    if (c.from) std::memcpy(c.to, c.from, 16);
+    else std::memset(c.to, 0, 16);
+  }
+  emu_lds_copies.clear();
+}
 inline uint32_t buffer_load_b32(BufRsrc r, uint32_t lane_off, uint32_t uniform_off = 0) {
   uint32_t v;
   std::memcpy(&v, r.base + (size_t)lane_off + (size_t)uniform_off, 4);

@@ -139,6 +139,16 @@ struct EmuBlock {
 inline thread_local EmuWave* emu_wave = nullptr;
 inline thread_local EmuBlock* emu_block = nullptr;
 
+// What a thread has on its way into LDS: there when it waits for it and not before, so that a read that comes too early finds
+// the old contents.  What no wait had brought in when its thread ended is counted.
+struct EmuLdsCopy {
+  const void* from;                  // null: zeros
+  void* to;
+};
+inline thread_local std::vector<EmuLdsCopy> emu_lds_copies;
+inline std::atomic<long long> emu_lds_copies_left{0};
+extern "C" inline __attribute__((used)) long long amoe_emu_lds_copies_left() { return emu_lds_copies_left.load(); }
+
 inline void __syncthreads() { emu_block->bar->arrive_and_wait(); }
 
 template <class T> inline T atomicAdd(T* p, T v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
@@ -179,6 +189,7 @@ inline void emu_launch(K kernel, dim3 grid, dim3 block, A... args) {
         emu_wave = &waves[t / 64];
         emu_block = &blk;
         kernel(args...);
+        emu_lds_copies_left += (long long)emu_lds_copies.size();
       });
     }
     for (auto& x : th) x.join();

@@ -274,6 +274,20 @@ def test_gpu_rest(dtype, S, d):
     check_rest(dtype, S, d, "cuda")
 
 
+def test_no_copy_into_lds_is_left_behind(emu_ops):
+    """What a workgroup has on its way into LDS when it ends would land in the next one's: every copy has been waited for."""
+    import ctypes
+    left = emu_ops.get_lib().amoe_emu_lds_copies_left
+    left.restype = ctypes.c_longlong
+    before = left()
+    for d in (64, 128):
+        for S, T, kw in ((40, 200, dict(starts=torch.tensor([30, 0]))), (3, 70, {}), (70, 40, dict(lengths=torch.tensor([40, 0])))):
+            q, k, v, go = inputs(2, S, T, 2, 1, d, "bf16")
+            out = A.attention_forward(q, k, v, **kw, want_lse=True)
+            A.attention_backward(go, q, k, v, *out, **kw)
+            assert left() == before, (d, S, T)
+
+
 def check_keys_that_no_query_sees(d, T, device="cpu"):
     """Zeros, beside gradients of keys that are seen; the workgroups of the former have nothing to wait for."""
     q, k, v, go = inputs(2, 40, T, 2, 1, d, "bf16")
