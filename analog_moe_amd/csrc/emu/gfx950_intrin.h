@@ -228,9 +228,6 @@ inline float fast_log2(float x) { return log2f(x); }
 inline float add_bf16x2(uint32_t w, float c) {
   return c + (__builtin_bit_cast(float, w << 16) + __builtin_bit_cast(float, w & 0xffff0000u));
 }
-inline float add_f16x2(uint32_t w, float c) {
-  return c + ((float)__builtin_bit_cast(_Float16, (uint16_t)w) + (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)));
-}
 inline float fast_exp2(float x) { return exp2f(x); }
 inline void sincos_half_turns(float x, float* s, float* c) {
   *s = (float)std::sin(3.14159265358979323846 * x);

@@ -145,14 +145,10 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
-// c plus the two bf16 (fp16) elements of a word, in fp32: a dot product with ones, one instruction
+// c plus the two bf16 elements of a word, in fp32: a dot product with ones, one instruction
 __device__ __forceinline__ float add_bf16x2(uint32_t w, float c) {
   typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
-}
-__device__ __forceinline__ float add_f16x2(uint32_t w, float c) {
-  typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), __builtin_bit_cast(f16x2_t, 0x3c003c00u), c, false);
 }
 
 // clamp(x, -r, r) for r >= 0 as one v_med3_f32 (a NaN input gives -r or r instead of NaN).

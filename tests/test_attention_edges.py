@@ -227,6 +227,39 @@ def test_gpu_equal_values(name):
     check_equal_values(name, "cuda")
 
 
+def check_tail(dtype, S, device="cpu"):
+    """A long tail of keys with 2^-22 of the largest probability: as fp16 operands subnormal numbers, which the sum has to count as
+    the product does.  Both are a mean of equal values."""
+    T, d = 4000, 64
+    q, k, v = torch.zeros(1, S, 2, d), torch.zeros(1, T, 1, d), torch.ones(1, T, 1, d)
+    q[..., 0] = 1.0
+    k[0, 1:, 0, 0] = -15.25
+    v[..., ::2] = 3.0
+    q, k, v = (t.to(DT[dtype]).to(device) for t in (q, k, v))
+    out, _, rest = A.attention_forward(q, k, v, causal=False, scale=1.0, want_lse=True)
+    have = (out.double() + (0 if rest is None else rest.double())).cpu()
+    want = v[:, :1].double().cpu().expand_as(have)
+    # a lane adds half the keys two by two, the product 16 at a time
+    assert ((have - want).abs() <= (T / 4 + T / 16 + 16) * 2.0 ** -24 * want).all()
+    # with other values in the tail: a thousandth of them arrives
+    v[:, 1:] = 0.0
+    have = A.attention_forward(q, k, v, causal=False, scale=1.0)[0].double().cpu()
+    tail = (T - 1) * math.exp(-15.25)
+    off = torch.finfo(q.dtype).eps / 2 + 2.0 ** -11 * tail + 2.0 ** -13
+    assert 9e-4 < tail and ((have - want / (1 + tail)).abs() <= off * want).all()
+
+
+@pytest.mark.parametrize("dtype, S", [("f16", 1), ("f16", 40), ("bf16", 1)])
+def test_tail(emu_ops, dtype, S):
+    check_tail(dtype, S)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, S", [("f16", 1), ("f16", 300), ("bf16", 1), ("bf16", 300)])
+def test_gpu_tail(dtype, S):
+    check_tail(dtype, S, "cuda")
+
+
 def check_rest(dtype, S, d, device="cpu"):
     """Queries of zeros: a row is the mean of the values it sees, its probabilities are exact (the maximum is 0, each 2^0, the sum
     a whole number), so that nothing but the output's rounding is off by more than some 2^-24."""
