@@ -15,8 +15,6 @@ template <typename T> inline constexpr float kGradShift = kIsF16<T> ? 15.f : 0.f
 // further from zero than kFar get theirs from a maximum and a sum made again: P = 2^((s - top) c - norm), with the maximum taken
 // out before the multiplication and norm the logarithm of the sum.  Other rows: top 0, norm lse.
 __device__ __forceinline__ bool attn_is_far(float lse, float limit) { return fabsf(lse) > limit && fabsf(lse) <= kMaxFloat; }
-// (a score made in another kernel may not be above the maximum either)
-__device__ __forceinline__ float attn_below(float s, float top) { return fminf(s - top, 0.f); }
 
 // top and norm of a wave's far rows, whose queries q holds: the keys they see once more, from memory
 template <typename T, int DP, bool EDGE>
@@ -190,14 +188,22 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
           if (e & 1) dp = attn_mma<T>(a, go[e / 2], dp);
           else s = attn_mma<T>(a, q[e / 2], s);
         });
-        if (any_far) {
-#pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = far ? attn_below(s[e], top) : s[e];
-        }
         float ds[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) ds[e] = fast_exp2(fmaf(s[e], p.c, -norm)) * (dp[e] - delta);
-        if (mask) {
+        if (mask || any_far) {
+          if (any_far) {
+            // (the products once more, within the branch that there is: a branch of its own before the exponentials, or scores kept
+            // for this one, cost every block more)
+            s = dp = f32x16_zero();
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+              s = attn_mma<T>(Tile::row_frag(lds_k, in, 32 * n, kk), q[kk], s);
+              dp = attn_mma<T>(Tile::row_frag(lds_v, in, 32 * n, kk), go[kk], dp);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) ds[e] = fast_exp2(fmaf(s[e] - top, p.c, -norm)) * (dp[e] - delta);
+          }
 #pragma unroll
           for (int e = 0; e < 16; e++)
             if (key0 + 32 * n + 8 * (e / 4) + 4 * h + e % 4 >= w.seen) ds[e] = 0.f;
@@ -263,8 +269,9 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   static_assert(KW * (QW - 1) <= 2 * kSumsPer, "the copies' sums fit the tiles' room");
   __shared__ __align__(1024) char lds_q[kTilesBytes], lds_g[kTilesBytes];
   __shared__ __align__(1024) char lds_k[Shape::kKInLds ? 32 * KW * DP * (int)sizeof(T) : 16], lds_v[Shape::kVInLds ? 32 * KW * DP * (int)sizeof(T) : 16];
-  __shared__ __align__(16) float lds_rows[3][2][BM];              // norm, delta, top
-  __shared__ int lds_far[2][QW];                                  // a block of 32 queries has one with a top
+  // norm, delta, top.  Scores here are those of the maximum to the last bit: the same products summed in the same order, whichever
+  // of q and k is the first operand
+  __shared__ __align__(16) float lds_rows[3][2][BM];
   T *const tq = reinterpret_cast<T*>(lds_q), *const tg = reinterpret_cast<T*>(lds_g);
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), kw = wave % KW, qw = wave / KW, h = lane >> 5;
   const int BG = p.B * p.G, bg = (int)(blockIdx.x % (unsigned)BG), tile = (int)(blockIdx.x / (unsigned)BG);
@@ -282,7 +289,7 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
   sq.init(tid, p.q.ss, p.d);
   sg.init(tid, p.go.ss, p.d);
   static_assert(3 * BM <= NT && BM % 64 == 0, "a thread for each, whole waves");
-  const int part = tid / BM;                          // threads 0 .. BM - 1: norm, the next BM: delta, the next: top
+  const int part = wave_uniform(tid / BM);            // threads 0 .. BM - 1: norm, the next BM: delta, the next: top
   float stat = 0.f;
   const auto fetch = [&](int t) {
     const int hd = g * p.R + t / per_head, q0 = (tile0 + t % per_head) * BM, buf = t & 1;
@@ -298,10 +305,6 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
     sq.store(tid, tq + buf * kTileElems);
     sg.store(tid, tg + buf * kTileElems);
     if (part < 3) lds_rows[part][buf][tid % BM] = stat;
-    if (part == 2) {
-      const uint64_t tops = wave_ballot(stat != 0.f);
-      if (lane % 32 == 0) lds_far[buf][tid % BM / 32] = (uint32_t)(tops >> lane) != 0;
-    }
   };
   if (n_tiles > 0) fetch(0);
   attn_frag<T> kf[NK], vf[NK];
@@ -367,22 +370,15 @@ __global__ __launch_bounds__((Shape::kThreads), (Shape::kWavesPerSimd)) void att
           dp = attn_mma<T>(rows, a, dp);
         }
       });
-      if (wave_uniform(lds_far[buf][qw]) != 0) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const f32x4 top = *reinterpret_cast<const f32x4*>(&lds_rows[2][buf][32 * qw + 8 * u + 4 * h]);
-#pragma unroll
-          for (int j = 0; j < 4; j++) s[4 * u + j] = top[j] != 0.f ? attn_below(s[4 * u + j], top[j]) : s[4 * u + j];
-        }
-      }
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const f32x4 norm = *reinterpret_cast<const f32x4*>(&lds_rows[0][buf][32 * qw + 8 * u + 4 * h]);
         const f32x4 del = *reinterpret_cast<const f32x4*>(&lds_rows[1][buf][32 * qw + 8 * u + 4 * h]);
+        const f32x4 top = *reinterpret_cast<const f32x4*>(&lds_rows[2][buf][32 * qw + 8 * u + 4 * h]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int e = 4 * u + j;
-          s[e] = fast_exp2(fmaf(s[e], p.c, kGradShift<T> - norm[j]));
+          s[e] = fast_exp2(fmaf(s[e] - top[j], p.c, kGradShift<T> - norm[j]));
           dp[e] = s[e] * (dp[e] - del[j]);
         }
       }
