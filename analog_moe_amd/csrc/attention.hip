@@ -41,13 +41,21 @@ int check_sizes(const amoe_attn_args* a) {
 }
 
 // Parts of the key axis for the kernel of few rows; 0: the kernel of many rows.
+//
+// Up to 32 rows share one read of the keys.  More are read for 32 by 32, which pays where blocks of 32 rows would not fill half the
+// CUs and every one of them would walk many keys by itself: with n of them, from 32 n keys on, and 1024.  Measured (us, many rows /
+// parts; 16 over 4 heads of 128, one sequence, then of 64, four; bf16): 40 queries (n = 32) over 600 keys 11.5 / 11.2, 1024
+// 15.3 / 11.8, 8192 92 / 23; 100 (64) over 1024 15.3 / 16.9, 2000 25 / 20, 8192 91 / 35; 250 (128) over 2000 25 / 28, 8192 90 / 65;
+// 4 x 40 (128) over 2000 15 / 19, 8192 49 / 29; 4 x 100 (256) over 2000 16 / 28, 8192 49 / 59, 32768 182 / 200.
 int attn_splits(const amoe_attn_args* a) {
   const int64_t rows = a->H / a->G * a->S, cus = num_compute_units();
-  const int64_t many = a->B * a->H * ((a->S + 127) / 128);
-  if (rows > 32 && (many * 2 > cus || a->T < 1024)) return 0;
+  const int64_t blocks = a->B * a->H * ((a->S + 31) / 32);
+  if (rows > 32 && (2 * blocks > cus || a->T < 1024 || a->T < 32 * blocks)) return 0;
   const int64_t groups = a->B * a->G * ((rows + 31) / 32);
   // parts of 512 keys or more, up to eight workgroups per CU (sequences differ in length, and the last round of workgroups
-  // is then short); where that leaves CUs without work, parts of down to 128 keys for two
+  // is then short); where that leaves CUs without work, parts of down to 128 keys for two.  One query over 131071 keys, 16 over 2
+  // heads of 128: 28 us, parts of 256 31.5, of 1024 28; 8 over 4096 to 8192, 16 over 4: 25, 27.6 and 26.7; 256 over 512 to 1024:
+  // 99, 100 and 87.  The smaller ones at least 256: one over 1024 keys, 16 heads of 64, 8.2 us for 7.8, over 4096 10.6 for 10.0
   const auto parts = [&](int64_t per_cu, int64_t keys) {
     const int64_t n = (per_cu * cus + groups - 1) / groups, most = (a->T + keys - 1) / keys;
     return n < most ? n : most;

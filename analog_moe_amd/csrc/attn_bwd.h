@@ -253,7 +253,8 @@ template <typename T, int DP, bool EDGE, int QW_> struct AttnKvShape {
   static constexpr int KW = 2, QW = QW_, kThreads = 64 * KW * QW;
   // k and v read from LDS for every product, for the registers that makes free.  16-bit heads past 96: v only, with dk, dv and k
   // the registers are full (both do not fit LDS).  Heads of 64, two copies: both, for a third workgroup on the CU (16 x 1024, 16 heads
-  // of 64, bf16: 123 us with two; with three 100 us, or 115 with k in registers and 4 of them in memory).
+  // of 64, bf16: 123 us with two; with three 100 us, or 115 with k in registers and 4 of them in memory).  Heads of 96 have room for
+  // neither third workgroup nor more reads ahead: v there or not is the same (16 x 1024, 16 heads: dq, dk and dv 324 us), both 430.
   static constexpr bool kVInLds = sizeof(T) == 2 && !EDGE && (DP == 128 || (DP == 64 && QW == 2)), kKInLds = kVInLds && DP == 64;
   static constexpr int kWavesPerSimd = sizeof(T) * DP > 256 || EDGE ? 1 : kKInLds ? 3 : 2;       // fp32 heads past 64: 512 registers a wave
   static constexpr int kAhead = kKInLds ? 4 : kVInLds ? 3 : kAttnAhead<T>;                       // (more do not fit the registers)

@@ -77,6 +77,29 @@ def test_gpu(name):
     check(sizes, dtype, layout, o, "cuda", sorted({(0, 0), (1, G - 1), (B // 2, G // 2), (B - 1, G - 1)}))
 
 
+# More than 32 rows that share keys, in parts of the key axis and in one.
+FEW = {
+    "parts_bf16": (1, 100, 2100, 16, 4, 128, "bf16", "cache", dict(lengths=[2090], starts=[1990])),
+    "parts_f16": (1, 250, 4200, 16, 4, 64, "f16", "own", {}),
+    "parts_f32": (2, 33, 4100, 4, 1, 64, "f32", "own", dict(lengths=[4100, 77], starts=[4067, 50])),
+    "one_bf16": (1, 250, 4000, 16, 4, 128, "bf16", "own", {}),
+    "one_f16": (4, 100, 2000, 16, 4, 64, "f16", "cache", {}),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(FEW))
+def test_gpu_few_rows(name):
+    from analog_moe_amd import ops
+    *sizes, dtype, layout, o = FEW[name]
+    q, k, v = (torch.empty(sizes[0], n, h, sizes[5], dtype=base.DT[dtype], device="cuda") for n, h in
+               ((sizes[1], sizes[3]), (sizes[2], sizes[4]), (sizes[2], sizes[4])))
+    need = ops.get_lib().amoe_attention_fwd_workspace(A._Call(q, k, v, None, None, True, None).pack(q, None, None))
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert (need > 0) == name.startswith("parts")
+    check(sizes, dtype, layout, o, "cuda", [(0, 0), (sizes[0] - 1, sizes[4] - 1)])
+
+
 # On one compute unit the same forms are reached by sizes that the host build can run.
 SMALL = {
     "bf16_64": (1, 200, 200, 2, 1, 64, "bf16", "packed", {}),
