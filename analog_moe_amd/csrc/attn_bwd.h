@@ -94,8 +94,8 @@ __device__ __forceinline__ void attn_pack_block(const V& v, attn_frag<T> (&f)[2]
 }
 
 // dq: 32 * RW queries of one head per workgroup, keys in tiles as in the forward pass; three products per block.  Also leaves
-// norm, delta and top of every row.  Bound as the forward pass is: 8192 queries, 16 over 4 heads of 128, bf16, causal: 394 us, 1050 TFLOP/s; 16 x 1024, 16
-// heads of 64: 78 us.
+// norm, delta and top of every row.  Bound as the forward pass is: 8192 queries, 16 over 4 heads of 128, bf16, causal: 398 us,
+// 1035 TFLOP/s; 16 x 1024, 16 heads of 64: 87 us.
 template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
 __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd_q_kernel(AttnParams p) {
   using Tile = AttnTile<T, DP>;
@@ -246,14 +246,14 @@ __global__ __launch_bounds__(kAttnThreads, (Shape::kWavesPerSimd)) void attn_bwd
 // reads what the other keys' waves read; more copies make shorter loops of the same work where there are few keys, and finer
 // workgroups where causal rows differ in length.  Four products per block; heads of 128 are bound by registers (two waves on a
 // SIMD with every one of them used, and operands no more than three reads ahead), heads of 64 by the vector work.  8192 keys, 16
-// over 4 heads of 128, bf16, causal: 650 us, 850 TFLOP/s; 16 x 1024, 16 heads of 64: 100 us.  Measured and not kept there: the
+// over 4 heads of 128, bf16, causal: 653 us, 840 TFLOP/s; 16 x 1024, 16 heads of 64: 122 us.  Measured and not kept there: the
 // exponentials between the products of one wave (900 us), two workgroups of four waves on a CU (1000 us), the queries from the
 // other end (no difference).
 template <typename T, int DP, bool EDGE, int QW_> struct AttnKvShape {
   static constexpr int KW = 2, QW = QW_, kThreads = 64 * KW * QW;
   // k and v read from LDS for every product, for the registers that makes free.  16-bit heads past 96: v only, with dk, dv and k
   // the registers are full (both do not fit LDS).  Heads of 64, two copies: both, for a third workgroup on the CU (16 x 1024, 16 heads
-  // of 64, bf16: 123 us with two; with three 100 us, or 115 with k in registers and 4 of them in memory).  Heads of 96 have room for
+  // of 64, bf16: 146 us with two; with three 122 us, and as much with k in registers).  Heads of 96 have room for
   // neither third workgroup nor more reads ahead: v there or not is the same (16 x 1024, 16 heads: dq, dk and dv 324 us), both 430.
   static constexpr bool kVInLds = sizeof(T) == 2 && !EDGE && (DP == 128 || (DP == 64 && QW == 2)), kKInLds = kVInLds && DP == 64;
   static constexpr int kWavesPerSimd = sizeof(T) * DP > 256 || EDGE ? 1 : kKInLds ? 3 : 2;       // fp32 heads past 64: 512 registers a wave

@@ -7,7 +7,7 @@ namespace amoe {
 
 // A row's scores are kept as s * c in the exponent of 2.  The maximum that is taken out of them lags behind: it follows only when
 // a larger one leaves it by more than 2^kMaxLag, which after a row's first keys it hardly ever does (following at every step
-// costs a multiplication of the whole output state: 8192 queries of 16 heads of 128, bf16, 350 us, so 309 us); sums in fp32 and
+// costs a multiplication of the whole output state: 8192 queries of 16 heads of 128, bf16, 311 us, so 285 us); sums in fp32 and
 // bf16 operands have the range for that.  fp16 probabilities are kept 2^7 times as large, which with the lag stays below 2^16:
 // what is 2^-21 of a row's largest is still a normal number, where at 1 times a long row's tail below 2^-14 would lose bits
 // that its sum counts.  The sum carries the same factor and the quotient none.
@@ -163,10 +163,11 @@ __device__ __forceinline__ void attn_add_acc(const f32x4* lds, int copy, f32x16 
 // tiles by turns with one barrier each.  Two products of 32 x 32 x d per block of 32 keys on the matrix unit, 16 exponentials and
 // about 55 other vector instructions a lane between them, which are the longer part for heads of 64; operands of one wave's
 // 32 queries only, as 64 would leave one wave on a SIMD with nobody to fill its waits.  8192 queries, 16 over 4 heads of 128,
-// bf16, causal: 283 us, 970 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 64 us, half
+// bf16, causal: 285 us, 965 TFLOP/s where a library product of 8192^3 reaches 1375; 16 x 1024, 16 heads of 64: 70 us, half
 // of it the time that q, k, v and the two results take to pass through memory.
 // Heads past 96 take one block of keys at a time, and with operands no more than four reads ahead three workgroups fit a CU (8192
-// queries as above: two blocks and two workgroups 312 us, one and three 294 us in turns on one card).
+// queries as above: two blocks and two workgroups 298 us, one and two 288, one and three 285).  Times of kernels in these files are
+// means of 20 launches in a trace; the least are 5 to 15 % shorter where launches in a row bring the clock down.
 template <typename T, int DP, bool EDGE, int RW>
 inline constexpr bool kAttnThree = sizeof(T) == 2 && DP == 128 && !EDGE && RW == 4;
 template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
 // Few rows: the R * S rows that share a key head, 32 per workgroup, and one of `splits` parts of the keys they see; every
 // wave takes every fourth block of 32 keys of the part.  K goes from global memory into the operands, V through a tile of the
 // wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.  Bound by
-// memory: 48 sequences over caches of 4096 to 8192, 16 over 4 heads of 128, bf16: 134 us for 604 MB (4.5 TB/s, a large copy
+// memory: 48 sequences over caches of 4096 to 8192, 16 over 4 heads of 128, bf16: 133 us for 604 MB (4.5 TB/s, a large copy
 // reaches 5.1); one over 131071 keys, 16 over 2 heads, fp16: 24 us for 134 MB (5.6 TB/s, part of it from the cache behind the
 // L2), and 5 us for the join.
 template <typename T, int DP, bool EDGE>

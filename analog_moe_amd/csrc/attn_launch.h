@@ -17,9 +17,9 @@ namespace amoe {
 
 // Waves over the rows of a workgroup (AttnShape) by how many workgroups there are: four where two can be on every CU, else two,
 // and one where those would not give every CU a workgroup; the tiles' room allowing.  Measured, forward pass: 256 workgroups of
-// 128 rows (2 sequences of 1024, 16 heads of 64, fp32) 88 us, 512 of 64 66 us, 1024 of 32 78 us; 256 of 128 (2 x 1003 queries over
-// 5003 keys, 16 heads of 128, bf16) 98 us, 512 of 64 90 us; 8 of 128 (2 x 100, 4 heads of 32, fp32) 14 us, 16 of 64 10 us, 32 of 32
-// 8 us; 2048 of 128 (16 x 1024, 16 heads of 64, bf16) 65 us, 4096 of 64 77 us.
+// 128 rows (2 sequences of 1024, 16 heads of 64, fp32) 87 us, 512 of 64 62 us, 1024 of 32 75 us; 256 of 128 (2 x 1003 queries over
+// 5003 keys, 16 heads of 128, bf16) 100 us, 512 of 64 75 us, 1024 of 32 168 us; 8 of 128 (2 x 100, 4 heads of 32, fp32) 14 us, 16 of
+// 64 10 us, 32 of 32 8 us; 2048 of 128 (16 x 1024, 16 heads of 64, bf16) 70 us, 4096 of 64 88 us.
 template <template <int> class Launch, bool FITS2, bool FITS1>
 int launch_attn_rows(const AttnParams& p, hipStream_t st) {
   const int64_t heads = (int64_t)p.B * p.H, want = 2 * num_compute_units();
@@ -76,8 +76,8 @@ int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
 }
 
 // Copies of the waves over the queries: two where there are two workgroups for every CU, else four.  Measured: 324 workgroups
-// (6 padded sequences of 1717, 2 key heads of 80, fp16) 146 us with two, 105 us with four; 512 (2 x 1024, 16 heads of 64, fp32) 116
-// and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 100 and 206 us.
+// (6 padded sequences of 1717, 2 key heads of 80, fp16) 141 us with two, 108 us with four; 512 (2 x 1024, 16 heads of 64, fp32) 119
+// and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 125 and 214 us.
 template <typename T, int DP, bool EDGE, int QW>
 int launch_attn_kv_of(const AttnParams& p, int64_t groups, hipStream_t st) {
   hipLaunchKernelGGL((&attn_bwd_kv_kernel<T, DP, EDGE, QW>), dim3((unsigned)groups), dim3(AttnKvShape<T, DP, EDGE, QW>::kThreads), 0, st, p);

@@ -205,9 +205,9 @@ template <typename T, int DP, bool EDGE, int RW_> struct AttnShape {
 };
 
 // A run of matrix products whose first operands come from LDS, with kAttnAhead of them on their way: a read takes as long as
-// three or four products, and left to itself the compiler has one in flight (dk and dv of 8192 keys, heads of 128: 2090 us so,
-// 1435 us with six; eight are no faster).  Nothing is moved across a step.  fp32 products take eight instructions each: two
-// ahead do.
+// three or four products, and left to itself the compiler has one in flight (8192 queries, 16 over 4 heads of 128: forward 325 us
+// with one ahead, 285 with four; dk and dv 728 with one, 653 with three).  Nothing is moved across a step.  fp32 products take
+// eight instructions each: two ahead do.
 template <typename T> inline constexpr int kAttnAhead = sizeof(T) == 4 ? 2 : 6;
 template <typename T, int N, int AHEAD = kAttnAhead<T>> struct AttnRun {
   static constexpr int D = AHEAD < N ? AHEAD : N;

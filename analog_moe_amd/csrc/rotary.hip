@@ -4,8 +4,8 @@
 // turns[i] is the fraction of a revolution per position times 2^64, so that the angle is the low 64 bits of an integer product:
 // exact for any position, where 32-bit floats lose the angle of far ones.  q and k go in one launch.  Bound by memory: every
 // element is read and written once, in 16-byte chunks; a token's sines and cosines are made once per workgroup, in LDS.  16 x 1024
-// tokens, 32 heads of 64, bf16: 27.5 us for 134 MB (4.9 TB/s, a large copy reaches 5.1); 50001 tokens, 20 heads of 128, half of
-// each turned, fp16: 117 us for 512 MB (4.4 TB/s).
+// tokens, 32 heads of 64, bf16: 26.7 us for 134 MB (5.0 TB/s, a large copy reaches 5.1); 50001 tokens, 20 heads of 128, half of
+// each turned, fp16: 116 us for 512 MB (4.4 TB/s).
 #include <amoe.h>
 
 #include "host_util.h"
