@@ -122,6 +122,10 @@ PROTOTYPES = {
     "amoe_attention_bwd_workspace": (SZ, [P]),
     "amoe_attention_bwd": (C.c_int, [P, P, SZ, P]),
     "amoe_attn_args_bytes": (SZ, []),
+    "amoe_layer_norm_fwd": (C.c_int, [P, P]),
+    "amoe_layer_norm_bwd_workspace": (SZ, [P]),
+    "amoe_layer_norm_bwd": (C.c_int, [P, P, SZ, P]),
+    "amoe_norm_args_bytes": (SZ, []),
     "amoe_select_workspace": (SZ, [I64, I32]),
     "amoe_select_fwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, SZ, P]),
     "amoe_select_bwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, P]),
@@ -140,7 +144,7 @@ FFN_ARGS = struct.Struct("<"
                          "6qq3d"       # dy grad_x grad_keys grad_values grad_gate grad_ir, gradient_relative, 3 scalars
                          "q")          # stage_events
 
-# amoe_rotary_args and amoe_attn_args, likewise
+# the decoder's, likewise
 ROTARY_ARGS = struct.Struct("<"
                             "9qd"         # dtype B S q_heads k_heads d R interleaved inverse, size
                             "q2q3q"       # turns, positions positions_are_i64, 2 strides start
@@ -151,6 +155,11 @@ ATTN_ARGS = struct.Struct("<"
                           "2q2q"          # lengths lengths_is_i64, starts starts_is_i64
                           "3q"            # out lse rest
                           "4q3q")         # go with 3 strides, dq dk dv
+NORM_ARGS = struct.Struct("<"
+                          "4qd"           # dtype weight_dtype rows D, eps
+                          "2q3q"          # x ldx, weight bias stats
+                          "2q2q"          # residual ldr, y sum
+                          "4q3q")         # gy ldgy gs ldgs, dx dweight dbias
 
 
 @functools.lru_cache(maxsize=256)
@@ -167,7 +176,7 @@ def bind(path: str) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS)):
+    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS), ("norm", NORM_ARGS)):
         if getattr(lib, f"amoe_{name}_args_bytes")() != layout.size:
             raise RuntimeError(f"{path}: amoe_{name}_args has another layout than this package packs")
     return lib

@@ -16,6 +16,7 @@ so every group of calls the Python layer makes is one opaque operator with a fak
   amoe::cvmm_backward       everything CVMM.backward launches (cvmm.py:772-897)
   amoe::ffn_fwd / ffn_bwd   the fused expert feed-forward, with its autograd formula registered
   amoe::attention_fwd / attention_bwd, amoe::rotary / rotary_into   the decoder's attention and rotary positions, likewise
+  amoe::layer_norm_fwd / layer_norm_bwd                             its layer norm, likewise
 
 Operators return an empty tensor where the Python interface returns ``None``.
 """
@@ -26,7 +27,7 @@ from typing import List, Optional
 import torch
 from torch import Tensor
 
-from . import attention, ffn, ops, rotary
+from . import attention, ffn, norm, ops, rotary
 
 _EMPTY_SHAPE = (0,)
 
@@ -452,3 +453,54 @@ def rotary_into(q, k, q_out, k_out, turns, positions, start, interleaved, size):
 @rotary_into.register_fake
 def _(q, k, q_out, k_out, turns, positions, start, interleaved, size):
     return None
+
+
+# --------------------------------------------------------------------------- layer norm
+@torch.library.custom_op(
+    "amoe::layer_norm_fwd", mutates_args=(),
+    schema="(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)")
+def layer_norm_fwd(x, residual, weight, bias, eps):
+    """(y, s or empty, stats [rows, 3])."""
+    y, s, stats = norm.layer_norm_forward(x, weight, bias, eps, residual, want_stats=True)
+    return y, x.new_empty(_EMPTY_SHAPE) if s is None else s, stats
+
+
+@layer_norm_fwd.register_fake
+def _(x, residual, weight, bias, eps):
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty(tuple(x.shape)), x.new_empty(_EMPTY_SHAPE if residual is None else tuple(x.shape)),
+            torch.empty((rows, 3), dtype=torch.float32, device=x.device))
+
+
+@torch.library.custom_op(
+    "amoe::layer_norm_bwd", mutates_args=(),
+    schema="(Tensor gy, Tensor s, Tensor? weight, Tensor? bias, Tensor stats, Tensor? gs) -> (Tensor, Tensor, Tensor)")
+def layer_norm_bwd(gy, s, weight, bias, stats, gs):
+    """(gradient of s, of weight or empty, of bias or empty)."""
+    dx, dw, db = norm.layer_norm_backward(gy, s, weight, bias, stats, gs)
+    return dx, s.new_empty(_EMPTY_SHAPE) if dw is None else dw, s.new_empty(_EMPTY_SHAPE) if db is None else db
+
+
+@layer_norm_bwd.register_fake
+def _(gy, s, weight, bias, stats, gs):
+    return (s.new_empty(tuple(s.shape)), *(s.new_empty(_EMPTY_SHAPE) if t is None else torch.empty_like(t) for t in (weight, bias)))
+
+
+def _layer_norm_setup_context(ctx, inputs, output):
+    x, residual, weight, bias, _ = inputs
+    _, s, stats = output
+    ctx.with_sum = residual is not None
+    ctx.save_for_backward(s if ctx.with_sum else x, weight, bias, stats)
+    ctx.set_materialize_grads(False)
+
+
+def _layer_norm_autograd(ctx, gy, gs, _grad_stats):
+    s, weight, bias, stats = ctx.saved_tensors
+    gs = gs if ctx.with_sum else None
+    if gy is None:
+        return gs, gs, None, None, None
+    dx, dw, db = torch.ops.amoe.layer_norm_bwd(gy, s, weight, bias, stats, gs)
+    return dx, dx if ctx.with_sum else None, None if weight is None else dw, None if bias is None else db, None
+
+
+layer_norm_fwd.register_autograd(_layer_norm_autograd, setup_context=_layer_norm_setup_context)

@@ -506,6 +506,36 @@ size_t amoe_attention_bwd_workspace(const amoe_attn_args* args);
 int amoe_attention_bwd(const amoe_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t amoe_attn_args_bytes(void);
 
+/* ---------------------------------------------------------------------------------------
+ * The decoder's layer norm (nothing of the reference's own is replaced here).  Every field is 8 bytes wide.
+ *
+ * y = (s - mean) / sqrt(var + eps) * weight + bias over rows of D elements, s = x, or x + residual rounded to the type and left in
+ * `sum` (both NULL: nothing is added).  weight and bias (either may be NULL) are of the rows' type or fp32.  stats: three floats a
+ * row for the backward call, NULL: not wanted.  Rows are ld* elements apart (0 too: the same row again), y, sum and dx are contiguous.
+ * D <= 32768, fewer than 2^31 rows (AMOE_EUNSUPPORTED otherwise).  The squares of what differs from the mean, and their sum, have to
+ * stay finite in fp32.
+ * The backward call reads x = s and stats and gives dx = the gradient of s: through y, whose gradient is gy, plus gs, that of s
+ * itself (NULL: none), rounded once; dweight and dbias [D] in the weights' type (each may be NULL, as may dx).  Both are sums in a
+ * fixed order in fp32, through the workspace: equal inputs give equal bits. */
+typedef struct amoe_norm_args {
+  int64_t dtype, weight_dtype, rows, D;
+  double eps;
+  const void* x;  int64_t ldx;
+  const void* weight;  const void* bias;                        /* [D] */
+  float* stats;                                                 /* [rows, 3] */
+  /* forward only */
+  const void* residual;  int64_t ldr;
+  void* y;  void* sum;                                          /* [rows, D] */
+  /* backward only */
+  const void* gy;  int64_t ldgy;
+  const void* gs;  int64_t ldgs;
+  void* dx;  void* dweight;  void* dbias;
+} amoe_norm_args;
+int amoe_layer_norm_fwd(const amoe_norm_args* args, void* stream);
+size_t amoe_layer_norm_bwd_workspace(const amoe_norm_args* args);
+int amoe_layer_norm_bwd(const amoe_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t amoe_norm_args_bytes(void);
+
 #ifdef __cplusplus
 }
 #endif
