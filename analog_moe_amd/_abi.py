@@ -126,6 +126,9 @@ PROTOTYPES = {
     "amoe_layer_norm_bwd_workspace": (SZ, [P]),
     "amoe_layer_norm_bwd": (C.c_int, [P, P, SZ, P]),
     "amoe_norm_args_bytes": (SZ, []),
+    "amoe_sample_workspace": (SZ, [P]),
+    "amoe_sample": (C.c_int, [P, P, SZ, P]),
+    "amoe_sample_args_bytes": (SZ, []),
     "amoe_select_workspace": (SZ, [I64, I32]),
     "amoe_select_fwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, SZ, P]),
     "amoe_select_bwd": (C.c_int, [I32, P, I64, I32, I32, P, P, P, P, P, P]),
@@ -160,6 +163,10 @@ NORM_ARGS = struct.Struct("<"
                           "2q3q"          # x ldx, weight bias stats
                           "2q2q"          # residual ldr, y sum
                           "4q3q")         # gy ldgy gs ldgs, dx dweight dbias
+SAMPLE_ARGS = struct.Struct("<"
+                            "3q2q2q"      # dtype rows V, logits ld, u u_is_f64
+                            "3q2q"        # temperature top_p min_p, top_k top_k_is_i64
+                            "3dq2q")      # the same for all rows (top_k last), ids logprob
 
 
 @functools.lru_cache(maxsize=256)
@@ -176,7 +183,8 @@ def bind(path: str) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS), ("norm", NORM_ARGS)):
+    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS), ("norm", NORM_ARGS),
+                         ("sample", SAMPLE_ARGS)):
         if getattr(lib, f"amoe_{name}_args_bytes")() != layout.size:
             raise RuntimeError(f"{path}: amoe_{name}_args has another layout than this package packs")
     return lib

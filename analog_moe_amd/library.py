@@ -17,6 +17,7 @@ so every group of calls the Python layer makes is one opaque operator with a fak
   amoe::ffn_fwd / ffn_bwd   the fused expert feed-forward, with its autograd formula registered
   amoe::attention_fwd / attention_bwd, amoe::rotary / rotary_into   the decoder's attention and rotary positions, likewise
   amoe::layer_norm_fwd / layer_norm_bwd                             its layer norm, likewise
+  amoe::sample                                                      the choice of its next token
 
 Operators return an empty tensor where the Python interface returns ``None``.
 """
@@ -27,7 +28,7 @@ from typing import List, Optional
 import torch
 from torch import Tensor
 
-from . import attention, ffn, norm, ops, rotary
+from . import attention, ffn, norm, ops, rotary, sampling
 
 _EMPTY_SHAPE = (0,)
 
@@ -504,3 +505,22 @@ def _layer_norm_autograd(ctx, gy, gs, _grad_stats):
 
 
 layer_norm_fwd.register_autograd(_layer_norm_autograd, setup_context=_layer_norm_setup_context)
+
+
+# --------------------------------------------------------------------------- the next token
+@torch.library.custom_op(
+    "amoe::sample", mutates_args=(),
+    schema="(Tensor logits, Tensor u, Tensor? temperature, Tensor? top_k, Tensor? top_p, Tensor? min_p, float temperature_all, "
+           "int top_k_all, float top_p_all, float min_p_all) -> (Tensor, Tensor)")
+def sample(logits, u, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all):
+    """(ids, logprob): each setting a tensor with one number per row, or None and the number for all."""
+    def one(t, v):
+        return v if t is None else t
+    return sampling.draw(logits, u, one(temperature, temperature_all), one(top_k, top_k_all), one(top_p, top_p_all), one(min_p, min_p_all),
+                         want_logprob=True)
+
+
+@sample.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all):
+    rows = tuple(logits.shape[:-1])
+    return torch.empty(rows, dtype=torch.int64, device=logits.device), torch.empty(rows, dtype=torch.float32, device=logits.device)

@@ -536,6 +536,32 @@ size_t amoe_layer_norm_bwd_workspace(const amoe_norm_args* args);
 int amoe_layer_norm_bwd(const amoe_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t amoe_norm_args_bytes(void);
 
+/* The choice of a token for every row of logits [rows, V] (nothing of the reference's own is replaced here).  Every field is 8 bytes
+ * wide.  With weight_i = exp((x_i - max) / temperature), tokens ranked by x and the lower index first among equals: kept are the
+ * first top_k (0 or >= V: all), of these the shortest run from the top with at least top_p of their weight (the first one always; 1:
+ * all), of these those of weight min_p (of the largest) or more.  ids[row]: the first, in the order of the indices, up to which the
+ * kept ones weigh more than u[row] times all of them (u outside [0, 1): the nearer end).  logprob[row]: log of its share of them.
+ * Temperature 0: the largest logit, the lowest index among equals, logprob 0.  Not-a-numbers count as minus infinity; infinite
+ * logits share the weight; a row with neither a number nor infinity gives id -1 and logprob minus infinity.
+ * Settings: one pointer each to a number per row, or NULL and the number for all.  A row's own settings are not refused: temperatures
+ * that are not above 0 count as 0, negative top_k as 0, top_p and min_p as the nearer end of [0, 1] (not a number: 1 and 0).
+ * Weights are multiples of 2^-44 of the largest (what weighs less than half of that is never drawn), sums of them exact: equal inputs
+ * give equal bits.  V < 2^20, fewer than 2^22 rows (AMOE_EUNSUPPORTED otherwise); rows ld elements apart, adjacent elements. */
+typedef struct amoe_sample_args {
+  int64_t dtype, rows, V;
+  const void* logits;  int64_t ld;
+  const void* u;  int64_t u_is_f64;                             /* [rows] fp32 or fp64 */
+  const float* temperature;  const float* top_p;  const float* min_p;
+  const void* top_k;  int64_t top_k_is_i64;                     /* [rows] int32 / int64 */
+  double temperature_all, top_p_all, min_p_all;
+  int64_t top_k_all;
+  int64_t* ids;
+  float* logprob;                                               /* may be NULL */
+} amoe_sample_args;
+size_t amoe_sample_workspace(const amoe_sample_args* args);
+int amoe_sample(const amoe_sample_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t amoe_sample_args_bytes(void);
+
 #ifdef __cplusplus
 }
 #endif
