@@ -122,6 +122,9 @@ PROTOTYPES = {
     "amoe_attention_bwd_workspace": (SZ, [P]),
     "amoe_attention_bwd": (C.c_int, [P, P, SZ, P]),
     "amoe_attn_args_bytes": (SZ, []),
+    "amoe_attention_shared_fwd_workspace": (SZ, [P]),
+    "amoe_attention_shared_fwd": (C.c_int, [P, P, SZ, P]),
+    "amoe_shared_attn_args_bytes": (SZ, []),
     "amoe_layer_norm_fwd": (C.c_int, [P, P]),
     "amoe_layer_norm_bwd_workspace": (SZ, [P]),
     "amoe_layer_norm_bwd": (C.c_int, [P, P, SZ, P]),
@@ -158,6 +161,11 @@ ATTN_ARGS = struct.Struct("<"
                           "2q2q"          # lengths lengths_is_i64, starts starts_is_i64
                           "3q"            # out lse rest
                           "4q3q")         # go with 3 strides, dq dk dv
+SHARED_ATTN_ARGS = struct.Struct("<"
+                                 "10qd"      # dtype B S T P prefixes H G d causal, scale
+                                 "4q4q4q4q4q"  # q, k, v, prefix_k, prefix_v with 3 strides each
+                                 "2q2q2q"    # lengths, starts, prefix_lengths, each with is_i64
+                                 "q")        # out
 NORM_ARGS = struct.Struct("<"
                           "4qd"           # dtype weight_dtype rows D, eps
                           "2q3q"          # x ldx, weight bias stats
@@ -183,7 +191,7 @@ def bind(path: str) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS), ("norm", NORM_ARGS),
+    for name, layout in (("ffn", FFN_ARGS), ("rotary", ROTARY_ARGS), ("attn", ATTN_ARGS), ("shared_attn", SHARED_ATTN_ARGS), ("norm", NORM_ARGS),
                          ("sample", SAMPLE_ARGS)):
         if getattr(lib, f"amoe_{name}_args_bytes")() != layout.size:
             raise RuntimeError(f"{path}: amoe_{name}_args has another layout than this package packs")

@@ -190,4 +190,56 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
     return Attention.apply(q, k, v, lengths, starts, causal, scale)
 
 
+def shared_attention_forward(q: Tensor, k: Tensor, v: Tensor, prefix_k: Tensor, prefix_v: Tensor, lengths: Optional[Tensor] = None,
+                             starts: Optional[Tensor] = None, prefix_lengths: Optional[Tensor] = None, causal: bool = True,
+                             scale: Optional[float] = None) -> Tensor:
+    """``amoe_attention_shared_fwd``; ``shared_attention`` describes it."""
+    ops._need_gpu(prefix_k, prefix_v, prefix_lengths)
+    call = _Call(q, k, v, lengths, starts, causal, scale)
+    code, B, S, T, H, G, d, causal, scale, *rest = call.head
+    shape = prefix_k.shape
+    if len(shape) != 4 or shape != prefix_v.shape or shape[2] != G or shape[3] != d:
+        raise ValueError(f"prefix_k {tuple(shape)} and prefix_v {tuple(prefix_v.shape)} do not match k {tuple(call.kv_shape)}")
+    if prefix_k.dtype != q.dtype or prefix_v.dtype != q.dtype:
+        raise TypeError("q, k, v and the prefix must share one dtype")
+    if prefix_k.device != q.device or prefix_v.device != q.device:
+        raise ValueError("q, k, v and the prefix must be on one device")
+    N, P = shape[:2]
+    if B and (N == 0 or B % N):
+        raise ValueError(f"{B} sequences cannot continue {N} prefixes evenly")
+    pk, pv = _rows(prefix_k), _rows(prefix_v)
+    n = n64 = 0
+    if prefix_lengths is not None:
+        prefix_lengths = _marks(prefix_lengths, N, q.device, "prefix_lengths")
+        n, n64 = prefix_lengths.data_ptr(), prefix_lengths.dtype == torch.int64
+    out = q.new_empty(call.shape)
+    ks, vs = pk.stride(), pv.stride()
+    args = _abi.SHARED_ATTN_ARGS.pack(code, B, S, T, P, N, H, G, d, causal, scale, *rest[:12], pk.data_ptr(), ks[0], ks[1], ks[2],
+                                      pv.data_ptr(), vs[0], vs[1], vs[2], *rest[12:], n, n64, out.data_ptr())
+    lib = ops.get_lib()
+    with ops.device_of(q):
+        need = lib.amoe_attention_shared_fwd_workspace(args)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.amoe_attention_shared_fwd(args, None if ws is None else ws.data_ptr(), need, ops._stream(q))
+    if rc:
+        _abi.check(lib, rc, "amoe_attention_shared_fwd")
+    return out
+
+
+def shared_attention(q: Tensor, k: Tensor, v: Tensor, prefix_k: Tensor, prefix_v: Tensor, *, causal: bool = True,
+                     scale: Optional[float] = None, lengths: Optional[Tensor] = None, starts: Optional[Tensor] = None,
+                     prefix_lengths: Optional[Tensor] = None) -> Tensor:
+    """``attention`` of q [B, S, H, d] over the keys of a prefix [N, P, G, d], then the sequence's own k, v [B, T, G, d]: every B / N
+    sequences in a row continue one prefix, which is read once for all of them.
+
+    All queries see the first prefix_lengths[n] keys of their prefix (None: P).  Own keys are as in ``attention``: lengths, starts
+    and the causal mask count among them (query i of sequence b sees own keys up to starts[b] + i; starts None: T - S + i).  T and P may
+    be 0.  A query that sees no key gives zeros.  For serving: no gradients."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, prefix_k, prefix_v)):
+        raise RuntimeError("shared_attention has no gradient: call it under torch.no_grad()")
+    if torch.compiler.is_compiling() or not ops.unwatched():
+        return torch.ops.amoe.attention_shared(q, k, v, prefix_k, prefix_v, lengths, starts, prefix_lengths, causal, scale)
+    return shared_attention_forward(q, k, v, prefix_k, prefix_v, lengths, starts, prefix_lengths, causal, scale)
+
+
 from . import library  # noqa: E402,F401  (registers the operators that traced calls go through; it imports this module)

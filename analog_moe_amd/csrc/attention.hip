@@ -79,6 +79,7 @@ void fill(AttnParams& p, const amoe_attn_args* a) {
   p.starts = a->starts; p.starts_i64 = (int)a->starts_is_i64;
   p.B = (int)a->B; p.S = (int)a->S; p.T = (int)a->T; p.H = (int)a->H; p.G = (int)a->G; p.R = (int)(a->H / a->G);
   p.d = (int)a->d; p.causal = a->causal != 0;
+  p.copies = 1;
   p.c = (float)(a->scale * 1.4426950408889634074);
   p.scale = (float)a->scale;
   p.lse = a->lse;
@@ -175,4 +176,130 @@ extern "C" int amoe_attention_bwd(const amoe_attn_args* a, void* workspace, size
   return a->dtype == AMOE_F32   ? launch_attn_bwd_f32(p, st)
          : a->dtype == AMOE_F16 ? launch_attn_bwd_f16(p, st)
                                 : launch_attn_bwd_bf16(p, st);
+}
+
+// ---- sequences that share a prefix ----------------------------------------------------------------
+namespace {
+
+// What is asked of one set of keys, in the terms of the other calls: the prefix's, B of which are seen by all queries of N = B / B'
+// sequences each, or the sequences' own.
+amoe_attn_args shared_part(const amoe_shared_attn_args* a, bool prefix) {
+  amoe_attn_args s{};
+  s.dtype = a->dtype; s.B = prefix ? a->prefixes : a->B; s.S = a->S; s.T = prefix ? a->P : a->T; s.H = a->H; s.G = a->G; s.d = a->d;
+  s.causal = prefix ? 0 : a->causal;
+  s.scale = a->scale;
+  s.q = a->q; s.q_sb = a->q_sb; s.q_ss = a->q_ss; s.q_sh = a->q_sh;
+  s.k = prefix ? a->prefix_k : a->k;
+  s.k_sb = prefix ? a->prefix_k_sb : a->k_sb; s.k_ss = prefix ? a->prefix_k_ss : a->k_ss; s.k_sh = prefix ? a->prefix_k_sh : a->k_sh;
+  s.v = prefix ? a->prefix_v : a->v;
+  s.v_sb = prefix ? a->prefix_v_sb : a->v_sb; s.v_ss = prefix ? a->prefix_v_ss : a->v_ss; s.v_sh = prefix ? a->prefix_v_sh : a->v_sh;
+  s.lengths = prefix ? a->prefix_lengths : a->lengths;
+  s.lengths_is_i64 = prefix ? a->prefix_lengths_is_i64 : a->lengths_is_i64;
+  s.starts = prefix ? nullptr : a->starts;
+  s.starts_is_i64 = a->starts_is_i64;
+  return s;
+}
+
+int check_shared(const amoe_shared_attn_args* a) {
+  if (!a) return AMOE_ENULL;
+  if (a->B < 0 || a->prefixes < 0 || a->P < 0) return AMOE_EINVAL;
+  if (a->B > 0 && (a->prefixes == 0 || a->B % a->prefixes)) return AMOE_ESHAPE;
+  const amoe_attn_args own = shared_part(a, false), prefix = shared_part(a, true);
+  if (int rc = check_sizes(&own)) return rc;
+  if (int rc = check_sizes(&prefix)) return rc;
+  if (a->B == 0 || a->S == 0) return AMOE_OK;
+  // threads of the join, and rows that share a key head, in 32 bits
+  if (a->B * a->H >= (INT64_C(1) << 23) / a->S) return AMOE_EUNSUPPORTED;
+  return a->B / a->prefixes * (a->H / a->G) * a->S > (INT64_C(1) << 30) ? AMOE_EUNSUPPORTED : AMOE_OK;
+}
+
+struct SharedPlan {
+  int rw = 0, splits = 0;
+};
+
+// Waves over the rows and parts of the keys, for `rows` rows that share a key head in each of `heads` of them and T keys.
+SharedPlan shared_plan(int64_t rows, int64_t heads, int64_t T, bool whole, size_t es) {
+  SharedPlan p;
+  if (T == 0) return p;
+  const int64_t cus = num_compute_units();
+  p.rw = rows <= 32 ? 0 : rows <= 64 && whole && es == 2 ? 2 : 4;
+  const int64_t block = p.rw ? 32 * p.rw : 32, groups = heads * ((rows + block - 1) / block);
+  const auto parts = [&](int64_t per_cu, int64_t keys) {
+    const int64_t n = (per_cu * cus + groups - 1) / groups, most = (T + keys - 1) / keys;
+    return n < most ? n : most;
+  };
+  int64_t n = p.rw ? parts(2, 256) : parts(8, 512);
+  const int64_t few = parts(2, 128);
+  if (!p.rw && few > n) n = few;
+  p.splits = (int)(n < 1 ? 1 : n > kAttnMaxSplits / 2 ? kAttnMaxSplits / 2 : n);
+  return p;
+}
+
+struct SharedPlans {
+  SharedPlan prefix, own;
+};
+SharedPlans shared_plans(const amoe_shared_attn_args* a, bool whole) {
+  const int64_t rows = a->H / a->G * a->S, copies = a->B / a->prefixes;
+  const size_t es = esize((int)a->dtype);
+  return {shared_plan(copies * rows, a->prefixes * a->G, a->P, whole, es), shared_plan(rows, a->B * a->G, a->T, whole, es)};
+}
+
+size_t shared_bytes(const amoe_shared_attn_args* a, int parts) {
+  return (size_t)parts * (size_t)(a->B * a->H * a->S) * (size_t)((a->d + 3) / 4 * 4 + 2) * 4;
+}
+
+}  // namespace
+
+extern "C" size_t amoe_shared_attn_args_bytes(void) { return sizeof(amoe_shared_attn_args); }
+
+extern "C" size_t amoe_attention_shared_fwd_workspace(const amoe_shared_attn_args* a) {
+  if (check_shared(a) || a->B == 0 || a->S == 0) return 0;
+  // (the strides decide between forms with as many parts or fewer)
+  const SharedPlans x = shared_plans(a, true), y = shared_plans(a, false);
+  const int m = x.prefix.splits + x.own.splits, n = y.prefix.splits + y.own.splits;
+  return shared_bytes(a, m > n ? m : n);
+}
+
+extern "C" int amoe_attention_shared_fwd(const amoe_shared_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_shared(a)) return rc;
+  if (a->B == 0 || a->S == 0) return AMOE_OK;
+  const amoe_attn_args own = shared_part(a, false), prefix = shared_part(a, true);
+  if (int rc = check_inputs(&own)) return rc;
+  if (int rc = check_inputs(&prefix)) return rc;
+  const size_t es = esize((int)a->dtype), need = amoe_attention_shared_fwd_workspace(a);
+  if (!a->out) return AMOE_ENULL;
+  if (!aligned(a->out, es)) return AMOE_EALIGN;
+  if (need && !workspace) return AMOE_ENULL;
+  if (workspace_bytes < need) return AMOE_EWORKSPACE;
+  if (!aligned(workspace, 16)) return AMOE_EALIGN;
+  AttnShared s{};
+  fill(s.own, &own);
+  fill(s.prefix, &prefix);
+  // the queries are those of all sequences
+  s.prefix.q = s.own.q;
+  s.prefix.copies = (int)(a->B / a->prefixes);
+  const int vec = operand_vec(s.own.q, a->S, a->d, es);
+  s.prefix.vec = a->P > 0 ? operand_vec(s.prefix.k, a->P, a->d, es) : 2;
+  if (a->P > 0 && operand_vec(s.prefix.v, a->P, a->d, es) < s.prefix.vec) s.prefix.vec = operand_vec(s.prefix.v, a->P, a->d, es);
+  if (vec < s.prefix.vec) s.prefix.vec = vec;
+  s.prefix.vec = s.own.vec = s.prefix.vec < s.own.vec ? s.prefix.vec : s.own.vec;
+  const SharedPlans plans = shared_plans(a, attn_whole_chunks(s.own, es));
+  s.prefix.splits = plans.prefix.splits; s.prefix_rw = plans.prefix.rw;
+  s.own.splits = plans.own.splits; s.own_rw = plans.own.rw;
+  const int parts = s.prefix.splits + s.own.splits;
+  const size_t rows = (size_t)(a->B * a->H * a->S), pad = (size_t)((a->d + 3) / 4 * 4);
+  // (the rows first: their 16-byte stores)
+  s.prefix.part_o = static_cast<float*>(workspace);
+  s.prefix.part_ml = s.prefix.part_o + parts * rows * pad;
+  s.own.part_o = s.prefix.part_o + s.prefix.splits * rows * pad;
+  s.own.part_ml = s.prefix.part_ml + s.prefix.splits * rows * 2;
+  s.join = s.own;
+  s.join.part_o = s.prefix.part_o;
+  s.join.part_ml = s.prefix.part_ml;
+  s.join.splits = parts;
+  s.join.out = a->out;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return a->dtype == AMOE_F32   ? launch_attn_shared_f32(s, st)
+         : a->dtype == AMOE_F16 ? launch_attn_shared_f16(s, st)
+                                : launch_attn_shared_bf16(s, st);
 }

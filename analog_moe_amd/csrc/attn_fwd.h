@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
   }
 }
 
-// Few rows: the R * S rows that share a key head, 32 per workgroup, and one of `splits` parts of the keys they see; every
+// Few rows: the copies * R * S rows that share a key head, 32 per workgroup, and one of `splits` parts of the keys they see; every
 // wave takes every fourth block of 32 keys of the part.  K goes from global memory into the operands, V through a tile of the
 // wave's own, both a block ahead; the waves' results are joined in LDS, and those of the parts by attn_join_kernel.  Bound by
 // memory: 48 sequences over caches of 4096 to 8192, 16 over 4 heads of 128, bf16: 133 us for 604 MB (4.5 TB/s, a large copy
@@ -287,15 +287,16 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   __shared__ __align__(16) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
   __shared__ float lds_m[4][32], lds_l[4][32];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
-  const int rows = p.R * p.S, row_tiles = (rows + 31) / 32;
+  const int rows = p.copies * p.R * p.S;
   int id = (int)blockIdx.x;
   const int bg = id % (p.B * p.G);
   id /= p.B * p.G;
   const int split = id % p.splits, r0 = (id / p.splits) * 32;
   const int b = bg / p.G, g = bg - b * p.G;
   const int length = attn_length(p, b), start = attn_start(p, b);
-  // row r is query r % S of the group's head r / S
-  const int r = r0 + (lane & 31), rr = r < rows ? r : rows - 1, hd = g * p.R + rr / p.S, i = rr % p.S;
+  // row r is query r % S of the group's head r / S, those of one sequence after those of another
+  const int r = r0 + (lane & 31), rr = r < rows ? r : rows - 1, hd = g * p.R + rr / p.S % p.R, i = rr % p.S;
+  const int seq0 = b * p.copies;
   const int seen = attn_seen(p, length, start, i);
   // keys that any row of the tile sees: with one head's rows in order it is the last row's, else the last query's
   const int r_last = r0 + 31 < rows ? r0 + 31 : rows - 1;
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
   T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
   attn_frag<T> q[NK], kf[NK];
-  const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
+  const T* qrow = static_cast<const T*>(p.q.p) + (seq0 + rr / (p.R * p.S)) * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
   AttnStage<T, DP, 32, 64, EDGE, true> sv;
   sv.init(lane, p.v.ss, p.d);
   const typename Tile::Lane at = typename Tile::Lane().in(wave * 32 * DP);
@@ -372,10 +373,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] += o[j];
     }
-    const int head = g * p.R + (r0 + row) / p.S, query = (r0 + row) % p.S;
-    const int64_t where = ((int64_t)b * p.H + head) * p.S + query;
-    if (p.splits > 1) {
-      const int64_t part = (int64_t)split * p.B * p.H * p.S + where;
+    const int head = g * p.R + (r0 + row) / p.S % p.R, query = (r0 + row) % p.S;
+    const int64_t seq = seq0 + (r0 + row) / (p.R * p.S), where = (seq * p.H + head) * p.S + query;
+    if (p.part_o) {
+      const int64_t part = (int64_t)split * p.B * p.copies * p.H * p.S + where;
       store4<float>(p.part_o + part * ((p.d + 3) & ~3) + e, v, 4, true);
       if (e == 0) {
         p.part_ml[2 * part] = mr;
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
       const float inv = lr == 0.f ? 0.f : 1.f / lr;
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] *= inv;
-      const int64_t to = (((int64_t)b * p.S + query) * p.H + head) * p.d + e;
+      const int64_t to = ((seq * p.S + query) * p.H + head) * p.d + e;
       store4<T>(static_cast<T*>(p.out) + to, v, EDGE ? p.d - e : 4, !EDGE);
       if (p.rest) {
         const float rest[4] = {attn_rest<T>(v[0]), attn_rest<T>(v[1]), attn_rest<T>(v[2]), attn_rest<T>(v[3])};
@@ -394,6 +395,175 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
       if (p.lse && e == 0) p.lse[where] = attn_lse<T>(mr, lr, p.c);
     }
   }
+}
+
+// Rows that share keys, 32 * RW of them per workgroup, and one of `splits` parts of the keys they see: as attn_fwd_rows_kernel, for
+// rows of several sequences and heads, whose results are joined with those of other parts.
+template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
+__global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Shape::kWavesPerSimd)) void attn_parts_kernel(AttnParams p) {
+  using Tile = AttnTile<T, DP>;
+  constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
+  constexpr int kElems = BN * DP, kTilesBytes = 2 * kElems * (int)sizeof(T);
+  static_assert((KG - 1) * RW * DP * 32 * 4 <= kTilesBytes, "the copies are joined in the keys' tiles");
+  __shared__ __align__(1024) char lds_k[kTilesBytes], lds_v[kTilesBytes];
+  __shared__ float lds_ml[KG][RW][2][64];
+  T *const tk = reinterpret_cast<T*>(lds_k), *const tv = reinterpret_cast<T*>(lds_v);
+  const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5, wave = wave_uniform(tid >> 6), rw = wave % RW, kg = wave / RW;
+  // blocks of rows over the same keys next to each other's on an XCD (ids go round the eight)
+  const int rows = p.copies * p.R * p.S, blocks = (rows + Shape::kRows - 1) / Shape::kRows, BG = p.B * p.G;
+  const int per_xcd = (int)gridDim.x / 8;
+  int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (id >= blocks * BG * p.splits) return;
+  const int r0 = id % blocks * Shape::kRows;
+  id /= blocks;
+  const int bg = id % BG, split = id / BG, b = bg / p.G, g = bg - b * p.G;
+  const int length = attn_length(p, b), start = attn_start(p, b);
+  const auto sees = [&](int first, int last) {       // keys that any of these rows sees: with one head's rows in order the last one's
+    last = last < rows ? last : rows - 1;
+    return first >= rows ? 0 : attn_seen(p, length, start, first / p.S == last / p.S ? last % p.S : p.S - 1);
+  };
+  const int group_sees = sees(r0, r0 + Shape::kRows - 1);
+  const int per = ((group_sees + p.splits - 1) / p.splits + BN - 1) / BN * BN;
+  const int64_t lo64 = (int64_t)split * per;
+  const int key_lo = lo64 < group_sees ? (int)lo64 : group_sees, key_hi = group_sees - key_lo < per ? group_sees : key_lo + per;
+  const int w0 = r0 + rw * 32, w1 = w0 + 31 < rows ? w0 + 31 : rows - 1;
+  const int wave_sees = sees(w0, w0 + 31), wave_all = attn_seen(p, length, start, w0 < rows && w0 / p.S == w1 / p.S ? w0 % p.S : 0);
+  const int r = w0 + (lane & 31), rr = r < rows ? r : rows - 1, hd = g * p.R + rr / p.S % p.R, i = rr % p.S;
+  const int64_t seq = b * p.copies + rr / (p.R * p.S);
+  const int all = attn_seen(p, length, start, i), seen = all < key_hi ? all : key_hi;
+
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
+  AttnStage<T, DP, BN, kAttnThreads, EDGE> sk, sv;
+  sk.init(tid, p.k.ss, p.d);
+  sv.init(tid, p.v.ss, p.d);
+  typename Tile::Lane at;
+  const int n_tiles = (key_hi - key_lo + BN - 1) / BN;
+  if (n_tiles > 0) {
+    sk.load(tid, tk, kb, p.k.ss, key_lo, key_hi, p.d, p.vec);
+    sv.load(tid, tv, vb, p.v.ss, key_lo, key_hi, p.d, p.vec);
+  }
+  attn_frag<T> q[NK];
+  const T* qrow = static_cast<const T*>(p.q.p) + seq * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
+#pragma unroll
+  for (int kk = 0; kk < NK; kk++) q[kk] = attn_global_frag<T, EDGE>(qrow, kk, p.d, r < rows, p.vec);
+
+  AttnState<T, DP> st;
+  st.clear();
+  if (n_tiles > 0) {
+    sk.store(tid, tk);
+    sv.store(tid, tv);
+  }
+  for (int t = 0; t < n_tiles; t++) {
+    const int cur = (t & 1) * kElems, next = kElems - cur;
+    sk.finish();
+    __syncthreads();       // tile t is there, and nobody reads the other one any more
+    if (t + 1 < n_tiles) {
+      sk.load(tid, tk + next, kb, p.k.ss, key_lo + (t + 1) * BN, key_hi, p.d, p.vec);
+      sv.load(tid, tv + next, vb, p.v.ss, key_lo + (t + 1) * BN, key_hi, p.d, p.vec);
+    }
+    const int key0 = key_lo + t * BN + 32 * NB * kg;
+    if (key0 < wave_sees && key0 < key_hi) {
+      constexpr int NS = NB * NK, NU = DP / 32;
+      const typename Tile::Lane in = at.in(cur + 32 * NB * kg * DP);
+      const auto load = [&](int e) -> attn_frag<T> {
+        return e < NS ? Tile::row_frag(lds_k, in, 32 * (e % NB), e / NB) : Tile::col_frag(lds_v, in, 16 * ((e - NS) / NU), (e - NS) % NU);
+      };
+      AttnRun<T, NS + 2 * NB * NU, kAttnThree<T, DP, EDGE, RW> ? 4 : kAttnAhead<T>> run;
+      run.begin(load);
+      f32x16 s[NB];
+      attn_frag<T> pr[2 * NB];
+#pragma unroll
+      for (int n = 0; n < NB; n++) s[n] = f32x16_zero();
+      run.steps(0, NS, load, [&](int e, const attn_frag<T>& a) { s[e % NB] = attn_mma<T>(a, q[e / NB], s[e % NB]); });
+      attn_softmax<T, DP, NB>(st, s, pr, key0, seen, key0 + 32 * NB > wave_all || key0 + 32 * NB > key_hi, p.c);
+      run.steps(NS, NS + 2 * NB * NU, load,
+                [&](int e, const attn_frag<T>& a) { st.o[(e - NS) % NU] = attn_mma<T>(a, pr[(e - NS) / NU], st.o[(e - NS) % NU]); });
+    }
+    if (t + 1 < n_tiles) {
+      sk.store(tid, tk + next);
+      sv.store(tid, tv + next);
+    }
+  }
+  float l = attn_pair_sum(st.l);
+  if constexpr (KG > 1) {
+    // the copies in units of the largest maximum; the first one takes the sums
+    __syncthreads();
+    f32x4* join = reinterpret_cast<f32x4*>(lds_k);
+    lds_ml[kg][rw][0][lane] = st.m;
+    lds_ml[kg][rw][1][lane] = l;
+    if (kg > 0) attn_put_acc<DP>(join, (kg - 1) * RW + rw, st.o, 1.f);
+    __syncthreads();
+    if (kg == 0) {
+      float m = st.m;
+#pragma unroll
+      for (int c = 1; c < KG; c++) m = fmaxf(m, lds_ml[c][rw][0][lane]);
+      const float own = st.m == -INFINITY ? 0.f : fast_exp2((st.m - m) * p.c);
+      l *= own;
+#pragma unroll
+      for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) st.o[t][e] *= own;
+#pragma unroll
+      for (int c = 1; c < KG; c++) {
+        const float mc = lds_ml[c][rw][0][lane], f = mc == -INFINITY ? 0.f : fast_exp2((mc - m) * p.c);
+        l = fmaf(lds_ml[c][rw][1][lane], f, l);
+        attn_add_acc<DP>(join, (c - 1) * RW + rw, st.o, f);
+      }
+      st.m = m;
+    }
+  }
+  if (kg == 0 && r < rows) {
+    const int64_t part = (int64_t)split * p.B * p.copies * p.H * p.S + (seq * p.H + hd) * p.S + i;
+    float* po = p.part_o + part * ((p.d + 3) & ~3);
+#pragma unroll
+    for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int e = 32 * t + 8 * u + 4 * h;
+        if (e < p.d) *reinterpret_cast<f32x4*>(po + e) = f32x4{st.o[t][4 * u], st.o[t][4 * u + 1], st.o[t][4 * u + 2], st.o[t][4 * u + 3]};
+      }
+    if (h == 0) {
+      p.part_ml[2 * part] = st.m;
+      p.part_ml[2 * part + 1] = l;
+    }
+  }
+}
+
+// The parts of a row joined, a wave per row, for up to 64 of them: a lane holds a part's maximum and sum, then two elements of the row.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_rows_kernel(AttnParams p) {
+  const int64_t n = (int64_t)p.B * p.H * p.S, row0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t at = row0 < n ? row0 : n - 1;
+  const int lane = lane_id(), pad = (p.d + 3) & ~3;
+  float m = -INFINITY, l = 0.f;
+  if (lane < p.splits) {
+    m = p.part_ml[2 * (lane * n + at)];
+    l = p.part_ml[2 * (lane * n + at) + 1];
+  }
+  float top = m;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, wave_shfl_xor(top, x));
+  const float f = m == -INFINITY ? 0.f : fast_exp2((m - top) * p.c);
+  l *= f;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += wave_shfl_xor(l, x);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int e = 2 * lane;
+  float a = 0.f, b = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.splits; s++) {
+    const float fs = as_f32(wave_read(as_u32(f), s));
+    if (e < p.d) {
+      const float* po = p.part_o + (s * n + at) * pad + e;
+      a = fmaf(po[0], fs, a);
+      b = fmaf(po[1], fs, b);
+    }
+  }
+  const int64_t bh = at / p.S, i = at - bh * p.S, seq = bh / p.H, hd = bh - seq * p.H;
+  T* out = static_cast<T*>(p.out) + ((seq * p.S + i) * p.H + hd) * p.d;
+  if (row0 < n && e < p.d) out[e] = Elem<T>::cvt(a * inv);
+  if (row0 < n && e + 1 < p.d) out[e + 1] = Elem<T>::cvt(b * inv);
 }
 
 // The parts of a row joined, a workgroup per row: sums in units of the largest maximum, eight runs of parts side by side and

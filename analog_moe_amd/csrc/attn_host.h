@@ -12,6 +12,14 @@ inline bool attn_whole_chunks(const AttnParams& p, size_t es) { return p.vec == 
 int launch_attn_fwd_f32(const AttnParams& p, hipStream_t st);
 int launch_attn_fwd_bf16(const AttnParams& p, hipStream_t st);
 int launch_attn_fwd_f16(const AttnParams& p, hipStream_t st);
+// rows that share `prefix` and have keys of their own in `own`: parts of both, and all of them joined
+struct AttnShared {
+  AttnParams prefix, own, join;
+  int prefix_rw, own_rw;             // waves over the rows of a workgroup; 0: attn_fwd_split_kernel
+};
+int launch_attn_shared_f32(const AttnShared& s, hipStream_t st);
+int launch_attn_shared_bf16(const AttnShared& s, hipStream_t st);
+int launch_attn_shared_f16(const AttnShared& s, hipStream_t st);
 int launch_attn_bwd_f32(const AttnParams& p, hipStream_t st);
 int launch_attn_bwd_bf16(const AttnParams& p, hipStream_t st);
 int launch_attn_bwd_f16(const AttnParams& p, hipStream_t st);

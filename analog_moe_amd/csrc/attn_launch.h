@@ -75,6 +75,53 @@ int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
   return rc;
 }
 
+template <typename T, int DP, bool EDGE>
+int launch_attn_parts_of(const AttnParams& p, int rw, hipStream_t st) {
+  const int64_t blocks = ((int64_t)p.copies * p.R * p.S + 32 * rw - 1) / (32 * rw);
+  const dim3 grid((unsigned)((p.B * p.G * blocks * p.splits + 7) / 8 * 8));
+  if constexpr (!EDGE && sizeof(T) == 2) {
+    if (rw == 2) {
+      hipLaunchKernelGGL((&attn_parts_kernel<T, DP, EDGE, 2>), grid, dim3(kAttnThreads), 0, st, p);
+      return launch_rc();
+    }
+  }
+  if (rw != 4) return AMOE_EUNSUPPORTED;
+  hipLaunchKernelGGL((&attn_parts_kernel<T, DP, EDGE, 4>), grid, dim3(kAttnThreads), 0, st, p);
+  return launch_rc();
+}
+
+// The parts of one set of keys.
+template <typename T>
+int launch_attn_parts(const AttnParams& p, int rw, hipStream_t st) {
+  int rc = AMOE_OK;
+  if (rw > 0) {
+#define AMOE_LAUNCH(TYPE, DP, EDGE) rc = launch_attn_parts_of<TYPE, DP, EDGE>(p, rw, st)
+    AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
+#undef AMOE_LAUNCH
+    return rc;
+  }
+  const dim3 grid((unsigned)((int64_t)p.B * p.G * p.splits * (((int64_t)p.copies * p.R * p.S + 31) / 32)));
+#define AMOE_LAUNCH(TYPE, DP, EDGE) hipLaunchKernelGGL((&attn_fwd_split_kernel<TYPE, DP, EDGE>), grid, dim3(kAttnThreads), 0, st, p)
+  AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
+#undef AMOE_LAUNCH
+  return launch_rc();
+}
+
+template <typename T>
+int launch_attn_shared(const AttnShared& s, hipStream_t st) {
+  if (s.prefix.splits > 0) {
+    if (int rc = launch_attn_parts<T>(s.prefix, s.prefix_rw, st)) return rc;
+  }
+  if (s.own.splits > 0) {
+    if (int rc = launch_attn_parts<T>(s.own, s.own_rw, st)) return rc;
+  }
+  const int64_t rows = (int64_t)s.join.B * s.join.H * s.join.S;
+  const dim3 block(kAttnThreads);
+  if (s.join.splits <= 64) hipLaunchKernelGGL((&attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, s.join);
+  else hipLaunchKernelGGL((&attn_join_kernel<T>), dim3((unsigned)rows), block, 0, st, s.join);
+  return launch_rc();
+}
+
 // Copies of the waves over the queries: two where there are two workgroups for every CU, else four.  Measured: 324 workgroups
 // (6 padded sequences of 1717, 2 key heads of 80, fp16) 141 us with two, 108 us with four; 512 (2 x 1024, 16 heads of 64, fp32) 119
 // and 104 us; 4096 (16 x 1024, 16 heads of 64, bf16) 125 and 214 us.

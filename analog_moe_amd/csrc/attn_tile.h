@@ -33,11 +33,12 @@ struct AttnParams {
   const void *lengths, *starts;      // [B] int32 / int64 or null
   int lengths_i64, starts_i64;
   int B, S, T, H, G, R, d, causal;   // G key heads, R = H / G query heads share one
+  int copies;                        // sequences of queries that share the keys of one (B counts the keys'): copies * b and on
   int vec;                           // every operand in whole aligned 16-byte chunks with offsets that fit 32 bits
   float c;                           // scale * log2(e)
   float scale;
   int splits;                        // forward of few rows: parts of the key axis
-  float *part_o, *part_ml;           // [splits][B * H * S][d rounded up to 4], [splits][B * H * S][2]
+  float *part_o, *part_ml;           // [splits][B * copies * H * S][d rounded up to 4], the same [2]; null: one part, the result
 };
 
 // keys that sequence b holds

@@ -16,6 +16,7 @@ so every group of calls the Python layer makes is one opaque operator with a fak
   amoe::cvmm_backward       everything CVMM.backward launches (cvmm.py:772-897)
   amoe::ffn_fwd / ffn_bwd   the fused expert feed-forward, with its autograd formula registered
   amoe::attention_fwd / attention_bwd, amoe::rotary / rotary_into   the decoder's attention and rotary positions, likewise
+  amoe::attention_shared                                            its attention over a shared prefix (no gradient)
   amoe::layer_norm_fwd / layer_norm_bwd                             its layer norm, likewise
   amoe::sample                                                      the choice of its next token
 
@@ -414,6 +415,19 @@ def _attention_autograd(ctx, go, _grad_lse, _grad_rest):
 
 
 attention_fwd.register_autograd(_attention_autograd, setup_context=_attention_setup_context)
+
+
+@torch.library.custom_op(
+    "amoe::attention_shared", mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor prefix_k, Tensor prefix_v, Tensor? lengths, Tensor? starts, Tensor? prefix_lengths, "
+           "bool causal, float? scale) -> Tensor")
+def attention_shared(q, k, v, prefix_k, prefix_v, lengths, starts, prefix_lengths, causal, scale):
+    return attention.shared_attention_forward(q, k, v, prefix_k, prefix_v, lengths, starts, prefix_lengths, causal, scale)
+
+
+@attention_shared.register_fake
+def _(q, k, v, prefix_k, prefix_v, lengths, starts, prefix_lengths, causal, scale):
+    return q.new_empty(tuple(q.shape))
 
 
 @torch.library.custom_op(

@@ -506,6 +506,28 @@ size_t amoe_attention_bwd_workspace(const amoe_attn_args* args);
 int amoe_attention_bwd(const amoe_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t amoe_attn_args_bytes(void);
 
+/* Attention of B sequences of which every B / prefixes in a row continue one prefix: out = softmax over the keys of the prefix, then
+ * the sequence's own.  q [B, S, H, d], k and v [B, T, G, d], prefix_k and prefix_v [prefixes, P, G, d]; sequence b reads prefix
+ * b / (B / prefixes), all keys [0, prefix_lengths) of it, and its own keys [0, lengths) as in amoe_attention_fwd (causal, starts: positions
+ * are those among the own keys).  T or P may be 0.  A prefix is read for all its sequences at once.  Limits as above, and B * H * S
+ * below 2^23 (AMOE_EUNSUPPORTED otherwise); results of parts of the keys pass through the workspace.  No gradients; no atomics. */
+typedef struct amoe_shared_attn_args {
+  int64_t dtype, B, S, T, P, prefixes, H, G, d, causal;
+  double scale;
+  const void* q;  int64_t q_sb, q_ss, q_sh;
+  const void* k;  int64_t k_sb, k_ss, k_sh;
+  const void* v;  int64_t v_sb, v_ss, v_sh;
+  const void* prefix_k;  int64_t prefix_k_sb, prefix_k_ss, prefix_k_sh;
+  const void* prefix_v;  int64_t prefix_v_sb, prefix_v_ss, prefix_v_sh;
+  const void* lengths;  int64_t lengths_is_i64;                 /* [B] int32 / int64, or NULL */
+  const void* starts;  int64_t starts_is_i64;
+  const void* prefix_lengths;  int64_t prefix_lengths_is_i64;   /* [prefixes] */
+  void* out;                                                    /* [B, S, H, d] */
+} amoe_shared_attn_args;
+size_t amoe_attention_shared_fwd_workspace(const amoe_shared_attn_args* args);
+int amoe_attention_shared_fwd(const amoe_shared_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t amoe_shared_attn_args_bytes(void);
+
 /* ---------------------------------------------------------------------------------------
  * The decoder's layer norm (nothing of the reference's own is replaced here).  Every field is 8 bytes wide.
  *
