@@ -4,10 +4,12 @@ The reference's example trains ``sigma_moe.SigmaMoEForCausalLM`` (example_aihwki
 third-party model whose feed-forward blocks are the SigmaMoE layers this package implements.  That model is
 not part of the reference checkout; this module provides the smallest stand-in that exercises the layer the
 same way: token + position embedding, pre-norm blocks of causal self-attention and an analog SigmaMoE
-feed-forward, final norm and language-model head.  Norms and embeddings are stock PyTorch; the
+feed-forward, final norm and language-model head.  Embeddings are stock PyTorch; the
 MoE feed-forward is ``AnalogSigmaMoELayer`` (or any module with its ``forward(x) -> (y, reg_loss)``).  Attention is stock
 PyTorch with a learned position table, or, with ``rotary``, this package's attention and rotary positions, which also
-serve: prompts and single tokens over a ``KVCache``, sequences of different lengths in one batch.
+serve: prompts and single tokens over a ``KVCache``, sequences of different lengths in one batch, several that continue one
+prompt, tokens drawn from the logits (``generate``).  Norms are ``nn.LayerNorm``, or, with ``norm=LayerNorm`` of this package, its
+kernels, which form the sum with the residual stream too.
 """
 from __future__ import annotations
 
@@ -18,8 +20,10 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
-from .attention import attention
+from .attention import attention, shared_attention
+from .norm import LayerNorm
 from .rotary import Rotary
+from .sampling import sample
 
 
 class CausalSelfAttention(nn.Module):
@@ -52,11 +56,26 @@ class KVCache:
             logits, _ = model(token, cache=cache)
             held.add_(1)
 
-    and replay no further than the room (past it the positions are an assertion on the device)."""
+    and replay no further than the room (past it the positions are an assertion on the device).
+
+    prefix: a cache that every batch / (its batch) sequences in a row continue (``share``); held and most count what comes after it."""
     keys: Tensor                                 # [layers, batch, room, key heads, head size]
     values: Tensor
     held: Tensor
     most: int = 0
+    prefix: Optional["KVCache"] = None
+
+    def share(self, copies: int, room: int) -> "KVCache":
+        """An empty cache for ``copies`` sequences after each of this one's, with room for ``room`` tokens of their own: what this one
+        holds now is read where it is, for all of them at once.  This one may go on by itself, but its tokens must stay."""
+        if self.prefix is not None:
+            raise ValueError("a cache that continues another one is not shared again")
+        if copies < 1 or room < 0:
+            raise ValueError(f"{copies} sequences with room for {room} tokens")
+        layers, batch, _, heads, head = self.keys.shape
+        keys, values = (t.new_empty((layers, batch * copies, room, heads, head)) for t in (self.keys, self.values))
+        held = self.held.new_zeros(batch * copies)
+        return KVCache(keys, values, held, 0, KVCache(self.keys, self.values, self.held.clone(), self.most))
 
 
 class RotarySelfAttention(nn.Module):
@@ -74,30 +93,35 @@ class RotarySelfAttention(nn.Module):
         self.proj = nn.Linear(d_model, d_model, bias=False)
 
     def forward(self, x: Tensor, lengths: Optional[Tensor] = None, cache: Optional[KVCache] = None, layer: int = 0,
-                positions: Optional[Tensor] = None) -> Tensor:
-        """lengths: tokens of each sequence that are not padding; with a cache, tokens held when x's are in it, and
-        positions [B, S] where x's stand."""
+                positions: Optional[Tensor] = None, places: Optional[Tensor] = None) -> Tensor:
+        """lengths: tokens of each sequence that are not padding; with a cache, tokens held when x's are in it, positions [B, S]
+        where x's stand, and places [B, S] where they stand in the cache (None: there too)."""
         B, S, D = x.shape
         q, k, v = self.qkv(x).view(B, S, -1, self.head).split((self.n_heads, self.kv_heads, self.kv_heads), dim=2)
         q, k = self.rotary(q, k, positions)
         starts = None
         if cache is not None:
-            at = (torch.arange(B, device=x.device)[:, None], positions)
+            at = (torch.arange(B, device=x.device)[:, None], positions if places is None else places)
             keys, values = cache.keys[layer], cache.values[layer]
             keys.index_put_(at, k.to(keys.dtype))
             values.index_put_(at, v.to(values.dtype))
             k, v, starts = keys[:, :cache.most + S], values[:, :cache.most + S], cache.held
         # (a cache of another type than q's: attention in the cache's)
-        out = attention(q.to(k.dtype), k, v, lengths=lengths, starts=starts).to(q.dtype)
+        if cache is not None and cache.prefix is not None:
+            pk, pv = (t[layer, :, :cache.prefix.most] for t in (cache.prefix.keys, cache.prefix.values))
+            out = shared_attention(q.to(k.dtype), k, v, pk, pv, lengths=lengths, starts=starts, prefix_lengths=cache.prefix.held).to(q.dtype)
+        else:
+            out = attention(q.to(k.dtype), k, v, lengths=lengths, starts=starts).to(q.dtype)
         return self.proj(out.reshape(B, S, D))
 
 
 class DecoderBlock(nn.Module):
-    def __init__(self, d_model: int, n_heads: int, ffn: nn.Module, attn: Optional[nn.Module] = None):
+    def __init__(self, d_model: int, n_heads: int, ffn: nn.Module, attn: Optional[nn.Module] = None,
+                 norm: Callable[[int], nn.Module] = nn.LayerNorm):
         super().__init__()
-        self.ln_attn = nn.LayerNorm(d_model)
+        self.ln_attn = norm(d_model)
         self.attn = CausalSelfAttention(d_model, n_heads) if attn is None else attn
-        self.ln_ffn = nn.LayerNorm(d_model)
+        self.ln_ffn = norm(d_model)
         self.ffn = ffn
 
     def forward(self, x: Tensor, **attn_args) -> Tuple[Tensor, Tensor]:
@@ -105,14 +129,22 @@ class DecoderBlock(nn.Module):
         y, reg = self.ffn(self.ln_ffn(x))
         return x + y, reg
 
+    def summed(self, x: Tensor, add: Optional[Tensor], **attn_args) -> Tuple[Tensor, Tensor, Tensor]:
+        """The block on the stream x + add, with norms that form the sums: (stream, what is to be added to it, regularisation)."""
+        n, x = (self.ln_attn(x), x) if add is None else self.ln_attn(add, x)
+        n, x = self.ln_ffn(self.attn(n, **attn_args), x)
+        y, reg = self.ffn(n)
+        return x, y, reg
+
 
 class SigmaMoEDecoder(nn.Module):
     """``make_ffn(layer_index) -> module`` builds the feed-forward of each block.  rotary: positions and attention of this
     package instead of a learned table of ``context`` positions and stock attention; kv_heads (None: n_heads) of its heads
-    hold keys and values."""
+    hold keys and values.  norm: ``nn.LayerNorm``, or ``analog_moe_amd.norm.LayerNorm`` (the same parameters)."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int, context: int,
-                 make_ffn: Callable[[int], nn.Module], rotary: Optional[Rotary] = None, kv_heads: Optional[int] = None):
+                 make_ffn: Callable[[int], nn.Module], rotary: Optional[Rotary] = None, kv_heads: Optional[int] = None,
+                 norm: Callable[[int], nn.Module] = nn.LayerNorm):
         super().__init__()
         if kv_heads is not None and rotary is None:
             raise ValueError("kv_heads goes with rotary: stock attention has as many key heads as heads")
@@ -121,8 +153,8 @@ class SigmaMoEDecoder(nn.Module):
 
         def attn():
             return None if rotary is None else RotarySelfAttention(d_model, n_heads, kv_heads or n_heads, rotary)
-        self.blocks = nn.ModuleList(DecoderBlock(d_model, n_heads, make_ffn(i), attn()) for i in range(n_layers))
-        self.ln_out = nn.LayerNorm(d_model)
+        self.blocks = nn.ModuleList(DecoderBlock(d_model, n_heads, make_ffn(i), attn(), norm) for i in range(n_layers))
+        self.ln_out = norm(d_model)
         self.head = nn.Linear(d_model, vocab_size, bias=False)
 
     def new_cache(self, batch: int, room: int) -> KVCache:
@@ -162,17 +194,54 @@ class SigmaMoEDecoder(nn.Module):
             # (within what ids have: positions past the cache's room are an assertion on the device)
             held = cache.held + (S if lengths is None else lengths.clamp(0, S))
             args = dict(lengths=held, cache=cache, positions=cache.held[:, None] + torch.arange(S, device=ids.device))
+            if cache.prefix is not None:
+                before = cache.prefix.held.repeat_interleave(B // cache.prefix.held.shape[0], output_size=B)
+                args.update(places=args["positions"], positions=args["positions"] + before[:, None])
         reg = x.new_zeros((), dtype=torch.float32)
+        summed, add = isinstance(self.ln_out, LayerNorm), None
         for i, blk in enumerate(self.blocks):
-            x, r = blk(x, layer=i, **args) if cache is not None else blk(x, **args)
+            if cache is not None:
+                args["layer"] = i
+            if summed:
+                x, add, r = blk.summed(x, add, **args)
+            else:
+                x, r = blk(x, **args)
             reg = reg + r.float()
         if cache is not None:
             cache.held, cache.most = held, cache.most + S
-        logits = self.head(self.ln_out(x))
+        logits = self.head(self.ln_out(x) if add is None else self.ln_out(add, x)[0])
         if labels is None:
             return logits, reg
         loss = F.cross_entropy(logits.float().view(B * S, -1), labels.reshape(-1))
         return loss + reg_weight * reg, reg
+
+    @torch.no_grad()
+    def generate(self, ids: Tensor, steps: int, copies: int = 1, lengths: Optional[Tensor] = None,
+                 generator: Optional[torch.Generator] = None, want_logprob: bool = False, **settings):
+        """``steps`` tokens after each prompt of ids [N, S] (lengths [N]: the tokens of each that are not padding, at least one), drawn
+        ``copies`` times: int64 [N * copies, steps], those of one prompt in a row; with want_logprob also the float32 logarithms of
+        their probabilities.  settings: temperature, top_k, top_p, min_p of ``sample`` (tensors hold one per sequence); temperature 0
+        makes all copies the same.  The prompts' keys are kept and read once for all copies."""
+        N, S = ids.shape
+        if S < 1 or steps < 0 or copies < 1:
+            raise ValueError(f"{steps} tokens after {copies} copies of prompts of {S}")
+        if lengths is not None:
+            lengths = lengths.clamp(1, S)
+        cache = self.new_cache(N, S if copies > 1 else S + steps)
+        logits, _ = self(ids, lengths=lengths, cache=cache)
+        last = logits[:, -1] if lengths is None else logits[torch.arange(N, device=ids.device), lengths.long() - 1]
+        if copies > 1:
+            cache, last = cache.share(copies, steps), last.repeat_interleave(copies, 0)
+        tokens = torch.empty(N * copies, steps, dtype=torch.int64, device=ids.device)
+        logprob = torch.empty(N * copies, steps, dtype=torch.float32, device=ids.device)
+        for s in range(steps):
+            u = torch.rand(N * copies, generator=generator, device=ids.device)
+            tokens[:, s], logprob[:, s] = sample(last, u, want_logprob=True, **settings)
+            if s + 1 < steps:
+                # (a row without a number has no token: -1 is not to be looked up)
+                logits, _ = self(tokens[:, s:s + 1].clamp_min(0), cache=cache)
+                last = logits[:, -1]
+        return (tokens, logprob) if want_logprob else tokens
 
     def post_update_step(self) -> None:
         """Weight clipping of the analog layers after an optimizer step (moe_layer_aihwkit_lightning.py:509-517)."""
