@@ -19,6 +19,8 @@
 namespace amoe {
 
 typedef unsigned long long u64;
+// (closures that are not inlined live in memory, and with them all that they refer to)
+#define AMOE_INLINE __attribute__((always_inline))
 
 struct SampleParams {
   const void* logits;                // [rows, V], ld elements apart
@@ -39,53 +41,60 @@ constexpr int kList = 2048;          // elements that are ranked at once
 constexpr u64 kOne = 1ull << 44;
 constexpr int kIndexBits = 20;
 
-// A row of V elements as chunks of 16 bytes that begin on 4: chunk 0 is the element before the first of them, if there is one, the
-// last chunk what is left.  Groups of 64 chunks go to the waves in units of `per`, four units at most to a wave.
+// A row of V elements: chunks of 16 bytes that begin on 4, and what is left before (one element) and behind them (less than a
+// chunk), which lanes of the first wave hold one by one.  Groups of 64 chunks go to the waves in units of `per`, four units at most to
+// a wave, 60 in all.  Chunks past the last one read as zeros from a resource that ends with it, so that no load waits for a branch.
 template <typename T, int W> struct SampleRow {
   static constexpr int C = Elem<T>::kChunk;
-  const T* p;
+  BufRsrc chunks_at;
   int head, body, tail, groups, per, units;
-  __device__ __forceinline__ SampleRow(const T* row, int V) : p(row) {
+  float edge;                        // of the first wave's lanes: lane 0 the element before the chunks, lanes 1 .. those behind
+  int edge_index;
+  __device__ __forceinline__ SampleRow(const T* row, int V) {
     head = sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(row) & 2) ? 1 : 0;
     body = (V - head) / C;
     tail = V - head - body * C;
-    groups = (body + 2 + 63) / 64;
-    const int even = (groups + W - 1) / W, most = (groups + 4 * W - 1) / (4 * W);
-    per = most > 4 ? most : (even < 4 ? even : 4);
+    groups = (body + 63) / 64;
+    const int even = (groups + W - 1) / W;
+    constexpr int kMost = 4 * W < 60 ? 4 * W : 60;
+    per = (groups + kMost - 1) / kMost;
+    if (per < 4) per = even < 4 ? (even > 1 ? even : 1) : 4;
     units = (groups + per - 1) / per;
+    chunks_at = make_rsrc_sized(const_cast<T*>(row + head), (uint32_t)body * 16u);
+    const int t = threadIdx.x;
+    edge_index = t == 0 ? 0 : V - tail + t - 1;
+    const bool there = t == 0 ? head == 1 : t <= tail;
+    edge = there ? Elem<T>::load(row + edge_index) : -INFINITY;
+    edge = edge == edge ? edge : -INFINITY;
   }
-  __device__ __forceinline__ int start(int j) const { return j == 0 ? 0 : head + (j - 1) * C; }
-  __device__ __forceinline__ int count(int j) const { return j == 0 ? head : j <= body ? C : j == body + 1 ? tail : 0; }
-  __device__ __forceinline__ Raw load(int j) const {
-    typedef u32x4 __attribute__((aligned(4))) RawU;
-    if (j > 0 && j <= body) return *reinterpret_cast<const RawU*>(p + start(j));
-    return raw_load<T>(p + start(j), count(j), false);
-  }
-  // f(values, index of the first, how many) for the chunks of groups [g, g_end) that are this lane's
+  __device__ __forceinline__ int start(int j) const { return head + j * C; }
+  // f(values, index of the first) for the chunks of groups [g, g_end) that are this lane's; minus infinity where there is no number
   template <class F>
   __device__ __forceinline__ void chunks(int g, int g_end, F f) const {
+    constexpr int kAhead = 4;
     const int lane = lane_id();
-    for (; g < g_end; g += 4) {
-      Raw r[4];
+    for (; g < g_end; g += kAhead) {
+      Raw r[kAhead];
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (g + i < g_end) r[i] = load((g + i) * 64 + lane);
+      for (int i = 0; i < kAhead; i++) r[i] = buffer_load_b128(chunks_at, (uint32_t)((g + i) * 64 + lane) * 16u, 0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < kAhead; i++) {
+        const int j = (g + i) * 64 + lane;
         if (g + i >= g_end) continue;
-        const int j = (g + i) * 64 + lane, n = count(j);
         float v[C];
         raw_unpack<T>(r[i], v);
 #pragma unroll
-        for (int e = 0; e < C; e++) v[e] = e < n && v[e] == v[e] ? v[e] : -INFINITY;      // (not a number: not a token)
-        if (n > 0) f(v, start(j), n);
+        for (int e = 0; e < C; e++) v[e] = j < body && v[e] == v[e] ? v[e] : -INFINITY;
+        f(v, start(j));
       }
     }
   }
-  template <class F>
-  __device__ __forceinline__ void all(F f) const {
+  // every element: f(values, index of the first) on chunks, one(value, index) on single ones
+  template <class F, class One>
+  __device__ __forceinline__ void all(F f, One one) const {
     const int wave = wave_uniform(threadIdx.x >> 6);
     for (int u = wave; u < units; u += W) chunks(u * per, (u + 1) * per < groups ? (u + 1) * per : groups, f);
+    if (threadIdx.x < 64 && edge != -INFINITY) one(edge, edge_index);
   }
 };
 
@@ -95,7 +104,6 @@ struct SampleWeight {
   bool flat;                         // only the largest weigh (temperature 0, or infinite logits)
   const double* table;               // 2^(j / 256)
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (flat) return x == top ? kOne : 0;
     // (what is so far below that it weighs nothing, and minus infinity, whose distance may be no number)
     const double t = __builtin_fmax(((double)x - (double)top) * scale, -46.0 * 256.0);
     const double n = __builtin_rint(t), f = t - n;
@@ -104,7 +112,8 @@ struct SampleWeight {
     const double q = f * __builtin_fma(f, __builtin_fma(f, __builtin_fma(f, a * a * a * a / 24, a * a * a / 6), a * a / 2), a);
     const double w = table[i & 255];
     // (256 + w: the last bit counts 2^-44)
-    return __builtin_bit_cast(u64, __builtin_ldexp(__builtin_fma(w, q, w), i >> 8) + 256.0) - __builtin_bit_cast(u64, 256.0);
+    const u64 r = __builtin_bit_cast(u64, __builtin_ldexp(__builtin_fma(w, q, w), i >> 8) + 256.0) - __builtin_bit_cast(u64, 256.0);
+    return flat ? (x == top ? kOne : 0) : r;
   }
 };
 
@@ -217,17 +226,20 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
       r.digit.w[i] = 0;
     }
     __syncthreads();
-    row.all([&](const float (&v)[SampleRow<T, W>::C], int first, int n) {
+    const auto count_one = [&](float x, int index) AMOE_INLINE {
+      if (bin(x) != b) return;
+      const u64 rank = sample_rank(x, index);
+      if (rank >> shift != prefix) return;
+      const int d = size - 1 - (int)((rank >> next) & (u64)(size - 1));
+      atomicAdd(&r.digit.n[d], 1u);
+      atomicAdd(&r.digit.w[d], weight(x));
+    };
+    row.all(
+        [&](const float (&v)[SampleRow<T, W>::C], int first) AMOE_INLINE {
 #pragma unroll
-      for (int e = 0; e < SampleRow<T, W>::C; e++) {
-        if (e >= n || bin(v[e]) != b) continue;
-        const u64 rank = sample_rank(v[e], first + e);
-        if (rank >> shift != prefix) continue;
-        const int d = size - 1 - (int)((rank >> next) & (u64)(size - 1));
-        atomicAdd(&r.digit.n[d], 1u);
-        atomicAdd(&r.digit.w[d], weight(v[e]));
-      }
-    });
+          for (int e = 0; e < SampleRow<T, W>::C; e++) count_one(v[e], first + e);
+        },
+        count_one);
     __syncthreads();
     sample_crossing<NT>(r.digit, size, by_weight, target - (by_weight ? before_w : before_n), sh);
     const int d = sh.found;
@@ -240,14 +252,17 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
   __syncthreads();
   if (tid == 0) sh.listed = 0;
   __syncthreads();
-  row.all([&](const float (&v)[SampleRow<T, W>::C], int first, int n) {
+  const auto list_one = [&](float x, int index) AMOE_INLINE {
+    if (bin(x) != b) return;
+    const u64 rank = sample_rank(x, index);
+    if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
+  };
+  row.all(
+      [&](const float (&v)[SampleRow<T, W>::C], int first) AMOE_INLINE {
 #pragma unroll
-    for (int e = 0; e < SampleRow<T, W>::C; e++) {
-      if (e >= n || bin(v[e]) != b) continue;
-      const u64 rank = sample_rank(v[e], first + e);
-      if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
-    }
-  });
+        for (int e = 0; e < SampleRow<T, W>::C; e++) list_one(v[e], first + e);
+      },
+      list_one);
   int size = 2;
   while (size < count) size *= 2;
   for (int i = count + tid; i < size; i += NT) r.list[i] = 0;
@@ -301,13 +316,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   for (int i = tid; i < 256; i += NT) sh.table[i] = ::exp2((double)i / 256.0);
 
   float mx = -INFINITY, mn = INFINITY;
-  row.all([&](const float (&v)[C], int, int) {
+  const auto extremes = [&](float x, int) AMOE_INLINE {
+    mx = fmaxf(mx, x);
+    if (CUT) mn = fminf(mn, x == -INFINITY ? INFINITY : x);
+  };
+  row.all(
+      [&](const float (&v)[C], int first) AMOE_INLINE {
 #pragma unroll
-    for (int e = 0; e < C; e++) {
-      mx = fmaxf(mx, v[e]);
-      if (CUT) mn = fminf(mn, v[e] == -INFINITY ? INFINITY : v[e]);
-    }
-  });
+        for (int e = 0; e < C; e++) extremes(v[e], first + e);
+      },
+      extremes);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     mx = fmaxf(mx, wave_shfl_xor(mx, d));
@@ -344,7 +362,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
       const float half = 0.5f * mx, reach = fminf(fmaf(-0.5f, mn, half), 16.f * temperature);
       const float step = reach > 0.f ? fminf((kBins - 2) / reach, 3.402823466e38f) : 0.f;
       const bool flat = weight.flat;
-      const auto bin = [=](float x) {
+      const auto bin = [=](float x) AMOE_INLINE {
         if (flat) return x == mx ? 0 : kBins - 1;
         return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins - 1));
       };
@@ -353,15 +371,18 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         hist.w[i] = 0;
       }
       __syncthreads();
-      row.all([&](const float (&v)[C], int, int n) {
+      const auto count_one = [&](float x, int) AMOE_INLINE {
+        const int b = bin(x);
+        if (b >= kBins - 1) return;
+        atomicAdd(&hist.n[b], 1u);
+        if (by_p) atomicAdd(&hist.w[b], weight(x));
+      };
+      row.all(
+          [&](const float (&v)[C], int first) AMOE_INLINE {
 #pragma unroll
-        for (int e = 0; e < C; e++) {
-          const int b = bin(v[e]);
-          if (e >= n || b >= kBins - 1) continue;
-          atomicAdd(&hist.n[b], 1u);
-          if (by_p) atomicAdd(&hist.w[b], weight(v[e]));
-        }
-      });
+            for (int e = 0; e < C; e++) count_one(v[e], first + e);
+          },
+          count_one);
       __syncthreads();
       u64 total = 0;
       bool cut_by_k = false;
@@ -405,23 +426,25 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   const int cut_i = cut ? sample_index(cut) : p.V;
   const u64 least = min_p > 0.f ? (u64)__builtin_ceil((double)fminf(min_p, 1.f) * (double)kOne) : 0;
   // weights of a chunk's kept elements
-  const auto weigh = [&](const float (&v)[C], int first, u64 (&w)[C]) {
+  const auto weigh_one = [&](float x, int index) AMOE_INLINE -> u64 {
+    const bool keep = (x > cut_x) | ((x == cut_x) & (index <= cut_i));
+    const u64 w = weight(x);
+    return keep & (w >= least) ? w : 0;
+  };
+  const auto weigh = [&](const float (&v)[C], int first, u64 (&w)[C]) AMOE_INLINE {
     bool any = false;
 #pragma unroll
-    for (int e = 0; e < C; e++) any = any || v[e] >= cut_x;
-#pragma unroll
-    for (int e = 0; e < C; e++) w[e] = 0;
+    for (int e = 0; e < C; e++) {
+      any = any | (v[e] >= cut_x);
+      w[e] = 0;
+    }
     if (!any) return;
 #pragma unroll
-    for (int e = 0; e < C; e++) {
-      const bool keep = v[e] > cut_x || (v[e] == cut_x && first + e <= cut_i);
-      const u64 x = weight(v[e]);
-      w[e] = keep && x >= least ? x : 0;
-    }
+    for (int e = 0; e < C; e++) w[e] = weigh_one(v[e], first + e);
   };
-  const auto group_sum = [&](int g, int g_end) {
+  const auto group_sum = [&](int g, int g_end) AMOE_INLINE {
     u64 s = 0;
-    row.chunks(g, g_end, [&](const float (&v)[C], int first, int) {
+    row.chunks(g, g_end, [&](const float (&v)[C], int first) AMOE_INLINE {
       u64 w[C];
       weigh(v, first, w);
 #pragma unroll
@@ -429,7 +452,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     });
     return s;
   };
-  const auto wave_total = [&](u64 s) {
+  const auto wave_total = [&](u64 s) AMOE_INLINE {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s += wave_shfl_xor(s, d);
     return s;
@@ -438,60 +461,79 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   for (int i = wave; i < row.units; i += W) {
     const int end = (i + 1) * row.per < row.groups ? (i + 1) * row.per : row.groups;
     const u64 s = wave_total(group_sum(i * row.per, end));
-    if (lane == 0) sh.unit[i] = s;
+    if (lane == 0) sh.unit[1 + i] = s;
+  }
+  // the element before the chunks and those behind them are units of their own, the first and the last
+  const u64 edge_w = wave == 0 && row.edge != -INFINITY ? weigh_one(row.edge, row.edge_index) : 0;
+  if (wave == 0) {
+    const u64 behind = wave_total(lane == 0 ? 0 : edge_w);
+    if (lane == 0) {
+      sh.unit[0] = edge_w;
+      sh.unit[1 + row.units] = behind;
+    }
   }
   __syncthreads();
   // the unit, then the group of chunks, then the chunk, then the element at which the sum passes u times the total
-  u64 mine = lane < row.units ? sh.unit[lane] : 0, run = wave_scan(mine);
+  u64 mine = lane < row.units + 2 ? sh.unit[lane] : 0, run = wave_scan(mine);
   const u64 total = wave_shfl(run, 63);
   const double want = (u > 0.0 ? u : 0.0) * (double)total;
   u64 target = want < (double)total ? (u64)want : total - 1;
   if (target >= total) target = total - 1;
-  const int unit = ctz64(wave_ballot(run > target));
-  target -= wave_shfl(run - mine, unit);
+  const int unit = ctz64(wave_ballot(run > target)) - 1;
+  target -= wave_shfl(run - mine, unit + 1);
+  const bool edges = unit < 0 || unit == row.units;
   const int g0 = unit * row.per, g1 = g0 + row.per < row.groups ? g0 + row.per : row.groups;
-  for (int g = g0 + wave; g < g1; g += W) {
-    const u64 s = wave_total(group_sum(g, g + 1));
-    if (lane == 0) sh.group[g - g0] = s;
+  if (!edges) {
+    for (int g = g0 + wave; g < g1; g += W) {
+      const u64 s = wave_total(group_sum(g, g + 1));
+      if (lane == 0) sh.group[g - g0] = s;
+    }
   }
   __syncthreads();
   if (wave != 0) return;
-  const u64 even = 2 * lane < g1 - g0 ? sh.group[2 * lane] : 0, odd = 2 * lane + 1 < g1 - g0 ? sh.group[2 * lane + 1] : 0;
-  run = wave_scan(even + odd);
-  const int pair = ctz64(wave_ballot(run > target));
-  target -= wave_shfl(run - even - odd, pair);
-  const u64 first_of_pair = wave_shfl(even, pair);
-  const bool second = target >= first_of_pair;
-  if (second) target -= first_of_pair;
-  const int group = g0 + 2 * pair + (second ? 1 : 0);
-  u64 w[C] = {};
-  float x[C] = {};
-  int start = 0;
-  row.chunks(group, group + 1, [&](const float (&v)[C], int first, int) {
-    weigh(v, first, w);
-    start = first;
-#pragma unroll
-    for (int e = 0; e < C; e++) x[e] = v[e];
-  });
-  mine = 0;
-#pragma unroll
-  for (int e = 0; e < C; e++) mine += w[e];
-  run = wave_scan(mine);
-  if (lane != ctz64(wave_ballot(run > target))) return;
-  u64 sum = run - mine;
   int which = 0;
-  float value = x[0];
-  bool found = false;
+  float value = 0.f;
+  if (edges) {
+    run = wave_scan((lane == 0) == (unit < 0) ? edge_w : 0);
+    if (lane != ctz64(wave_ballot(run > target))) return;
+    which = row.edge_index;
+    value = row.edge;
+  } else {
+    const u64 even = 2 * lane < g1 - g0 ? sh.group[2 * lane] : 0, odd = 2 * lane + 1 < g1 - g0 ? sh.group[2 * lane + 1] : 0;
+    run = wave_scan(even + odd);
+    const int pair = ctz64(wave_ballot(run > target));
+    target -= wave_shfl(run - even - odd, pair);
+    const u64 first_of_pair = wave_shfl(even, pair);
+    const bool second = target >= first_of_pair;
+    if (second) target -= first_of_pair;
+    const int group = g0 + 2 * pair + (second ? 1 : 0);
+    u64 w[C] = {};
+    float x[C] = {};
+    int start = 0;
+    row.chunks(group, group + 1, [&](const float (&v)[C], int first) AMOE_INLINE {
+      weigh(v, first, w);
+      start = first;
 #pragma unroll
-  for (int e = 0; e < C; e++) {
-    sum += w[e];
-    if (!found && sum > target) {
-      found = true;
-      which = e;
-      value = x[e];
+      for (int e = 0; e < C; e++) x[e] = v[e];
+    });
+    mine = 0;
+#pragma unroll
+    for (int e = 0; e < C; e++) mine += w[e];
+    run = wave_scan(mine);
+    if (lane != ctz64(wave_ballot(run > target))) return;
+    u64 sum = run - mine;
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < C; e++) {
+      sum += w[e];
+      if (!found && sum > target) {
+        found = true;
+        which = start + e;
+        value = x[e];
+      }
     }
   }
-  p.ids[at] = start + which;
+  p.ids[at] = which;
   if (p.logprob) {
     const double log_total = ::log((double)total * 0x1p-44);
     p.logprob[at] = greedy ? 0.f : (float)((weight.flat ? 0.0 : ((double)value - (double)mx) / (double)temperature) - log_total);
