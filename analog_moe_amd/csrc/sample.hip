@@ -9,9 +9,8 @@
 // within 2^-44 of the largest weight.  (In fp32 a row of 10^5 logits would go to a neighbour about once in a thousand draws.)
 // What weighs less than 2^-45 of the largest is never drawn.
 //
-// The cut that top_k and top_p make in the ranking is found without a sort: the distances from the maximum are counted (and weighed)
-// in 2047 equal intervals, and only the interval with the cut is ranked.  Bound by LDS atomics and 64-bit arithmetic where rows are
-// truncated, by the weights' arithmetic and memory where not.
+// The cut that top_k and top_p make in the ranking is found without a sort: tokens are counted, or weighed, by their weight's binary
+// logarithm in up to 2047 bins, and only those of the bin with the cut are ranked.
 #include <amoe.h>
 
 #include "host_util.h"
@@ -36,18 +35,21 @@ struct SampleParams {
 };
 
 constexpr int64_t kSampleMaxV = (1 << 20) - 1;       // (as many largest weights are less than 2^64)
-constexpr int kBins = 2048;          // the last one holds what weighs nothing and is not counted
+constexpr int kBins = 2048;          // the last one holds what is not looked at
 constexpr int kList = 2048;          // elements that are ranked at once
+constexpr int kUnits = 240;
+constexpr int kLevels = 46 * 256;    // below the largest weight by this many 256ths of a factor of two: 0 as a multiple of 2^-44
 constexpr u64 kOne = 1ull << 44;
 constexpr int kIndexBits = 20;
 
 // A row of V elements: chunks of 16 bytes that begin on 4, and what is left before (one element) and behind them (less than a
-// chunk), which lanes of the first wave hold one by one.  Groups of 64 chunks go to the waves in units of `per`, four units at most to
-// a wave, 60 in all.  Chunks past the last one read as zeros from a resource that ends with it, so that no load waits for a branch.
+// chunk), which lanes of the first wave hold one by one.  `per` groups of 64 chunks are a unit; units are counted from 1, what is
+// before the chunks is unit 0 and what is behind them the last.  Chunks past the end read as zeros from a resource that ends with
+// them, so that no load waits for a branch.
 template <typename T, int W> struct SampleRow {
   static constexpr int C = Elem<T>::kChunk;
   BufRsrc chunks_at;
-  int head, body, tail, groups, per, units;
+  int head, body, tail, groups, per, units, last;
   float edge;                        // of the first wave's lanes: lane 0 the element before the chunks, lanes 1 .. those behind
   int edge_index;
   __device__ __forceinline__ SampleRow(const T* row, int V) {
@@ -55,11 +57,11 @@ template <typename T, int W> struct SampleRow {
     body = (V - head) / C;
     tail = V - head - body * C;
     groups = (body + 63) / 64;
-    const int even = (groups + W - 1) / W;
-    constexpr int kMost = 4 * W < 60 ? 4 * W : 60;
-    per = (groups + kMost - 1) / kMost;
-    if (per < 4) per = even < 4 ? (even > 1 ? even : 1) : 4;
+    const int least = groups / (4 * W);
+    per = (groups + kUnits - 1) / kUnits;
+    if (per < 4) per = least >= 4 ? 4 : least > per ? least : per > 1 ? per : 1;
     units = (groups + per - 1) / per;
+    last = units + 1;
     chunks_at = make_rsrc_sized(const_cast<T*>(row + head), (uint32_t)body * 16u);
     const int t = threadIdx.x;
     edge_index = t == 0 ? 0 : V - tail + t - 1;
@@ -68,52 +70,84 @@ template <typename T, int W> struct SampleRow {
     edge = edge == edge ? edge : -INFINITY;
   }
   __device__ __forceinline__ int start(int j) const { return head + j * C; }
-  // f(values, index of the first) for the chunks of groups [g, g_end) that are this lane's; minus infinity where there is no number
-  template <class F>
-  __device__ __forceinline__ void chunks(int g, int g_end, F f) const {
-    constexpr int kAhead = 4;
+  __device__ __forceinline__ int unit_of(int index) const {
+    if (index < head) return 0;
+    const int j = (index - head) / C;
+    return j >= body ? last : 1 + j / 64 / per;
+  }
+  // f(values, index of the first, whether the chunk is in the row) for the chunks of groups [g, g_end) that are this lane's, done(unit)
+  // after each unit; minus infinity where there is no number
+  template <class F, class Done>
+  __device__ __forceinline__ void scan(int g, int g_end, F f, Done done) const {
+    constexpr int kAhead = sizeof(T) == 4 ? 8 : 4;
     const int lane = lane_id();
+    int in_unit = g % per, unit = 1 + g / per;
     for (; g < g_end; g += kAhead) {
       Raw r[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; i++) r[i] = buffer_load_b128(chunks_at, (uint32_t)((g + i) * 64 + lane) * 16u, 0);
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
+        if (g + i >= g_end) break;
         const int j = (g + i) * 64 + lane;
-        if (g + i >= g_end) continue;
+        const bool inside = j < body;
         float v[C];
         raw_unpack<T>(r[i], v);
 #pragma unroll
-        for (int e = 0; e < C; e++) v[e] = j < body && v[e] == v[e] ? v[e] : -INFINITY;
-        f(v, start(j));
+        for (int e = 0; e < C; e++) v[e] = inside & (v[e] == v[e]) ? v[e] : -INFINITY;
+        f(v, start(j), inside);
+        if (++in_unit == per || g + i + 1 == g_end) {
+          done(unit++);
+          in_unit = 0;
+        }
       }
     }
   }
-  // every element: f(values, index of the first) on chunks, one(value, index) on single ones
-  template <class F, class One>
-  __device__ __forceinline__ void all(F f, One one) const {
-    const int wave = wave_uniform(threadIdx.x >> 6);
-    for (int u = wave; u < units; u += W) chunks(u * per, (u + 1) * per < groups ? (u + 1) * per : groups, f);
-    if (threadIdx.x < 64 && edge != -INFINITY) one(edge, edge_index);
+  // the whole row: a wave's units lie next to each other
+  template <class F, class Done>
+  __device__ __forceinline__ void all(F f, Done done) const {
+    const int wave = wave_uniform(threadIdx.x >> 6), share = (units + W - 1) / W;
+    const int g = wave * share * per, end = g + share * per;
+    scan(g, end < groups ? end : groups, f, done);
   }
 };
 
+// The weight of an element, in multiples of 2^-44 of the largest, and its level, the logarithm of that (256 to a factor of two).
 struct SampleWeight {
-  float top;
-  double scale;                      // 256 log2(e) / temperature
-  bool flat;                         // only the largest weigh (temperature 0, or infinite logits)
+  float floor;                       // weighs nothing
+  bool hot;                          // not even minus infinity is below the floor by itself
+  double top, scale;                 // 256 log2(e) / temperature
   const double* table;               // 2^(j / 256)
-  __device__ __forceinline__ u64 operator()(float x) const {
-    // (what is so far below that it weighs nothing, and minus infinity, whose distance may be no number)
-    const double t = __builtin_fmax(((double)x - (double)top) * scale, -46.0 * 256.0);
-    const double n = __builtin_rint(t), f = t - n;
-    const int i = (int)n;
+  __device__ __forceinline__ SampleWeight(float mx, float temperature, const double* table_) : top(mx), table(table_) {
+    // (the next float down, where 33 temperatures are less than that: then nothing but the largest weighs)
+    const uint32_t b = as_u32(mx);
+    const float next = mx == 0.f ? -1e-45f : as_f32(mx > 0.f ? b - 1 : b + 1);
+    const float down = mx - 33.f * temperature;
+    floor = fmaxf(fminf(down, next), -3.402823466e38f);
+    hot = !(down > -3.3e38f);
+    const double most = (kLevels + 1000.0) / (top - (double)floor);
+    scale = 256 * 1.44269504088896340736 / (double)temperature;
+    if (!(scale < most) && !hot) scale = most;
+  }
+  __device__ __forceinline__ int level(float x, double& rest) const {
+    constexpr double kMagic = 6755399441055744.0;          // 1.5 * 2^52: whole numbers are its last bits
+    const double t = ((double)fmaxf(x, floor) - top) * scale, m = t + kMagic;
+    rest = t - (m - kMagic);
+    return (int)(uint32_t)__builtin_bit_cast(u64, m);
+  }
+  __device__ __forceinline__ u64 of(float x, int level, double f) const {
     constexpr double a = 0.69314718055994530942 / 256;
     const double q = f * __builtin_fma(f, __builtin_fma(f, __builtin_fma(f, a * a * a * a / 24, a * a * a / 6), a * a / 2), a);
-    const double w = table[i & 255];
+    const u64 bits = __builtin_bit_cast(u64, table[level & 255]) + ((u64)(uint32_t)((level & ~255) << 12) << 32);
+    const double w = __builtin_bit_cast(double, bits);
     // (256 + w: the last bit counts 2^-44)
-    const u64 r = __builtin_bit_cast(u64, __builtin_ldexp(__builtin_fma(w, q, w), i >> 8) + 256.0) - __builtin_bit_cast(u64, 256.0);
-    return flat ? (x == top ? kOne : 0) : r;
+    const u64 r = __builtin_bit_cast(u64, __builtin_fma(w, q, w) + 256.0) - __builtin_bit_cast(u64, 256.0);
+    return hot && x == -INFINITY ? 0 : r;
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    double f;
+    const int l = level(x, f);
+    return of(x, l, f);
   }
 };
 
@@ -138,14 +172,24 @@ __device__ __forceinline__ V wave_scan(V v) {       // sums up to and with the l
   }
   return v;
 }
+__device__ __forceinline__ u64 wave_total(u64 s) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) s += wave_shfl_xor(s, d);
+  return s;
+}
+__device__ __forceinline__ float wave_largest(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, wave_shfl_xor(v, d));
+  return v;
+}
 
 // What a workgroup shares beside the histogram.
 template <int W> struct SampleShared {
   double table[256];
-  u64 unit[64], group[128], wave_w[W];
-  float wave_max[W], wave_min[W];
+  u64 unit[kUnits + 2], group[32], wave_w[W];
+  float unit_max[kUnits + 2], wave_max[W], wave_min[W];
   int wave_n[W], found, listed;
-  u64 found_w, found_n, cut;
+  u64 found_w, found_n, cut, rest;
 };
 struct SampleBins {
   uint32_t n[kBins];
@@ -207,67 +251,16 @@ __device__ __forceinline__ void sample_crossing(const SampleBins& bins, int size
   __syncthreads();
 }
 
-// The rank at which `target` is reached within one bin of the row (n of its elements, w of weight before the bin): sh.cut, and in
-// found_w the weight up to and with it.
-template <typename T, int NT, class Bin>
-__device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, const SampleWeight& weight, Bin bin, int b, int count,
-                                              bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked& r,
-                                              SampleShared<NT / 64>& sh) {
-  constexpr int W = NT / 64;
+// The list of `count` ranks, the largest first, and where `target` is reached in it (before_n elements and before_w of weight come
+// before it): sh.cut, and in found_w the weight up to and with it.
+template <int NT>
+__device__ __forceinline__ void sample_sort(const SampleWeight& weight, int count, bool by_weight, u64 target, u64 before_n, u64 before_w,
+                                            SampleRanked& r, SampleShared<NT / 64>& sh) {
   const int tid = threadIdx.x;
-  // too many to rank at once: by 11 bits of their ranks at a time
-  int shift = 32 + kIndexBits;
-  u64 prefix = 0;
-  while (count > kList) {
-    const int next = shift > 11 ? shift - 11 : 0, size = 1 << (shift - next);
-    __syncthreads();
-    for (int i = tid; i < kBins; i += NT) {
-      r.digit.n[i] = 0;
-      r.digit.w[i] = 0;
-    }
-    __syncthreads();
-    const auto count_one = [&](float x, int index) AMOE_INLINE {
-      if (bin(x) != b) return;
-      const u64 rank = sample_rank(x, index);
-      if (rank >> shift != prefix) return;
-      const int d = size - 1 - (int)((rank >> next) & (u64)(size - 1));
-      atomicAdd(&r.digit.n[d], 1u);
-      atomicAdd(&r.digit.w[d], weight(x));
-    };
-    row.all(
-        [&](const float (&v)[SampleRow<T, W>::C], int first) AMOE_INLINE {
-#pragma unroll
-          for (int e = 0; e < SampleRow<T, W>::C; e++) count_one(v[e], first + e);
-        },
-        count_one);
-    __syncthreads();
-    sample_crossing<NT>(r.digit, size, by_weight, target - (by_weight ? before_w : before_n), sh);
-    const int d = sh.found;
-    count = (int)r.digit.n[d];
-    before_n += sh.found_n;
-    before_w += sh.found_w;
-    prefix = (prefix << (shift - next)) | (u64)(size - 1 - d);
-    shift = next;
-  }
-  __syncthreads();
-  if (tid == 0) sh.listed = 0;
-  __syncthreads();
-  const auto list_one = [&](float x, int index) AMOE_INLINE {
-    if (bin(x) != b) return;
-    const u64 rank = sample_rank(x, index);
-    if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
-  };
-  row.all(
-      [&](const float (&v)[SampleRow<T, W>::C], int first) AMOE_INLINE {
-#pragma unroll
-        for (int e = 0; e < SampleRow<T, W>::C; e++) list_one(v[e], first + e);
-      },
-      list_one);
   int size = 2;
   while (size < count) size *= 2;
   for (int i = count + tid; i < size; i += NT) r.list[i] = 0;
   __syncthreads();
-  // the largest first
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
       for (int i = tid; i < size / 2; i += NT) {
@@ -288,7 +281,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
     w[i] = tid * P + i < count ? weight(sample_value(r.list[tid * P + i])) : 0;
     sum += w[i];
   }
-  sample_scan<W>(none, sum, sh);
+  sample_scan<NT / 64>(none, sum, sh);
 #pragma unroll
   for (int i = 0; i < P; i++) {
     const int at = tid * P + i;
@@ -302,6 +295,155 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
   __syncthreads();
 }
 
+// The same for one bin of the row, whatever number of elements (`count`) it has.
+template <typename T, int NT, class Bin>
+__device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, const SampleWeight& weight, Bin bin, int b, int count,
+                                              bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked& r,
+                                              SampleShared<NT / 64>& sh) {
+  constexpr int W = NT / 64, C = SampleRow<T, W>::C;
+  const int tid = threadIdx.x;
+  const auto none = [](int) AMOE_INLINE {};
+  // too many to rank at once: by 11 bits of their ranks at a time
+  int shift = 32 + kIndexBits;
+  u64 prefix = 0;
+  while (count > kList) {
+    const int next = shift > 11 ? shift - 11 : 0, size = 1 << (shift - next);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += NT) {
+      r.digit.n[i] = 0;
+      r.digit.w[i] = 0;
+    }
+    __syncthreads();
+    const auto count_one = [&](float x, int index) AMOE_INLINE {
+      if (bin(x) != b) return;
+      const u64 rank = sample_rank(x, index);
+      if (rank >> shift != prefix) return;
+      const int d = size - 1 - (int)((rank >> next) & (u64)(size - 1));
+      atomicAdd(&r.digit.n[d], 1u);
+      atomicAdd(&r.digit.w[d], weight(x));
+    };
+    row.all(
+        [&](const float (&v)[C], int first, bool) AMOE_INLINE {
+#pragma unroll
+          for (int e = 0; e < C; e++) count_one(v[e], first + e);
+        },
+        none);
+    if (tid < 64) count_one(row.edge, row.edge_index);
+    __syncthreads();
+    sample_crossing<NT>(r.digit, size, by_weight, target - (by_weight ? before_w : before_n), sh);
+    const int d = sh.found;
+    count = (int)r.digit.n[d];
+    before_n += sh.found_n;
+    before_w += sh.found_w;
+    prefix = (prefix << (shift - next)) | (u64)(size - 1 - d);
+    shift = next;
+  }
+  __syncthreads();
+  if (tid == 0) sh.listed = 0;
+  __syncthreads();
+  const auto list_one = [&](float x, int index) AMOE_INLINE {
+    if (bin(x) != b) return;
+    const u64 rank = sample_rank(x, index);
+    if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
+  };
+  row.all(
+      [&](const float (&v)[C], int first, bool) AMOE_INLINE {
+#pragma unroll
+        for (int e = 0; e < C; e++) list_one(v[e], first + e);
+      },
+      none);
+  if (tid < 64) list_one(row.edge, row.edge_index);
+  __syncthreads();
+  sample_sort<NT>(weight, count, by_weight, target, before_n, before_w, r, sh);
+}
+
+// The element at which the sum of weights passes `target`, from the units' sums: weigh(value, index).  True for the thread that has
+// it.  Every thread calls this.
+template <typename T, int W, class Weigh>
+__device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, u64 target, Weigh weigh, SampleShared<W>& sh, int& index, float& value) {
+  constexpr int C = SampleRow<T, W>::C, P = (kUnits + 2 + 63) / 64;
+  const int lane = lane_id(), wave = wave_uniform(threadIdx.x >> 6);
+  const auto none = [](int) AMOE_INLINE {};
+  u64 part[P], mine = 0;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    part[i] = P * lane + i <= row.last ? sh.unit[P * lane + i] : 0;
+    mine += part[i];
+  }
+  u64 run = wave_scan(mine);
+  const int at = ctz64(wave_ballot(run > target));
+  run -= mine;
+  int in = -1;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    if (in < 0 && run + part[i] > target) in = i;
+    if (in < 0) run += part[i];
+  }
+  target -= wave_shfl(run, at);
+  const int unit = P * at + wave_shfl(in, at);
+  const bool edges = unit == 0 || unit == row.last;
+  const int g0 = (unit - 1) * row.per, g1 = g0 + row.per < row.groups ? g0 + row.per : row.groups;
+  const auto group_sum = [&](int g, u64 (&w)[C], float (&x)[C], int& start) AMOE_INLINE {
+    u64 s = 0;
+    row.scan(
+        g, g + 1,
+        [&](const float (&v)[C], int first, bool) AMOE_INLINE {
+#pragma unroll
+          for (int e = 0; e < C; e++) {
+            x[e] = v[e];
+            w[e] = weigh(v[e], first + e);
+            s += w[e];
+          }
+          start = first;
+        },
+        none);
+    return s;
+  };
+  u64 w[C];
+  float x[C];
+  int start = 0;
+  if (!edges) {
+    for (int g = g0 + wave; g < g1; g += W) {
+      const u64 s = wave_total(group_sum(g, w, x, start));
+      if (lane == 0) sh.group[g - g0] = s;
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return false;
+  if (edges) {
+    run = wave_scan((lane == 0) == (unit == 0) && row.edge != -INFINITY ? weigh(row.edge, row.edge_index) : 0);
+    index = row.edge_index;
+    value = row.edge;
+    return lane == ctz64(wave_ballot(run > target));
+  }
+  mine = lane < g1 - g0 ? sh.group[lane] : 0;
+  run = wave_scan(mine);
+  const int group = ctz64(wave_ballot(run > target));
+  target -= wave_shfl(run - mine, group);
+  mine = group_sum(g0 + group, w, x, start);
+  run = wave_scan(mine);
+  const bool here = lane == ctz64(wave_ballot(run > target));
+  u64 sum = run - mine;
+  bool found = false;
+#pragma unroll
+  for (int e = 0; e < C; e++) {
+    sum += w[e];
+    if (!found && sum > target) {
+      found = true;
+      index = start + e;
+      value = x[e];
+    }
+  }
+  return here;
+}
+
+// The number of [0, total) that u stands for
+__device__ __forceinline__ u64 sample_target(double u, u64 total) {
+  const double want = (u > 0.0 ? u : 0.0) * (double)total;
+  const u64 target = want < (double)total ? (u64)want : total - 1;
+  return target < total ? target : total - 1;
+}
+
 template <typename T, int NT, bool CUT>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   constexpr int W = NT / 64, C = Elem<T>::kChunk;
@@ -312,25 +454,36 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   const float temperature = p.temperature ? p.temperature[at] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[at] : p.top_p_all, min_p = p.min_p ? p.min_p[at] : p.min_p_all;
   const int64_t top_k = !p.top_k ? p.top_k_all : p.top_k_i64 ? static_cast<const int64_t*>(p.top_k)[at] : static_cast<const int32_t*>(p.top_k)[at];
-  double u = p.u_f64 ? static_cast<const double*>(p.u)[at] : (double)static_cast<const float*>(p.u)[at];
+  const double u = p.u_f64 ? static_cast<const double*>(p.u)[at] : (double)static_cast<const float*>(p.u)[at];
   for (int i = tid; i < 256; i += NT) sh.table[i] = ::exp2((double)i / 256.0);
 
-  float mx = -INFINITY, mn = INFINITY;
-  const auto extremes = [&](float x, int) AMOE_INLINE {
-    mx = fmaxf(mx, x);
-    if (CUT) mn = fminf(mn, x == -INFINITY ? INFINITY : x);
-  };
+  float mx = -INFINITY, mn = INFINITY, unit_max = -INFINITY;
   row.all(
-      [&](const float (&v)[C], int first) AMOE_INLINE {
+      [&](const float (&v)[C], int, bool inside) AMOE_INLINE {
+        float lo = v[0];
 #pragma unroll
-        for (int e = 0; e < C; e++) extremes(v[e], first + e);
+        for (int e = 0; e < C; e++) {
+          unit_max = fmaxf(unit_max, v[e]);
+          if (CUT) lo = fminf(lo, v[e]);
+        }
+        if (CUT) mn = inside ? fminf(mn, lo) : mn;
       },
-      extremes);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    mx = fmaxf(mx, wave_shfl_xor(mx, d));
-    if (CUT) mn = fminf(mn, wave_shfl_xor(mn, d));
+      [&](int unit) AMOE_INLINE {
+        unit_max = wave_largest(unit_max);
+        if (lane == 0) sh.unit_max[unit] = unit_max;
+        mx = fmaxf(mx, unit_max);
+        unit_max = -INFINITY;
+      });
+  if (wave == 0) {
+    const float behind = wave_largest(lane == 0 ? -INFINITY : row.edge);
+    if (lane == 0) {
+      sh.unit_max[0] = row.edge;
+      sh.unit_max[row.last] = behind;
+    }
+    mx = fmaxf(fmaxf(mx, behind), wave_shfl(row.edge, 0));
+    if (CUT && row.edge != -INFINITY) mn = fminf(mn, row.edge);
   }
+  if (CUT) mn = -wave_largest(-mn);
   if (lane == 0) {
     sh.wave_max[wave] = mx;
     sh.wave_min[wave] = mn;
@@ -341,6 +494,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     mx = fmaxf(mx, sh.wave_max[i]);
     mn = fminf(mn, sh.wave_min[i]);
   }
+  int index = 0;
+  float value = 0.f;
   if (mx == -INFINITY) {
     if (tid == 0) {
       p.ids[at] = -1;
@@ -349,56 +504,128 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     return;
   }
   const bool greedy = !(temperature > 0.f);
-  const SampleWeight weight{mx, greedy ? 0.0 : 256 * 1.44269504088896340736 / (double)temperature, greedy || mx == INFINITY, sh.table};
-  if (greedy) u = 0.0;                               // (the first of those that weigh)
+  if (greedy || mx == INFINITY) {
+    // only those as large as the largest weigh, and all the same
+    const auto weigh = [&](float x, int) AMOE_INLINE { return (u64)(x == mx); };
+    for (int i = wave; i <= row.last; i += W) {
+      u64 s = 0;
+      if (sh.unit_max[i] == mx) {
+        if (i == 0 || i == row.last) {
+          s = (u64)((lane == 0) == (i == 0) && row.edge == mx);        // (the edges are the first wave's)
+        } else {
+          const int g = (i - 1) * row.per, end = g + row.per;
+          row.scan(
+              g, end < row.groups ? end : row.groups,
+              [&](const float (&v)[C], int, bool) AMOE_INLINE {
+#pragma unroll
+                for (int e = 0; e < C; e++) s += weigh(v[e], 0);
+              },
+              [](int) AMOE_INLINE {});
+        }
+        s = wave_total(s);
+      }
+      if (lane == 0 && i != row.last && i != 0) sh.unit[i] = s;
+    }
+    if (wave == 0) {
+      const u64 behind = wave_total(lane != 0 && row.edge == mx);
+      if (lane == 0) {
+        sh.unit[0] = row.edge == mx;
+        sh.unit[row.last] = behind;
+      }
+    }
+    __syncthreads();
+    u64 kept = 1;
+    if (!greedy) {
+      kept = 0;
+      for (int i = lane; i <= row.last; i += 64) kept += sh.unit[i];
+      kept = wave_total(kept);
+      if (top_k > 0 && (u64)top_k < kept) kept = (u64)top_k;
+      if (top_p < 1.f) {
+        const double part = top_p > 0.f ? __builtin_ceil((double)top_p * (double)kept) : 1.0;
+        kept = part < 1.0 ? 1 : (u64)part;
+      }
+    }
+    if (sample_find<T, W>(row, greedy ? 0 : sample_target(u, kept), weigh, sh, index, value)) {
+      p.ids[at] = index;
+      if (p.logprob) p.logprob[at] = greedy ? 0.f : (float)-::log((double)kept);
+    }
+    return;
+  }
 
+  const SampleWeight weight(mx, temperature, sh.table);
+  const u64 least = min_p > 0.f ? (u64)__builtin_ceil((double)fminf(min_p, 1.f) * (double)kOne) : 0;
+  // What is kept: ranks of `cut` and more; while that is not known, bins before `edge_bin`
   u64 cut = 0;
+  bool summed = false;
   if constexpr (CUT) {
     __shared__ SampleBins hist;
     __shared__ SampleRanked ranked;
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
-    if (!greedy && (by_k || by_p)) {
-      // (half the distances: they may be twice the largest float)
-      const float half = 0.5f * mx, reach = fminf(fmaf(-0.5f, mn, half), 16.f * temperature);
-      const float step = reach > 0.f ? fminf((kBins - 2) / reach, 3.402823466e38f) : 0.f;
-      const bool flat = weight.flat;
-      const auto bin = [=](float x) AMOE_INLINE {
-        if (flat) return x == mx ? 0 : kBins - 1;
-        return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins - 1));
+    if (by_k || by_p) {
+      // Levels that bins are made for: those that occur, that weigh anything and, without top_k, that may be kept: all tokens of less
+      // than (1 - top_p) / V of the largest weight are together less than what top_p may leave out.
+      double f;
+      int most = mn == -INFINITY ? kLevels : -weight.level(mn, f);
+      if (most > kLevels) most = kLevels;
+      if (!by_k) {
+        const float left = 1.f - fmaxf(top_p, 0.f);
+        const int may = (int)(256.f * (fast_log2((float)p.V) - fast_log2(left))) + 512;
+        if (may < most) most = may;
+      }
+      int shift = 0;
+      while (most >> shift >= kBins - 1) shift++;
+      const int n_bins = (most >> shift) + 1;
+      const auto bin_of = [=](int level) AMOE_INLINE {
+        const int b = -level >> shift;
+        return b < kBins - 1 ? b : kBins - 1;
+      };
+      const auto bin = [=, &weight](float x) AMOE_INLINE {
+        double rest;
+        return bin_of(weight.level(x, rest));
       };
       for (int i = tid; i < kBins; i += NT) {
         hist.n[i] = 0;
         hist.w[i] = 0;
       }
+      if (tid == 0) sh.rest = 0;
       __syncthreads();
+      u64 rest = 0;
       const auto count_one = [&](float x, int) AMOE_INLINE {
-        const int b = bin(x);
-        if (b >= kBins - 1) return;
-        atomicAdd(&hist.n[b], 1u);
-        if (by_p) atomicAdd(&hist.w[b], weight(x));
+        double f;
+        const int level = weight.level(x, f), b = bin_of(level);
+        if (by_p) {
+          const u64 w = weight.of(x, level, f);
+          if (b < n_bins) atomicAdd(&hist.w[b], w);
+          else rest += w;
+        }
+        if (by_k && b < n_bins) atomicAdd(&hist.n[b], 1u);
       };
       row.all(
-          [&](const float (&v)[C], int first) AMOE_INLINE {
+          [&](const float (&v)[C], int first, bool) AMOE_INLINE {
 #pragma unroll
             for (int e = 0; e < C; e++) count_one(v[e], first + e);
           },
-          count_one);
+          [](int) AMOE_INLINE {});
+      if (wave == 0 && row.edge != -INFINITY) count_one(row.edge, 0);
+      if (by_p) {
+        rest = wave_total(rest);
+        if (lane == 0 && rest) atomicAdd(&sh.rest, rest);
+      }
       __syncthreads();
-      u64 total = 0;
-      bool cut_by_k = false;
+      u64 total = 0, target = (u64)top_k;
+      int b = -1;
       if (by_k) {
-        sample_crossing<NT>(hist, kBins, false, (u64)top_k, sh);
-        const int b = sh.found;
-        if (b >= 0) {
+        sample_crossing<NT>(hist, n_bins, false, target, sh);
+        b = sh.found;
+        if (b >= 0 && by_p) {
           const u64 before_n = sh.found_n, before_w = sh.found_w;
-          sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], false, (u64)top_k, before_n, before_w, ranked, sh);
-          cut_by_k = true;
+          sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], false, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
           total = sh.found_w;
         }
       }
       if (by_p) {
-        if (!cut_by_k) {
+        if (b < 0) {
           int n = 0;
           u64 w = 0;
           for (int i = tid; i < kBins; i += NT) w += hist.w[i];
@@ -407,137 +634,106 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
           __syncthreads();
           if (tid == NT - 1) sh.found_w = w + mine;
           __syncthreads();
-          total = sh.found_w;
+          total = sh.found_w + sh.rest;
         }
         const double part = top_p > 0.f ? __builtin_ceil((double)top_p * (double)total) : 1.0;
-        const u64 target = part < 1.0 ? 1 : (u64)part;
+        target = part < 1.0 ? 1 : (u64)part;
         __syncthreads();
-        sample_crossing<NT>(hist, kBins, true, target, sh);
-        const int b = sh.found;
-        if (b >= 0) {
-          const u64 before_n = sh.found_n, before_w = sh.found_w;
-          sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], true, target, before_n, before_w, ranked, sh);
-          if (sh.cut > cut) cut = sh.cut;
+        sample_crossing<NT>(hist, n_bins, true, target, sh);
+        b = sh.found;
+      }
+      if (b >= 0) {
+        // one more pass: the sums of the bins before b, and a list of b's elements
+        const u64 before_n = sh.found_n, before_w = sh.found_w;
+        const float above = (float)(weight.top - (double)(((b + 1) << shift) + 2) / weight.scale);
+        const float low = fminf(above - fabsf(above) * 0x1p-22f, mx);      // (nothing smaller is in these bins)
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+        u64 s = 0;
+        const auto take = [&](float x, int i) AMOE_INLINE -> u64 {
+          double f;
+          const int level = weight.level(x, f), at_bin = bin_of(level);
+          const u64 w = weight.of(x, level, f);
+          if (at_bin == b) {
+            const int n = atomicAdd(&sh.listed, 1);
+            if (n < kList) ranked.list[n] = sample_rank(x, i);
+          }
+          return (at_bin < b) & (w >= least) ? w : 0;
+        };
+        row.all(
+            [&](const float (&v)[C], int first, bool) AMOE_INLINE {
+              bool any = false;
+#pragma unroll
+              for (int e = 0; e < C; e++) any = any | (v[e] >= low);
+              if (any) {
+#pragma unroll
+                for (int e = 0; e < C; e++) s += take(v[e], first + e);
+              }
+            },
+            [&](int unit) AMOE_INLINE {
+              s = wave_total(s);
+              if (lane == 0) sh.unit[unit] = s;
+              s = 0;
+            });
+        if (wave == 0) {
+          const u64 w = row.edge >= low ? take(row.edge, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
+          if (lane == 0) {
+            sh.unit[0] = w;
+            sh.unit[row.last] = behind;
+          }
+        }
+        __syncthreads();
+        const int listed = sh.listed;
+        if (listed <= kList) {
+          sample_sort<NT>(weight, listed, by_p, target, before_n, before_w, ranked, sh);
+          cut = sh.cut;
+          for (int i = tid; i < listed; i += NT) {
+            const u64 rank = ranked.list[i], w = weight(sample_value(rank));
+            if (rank >= cut && w >= least) atomicAdd(&sh.unit[row.unit_of(sample_index(rank))], w);
+          }
+          summed = true;
+        } else {
+          sample_refine<T, NT>(row, weight, bin, b, listed, by_p, target, before_n, before_w, ranked, sh);
+          cut = sh.cut;
         }
       }
     }
   }
   const float cut_x = cut ? sample_value(cut) : -INFINITY;
   const int cut_i = cut ? sample_index(cut) : p.V;
-  const u64 least = min_p > 0.f ? (u64)__builtin_ceil((double)fminf(min_p, 1.f) * (double)kOne) : 0;
-  // weights of a chunk's kept elements
-  const auto weigh_one = [&](float x, int index) AMOE_INLINE -> u64 {
-    const bool keep = (x > cut_x) | ((x == cut_x) & (index <= cut_i));
+  const auto weigh = [&](float x, int i) AMOE_INLINE -> u64 {
+    const bool keep = (x > cut_x) | ((x == cut_x) & (i <= cut_i));
     const u64 w = weight(x);
     return keep & (w >= least) ? w : 0;
   };
-  const auto weigh = [&](const float (&v)[C], int first, u64 (&w)[C]) AMOE_INLINE {
-    bool any = false;
-#pragma unroll
-    for (int e = 0; e < C; e++) {
-      any = any | (v[e] >= cut_x);
-      w[e] = 0;
-    }
-    if (!any) return;
-#pragma unroll
-    for (int e = 0; e < C; e++) w[e] = weigh_one(v[e], first + e);
-  };
-  const auto group_sum = [&](int g, int g_end) AMOE_INLINE {
-    u64 s = 0;
-    row.chunks(g, g_end, [&](const float (&v)[C], int first) AMOE_INLINE {
-      u64 w[C];
-      weigh(v, first, w);
-#pragma unroll
-      for (int e = 0; e < C; e++) s += w[e];
-    });
-    return s;
-  };
-  const auto wave_total = [&](u64 s) AMOE_INLINE {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += wave_shfl_xor(s, d);
-    return s;
-  };
   __syncthreads();                                    // (the table, where nothing was cut)
-  for (int i = wave; i < row.units; i += W) {
-    const int end = (i + 1) * row.per < row.groups ? (i + 1) * row.per : row.groups;
-    const u64 s = wave_total(group_sum(i * row.per, end));
-    if (lane == 0) sh.unit[1 + i] = s;
-  }
-  // the element before the chunks and those behind them are units of their own, the first and the last
-  const u64 edge_w = wave == 0 && row.edge != -INFINITY ? weigh_one(row.edge, row.edge_index) : 0;
-  if (wave == 0) {
-    const u64 behind = wave_total(lane == 0 ? 0 : edge_w);
-    if (lane == 0) {
-      sh.unit[0] = edge_w;
-      sh.unit[1 + row.units] = behind;
-    }
-  }
-  __syncthreads();
-  // the unit, then the group of chunks, then the chunk, then the element at which the sum passes u times the total
-  u64 mine = lane < row.units + 2 ? sh.unit[lane] : 0, run = wave_scan(mine);
-  const u64 total = wave_shfl(run, 63);
-  const double want = (u > 0.0 ? u : 0.0) * (double)total;
-  u64 target = want < (double)total ? (u64)want : total - 1;
-  if (target >= total) target = total - 1;
-  const int unit = ctz64(wave_ballot(run > target)) - 1;
-  target -= wave_shfl(run - mine, unit + 1);
-  const bool edges = unit < 0 || unit == row.units;
-  const int g0 = unit * row.per, g1 = g0 + row.per < row.groups ? g0 + row.per : row.groups;
-  if (!edges) {
-    for (int g = g0 + wave; g < g1; g += W) {
-      const u64 s = wave_total(group_sum(g, g + 1));
-      if (lane == 0) sh.group[g - g0] = s;
-    }
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  int which = 0;
-  float value = 0.f;
-  if (edges) {
-    run = wave_scan((lane == 0) == (unit < 0) ? edge_w : 0);
-    if (lane != ctz64(wave_ballot(run > target))) return;
-    which = row.edge_index;
-    value = row.edge;
-  } else {
-    const u64 even = 2 * lane < g1 - g0 ? sh.group[2 * lane] : 0, odd = 2 * lane + 1 < g1 - g0 ? sh.group[2 * lane + 1] : 0;
-    run = wave_scan(even + odd);
-    const int pair = ctz64(wave_ballot(run > target));
-    target -= wave_shfl(run - even - odd, pair);
-    const u64 first_of_pair = wave_shfl(even, pair);
-    const bool second = target >= first_of_pair;
-    if (second) target -= first_of_pair;
-    const int group = g0 + 2 * pair + (second ? 1 : 0);
-    u64 w[C] = {};
-    float x[C] = {};
-    int start = 0;
-    row.chunks(group, group + 1, [&](const float (&v)[C], int first) AMOE_INLINE {
-      weigh(v, first, w);
-      start = first;
+  if (!summed) {
+    u64 s = 0;
+    row.all(
+        [&](const float (&v)[C], int first, bool) AMOE_INLINE {
 #pragma unroll
-      for (int e = 0; e < C; e++) x[e] = v[e];
-    });
-    mine = 0;
-#pragma unroll
-    for (int e = 0; e < C; e++) mine += w[e];
-    run = wave_scan(mine);
-    if (lane != ctz64(wave_ballot(run > target))) return;
-    u64 sum = run - mine;
-    bool found = false;
-#pragma unroll
-    for (int e = 0; e < C; e++) {
-      sum += w[e];
-      if (!found && sum > target) {
-        found = true;
-        which = start + e;
-        value = x[e];
+          for (int e = 0; e < C; e++) s += weigh(v[e], first + e);
+        },
+        [&](int unit) AMOE_INLINE {
+          s = wave_total(s);
+          if (lane == 0) sh.unit[unit] = s;
+          s = 0;
+        });
+    if (wave == 0) {
+      const u64 w = row.edge != -INFINITY ? weigh(row.edge, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
+      if (lane == 0) {
+        sh.unit[0] = w;
+        sh.unit[row.last] = behind;
       }
     }
+    __syncthreads();
   }
-  p.ids[at] = which;
-  if (p.logprob) {
-    const double log_total = ::log((double)total * 0x1p-44);
-    p.logprob[at] = greedy ? 0.f : (float)((weight.flat ? 0.0 : ((double)value - (double)mx) / (double)temperature) - log_total);
-  }
+  u64 total = 0;
+  for (int i = lane; i <= row.last; i += 64) total += sh.unit[i];
+  total = wave_total(total);
+  if (!sample_find<T, W>(row, sample_target(u, total), weigh, sh, index, value)) return;
+  p.ids[at] = index;
+  if (p.logprob) p.logprob[at] = (float)(((double)value - (double)mx) / (double)temperature - ::log((double)total * 0x1p-44));
 }
 
 namespace {
