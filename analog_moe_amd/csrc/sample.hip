@@ -38,7 +38,8 @@ constexpr int64_t kSampleMaxV = (1 << 20) - 1;       // (as many largest weights
 constexpr int kBins = 2048;          // the last one holds what is not looked at
 constexpr int kList = 2048;          // elements that are ranked at once
 constexpr int kUnits = 240;
-constexpr int kLevels = 46 * 256;    // below the largest weight by this many 256ths of a factor of two: 0 as a multiple of 2^-44
+constexpr int kSteps = 32;           // table entries to a factor of two
+constexpr int kCopies = 16;          // of the table, for 16 lanes side by side: random entries then meet on no bank
 constexpr u64 kOne = 1ull << 44;
 constexpr int kIndexBits = 20;
 
@@ -76,9 +77,9 @@ template <typename T, int W> struct SampleRow {
     return j >= body ? last : 1 + j / 64 / per;
   }
   // f(values, index of the first, whether the chunk is in the row) for the chunks of groups [g, g_end) that are this lane's, done(unit)
-  // after each unit; minus infinity where there is no number
+  // after each unit; `low` for what is smaller, no number or not there
   template <class F, class Done>
-  __device__ __forceinline__ void scan(int g, int g_end, F f, Done done) const {
+  __device__ __forceinline__ void scan(float low, int g, int g_end, F f, Done done) const {
     constexpr int kAhead = sizeof(T) == 4 ? 8 : 4;
     const int lane = lane_id();
     int in_unit = g % per, unit = 1 + g / per;
@@ -94,7 +95,7 @@ template <typename T, int W> struct SampleRow {
         float v[C];
         raw_unpack<T>(r[i], v);
 #pragma unroll
-        for (int e = 0; e < C; e++) v[e] = inside & (v[e] == v[e]) ? v[e] : -INFINITY;
+        for (int e = 0; e < C; e++) v[e] = inside & (v[e] > low) ? v[e] : low;
         f(v, start(j), inside);
         if (++in_unit == per || g + i + 1 == g_end) {
           done(unit++);
@@ -105,49 +106,73 @@ template <typename T, int W> struct SampleRow {
   }
   // the whole row: a wave's units lie next to each other
   template <class F, class Done>
-  __device__ __forceinline__ void all(F f, Done done) const {
+  __device__ __forceinline__ void all(float low, F f, Done done) const {
     const int wave = wave_uniform(threadIdx.x >> 6), share = (units + W - 1) / W;
     const int g = wave * share * per, end = g + share * per;
-    scan(g, end < groups ? end : groups, f, done);
+    scan(low, g, end < groups ? end : groups, f, done);
   }
 };
 
-// The weight of an element, in multiples of 2^-44 of the largest, and its level, the logarithm of that (256 to a factor of two).
+// The weight of an element, in multiples of 2^-44 of the largest: 2^(j / 32) from a table, e^z for the rest, |z| < 0.0109, by five
+// terms of its series, which leave 2^-48.
 struct SampleWeight {
-  float floor;                       // weighs nothing
-  bool hot;                          // not even minus infinity is below the floor by itself
-  double top, scale;                 // 256 log2(e) / temperature
-  const double* table;               // 2^(j / 256)
-  __device__ __forceinline__ SampleWeight(float mx, float temperature, const double* table_) : top(mx), table(table_) {
+  float low;                         // weighs nothing: this and what is smaller
+  bool hot;                          // that is minus infinity alone
+  double top, scale;                 // 32 log2(e) / temperature
+  const double* table;               // the lane's copy of 2^(j / 32)
+  __device__ __forceinline__ SampleWeight(float mx, float temperature, const double* tables) : top(mx), table(tables + (threadIdx.x & (kCopies - 1))) {
     // (the next float down, where 33 temperatures are less than that: then nothing but the largest weighs)
     const uint32_t b = as_u32(mx);
     const float next = mx == 0.f ? -1e-45f : as_f32(mx > 0.f ? b - 1 : b + 1);
-    const float down = mx - 33.f * temperature;
-    floor = fmaxf(fminf(down, next), -3.402823466e38f);
-    hot = !(down > -3.3e38f);
-    const double most = (kLevels + 1000.0) / (top - (double)floor);
-    scale = 256 * 1.44269504088896340736 / (double)temperature;
+    low = fminf(mx - 33.f * temperature, next);
+    hot = !(low > -3.3e38f);
+    if (hot) low = -INFINITY;
+    scale = kSteps * 1.44269504088896340736 / (double)temperature;
+    const double most = 50.0 * kSteps / (top - (double)low);           // (33 temperatures: 47.6 factors of two)
     if (!(scale < most) && !hot) scale = most;
   }
-  __device__ __forceinline__ int level(float x, double& rest) const {
+  // of N elements, none below `low`: side by side, as each is a chain of 13 operations and a read
+  template <int N>
+  __device__ __forceinline__ void operator()(const float (&x)[N], u64 (&r)[N]) const {
     constexpr double kMagic = 6755399441055744.0;          // 1.5 * 2^52: whole numbers are its last bits
-    const double t = ((double)fmaxf(x, floor) - top) * scale, m = t + kMagic;
-    rest = t - (m - kMagic);
-    return (int)(uint32_t)__builtin_bit_cast(u64, m);
-  }
-  __device__ __forceinline__ u64 of(float x, int level, double f) const {
-    constexpr double a = 0.69314718055994530942 / 256;
-    const double q = f * __builtin_fma(f, __builtin_fma(f, __builtin_fma(f, a * a * a * a / 24, a * a * a / 6), a * a / 2), a);
-    const u64 bits = __builtin_bit_cast(u64, table[level & 255]) + ((u64)(uint32_t)((level & ~255) << 12) << 32);
-    const double w = __builtin_bit_cast(double, bits);
-    // (256 + w: the last bit counts 2^-44)
-    const u64 r = __builtin_bit_cast(u64, __builtin_fma(w, q, w) + 256.0) - __builtin_bit_cast(u64, 256.0);
-    return hot && x == -INFINITY ? 0 : r;
+    constexpr double a = 0.69314718055994530942 / kSteps;
+    double f[N], m[N], q[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] = ((double)x[e] - top) * scale;
+#pragma unroll
+    for (int e = 0; e < N; e++) m[e] = f[e] + kMagic;
+    u64 bits[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const int step = (int)(uint32_t)__builtin_bit_cast(u64, m[e]);
+      bits[e] = __builtin_bit_cast(u64, table[(step & (kSteps - 1)) * kCopies]) + ((u64)(uint32_t)((step >> 5) * (1 << 20)) << 32);
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] -= m[e] - kMagic;
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = __builtin_fma(f[e], a * a * a * a * a / 120, a * a * a * a / 24);
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = __builtin_fma(f[e], q[e], a * a * a / 6);
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = __builtin_fma(f[e], q[e], a * a / 2);
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = __builtin_fma(f[e], q[e], a);
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const double w = __builtin_bit_cast(double, bits[e]);
+      // (256 + w: the last bit counts 2^-44)
+      r[e] = __builtin_bit_cast(u64, __builtin_fma(w * f[e], q[e], w) + 256.0) - __builtin_bit_cast(u64, 256.0);
+    }
+    if (hot) {
+#pragma unroll
+      for (int e = 0; e < N; e++) r[e] = x[e] == -INFINITY ? 0 : r[e];
+    }
   }
   __device__ __forceinline__ u64 operator()(float x) const {
-    double f;
-    const int l = level(x, f);
-    return of(x, l, f);
+    const float one[1] = {x > low ? x : low};
+    u64 r[1];
+    (*this)(one, r);
+    return r[0];
   }
 };
 
@@ -185,7 +210,7 @@ __device__ __forceinline__ float wave_largest(float v) {
 
 // What a workgroup shares beside the histogram.
 template <int W> struct SampleShared {
-  double table[256];
+  double table[kSteps * kCopies];
   u64 unit[kUnits + 2], group[32], wave_w[W];
   float unit_max[kUnits + 2], wave_max[W], wave_min[W];
   int wave_n[W], found, listed;
@@ -323,6 +348,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
       atomicAdd(&r.digit.w[d], weight(x));
     };
     row.all(
+        -INFINITY,
         [&](const float (&v)[C], int first, bool) AMOE_INLINE {
 #pragma unroll
           for (int e = 0; e < C; e++) count_one(v[e], first + e);
@@ -347,6 +373,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
     if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
   };
   row.all(
+      -INFINITY,
       [&](const float (&v)[C], int first, bool) AMOE_INLINE {
 #pragma unroll
         for (int e = 0; e < C; e++) list_one(v[e], first + e);
@@ -360,7 +387,8 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
 // The element at which the sum of weights passes `target`, from the units' sums: weigh(value, index).  True for the thread that has
 // it.  Every thread calls this.
 template <typename T, int W, class Weigh>
-__device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, u64 target, Weigh weigh, SampleShared<W>& sh, int& index, float& value) {
+__device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float low, u64 target, Weigh weigh, SampleShared<W>& sh, int& index,
+                                            float& value) {
   constexpr int C = SampleRow<T, W>::C, P = (kUnits + 2 + 63) / 64;
   const int lane = lane_id(), wave = wave_uniform(threadIdx.x >> 6);
   const auto none = [](int) AMOE_INLINE {};
@@ -386,7 +414,7 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, u64 targ
   const auto group_sum = [&](int g, u64 (&w)[C], float (&x)[C], int& start) AMOE_INLINE {
     u64 s = 0;
     row.scan(
-        g, g + 1,
+        low, g, g + 1,
         [&](const float (&v)[C], int first, bool) AMOE_INLINE {
 #pragma unroll
           for (int e = 0; e < C; e++) {
@@ -445,7 +473,7 @@ __device__ __forceinline__ u64 sample_target(double u, u64 total) {
 }
 
 template <typename T, int NT, bool CUT>
-__global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
+__global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
   constexpr int W = NT / 64, C = Elem<T>::kChunk;
   __shared__ SampleShared<W> sh;
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6);
@@ -455,10 +483,11 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   const float top_p = p.top_p ? p.top_p[at] : p.top_p_all, min_p = p.min_p ? p.min_p[at] : p.min_p_all;
   const int64_t top_k = !p.top_k ? p.top_k_all : p.top_k_i64 ? static_cast<const int64_t*>(p.top_k)[at] : static_cast<const int32_t*>(p.top_k)[at];
   const double u = p.u_f64 ? static_cast<const double*>(p.u)[at] : (double)static_cast<const float*>(p.u)[at];
-  for (int i = tid; i < 256; i += NT) sh.table[i] = ::exp2((double)i / 256.0);
+  for (int i = tid; i < kSteps * kCopies; i += NT) sh.table[i] = ::exp2((double)(i / kCopies) / kSteps);
 
   float mx = -INFINITY, mn = INFINITY, unit_max = -INFINITY;
   row.all(
+      -INFINITY,
       [&](const float (&v)[C], int, bool inside) AMOE_INLINE {
         float lo = v[0];
 #pragma unroll
@@ -515,7 +544,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         } else {
           const int g = (i - 1) * row.per, end = g + row.per;
           row.scan(
-              g, end < row.groups ? end : row.groups,
+              -INFINITY, g, end < row.groups ? end : row.groups,
               [&](const float (&v)[C], int, bool) AMOE_INLINE {
 #pragma unroll
                 for (int e = 0; e < C; e++) s += weigh(v[e], 0);
@@ -545,7 +574,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         kept = part < 1.0 ? 1 : (u64)part;
       }
     }
-    if (sample_find<T, W>(row, greedy ? 0 : sample_target(u, kept), weigh, sh, index, value)) {
+    if (sample_find<T, W>(row, -INFINITY, greedy ? 0 : sample_target(u, kept), weigh, sh, index, value)) {
       p.ids[at] = index;
       if (p.logprob) p.logprob[at] = greedy ? 0.f : (float)-::log((double)kept);
     }
@@ -562,27 +591,14 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     __shared__ SampleRanked ranked;
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
     if (by_k || by_p) {
-      // Levels that bins are made for: those that occur, that weigh anything and, without top_k, that may be kept: all tokens of less
-      // than (1 - top_p) / V of the largest weight are together less than what top_p may leave out.
-      double f;
-      int most = mn == -INFINITY ? kLevels : -weight.level(mn, f);
-      if (most > kLevels) most = kLevels;
-      if (!by_k) {
-        const float left = 1.f - fmaxf(top_p, 0.f);
-        const int may = (int)(256.f * (fast_log2((float)p.V) - fast_log2(left))) + 512;
-        if (may < most) most = may;
-      }
-      int shift = 0;
-      while (most >> shift >= kBins - 1) shift++;
-      const int n_bins = (most >> shift) + 1;
-      const auto bin_of = [=](int level) AMOE_INLINE {
-        const int b = -level >> shift;
-        return b < kBins - 1 ? b : kBins - 1;
-      };
-      const auto bin = [=, &weight](float x) AMOE_INLINE {
-        double rest;
-        return bin_of(weight.level(x, rest));
-      };
+      // Bins are equal intervals of the distance to the largest, up to where tokens occur, weigh anything and, without top_k, may be
+      // kept: all that weigh less than (1 - top_p) / V are together less than what top_p may leave out.  (Half the distances: they
+      // may be twice the largest float.)
+      const float half = 0.5f * mx;
+      float reach = fminf(fmaf(-0.5f, mn, half), 16.25f * temperature);
+      if (!by_k) reach = fminf(reach, 0.3466f * temperature * (fast_log2((float)p.V) - fast_log2(1.f - fmaxf(top_p, 0.f)) + 1.f));
+      const float step = reach > 0.f ? fminf((kBins - 2) / reach, 3.402823466e38f) : 0.f;
+      const auto bin = [=](float x) AMOE_INLINE { return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins - 1)); };
       for (int i = tid; i < kBins; i += NT) {
         hist.n[i] = 0;
         hist.w[i] = 0;
@@ -590,23 +606,32 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
       if (tid == 0) sh.rest = 0;
       __syncthreads();
       u64 rest = 0;
-      const auto count_one = [&](float x, int) AMOE_INLINE {
-        double f;
-        const int level = weight.level(x, f), b = bin_of(level);
+      const auto count = [&](const auto& v) AMOE_INLINE {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+        int b[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) b[e] = bin(v[e]);
         if (by_p) {
-          const u64 w = weight.of(x, level, f);
-          if (b < n_bins) atomicAdd(&hist.w[b], w);
-          else rest += w;
+          u64 w[N];
+          weight(v, w);
+#pragma unroll
+          for (int e = 0; e < N; e++) {
+            if (b[e] < kBins - 1) atomicAdd(&hist.w[b[e]], w[e]);
+            else rest += w[e];
+          }
         }
-        if (by_k && b < n_bins) atomicAdd(&hist.n[b], 1u);
+        if (by_k) {
+#pragma unroll
+          for (int e = 0; e < N; e++)
+            if (b[e] < kBins - 1) atomicAdd(&hist.n[b[e]], 1u);
+        }
       };
       row.all(
-          [&](const float (&v)[C], int first, bool) AMOE_INLINE {
-#pragma unroll
-            for (int e = 0; e < C; e++) count_one(v[e], first + e);
-          },
-          [](int) AMOE_INLINE {});
-      if (wave == 0 && row.edge != -INFINITY) count_one(row.edge, 0);
+          weight.low, [&](const float (&v)[C], int, bool) AMOE_INLINE { count(v); }, [](int) AMOE_INLINE {});
+      if (wave == 0 && row.edge > weight.low) {
+        const float one[1] = {row.edge};
+        count(one);
+      }
       if (by_p) {
         rest = wave_total(rest);
         if (lane == 0 && rest) atomicAdd(&sh.rest, rest);
@@ -615,7 +640,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
       u64 total = 0, target = (u64)top_k;
       int b = -1;
       if (by_k) {
-        sample_crossing<NT>(hist, n_bins, false, target, sh);
+        sample_crossing<NT>(hist, kBins - 1, false, target, sh);
         b = sh.found;
         if (b >= 0 && by_p) {
           const u64 before_n = sh.found_n, before_w = sh.found_w;
@@ -639,44 +664,47 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         const double part = top_p > 0.f ? __builtin_ceil((double)top_p * (double)total) : 1.0;
         target = part < 1.0 ? 1 : (u64)part;
         __syncthreads();
-        sample_crossing<NT>(hist, n_bins, true, target, sh);
+        sample_crossing<NT>(hist, kBins - 1, true, target, sh);
         b = sh.found;
       }
       if (b >= 0) {
         // one more pass: the sums of the bins before b, and a list of b's elements
         const u64 before_n = sh.found_n, before_w = sh.found_w;
-        const float above = (float)(weight.top - (double)(((b + 1) << shift) + 2) / weight.scale);
-        const float low = fminf(above - fabsf(above) * 0x1p-22f, mx);      // (nothing smaller is in these bins)
         if (tid == 0) sh.listed = 0;
         __syncthreads();
         u64 s = 0;
-        const auto take = [&](float x, int i) AMOE_INLINE -> u64 {
-          double f;
-          const int level = weight.level(x, f), at_bin = bin_of(level);
-          const u64 w = weight.of(x, level, f);
-          if (at_bin == b) {
-            const int n = atomicAdd(&sh.listed, 1);
-            if (n < kList) ranked.list[n] = sample_rank(x, i);
+        const auto take = [&](const auto& v, int first) AMOE_INLINE -> u64 {
+          constexpr int N = sizeof(v) / sizeof(v[0]);
+          int in[N];
+          bool any = false;
+#pragma unroll
+          for (int e = 0; e < N; e++) {
+            in[e] = bin(v[e]);
+            any = any | (in[e] <= b);
           }
-          return (at_bin < b) & (w >= least) ? w : 0;
+          if (!any) return 0;
+          u64 w[N], sum = 0;
+          weight(v, w);
+#pragma unroll
+          for (int e = 0; e < N; e++) {
+            if (in[e] == b) {
+              const int n = atomicAdd(&sh.listed, 1);
+              if (n < kList) ranked.list[n] = sample_rank(v[e], first + e);
+            }
+            sum += (in[e] < b) & (w[e] >= least) ? w[e] : 0;
+          }
+          return sum;
         };
         row.all(
-            [&](const float (&v)[C], int first, bool) AMOE_INLINE {
-              bool any = false;
-#pragma unroll
-              for (int e = 0; e < C; e++) any = any | (v[e] >= low);
-              if (any) {
-#pragma unroll
-                for (int e = 0; e < C; e++) s += take(v[e], first + e);
-              }
-            },
+            weight.low, [&](const float (&v)[C], int first, bool) AMOE_INLINE { s += take(v, first); },
             [&](int unit) AMOE_INLINE {
               s = wave_total(s);
               if (lane == 0) sh.unit[unit] = s;
               s = 0;
             });
         if (wave == 0) {
-          const u64 w = row.edge >= low ? take(row.edge, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
+          const float one[1] = {row.edge};
+          const u64 w = row.edge > weight.low ? take(one, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
           if (lane == 0) {
             sh.unit[0] = w;
             sh.unit[row.last] = behind;
@@ -709,10 +737,22 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   __syncthreads();                                    // (the table, where nothing was cut)
   if (!summed) {
     u64 s = 0;
+    const bool all = !CUT || cut == 0;
     row.all(
+        weight.low,
         [&](const float (&v)[C], int first, bool) AMOE_INLINE {
+          u64 w[C];
+          weight(v, w);
+          if (least) {
 #pragma unroll
-          for (int e = 0; e < C; e++) s += weigh(v[e], first + e);
+            for (int e = 0; e < C; e++) w[e] = w[e] >= least ? w[e] : 0;
+          }
+          if (!all) {
+#pragma unroll
+            for (int e = 0; e < C; e++) w[e] = (v[e] > cut_x) | ((v[e] == cut_x) & (first + e <= cut_i)) ? w[e] : 0;
+          }
+#pragma unroll
+          for (int e = 0; e < C; e++) s += w[e];
         },
         [&](int unit) AMOE_INLINE {
           s = wave_total(s);
@@ -731,7 +771,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
   u64 total = 0;
   for (int i = lane; i <= row.last; i += 64) total += sh.unit[i];
   total = wave_total(total);
-  if (!sample_find<T, W>(row, sample_target(u, total), weigh, sh, index, value)) return;
+  if (!sample_find<T, W>(row, weight.low, sample_target(u, total), weigh, sh, index, value)) return;
   p.ids[at] = index;
   if (p.logprob) p.logprob[at] = (float)(((double)value - (double)mx) / (double)temperature - ::log((double)total * 0x1p-44));
 }
