@@ -32,12 +32,16 @@ struct SampleParams {
   int64_t ld, rows, top_k_all;
   int V, u_f64, top_k_i64;
   float temperature_all, top_p_all, min_p_all;
+  char* work;                        // rows worked on in parts: what their launches leave for one another
+  int parts;
 };
 
 constexpr int64_t kSampleMaxV = (1 << 20) - 1;       // (as many largest weights are less than 2^64)
-constexpr int kBins = 2048;          // the last one holds what is not looked at
-constexpr int kList = 2048;          // elements that are ranked at once
+// bins of a workgroup of NT threads, the last of which holds what is not looked at, and elements that it ranks at once
+template <int NT> inline constexpr int kBins = 2 * NT;
 constexpr int kUnits = 240;
+constexpr int kMaxParts = 32;
+constexpr int kPartList = 256;       // elements of the cut's bin that a part of a row can hand on
 constexpr int kSteps = 32;           // table entries to a factor of two
 constexpr int kCopies = 16;          // of the table, for 16 lanes side by side: random entries then meet on no bank
 constexpr u64 kOne = 1ull << 44;
@@ -104,12 +108,16 @@ template <typename T, int W> struct SampleRow {
       }
     }
   }
-  // the whole row: a wave's units lie next to each other
+  // units [first, end) of the chunks, counted from 0: a wave's lie next to each other
+  template <class F, class Done>
+  __device__ __forceinline__ void some(float low, int first, int end, F f, Done done) const {
+    const int wave = wave_uniform(threadIdx.x >> 6), share = (end - first + W - 1) / W;
+    const int u = first + wave * share, u_end = u + share < end ? u + share : end;
+    if (u < u_end) scan(low, u * per, u_end * per < groups ? u_end * per : groups, f, done);
+  }
   template <class F, class Done>
   __device__ __forceinline__ void all(float low, F f, Done done) const {
-    const int wave = wave_uniform(threadIdx.x >> 6), share = (units + W - 1) / W;
-    const int g = wave * share * per, end = g + share * per;
-    scan(low, g, end < groups ? end : groups, f, done);
+    some(low, 0, units, f, done);
   }
 };
 
@@ -121,14 +129,15 @@ struct SampleWeight {
   double top, scale;                 // 32 log2(e) / temperature
   const double* table;               // the lane's copy of 2^(j / 32)
   __device__ __forceinline__ SampleWeight(float mx, float temperature, const double* tables) : top(mx), table(tables + (threadIdx.x & (kCopies - 1))) {
-    // (the next float down, where 33 temperatures are less than that: then nothing but the largest weighs)
-    const uint32_t b = as_u32(mx);
-    const float next = mx == 0.f ? -1e-45f : as_f32(mx > 0.f ? b - 1 : b + 1);
-    low = fminf(mx - 33.f * temperature, next);
-    hot = !(low > -3.3e38f);
+    // 33 temperatures down, and a float further (the rounding; where that is more, nothing but the largest weighs, and the scale is what
+    // keeps 2^t a normal number)
+    const float down = fminf(mx - 33.f * temperature, mx);
+    const uint32_t b = as_u32(down);
+    low = down == 0.f ? -1e-45f : as_f32(down > 0.f ? b - 1 : b + 1);
+    hot = !(down > -3.3e38f);
     if (hot) low = -INFINITY;
     scale = kSteps * 1.44269504088896340736 / (double)temperature;
-    const double most = 50.0 * kSteps / (top - (double)low);           // (33 temperatures: 47.6 factors of two)
+    const double most = 30000.0 / (top - (double)low);
     if (!(scale < most) && !hot) scale = most;
   }
   // of N elements, none below `low`: side by side, as each is a chain of 13 operations and a read
@@ -216,13 +225,13 @@ template <int W> struct SampleShared {
   int wave_n[W], found, listed;
   u64 found_w, found_n, cut, rest;
 };
-struct SampleBins {
-  uint32_t n[kBins];
-  u64 w[kBins];
+template <int NT> struct SampleBins {
+  uint32_t n[kBins<NT>];
+  u64 w[kBins<NT>];
 };
-union SampleRanked {
-  u64 list[kList];
-  SampleBins digit;
+template <int NT> union SampleRanked {
+  u64 list[kBins<NT>];
+  SampleBins<NT> digit;
 };
 
 // Sums of (n, w) over the threads before this one.
@@ -247,8 +256,8 @@ __device__ __forceinline__ void sample_scan(int& n, u64& w, SampleShared<W>& sh)
 // The first bin up to which there are at least `target` (of what is counted, or weighed): sh.found (-1: there are fewer), and in
 // found_n and found_w what is before it.
 template <int NT>
-__device__ __forceinline__ void sample_crossing(const SampleBins& bins, int size, bool by_weight, u64 target, SampleShared<NT / 64>& sh) {
-  constexpr int P = kBins / NT;
+__device__ __forceinline__ void sample_crossing(const SampleBins<NT>& bins, int size, bool by_weight, u64 target, SampleShared<NT / 64>& sh) {
+  constexpr int P = 2;
   const int first = threadIdx.x * P;
   int n[P], before_n = 0;
   u64 w[P], before_w = 0;
@@ -280,7 +289,7 @@ __device__ __forceinline__ void sample_crossing(const SampleBins& bins, int size
 // before it): sh.cut, and in found_w the weight up to and with it.
 template <int NT>
 __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int count, bool by_weight, u64 target, u64 before_n, u64 before_w,
-                                            SampleRanked& r, SampleShared<NT / 64>& sh) {
+                                            SampleRanked<NT>& r, SampleShared<NT / 64>& sh) {
   const int tid = threadIdx.x;
   int size = 2;
   while (size < count) size *= 2;
@@ -298,7 +307,7 @@ __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int coun
       }
       __syncthreads();
     }
-  constexpr int P = kList / NT;
+  constexpr int P = 2;
   u64 w[P], sum = 0;
   int none = 0;
 #pragma unroll
@@ -323,18 +332,20 @@ __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int coun
 // The same for one bin of the row, whatever number of elements (`count`) it has.
 template <typename T, int NT, class Bin>
 __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, const SampleWeight& weight, Bin bin, int b, int count,
-                                              bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked& r,
+                                              bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked<NT>& r,
                                               SampleShared<NT / 64>& sh) {
   constexpr int W = NT / 64, C = SampleRow<T, W>::C;
   const int tid = threadIdx.x;
   const auto none = [](int) AMOE_INLINE {};
-  // too many to rank at once: by 11 bits of their ranks at a time
+  // too many to rank at once: by as many bits of their ranks at a time as there are bins
+  constexpr int kDigit = NT == 1024 ? 11 : 9;
+  static_assert(1 << kDigit == kBins<NT>, "a bin for each digit");
   int shift = 32 + kIndexBits;
   u64 prefix = 0;
-  while (count > kList) {
-    const int next = shift > 11 ? shift - 11 : 0, size = 1 << (shift - next);
+  while (count > kBins<NT>) {
+    const int next = shift > kDigit ? shift - kDigit : 0, size = 1 << (shift - next);
     __syncthreads();
-    for (int i = tid; i < kBins; i += NT) {
+    for (int i = tid; i < kBins<NT>; i += NT) {
       r.digit.n[i] = 0;
       r.digit.w[i] = 0;
     }
@@ -472,88 +483,144 @@ __device__ __forceinline__ u64 sample_target(double u, u64 total) {
   return target < total ? target : total - 1;
 }
 
-template <typename T, int NT, bool CUT>
+// What the launches for a row that is worked on in parts leave for one another.
+struct SamplePart {
+  u64 list[2][kPartList];
+  float mx, mn;
+  int listed[2];
+};
+struct SampleWork {
+  SampleBins<1024> hist;             // cleared by the first launch, added to by the parts (whole numbers: in any order)
+  u64 rest, unit[kUnits + 2];
+  float unit_max[kUnits + 2];
+  SamplePart part[1];                // as many as there are
+};
+__device__ __host__ inline size_t sample_work_bytes(int parts) { return sizeof(SampleWork) + (size_t)(parts - 1) * sizeof(SamplePart); }
+
+// The launches for a row: all in one, or, of a row in parts, its extremes, its bins, the list of top_k's bin (where top_p needs its
+// weight), sums and the list of the cut's bin, and the rest by one workgroup again.
+enum SampleStage { kAll, kExtremes, kHistogram, kTopList, kSums, kFinish };
+
+template <typename T, int NT, bool CUT, int STAGE>
 __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
   constexpr int W = NT / 64, C = Elem<T>::kChunk;
+  constexpr bool kParted = STAGE != kAll;
   __shared__ SampleShared<W> sh;
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6);
-  const int64_t at = blockIdx.x;
+  const int parts = kParted && STAGE != kFinish ? p.parts : 1, part = (int)(blockIdx.x % (unsigned)parts);
+  const int64_t at = blockIdx.x / (unsigned)parts;
   const SampleRow<T, W> row(static_cast<const T*>(p.logits) + at * p.ld, p.V);
+  SampleWork* const work = kParted ? reinterpret_cast<SampleWork*>(p.work + at * (int64_t)sample_work_bytes(p.parts)) : nullptr;
+  // this workgroup's units; the edges are the first part's
+  const int first_unit = row.units * part / parts, end_unit = row.units * (part + 1) / parts;
+  const bool has_edges = part == 0 && wave == 0;
   const float temperature = p.temperature ? p.temperature[at] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[at] : p.top_p_all, min_p = p.min_p ? p.min_p[at] : p.min_p_all;
   const int64_t top_k = !p.top_k ? p.top_k_all : p.top_k_i64 ? static_cast<const int64_t*>(p.top_k)[at] : static_cast<const int32_t*>(p.top_k)[at];
   const double u = p.u_f64 ? static_cast<const double*>(p.u)[at] : (double)static_cast<const float*>(p.u)[at];
-  for (int i = tid; i < kSteps * kCopies; i += NT) sh.table[i] = ::exp2((double)(i / kCopies) / kSteps);
+  const bool greedy = !(temperature > 0.f), by_k = CUT && top_k > 0 && top_k < p.V, by_p = CUT && top_p < 1.f;
+  if (STAGE != kExtremes)
+    for (int i = tid; i < kSteps * kCopies; i += NT) sh.table[i] = ::exp2((double)(i / kCopies) / kSteps);
 
-  float mx = -INFINITY, mn = INFINITY, unit_max = -INFINITY;
-  row.all(
-      -INFINITY,
-      [&](const float (&v)[C], int, bool inside) AMOE_INLINE {
-        float lo = v[0];
+  // ---- the extremes
+  float mx = -INFINITY, mn = INFINITY;
+  if constexpr (STAGE == kAll || STAGE == kExtremes) {
+    float unit_max = -INFINITY;
+    row.some(
+        -INFINITY, first_unit, end_unit,
+        [&](const float (&v)[C], int, bool inside) AMOE_INLINE {
+          float lo = v[0];
 #pragma unroll
-        for (int e = 0; e < C; e++) {
-          unit_max = fmaxf(unit_max, v[e]);
-          if (CUT) lo = fminf(lo, v[e]);
-        }
-        if (CUT) mn = inside ? fminf(mn, lo) : mn;
-      },
-      [&](int unit) AMOE_INLINE {
-        unit_max = wave_largest(unit_max);
-        if (lane == 0) sh.unit_max[unit] = unit_max;
-        mx = fmaxf(mx, unit_max);
-        unit_max = -INFINITY;
-      });
-  if (wave == 0) {
-    const float behind = wave_largest(lane == 0 ? -INFINITY : row.edge);
-    if (lane == 0) {
-      sh.unit_max[0] = row.edge;
-      sh.unit_max[row.last] = behind;
+          for (int e = 0; e < C; e++) {
+            unit_max = fmaxf(unit_max, v[e]);
+            if (CUT) lo = fminf(lo, v[e]);
+          }
+          if (CUT) mn = inside ? fminf(mn, lo) : mn;
+        },
+        [&](int unit) AMOE_INLINE {
+          unit_max = wave_largest(unit_max);
+          if (lane == 0) {
+            if constexpr (kParted) work->unit_max[unit] = unit_max;
+            else sh.unit_max[unit] = unit_max;
+          }
+          mx = fmaxf(mx, unit_max);
+          unit_max = -INFINITY;
+        });
+    if (has_edges) {
+      const float behind = wave_largest(lane == 0 ? -INFINITY : row.edge);
+      if (lane == 0) {
+        float* const to = kParted ? work->unit_max : sh.unit_max;
+        to[0] = row.edge;
+        to[row.last] = behind;
+      }
+      mx = fmaxf(fmaxf(mx, behind), wave_shfl(row.edge, 0));
+      if (CUT && row.edge != -INFINITY) mn = fminf(mn, row.edge);
     }
-    mx = fmaxf(fmaxf(mx, behind), wave_shfl(row.edge, 0));
-    if (CUT && row.edge != -INFINITY) mn = fminf(mn, row.edge);
-  }
-  if (CUT) mn = -wave_largest(-mn);
-  if (lane == 0) {
-    sh.wave_max[wave] = mx;
-    sh.wave_min[wave] = mn;
-  }
-  __syncthreads();
+    if (CUT) mn = -wave_largest(-mn);
+    if (lane == 0) {
+      sh.wave_max[wave] = mx;
+      sh.wave_min[wave] = mn;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < W; i++) {
-    mx = fmaxf(mx, sh.wave_max[i]);
-    mn = fminf(mn, sh.wave_min[i]);
+    for (int i = 0; i < W; i++) {
+      mx = fmaxf(mx, sh.wave_max[i]);
+      mn = fminf(mn, sh.wave_min[i]);
+    }
+    if constexpr (STAGE == kExtremes) {
+      if constexpr (CUT) {
+        for (int i = part * NT + tid; i < kBins<NT>; i += parts * NT) {
+          work->hist.n[i] = 0;
+          work->hist.w[i] = 0;
+        }
+        if (part == 0 && tid == 0) work->rest = 0;
+      }
+      if (tid == 0) {
+        work->part[part].mx = mx;
+        work->part[part].mn = mn;
+      }
+      return;
+    }
+  } else {
+    for (int i = 0; i < p.parts; i++) {
+      mx = fmaxf(mx, work->part[i].mx);
+      mn = fminf(mn, work->part[i].mn);
+    }
+    if (STAGE == kFinish)
+      for (int i = tid; i <= row.last; i += NT) {
+        sh.unit[i] = work->unit[i];
+        sh.unit_max[i] = work->unit_max[i];
+      }
+    __syncthreads();
   }
   int index = 0;
   float value = 0.f;
   if (mx == -INFINITY) {
-    if (tid == 0) {
+    if ((STAGE == kAll || STAGE == kFinish) && tid == 0) {
       p.ids[at] = -1;
       if (p.logprob) p.logprob[at] = -INFINITY;
     }
     return;
   }
-  const bool greedy = !(temperature > 0.f);
+
+  // ---- only those as large as the largest weigh, and all the same
   if (greedy || mx == INFINITY) {
-    // only those as large as the largest weigh, and all the same
+    if (STAGE != kAll && STAGE != kFinish) return;
     const auto weigh = [&](float x, int) AMOE_INLINE { return (u64)(x == mx); };
-    for (int i = wave; i <= row.last; i += W) {
+    for (int i = 1 + wave; i < row.last; i += W) {
       u64 s = 0;
       if (sh.unit_max[i] == mx) {
-        if (i == 0 || i == row.last) {
-          s = (u64)((lane == 0) == (i == 0) && row.edge == mx);        // (the edges are the first wave's)
-        } else {
-          const int g = (i - 1) * row.per, end = g + row.per;
-          row.scan(
-              -INFINITY, g, end < row.groups ? end : row.groups,
-              [&](const float (&v)[C], int, bool) AMOE_INLINE {
+        const int g = (i - 1) * row.per, end = g + row.per;
+        row.scan(
+            -INFINITY, g, end < row.groups ? end : row.groups,
+            [&](const float (&v)[C], int, bool) AMOE_INLINE {
 #pragma unroll
-                for (int e = 0; e < C; e++) s += weigh(v[e], 0);
-              },
-              [](int) AMOE_INLINE {});
-        }
+              for (int e = 0; e < C; e++) s += weigh(v[e], 0);
+            },
+            [](int) AMOE_INLINE {});
         s = wave_total(s);
       }
-      if (lane == 0 && i != row.last && i != 0) sh.unit[i] = s;
+      if (lane == 0) sh.unit[i] = s;
     }
     if (wave == 0) {
       const u64 behind = wave_total(lane != 0 && row.edge == mx);
@@ -570,8 +637,8 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
       kept = wave_total(kept);
       if (top_k > 0 && (u64)top_k < kept) kept = (u64)top_k;
       if (top_p < 1.f) {
-        const double part = top_p > 0.f ? __builtin_ceil((double)top_p * (double)kept) : 1.0;
-        kept = part < 1.0 ? 1 : (u64)part;
+        const double share = top_p > 0.f ? __builtin_ceil((double)top_p * (double)kept) : 1.0;
+        kept = share < 1.0 ? 1 : (u64)share;
       }
     }
     if (sample_find<T, W>(row, -INFINITY, greedy ? 0 : sample_target(u, kept), weigh, sh, index, value)) {
@@ -583,136 +650,183 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
 
   const SampleWeight weight(mx, temperature, sh.table);
   const u64 least = min_p > 0.f ? (u64)__builtin_ceil((double)fminf(min_p, 1.f) * (double)kOne) : 0;
-  // What is kept: ranks of `cut` and more; while that is not known, bins before `edge_bin`
+  u64* const unit_to = STAGE == kSums ? work->unit : sh.unit;
+  // ---- what is kept: ranks of `cut` and more
   u64 cut = 0;
-  bool summed = false;
+  bool summed = STAGE == kFinish;
   if constexpr (CUT) {
-    __shared__ SampleBins hist;
-    __shared__ SampleRanked ranked;
-    const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
+    __shared__ SampleBins<NT> hist;
+    __shared__ SampleRanked<NT> ranked;
     if (by_k || by_p) {
+      if (STAGE == kTopList && !(by_k && by_p)) return;
       // Bins are equal intervals of the distance to the largest, up to where tokens occur, weigh anything and, without top_k, may be
       // kept: all that weigh less than (1 - top_p) / V are together less than what top_p may leave out.  (Half the distances: they
       // may be twice the largest float.)
       const float half = 0.5f * mx;
       float reach = fminf(fmaf(-0.5f, mn, half), 16.25f * temperature);
       if (!by_k) reach = fminf(reach, 0.3466f * temperature * (fast_log2((float)p.V) - fast_log2(1.f - fmaxf(top_p, 0.f)) + 1.f));
-      const float step = reach > 0.f ? fminf((kBins - 2) / reach, 3.402823466e38f) : 0.f;
-      const auto bin = [=](float x) AMOE_INLINE { return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins - 1)); };
-      for (int i = tid; i < kBins; i += NT) {
-        hist.n[i] = 0;
-        hist.w[i] = 0;
-      }
+      const float step = reach > 0.f ? fminf((kBins<NT> - 2) / reach, 3.402823466e38f) : 0.f;
+      const auto bin = [=](float x) AMOE_INLINE { return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins<NT> - 1)); };
       if (tid == 0) sh.rest = 0;
-      __syncthreads();
-      u64 rest = 0;
-      const auto count = [&](const auto& v) AMOE_INLINE {
-        constexpr int N = sizeof(v) / sizeof(v[0]);
-        int b[N];
+      if constexpr (STAGE == kAll || STAGE == kHistogram) {
+        for (int i = tid; i < kBins<NT>; i += NT) {
+          hist.n[i] = 0;
+          hist.w[i] = 0;
+        }
+        __syncthreads();
+        u64 rest = 0;
+        const auto count = [&](const auto& v) AMOE_INLINE {
+          constexpr int N = sizeof(v) / sizeof(v[0]);
+          int b[N];
 #pragma unroll
-        for (int e = 0; e < N; e++) b[e] = bin(v[e]);
-        if (by_p) {
-          u64 w[N];
-          weight(v, w);
+          for (int e = 0; e < N; e++) b[e] = bin(v[e]);
+          if (by_p) {
+            u64 w[N];
+            weight(v, w);
 #pragma unroll
-          for (int e = 0; e < N; e++) {
-            if (b[e] < kBins - 1) atomicAdd(&hist.w[b[e]], w[e]);
-            else rest += w[e];
+            for (int e = 0; e < N; e++) {
+              if (b[e] < kBins<NT> - 1) atomicAdd(&hist.w[b[e]], w[e]);
+              else rest += w[e];
+            }
           }
-        }
-        if (by_k) {
+          if (by_k) {
 #pragma unroll
-          for (int e = 0; e < N; e++)
-            if (b[e] < kBins - 1) atomicAdd(&hist.n[b[e]], 1u);
+            for (int e = 0; e < N; e++)
+              if (b[e] < kBins<NT> - 1) atomicAdd(&hist.n[b[e]], 1u);
+          }
+        };
+        row.some(
+            weight.low, first_unit, end_unit, [&](const float (&v)[C], int, bool) AMOE_INLINE { count(v); }, [](int) AMOE_INLINE {});
+        if (has_edges && row.edge > weight.low) {
+          const float one[1] = {row.edge};
+          count(one);
         }
+        if (by_p) {
+          rest = wave_total(rest);
+          if (lane == 0 && rest) atomicAdd(&sh.rest, rest);
+        }
+        __syncthreads();
+        if constexpr (STAGE == kHistogram) {
+          for (int i = tid; i < kBins<NT> - 1; i += NT) {
+            if (hist.n[i]) atomicAdd(&work->hist.n[i], hist.n[i]);
+            if (hist.w[i]) atomicAdd(&work->hist.w[i], hist.w[i]);
+          }
+          if (tid == 0 && sh.rest) atomicAdd(&work->rest, sh.rest);
+          return;
+        }
+      } else if constexpr (NT == 1024) {
+        for (int i = tid; i < kBins<NT>; i += NT) {
+          hist.n[i] = work->hist.n[i];
+          hist.w[i] = work->hist.w[i];
+        }
+        if (tid == 0) sh.rest = work->rest;
+        __syncthreads();
+      }
+      // the elements of bin b, from the parts' lists (l: of top_k's bin or the cut's); false if some did not fit
+      const auto gather = [&](int l) AMOE_INLINE {
+        int n = 0;
+        bool fit = true;
+        for (int j = 0; j < p.parts; j++) {
+          const int m = work->part[j].listed[l];
+          fit = fit && m <= kPartList && n + m <= kBins<NT>;
+          if (!fit) break;
+          for (int i = tid; i < m; i += NT) ranked.list[n + i] = work->part[j].list[l][i];
+          n += m;
+        }
+        if (tid == 0) sh.listed = n;
+        __syncthreads();
+        return fit;
       };
-      row.all(
-          weight.low, [&](const float (&v)[C], int, bool) AMOE_INLINE { count(v); }, [](int) AMOE_INLINE {});
-      if (wave == 0 && row.edge > weight.low) {
-        const float one[1] = {row.edge};
-        count(one);
-      }
-      if (by_p) {
-        rest = wave_total(rest);
-        if (lane == 0 && rest) atomicAdd(&sh.rest, rest);
-      }
-      __syncthreads();
       u64 total = 0, target = (u64)top_k;
       int b = -1;
       if (by_k) {
-        sample_crossing<NT>(hist, kBins - 1, false, target, sh);
+        sample_crossing<NT>(hist, kBins<NT> - 1, false, target, sh);
         b = sh.found;
-        if (b >= 0 && by_p) {
+        if (b >= 0 && by_p && STAGE != kTopList) {
           const u64 before_n = sh.found_n, before_w = sh.found_w;
-          sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], false, target, before_n, before_w, ranked, sh);
+          if (STAGE == kAll || !gather(0)) sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], false, target, before_n, before_w, ranked, sh);
+          else sample_sort<NT>(weight, sh.listed, false, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
           total = sh.found_w;
         }
       }
-      if (by_p) {
+      if (by_p && STAGE != kTopList) {
         if (b < 0) {
-          int n = 0;
           u64 w = 0;
-          for (int i = tid; i < kBins; i += NT) w += hist.w[i];
-          const u64 mine = w;
-          sample_scan<W>(n, w, sh);
+          for (int i = tid; i < kBins<NT>; i += NT) w += hist.w[i];
+          w = wave_total(w);
+          if (lane == 0 && w) atomicAdd(&sh.rest, w);
           __syncthreads();
-          if (tid == NT - 1) sh.found_w = w + mine;
-          __syncthreads();
-          total = sh.found_w + sh.rest;
+          total = sh.rest;
         }
-        const double part = top_p > 0.f ? __builtin_ceil((double)top_p * (double)total) : 1.0;
-        target = part < 1.0 ? 1 : (u64)part;
+        const double share = top_p > 0.f ? __builtin_ceil((double)top_p * (double)total) : 1.0;
+        target = share < 1.0 ? 1 : (u64)share;
         __syncthreads();
-        sample_crossing<NT>(hist, kBins - 1, true, target, sh);
+        sample_crossing<NT>(hist, kBins<NT> - 1, true, target, sh);
         b = sh.found;
       }
       if (b >= 0) {
         // one more pass: the sums of the bins before b, and a list of b's elements
         const u64 before_n = sh.found_n, before_w = sh.found_w;
-        if (tid == 0) sh.listed = 0;
-        __syncthreads();
-        u64 s = 0;
-        const auto take = [&](const auto& v, int first) AMOE_INLINE -> u64 {
-          constexpr int N = sizeof(v) / sizeof(v[0]);
-          int in[N];
-          bool any = false;
+        if constexpr (STAGE != kFinish) {
+          if (tid == 0) sh.listed = 0;
+          __syncthreads();
+          constexpr int kRoom = STAGE == kAll ? kBins<NT> : kPartList;
+          u64 s = 0;
+          const auto take = [&](const auto& v, int first) AMOE_INLINE -> u64 {
+            constexpr int N = sizeof(v) / sizeof(v[0]);
+            int in[N];
+            bool any = false;
 #pragma unroll
-          for (int e = 0; e < N; e++) {
-            in[e] = bin(v[e]);
-            any = any | (in[e] <= b);
-          }
-          if (!any) return 0;
-          u64 w[N], sum = 0;
-          weight(v, w);
-#pragma unroll
-          for (int e = 0; e < N; e++) {
-            if (in[e] == b) {
-              const int n = atomicAdd(&sh.listed, 1);
-              if (n < kList) ranked.list[n] = sample_rank(v[e], first + e);
+            for (int e = 0; e < N; e++) {
+              in[e] = bin(v[e]);
+              any = any | (STAGE == kTopList ? in[e] == b : in[e] <= b);
             }
-            sum += (in[e] < b) & (w[e] >= least) ? w[e] : 0;
+            if (!any) return 0;
+#pragma unroll
+            for (int e = 0; e < N; e++)
+              if (in[e] == b) {
+                const int n = atomicAdd(&sh.listed, 1);
+                if (n < kRoom) ranked.list[n] = sample_rank(v[e], first + e);
+              }
+            if (STAGE == kTopList) return 0;
+            u64 w[N], sum = 0;
+            weight(v, w);
+#pragma unroll
+            for (int e = 0; e < N; e++) sum += (in[e] < b) & (w[e] >= least) ? w[e] : 0;
+            return sum;
+          };
+          row.some(
+              weight.low, first_unit, end_unit, [&](const float (&v)[C], int first, bool) AMOE_INLINE { s += take(v, first); },
+              [&](int unit) AMOE_INLINE {
+                if (STAGE != kTopList) {
+                  s = wave_total(s);
+                  if (lane == 0) unit_to[unit] = s;
+                }
+                s = 0;
+              });
+          if (has_edges) {
+            const float one[1] = {row.edge};
+            const u64 w = row.edge > weight.low ? take(one, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
+            if (lane == 0 && STAGE != kTopList) {
+              unit_to[0] = w;
+              unit_to[row.last] = behind;
+            }
           }
-          return sum;
-        };
-        row.all(
-            weight.low, [&](const float (&v)[C], int first, bool) AMOE_INLINE { s += take(v, first); },
-            [&](int unit) AMOE_INLINE {
-              s = wave_total(s);
-              if (lane == 0) sh.unit[unit] = s;
-              s = 0;
-            });
-        if (wave == 0) {
-          const float one[1] = {row.edge};
-          const u64 w = row.edge > weight.low ? take(one, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
-          if (lane == 0) {
-            sh.unit[0] = w;
-            sh.unit[row.last] = behind;
+          __syncthreads();
+          if constexpr (STAGE != kAll) {
+            constexpr int l = STAGE == kTopList ? 0 : 1;
+            SamplePart& to = work->part[part];
+            const int n = sh.listed;
+            for (int i = tid; i < (n < kRoom ? n : kRoom); i += NT) to.list[l][i] = ranked.list[i];
+            if (tid == 0) to.listed[l] = n;
+            return;
           }
         }
-        __syncthreads();
+        bool fit = sh.listed <= kBins<NT>;
+        if constexpr (STAGE == kFinish) fit = gather(1);
         const int listed = sh.listed;
-        if (listed <= kList) {
+        if (fit) {
           sample_sort<NT>(weight, listed, by_p, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
           for (int i = tid; i < listed; i += NT) {
@@ -721,12 +835,19 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
           }
           summed = true;
         } else {
-          sample_refine<T, NT>(row, weight, bin, b, listed, by_p, target, before_n, before_w, ranked, sh);
+          int count = listed;
+          if constexpr (STAGE == kFinish) {
+            count = 0;
+            for (int j = 0; j < p.parts; j++) count += work->part[j].listed[1];
+          }
+          sample_refine<T, NT>(row, weight, bin, b, count, by_p, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
+          summed = false;
         }
       }
     }
   }
+  if (STAGE == kHistogram || STAGE == kTopList) return;
   const float cut_x = cut ? sample_value(cut) : -INFINITY;
   const int cut_i = cut ? sample_index(cut) : p.V;
   const auto weigh = [&](float x, int i) AMOE_INLINE -> u64 {
@@ -737,9 +858,9 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
   __syncthreads();                                    // (the table, where nothing was cut)
   if (!summed) {
     u64 s = 0;
-    const bool all = !CUT || cut == 0;
-    row.all(
-        weight.low,
+    const bool every = !CUT || cut == 0;
+    row.some(
+        weight.low, first_unit, end_unit,
         [&](const float (&v)[C], int first, bool) AMOE_INLINE {
           u64 w[C];
           weight(v, w);
@@ -747,7 +868,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
 #pragma unroll
             for (int e = 0; e < C; e++) w[e] = w[e] >= least ? w[e] : 0;
           }
-          if (!all) {
+          if (!every) {
 #pragma unroll
             for (int e = 0; e < C; e++) w[e] = (v[e] > cut_x) | ((v[e] == cut_x) & (first + e <= cut_i)) ? w[e] : 0;
           }
@@ -756,18 +877,19 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
         },
         [&](int unit) AMOE_INLINE {
           s = wave_total(s);
-          if (lane == 0) sh.unit[unit] = s;
+          if (lane == 0) unit_to[unit] = s;
           s = 0;
         });
-    if (wave == 0) {
+    if (has_edges) {
       const u64 w = row.edge != -INFINITY ? weigh(row.edge, row.edge_index) : 0, behind = wave_total(lane == 0 ? 0 : w);
       if (lane == 0) {
-        sh.unit[0] = w;
-        sh.unit[row.last] = behind;
+        unit_to[0] = w;
+        unit_to[row.last] = behind;
       }
     }
     __syncthreads();
   }
+  if (STAGE == kSums) return;
   u64 total = 0;
   for (int i = lane; i <= row.last; i += 64) total += sh.unit[i];
   total = wave_total(total);
@@ -778,17 +900,34 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
 
 namespace {
 
-template <typename T>
-int launch_sample(const SampleParams& p, bool cut, hipStream_t st) {
-  const dim3 grid((unsigned)p.rows);
-  const bool wide = p.V > 16384 || p.rows < 2 * num_compute_units();
-#define AMOE_LAUNCH(NT, CUT) hipLaunchKernelGGL((&sample_kernel<T, NT, CUT>), grid, dim3(NT), 0, st, p)
-  if (wide && cut) AMOE_LAUNCH(1024, true);
-  else if (wide) AMOE_LAUNCH(1024, false);
-  else if (cut) AMOE_LAUNCH(256, true);
-  else AMOE_LAUNCH(256, false);
-#undef AMOE_LAUNCH
+// Parts that a row is worked on in, 1: all in one launch.
+int sample_parts(const amoe_sample_args* a) {
+  const int64_t most = num_compute_units() / (a->rows < 1 ? 1 : a->rows), n = a->V / 4096;
+  const int64_t parts = n < most ? n : most;
+  return (int)(parts < 4 ? 1 : parts > kMaxParts ? kMaxParts : parts);
+}
+
+template <typename T, bool CUT>
+int launch_sample_cut(const SampleParams& p, bool both, hipStream_t st) {
+  const dim3 grid((unsigned)p.rows), parts((unsigned)(p.rows * p.parts)), block(1024);
+  if (p.parts > 1) {
+    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kExtremes>), parts, block, 0, st, p);
+    if constexpr (CUT) {
+      hipLaunchKernelGGL((&sample_kernel<T, 1024, true, kHistogram>), parts, block, 0, st, p);
+      if (both) hipLaunchKernelGGL((&sample_kernel<T, 1024, true, kTopList>), parts, block, 0, st, p);
+    }
+    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kSums>), parts, block, 0, st, p);
+    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kFinish>), grid, block, 0, st, p);
+  } else if (p.V > 16384 || p.rows < 2 * num_compute_units()) {
+    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kAll>), grid, block, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((&sample_kernel<T, 256, CUT, kAll>), grid, dim3(256), 0, st, p);
+  }
   return launch_rc();
+}
+template <typename T>
+int launch_sample(const SampleParams& p, bool cut, bool both, hipStream_t st) {
+  return cut ? launch_sample_cut<T, true>(p, both, st) : launch_sample_cut<T, false>(p, both, st);
 }
 
 int sample_check(const amoe_sample_args* a) {
@@ -811,9 +950,13 @@ using namespace amoe;
 
 extern "C" size_t amoe_sample_args_bytes(void) { return sizeof(amoe_sample_args); }
 
-extern "C" size_t amoe_sample_workspace(const amoe_sample_args*) { return 0; }
+extern "C" size_t amoe_sample_workspace(const amoe_sample_args* a) {
+  if (sample_check(a) || a->rows == 0) return 0;
+  const int parts = sample_parts(a);
+  return parts > 1 ? (size_t)a->rows * sample_work_bytes(parts) : 0;
+}
 
-extern "C" int amoe_sample(const amoe_sample_args* a, void*, size_t, void* stream) {
+extern "C" int amoe_sample(const amoe_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = sample_check(a)) return rc;
   if (a->rows == 0) return AMOE_OK;
   if (!a->logits || !a->u || !a->ids) return AMOE_ENULL;
@@ -821,7 +964,13 @@ extern "C" int amoe_sample(const amoe_sample_args* a, void*, size_t, void* strea
   if (!aligned(a->logits, esize((int)a->dtype)) || !aligned(a->u, a->u_is_f64 ? 8 : 4) || !aligned(a->ids, 8) || !aligned(a->logprob, 4) ||
       !aligned(a->temperature, 4) || !aligned(a->top_p, 4) || !aligned(a->min_p, 4) || !aligned(a->top_k, a->top_k_is_i64 ? 8 : 4))
     return AMOE_EALIGN;
+  const size_t need = amoe_sample_workspace(a);
+  if (need && !workspace) return AMOE_ENULL;
+  if (workspace_bytes < need) return AMOE_EWORKSPACE;
+  if (need && !aligned(workspace, 8)) return AMOE_EALIGN;
   SampleParams p{};
+  p.work = static_cast<char*>(workspace);
+  p.parts = sample_parts(a);
   p.logits = a->logits; p.ld = a->rows == 1 ? 0 : a->ld;
   p.u = a->u; p.u_f64 = a->u_is_f64 != 0;
   p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p;
@@ -830,9 +979,10 @@ extern "C" int amoe_sample(const amoe_sample_args* a, void*, size_t, void* strea
   p.top_k_all = a->top_k_all;
   p.ids = a->ids; p.logprob = a->logprob;
   p.rows = a->rows; p.V = (int)a->V;
-  const bool cut = a->top_k || a->top_p || (a->top_k_all > 0 && a->top_k_all < a->V) || p.top_p_all < 1.f;
+  const bool by_k = a->top_k || (a->top_k_all > 0 && a->top_k_all < a->V), by_p = a->top_p || p.top_p_all < 1.f;
+  const bool cut = by_k || by_p, both = by_k && by_p;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a->dtype == AMOE_F32   ? launch_sample<float>(p, cut, st)
-         : a->dtype == AMOE_F16 ? launch_sample<f16_t>(p, cut, st)
-                                : launch_sample<uint16_t>(p, cut, st);
+  return a->dtype == AMOE_F32   ? launch_sample<float>(p, cut, both, st)
+         : a->dtype == AMOE_F16 ? launch_sample<f16_t>(p, cut, both, st)
+                                : launch_sample<uint16_t>(p, cut, both, st);
 }

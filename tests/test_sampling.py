@@ -1,5 +1,8 @@
 """The choice of a token against its definition: the kernel's source on the CPU, and the built library on the GPU."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -157,6 +160,51 @@ def test_cuts_within_many_equal_logits(emu_ops):
     check(x, torch.tensor([0.999]), top_p=0.97)
 
 
+PARTED = {
+    # rows worked on in parts: as CASES, and more equal logits at a cut than the parts hand on
+    "full": (2, 16500, "f32", "normal", "own", {}),
+    "greedy": (2, 17001, "bf16", "coarse", "odd", dict(temperature=0.0)),
+    "k": (2, 16500, "f32", "normal", "odd", dict(top_k=700)),
+    "p": (2, 17003, "bf16", "masked", "odd", dict(top_p=0.9)),
+    "both": (2, 20011, "f16", "normal", "own", dict(top_k=900, top_p=0.8, min_p=0.001)),
+    "both_equal": (2, 16400, "f32", "equal", "own", dict(top_k=9000, top_p=0.5)),
+    "k_two": (1, 16400, "bf16", "two", "odd", dict(top_k=5000)),
+    "p_two": (1, 16400, "f32", "two", "own", dict(top_p=0.97)),
+    "cold": (2, 16400, "f32", "normal", "own", dict(top_p=0.6, temperature=1e-30)),
+}
+
+
+def check_parted(names, device="cpu"):
+    for name in names:
+        if name == "rows":                                # settings of each row's own, infinities and rows of nothing
+            how = allowed(mixed(5))
+            x = logits(5, 16500, "bf16", seed=5)
+            x[1, 400], x[1, 16400] = INF, INF
+            how["temperature"][1] = 1.0
+            x[4] = -INF
+            check(x, numbers(5, 5), device, **how)
+            continue
+        rows, V, dtype, kind, layout, how = PARTED[name]
+        check(logits(rows, V, dtype, kind, len(name), layout), numbers(rows, len(name)), device, **how)
+
+
+@pytest.mark.parametrize("names", [list(PARTED)[:5], list(PARTED)[5:] + ["rows"]])
+def test_rows_in_parts(emu_ops, names):
+    """On a device of 64 compute units (a process of its own: the library asks once how many there are)."""
+    child = ("import sys\nfrom analog_moe_amd import _abi, ops\nfrom tests import test_emu_kernels as t, test_sampling as f\n"
+             "ops._LIB, ops._stream, ops._need_gpu = _abi.bind(t.EMU_SO), (lambda x: None), (lambda *a: None)\n"
+             "f.check_parted(sys.argv[1:])\nprint('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = subprocess.run([sys.executable, "-c", child, *names], cwd=root, env={**os.environ, "AMOE_EMU_CUS": "64"}, capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout.endswith("done\n"), got.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(PARTED) + ["rows"])
+def test_gpu_rows_in_parts(name):
+    check_parted([name], "cuda")
+
+
 def test_every_token_has_its_share(emu_ops):
     """u from 0 to 1 in equal steps: each token is drawn as often as its weight says, and in the order of the indices."""
     w = torch.tensor([3.0, 0.0, 1.0, 4.0, 0.0, 8.0])
@@ -262,8 +310,12 @@ GPU_CASES = dict(CASES, **{
     "large_bf16": (5, 50001, "bf16", "normal", "own", dict(top_p=0.99)),
     "large_masked": (5, 50001, "f16", "masked", "odd", dict(top_p=0.9, min_p=0.01)),
     "large_coarse": (3, 200000, "f32", "coarse", "own", dict(top_k=30001, top_p=0.97)),
+    "parted_f32": (30, 130001, "f32", "normal", "own", dict(top_k=60000, top_p=0.95, temperature=1.2)),
+    "parted_bf16": (60, 50001, "bf16", "normal", "odd", dict(top_p=0.99)),
+    "parted_full": (7, 200003, "bf16", "normal", "odd", dict(min_p=1e-4)),
     "large_equal": (2, 100003, "bf16", "equal", "own", dict(top_k=77777, top_p=0.9)),
     "large_two": (3, 100003, "f32", "two", "own", dict(top_k=90000, top_p=0.9)),
+    "large_rows": (100, 50001, "f32", "masked", "own", dict(top_k=5000, top_p=0.95)),
     "largest": (2, (1 << 20) - 1, "f32", "normal", "own", dict(top_p=0.9)),
     "largest_full": (2, (1 << 20) - 1, "bf16", "equal", "own", {}),
 })
