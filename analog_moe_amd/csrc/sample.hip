@@ -582,10 +582,9 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
       return;
     }
   } else {
-    for (int i = 0; i < p.parts; i++) {
-      mx = fmaxf(mx, work->part[i].mx);
-      mn = fminf(mn, work->part[i].mn);
-    }
+    // (a lane per part: one after the other they are a round trip to memory each)
+    mx = wave_largest(lane < p.parts ? work->part[lane].mx : -INFINITY);
+    mn = -wave_largest(lane < p.parts ? -work->part[lane].mn : -INFINITY);
     if (STAGE == kFinish)
       for (int i = tid; i <= row.last; i += NT) {
         sh.unit[i] = work->unit[i];
@@ -723,19 +722,16 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
         __syncthreads();
       }
       // the elements of bin b, from the parts' lists (l: of top_k's bin or the cut's); false if some did not fit
-      const auto gather = [&](int l) AMOE_INLINE {
-        int n = 0;
-        bool fit = true;
-        for (int j = 0; j < p.parts; j++) {
-          const int m = work->part[j].listed[l];
-          fit = fit && m <= kPartList && n + m <= kBins<NT>;
-          if (!fit) break;
-          for (int i = tid; i < m; i += NT) ranked.list[n + i] = work->part[j].list[l][i];
-          n += m;
+      const auto gather = [&](int l, int& count) AMOE_INLINE {
+        const int mine = lane < p.parts ? work->part[lane].listed[l] : 0, before = wave_scan(mine) - mine;
+        count = wave_shfl(before + mine, 63);
+        if (wave_ballot(mine > kPartList) != 0 || count > kBins<NT>) return false;
+        for (int j = wave; j < p.parts; j += W) {
+          const int m = wave_shfl(mine, j), to = wave_shfl(before, j);
+          for (int i = lane; i < m; i += 64) ranked.list[to + i] = work->part[j].list[l][i];
         }
-        if (tid == 0) sh.listed = n;
         __syncthreads();
-        return fit;
+        return true;
       };
       u64 total = 0, target = (u64)top_k;
       int b = -1;
@@ -744,8 +740,9 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
         b = sh.found;
         if (b >= 0 && by_p && STAGE != kTopList) {
           const u64 before_n = sh.found_n, before_w = sh.found_w;
-          if (STAGE == kAll || !gather(0)) sample_refine<T, NT>(row, weight, bin, b, (int)hist.n[b], false, target, before_n, before_w, ranked, sh);
-          else sample_sort<NT>(weight, sh.listed, false, target, before_n, before_w, ranked, sh);
+          int n = (int)hist.n[b];
+          if (STAGE != kAll && gather(0, n)) sample_sort<NT>(weight, n, false, target, before_n, before_w, ranked, sh);
+          else sample_refine<T, NT>(row, weight, bin, b, n, false, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
           total = sh.found_w;
         }
@@ -823,9 +820,9 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
             return;
           }
         }
-        bool fit = sh.listed <= kBins<NT>;
-        if constexpr (STAGE == kFinish) fit = gather(1);
-        const int listed = sh.listed;
+        int listed = sh.listed;
+        bool fit = listed <= kBins<NT>;
+        if constexpr (STAGE == kFinish) fit = gather(1, listed);
         if (fit) {
           sample_sort<NT>(weight, listed, by_p, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
@@ -835,12 +832,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
           }
           summed = true;
         } else {
-          int count = listed;
-          if constexpr (STAGE == kFinish) {
-            count = 0;
-            for (int j = 0; j < p.parts; j++) count += work->part[j].listed[1];
-          }
-          sample_refine<T, NT>(row, weight, bin, b, count, by_p, target, before_n, before_w, ranked, sh);
+          sample_refine<T, NT>(row, weight, bin, b, listed, by_p, target, before_n, before_w, ranked, sh);
           cut = sh.cut;
           summed = false;
         }
