@@ -72,6 +72,24 @@ inline void swap_half_waves(uint32_t& a, uint32_t& b) {
   const uint32_t got = emu_exchange(upper ? a : b, lane_id() ^ 32);
   (upper ? a : b) = got;
 }
+inline void swap_odd_rows(uint32_t& a, uint32_t& b) {
+  const bool odd = lane_id() & 16;
+  const uint32_t got = emu_exchange(odd ? a : b, lane_id() ^ 16);
+  (odd ? a : b) = got;
+}
+template <int N> inline uint32_t row_rotate(uint32_t v) { return emu_exchange(v, (lane_id() & ~15) | ((lane_id() - N) & 15)); }
+template <int N> inline uint32_t row_from_below(uint32_t v) {
+  const uint32_t got = emu_exchange(v, lane_id() - N);
+  return (lane_id() & 15) >= N ? got : 0u;
+}
+inline uint32_t odd_rows_from_below(uint32_t v) {
+  const uint32_t got = emu_exchange(v, ((lane_id() & ~15) - 1) & 63);
+  return lane_id() & 16 ? got : 0u;
+}
+inline uint32_t upper_half_from_below(uint32_t v) {
+  const uint32_t got = emu_exchange(v, 31);
+  return lane_id() >= 32 ? got : 0u;
+}
 template <class V> inline V wave_shfl_up(V v, int d) {
   int l = lane_id();
   return emu_exchange(v, l >= d ? l - d : l);

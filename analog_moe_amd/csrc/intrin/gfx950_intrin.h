@@ -119,6 +119,26 @@ __device__ __forceinline__ void swap_half_waves(uint32_t& a, uint32_t& b) {
   a = r[0];
   b = r[1];
 }
+// The odd rows of 16 lanes of a and the even rows of b change places.
+__device__ __forceinline__ void swap_odd_rows(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// Moves between lanes that take no trip through LDS: a row's 16 lanes rotated by N; from N lanes below in the row (zero for the first
+// N); rows 1 and 3 the last lane of the row below, the others zero; the upper half wave the last lane of the lower, which gets zero.
+template <int N> __device__ __forceinline__ uint32_t row_rotate(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, false);
+}
+template <int N> __device__ __forceinline__ uint32_t row_from_below(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x110 + N, 0xf, 0xf, false);
+}
+__device__ __forceinline__ uint32_t odd_rows_from_below(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+}
+__device__ __forceinline__ uint32_t upper_half_from_below(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+}
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
 template <typename V>

@@ -8,6 +8,7 @@
 #include <amoe.h>
 
 #include "host_util.h"
+#include "wave_ops.h"
 
 namespace amoe {
 
@@ -83,11 +84,8 @@ __device__ __forceinline__ void norm_weight(const void* w, int f32, int c, int D
 // barrier each does.
 template <int NT>
 __device__ __forceinline__ void norm_sum2(float& a, float& b, float (*lds)[2][16], int turn) {
-#pragma unroll
-  for (int m = 1; m < (NT < 64 ? NT : 64); m <<= 1) {
-    a += wave_shfl_xor(a, m);
-    b += wave_shfl_xor(b, m);
-  }
+  a = lanes_sum<(NT < 64 ? NT : 64)>(a);
+  b = lanes_sum<(NT < 64 ? NT : 64)>(b);
   if constexpr (NT > 64) {
     constexpr int W = NT / 64;
     const int wave = threadIdx.x >> 6, first = wave / W * W;

@@ -14,10 +14,10 @@
 #include <amoe.h>
 
 #include "host_util.h"
+#include "wave_ops.h"
 
 namespace amoe {
 
-typedef unsigned long long u64;
 // (closures that are not inlined live in memory, and with them all that they refer to)
 #define AMOE_INLINE __attribute__((always_inline))
 
@@ -197,26 +197,6 @@ __device__ __forceinline__ float sample_value(u64 rank) {
 }
 __device__ __forceinline__ int sample_index(u64 rank) { return (1 << kIndexBits) - 1 - (int)(rank & ((1 << kIndexBits) - 1)); }
 
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v) {       // sums up to and with the lane's
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const V up = wave_shfl_up(v, d);
-    if (lane_id() >= d) v += up;
-  }
-  return v;
-}
-__device__ __forceinline__ u64 wave_total(u64 s) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) s += wave_shfl_xor(s, d);
-  return s;
-}
-__device__ __forceinline__ float wave_largest(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, wave_shfl_xor(v, d));
-  return v;
-}
-
 // What a workgroup shares beside the histogram.
 template <int W> struct SampleShared {
   double table[kSteps * kCopies];
@@ -245,12 +225,10 @@ __device__ __forceinline__ void sample_scan(int& n, u64& w, SampleShared<W>& sh)
     sh.wave_w[wave] = iw;
   }
   __syncthreads();
-  n = in - n;
-  w = iw - w;
-  for (int i = 0; i < wave; i++) {
-    n += sh.wave_n[i];
-    w += sh.wave_w[i];
-  }
+  // (those of the waves before, a lane each)
+  const bool before = lane < wave;
+  n = in - n + (int)wave_read((uint32_t)wave_scan(before ? sh.wave_n[lane] : 0), 63);
+  w = iw - w + wave_total(before ? sh.wave_w[lane] : 0);
 }
 
 // The first bin up to which there are at least `target` (of what is counted, or weighed): sh.found (-1: there are fewer), and in
@@ -418,8 +396,8 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float lo
     if (in < 0 && run + part[i] > target) in = i;
     if (in < 0) run += part[i];
   }
-  target -= wave_shfl(run, at);
-  const int unit = P * at + wave_shfl(in, at);
+  target -= wave_read(run, at);
+  const int unit = P * at + (int)wave_read((uint32_t)in, at);
   const bool edges = unit == 0 || unit == row.last;
   const int g0 = (unit - 1) * row.per, g1 = g0 + row.per < row.groups ? g0 + row.per : row.groups;
   const auto group_sum = [&](int g, u64 (&w)[C], float (&x)[C], int& start) AMOE_INLINE {
@@ -458,7 +436,7 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float lo
   mine = lane < g1 - g0 ? sh.group[lane] : 0;
   run = wave_scan(mine);
   const int group = ctz64(wave_ballot(run > target));
-  target -= wave_shfl(run - mine, group);
+  target -= wave_read(run - mine, group);
   mine = group_sum(g0 + group, w, x, start);
   run = wave_scan(mine);
   const bool here = lane == ctz64(wave_ballot(run > target));
@@ -553,7 +531,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
         to[0] = row.edge;
         to[row.last] = behind;
       }
-      mx = fmaxf(fmaxf(mx, behind), wave_shfl(row.edge, 0));
+      mx = fmaxf(fmaxf(mx, behind), as_f32(wave_read(as_u32(row.edge), 0)));
       if (CUT && row.edge != -INFINITY) mn = fminf(mn, row.edge);
     }
     if (CUT) mn = -wave_largest(-mn);
@@ -724,10 +702,10 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
       // the elements of bin b, from the parts' lists (l: of top_k's bin or the cut's); false if some did not fit
       const auto gather = [&](int l, int& count) AMOE_INLINE {
         const int mine = lane < p.parts ? work->part[lane].listed[l] : 0, before = wave_scan(mine) - mine;
-        count = wave_shfl(before + mine, 63);
+        count = (int)wave_read((uint32_t)(before + mine), 63);
         if (wave_ballot(mine > kPartList) != 0 || count > kBins<NT>) return false;
         for (int j = wave; j < p.parts; j += W) {
-          const int m = wave_shfl(mine, j), to = wave_shfl(before, j);
+          const int m = (int)wave_read((uint32_t)mine, j), to = (int)wave_read((uint32_t)before, j);
           for (int i = lane; i < m; i += 64) ranked.list[to + i] = work->part[j].list[l][i];
         }
         __syncthreads();
