@@ -241,7 +241,9 @@ struct SharedPlans {
 SharedPlans shared_plans(const amoe_shared_attn_args* a, bool whole) {
   const int64_t rows = a->H / a->G * a->S, copies = a->B / a->prefixes;
   const size_t es = esize((int)a->dtype);
-  return {shared_plan(copies * rows, a->prefixes * a->G, a->P, whole, es), shared_plan(rows, a->B * a->G, a->T, whole, es)};
+  SharedPlans p{shared_plan(copies * rows, a->prefixes * a->G, a->P, whole, es), shared_plan(rows, a->B * a->G, a->T, whole, es)};
+  if (p.own.rw) p.own.rw = p.prefix.rw = 4;
+  return p;
 }
 
 size_t shared_bytes(const amoe_shared_attn_args* a, int parts) {

@@ -2,6 +2,7 @@
 // row; a row that sees no key gives zeros.
 #pragma once
 #include "attn_tile.h"
+#include "wave_ops.h"
 
 namespace amoe {
 
@@ -279,16 +280,15 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
 // memory: 48 sequences over caches of 4096 to 8192, 16 over 4 heads of 128, bf16: 133 us for 604 MB (4.5 TB/s, a large copy
 // reaches 5.1); one over 131071 keys, 16 over 2 heads, fp16: 24 us for 134 MB (5.6 TB/s, part of it from the cache behind the
 // L2), and 5 us for the join.
+//
+// LDS: two halves, of two waves each.
+template <int DP> inline constexpr int kAttnSplitHalf = 2 * 32 * (DP + 4) * 4;
 template <typename T, int DP, bool EDGE>
-__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_split_kernel(AttnParams p) {
+__device__ __forceinline__ void attn_split_body(const AttnParams& p, int id, char* lds_lo, char* lds_hi, float (*lds_m)[32], float (*lds_l)[32]) {
   using Tile = AttnTile<T, DP>;
   constexpr int NK = DP / 16, kRowF = DP + 4;     // floats between joined rows
-  constexpr int kTileBytes = 4 * 32 * DP * (int)sizeof(T), kJoinBytes = 4 * 32 * kRowF * 4;
-  __shared__ __align__(16) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
-  __shared__ float lds_m[4][32], lds_l[4][32];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_uniform(tid >> 6), h = lane >> 5;
   const int rows = p.copies * p.R * p.S;
-  int id = (int)blockIdx.x;
   const int bg = id % (p.B * p.G);
   id /= p.B * p.G;
   const int split = id % p.splits, r0 = (id / p.splits) * 32;
@@ -307,12 +307,13 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
 
   const T* kb = static_cast<const T*>(p.k.p) + b * p.k.sb + g * p.k.sh;
   const T* vb = static_cast<const T*>(p.v.p) + b * p.v.sb + g * p.v.sh;
-  T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
+  char* const lds = wave < 2 ? lds_lo : lds_hi;
+  T* tile = reinterpret_cast<T*>(lds) + (wave & 1) * 32 * DP;
   attn_frag<T> q[NK], kf[NK];
   const T* qrow = static_cast<const T*>(p.q.p) + (seq0 + rr / (p.R * p.S)) * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
   AttnStage<T, DP, 32, 64, EDGE, true> sv;
   sv.init(lane, p.v.ss, p.d);
-  const typename Tile::Lane at = typename Tile::Lane().in(wave * 32 * DP);
+  const typename Tile::Lane at = typename Tile::Lane().in((wave & 1) * 32 * DP);
   const auto fetch = [&](int key0) {
     attn_row_frags<T, DP, EDGE>(kf, kb, p.k.ss, key0, key_hi, p.d, p.vec);
     sv.load(lane, nullptr, vb, p.v.ss, key0, key_hi, p.d, p.vec);
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   float m = lds_m[0][lane & 31];
   for (int w = 1; w < 4; w++) m = fmaxf(m, lds_m[w][lane & 31]);
   const float f = st.m == -INFINITY ? 0.f : fast_exp2((st.m - m) * p.c);
-  float* mine = reinterpret_cast<float*>(lds) + (wave * 32 + (lane & 31)) * kRowF;
+  float* mine = reinterpret_cast<float*>(lds) + ((wave & 1) * 32 + (lane & 31)) * kRowF;
 #pragma unroll
   for (int t = 0; t < DP / 32; t++)
 #pragma unroll
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
     for (int w = 0; w < 4; w++) {
       const float mw = lds_m[w][row];
       lr += lds_l[w][row] * (mw == -INFINITY ? 0.f : fast_exp2((mw - mr) * p.c));
-      const f32x4 o = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * 32 + row) * kRowF + e);
+      const f32x4 o = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(w < 2 ? lds_lo : lds_hi) + ((w & 1) * 32 + row) * kRowF + e);
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] += o[j];
     }
@@ -397,23 +398,32 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd
   }
 }
 
+template <typename T, int DP, bool EDGE>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_fwd_split_kernel(AttnParams p) {
+  __shared__ __align__(16) char lds_lo[kAttnSplitHalf<DP>], lds_hi[kAttnSplitHalf<DP>];
+  __shared__ float lds_m[4][32], lds_l[4][32];
+  attn_split_body<T, DP, EDGE>(p, (int)blockIdx.x, lds_lo, lds_hi, lds_m, lds_l);
+}
+
 // Rows that share keys, 32 * RW of them per workgroup, and one of `splits` parts of the keys they see: as attn_fwd_rows_kernel, for
-// rows of several sequences and heads, whose results are joined with those of other parts.
-template <typename T, int DP, bool EDGE, int RW, class Shape = AttnShape<T, DP, EDGE, RW>>
-__global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Shape::kWavesPerSimd)) void attn_parts_kernel(AttnParams p) {
+// rows of several sequences and heads, whose results are joined with those of other parts.  Keys come from memory for the first
+// time here: as many tiles as LDS has room for are on their way at once.
+template <typename T, int DP, bool EDGE, int RW> struct AttnParts {
+  static constexpr int KG = 4 / RW, kRows = 32 * RW;
+  // (two blocks of keys where one is no whole number of chunks for every thread)
+  static constexpr int kBlocks = KG == 1 && sizeof(T) == 2 && DP == 96 ? 2 : 1, BN = 32 * KG * kBlocks, kTile = BN * DP * (int)sizeof(T);
+  // two workgroups on a CU
+  static constexpr int kMost = (36 << 10) / kTile, kStages = EDGE || kMost < 3 ? 2 : kMost < 4 ? kMost : 4;
+  static constexpr int kJoin = (KG - 1) * RW * DP * 32 * 4, kBytes = kStages * kTile > kJoin ? kStages * kTile : kJoin;
+};
+template <typename T, int DP, bool EDGE, int RW>
+__device__ __forceinline__ void attn_parts_body(const AttnParams& p, int id, char* lds_k, char* lds_v, float (*lds_ml)[2][64]) {
   using Tile = AttnTile<T, DP>;
-  constexpr int KG = Shape::KG, BN = Shape::kKeys, NB = Shape::kBlocks, NK = DP / 16;
-  constexpr int kElems = BN * DP, kTilesBytes = 2 * kElems * (int)sizeof(T);
-  static_assert((KG - 1) * RW * DP * 32 * 4 <= kTilesBytes, "the copies are joined in the keys' tiles");
-  __shared__ __align__(1024) char lds_k[kTilesBytes], lds_v[kTilesBytes];
-  __shared__ float lds_ml[KG][RW][2][64];
+  using Shape = AttnParts<T, DP, EDGE, RW>;
+  constexpr int KG = Shape::KG, BN = Shape::BN, NB = Shape::kBlocks, NK = DP / 16, kElems = BN * DP, kStages = Shape::kStages;
   T *const tk = reinterpret_cast<T*>(lds_k), *const tv = reinterpret_cast<T*>(lds_v);
   const int tid = threadIdx.x, lane = lane_id(), h = lane >> 5, wave = wave_uniform(tid >> 6), rw = wave % RW, kg = wave / RW;
-  // blocks of rows over the same keys next to each other's on an XCD (ids go round the eight)
   const int rows = p.copies * p.R * p.S, blocks = (rows + Shape::kRows - 1) / Shape::kRows, BG = p.B * p.G;
-  const int per_xcd = (int)gridDim.x / 8;
-  int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-  if (id >= blocks * BG * p.splits) return;
   const int r0 = id % blocks * Shape::kRows;
   id /= blocks;
   const int bg = id % BG, split = id / BG, b = bg / p.G, g = bg - b * p.G;
@@ -439,10 +449,12 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
   sv.init(tid, p.v.ss, p.d);
   typename Tile::Lane at;
   const int n_tiles = (key_hi - key_lo + BN - 1) / BN;
-  if (n_tiles > 0) {
-    sk.load(tid, tk, kb, p.k.ss, key_lo, key_hi, p.d, p.vec);
-    sv.load(tid, tv, vb, p.v.ss, key_lo, key_hi, p.d, p.vec);
-  }
+  // tile t on its way to its place (past the last one: nothing is read, but it counts as asked for)
+  const auto ask = [&](int t) __attribute__((always_inline)) {
+    const int key = key_lo + t * BN, to = t % kStages * kElems;
+    sk.load(tid, tk + to, kb, p.k.ss, key < key_hi ? key : key_hi, key_hi, p.d, p.vec);
+    sv.load(tid, tv + to, vb, p.v.ss, key < key_hi ? key : key_hi, key_hi, p.d, p.vec);
+  };
   attn_frag<T> q[NK];
   const T* qrow = static_cast<const T*>(p.q.p) + seq * p.q.sb + hd * p.q.sh + (int64_t)i * p.q.ss;
 #pragma unroll
@@ -450,17 +462,25 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
 
   AttnState<T, DP> st;
   st.clear();
-  if (n_tiles > 0) {
-    sk.store(tid, tk);
-    sv.store(tid, tv);
+  if constexpr (EDGE) {
+    if (n_tiles > 0) {
+      ask(0);
+      sk.store(tid, tk);
+      sv.store(tid, tv);
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < kStages - 1; t++) ask(t);
   }
   for (int t = 0; t < n_tiles; t++) {
-    const int cur = (t & 1) * kElems, next = kElems - cur;
-    sk.finish();
-    __syncthreads();       // tile t is there, and nobody reads the other one any more
-    if (t + 1 < n_tiles) {
-      sk.load(tid, tk + next, kb, p.k.ss, key_lo + (t + 1) * BN, key_hi, p.d, p.vec);
-      sv.load(tid, tv + next, vb, p.v.ss, key_lo + (t + 1) * BN, key_hi, p.d, p.vec);
+    const int cur = t % kStages * kElems;
+    if constexpr (EDGE) {
+      __syncthreads();     // tile t is there, and nobody reads the other one any more
+      if (t + 1 < n_tiles) ask(t + 1);
+    } else {
+      lds_dma_wait_but<(kStages - 2) * 2 * decltype(sk)::kN>();
+      __syncthreads();     // tile t is there, and nobody reads the one before any more
+      ask(t + kStages - 1);
     }
     const int key0 = key_lo + t * BN + 32 * NB * kg;
     if (key0 < wave_sees && key0 < key_hi) {
@@ -469,7 +489,7 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
       const auto load = [&](int e) -> attn_frag<T> {
         return e < NS ? Tile::row_frag(lds_k, in, 32 * (e % NB), e / NB) : Tile::col_frag(lds_v, in, 16 * ((e - NS) / NU), (e - NS) % NU);
       };
-      AttnRun<T, NS + 2 * NB * NU, kAttnThree<T, DP, EDGE, RW> ? 4 : kAttnAhead<T>> run;
+      AttnRun<T, NS + 2 * NB * NU> run;
       run.begin(load);
       f32x16 s[NB];
       attn_frag<T> pr[2 * NB];
@@ -480,24 +500,28 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
       run.steps(NS, NS + 2 * NB * NU, load,
                 [&](int e, const attn_frag<T>& a) { st.o[(e - NS) % NU] = attn_mma<T>(a, pr[(e - NS) / NU], st.o[(e - NS) % NU]); });
     }
-    if (t + 1 < n_tiles) {
-      sk.store(tid, tk + next);
-      sv.store(tid, tv + next);
+    if constexpr (EDGE) {
+      if (t + 1 < n_tiles) {
+        const int next = (t + 1) % kStages * kElems;
+        sk.store(tid, tk + next);
+        sv.store(tid, tv + next);
+      }
     }
   }
+  if constexpr (!EDGE) lds_dma_wait();     // (what was asked for past the last tile)
   float l = attn_pair_sum(st.l);
   if constexpr (KG > 1) {
     // the copies in units of the largest maximum; the first one takes the sums
     __syncthreads();
     f32x4* join = reinterpret_cast<f32x4*>(lds_k);
-    lds_ml[kg][rw][0][lane] = st.m;
-    lds_ml[kg][rw][1][lane] = l;
+    lds_ml[kg * RW + rw][0][lane] = st.m;
+    lds_ml[kg * RW + rw][1][lane] = l;
     if (kg > 0) attn_put_acc<DP>(join, (kg - 1) * RW + rw, st.o, 1.f);
     __syncthreads();
     if (kg == 0) {
       float m = st.m;
 #pragma unroll
-      for (int c = 1; c < KG; c++) m = fmaxf(m, lds_ml[c][rw][0][lane]);
+      for (int c = 1; c < KG; c++) m = fmaxf(m, lds_ml[c * RW + rw][0][lane]);
       const float own = st.m == -INFINITY ? 0.f : fast_exp2((st.m - m) * p.c);
       l *= own;
 #pragma unroll
@@ -506,8 +530,8 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
         for (int e = 0; e < 16; e++) st.o[t][e] *= own;
 #pragma unroll
       for (int c = 1; c < KG; c++) {
-        const float mc = lds_ml[c][rw][0][lane], f = mc == -INFINITY ? 0.f : fast_exp2((mc - m) * p.c);
-        l = fmaf(lds_ml[c][rw][1][lane], f, l);
+        const float mc = lds_ml[c * RW + rw][0][lane], f = mc == -INFINITY ? 0.f : fast_exp2((mc - m) * p.c);
+        l = fmaf(lds_ml[c * RW + rw][1][lane], f, l);
         attn_add_acc<DP>(join, (c - 1) * RW + rw, st.o, f);
       }
       st.m = m;
@@ -530,34 +554,69 @@ __global__ __launch_bounds__(kAttnThreads, (kAttnThree<T, DP, EDGE, RW> ? 3 : Sh
   }
 }
 
-// The parts of a row joined, a wave per row, for up to 64 of them: a lane holds a part's maximum and sum, then two elements of the row.
+// Parts of a prefix and of the sequences' own keys in one launch: the first kind waits for the matrix unit, the second for memory.
+// RWP, RWO: rows of a workgroup of either kind (32 times this; 0: attn_split_body).  Ids go round the eight XCDs; each of them
+// has its run of both kinds, next to each other what reads the same keys, the kinds mixed in proportion.
+struct AttnSharedParams {
+  AttnParams prefix, own;
+  int n_prefix, n_own;               // workgroups
+};
+template <typename T, int DP, bool EDGE, int RWP, int RWO>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 4 ? 1 : 2) void attn_shared_kernel(AttnSharedParams p) {
+  constexpr int kSplit = RWP == 0 || RWO == 0 ? kAttnSplitHalf<DP> : 0;
+  constexpr int kPrefix = RWP ? AttnParts<T, DP, EDGE, RWP ? RWP : 4>::kBytes : 0, kOwn = RWO ? AttnParts<T, DP, EDGE, RWO ? RWO : 4>::kBytes : 0;
+  constexpr int kParts = kPrefix > kOwn ? kPrefix : kOwn, kHalf = kSplit > kParts ? kSplit : kParts;
+  __shared__ __align__(1024) char lds_lo[kHalf], lds_hi[kHalf];
+  __shared__ float lds_ml[4][2][64];
+  const auto split = [&](const AttnParams& a, int id) __attribute__((always_inline)) {
+    attn_split_body<T, DP, EDGE>(a, id, lds_lo, lds_hi, reinterpret_cast<float(*)[32]>(lds_ml), reinterpret_cast<float(*)[32]>(lds_ml) + 8);
+  };
+  const int xcd = (int)(blockIdx.x % 8), slot = (int)(blockIdx.x / 8), each_p = (p.n_prefix + 7) / 8, each_o = (p.n_own + 7) / 8;
+  const int before = (int)((int64_t)slot * each_p / (each_p + each_o)), after = (int)((int64_t)(slot + 1) * each_p / (each_p + each_o));
+  if (after > before) {
+    const int id = xcd * each_p + before;
+    if (id >= p.n_prefix) return;
+    if constexpr (RWP == 0) split(p.prefix, id);
+    else attn_parts_body<T, DP, EDGE, RWP>(p.prefix, id, lds_lo, lds_hi, lds_ml);
+  } else {
+    const int id = xcd * each_o + slot - before;
+    if (id >= p.n_own) return;
+    if constexpr (RWO == 0) split(p.own, id);
+    else attn_parts_body<T, DP, EDGE, RWO>(p.own, id, lds_lo, lds_hi, lds_ml);
+  }
+}
+
+// The parts of a row joined, a wave per row, for up to 128 of them: a lane holds two parts' maxima and sums, then two elements of the
+// row.  Parts in which a row sees nothing are not read.
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_rows_kernel(AttnParams p) {
   const int64_t n = (int64_t)p.B * p.H * p.S, row0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t at = row0 < n ? row0 : n - 1;
   const int lane = lane_id(), pad = (p.d + 3) & ~3;
-  float m = -INFINITY, l = 0.f;
-  if (lane < p.splits) {
-    m = p.part_ml[2 * (lane * n + at)];
-    l = p.part_ml[2 * (lane * n + at) + 1];
+  float m[2], l[2], f[2];
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int s = lane + 64 * u;
+    m[u] = s < p.splits ? p.part_ml[2 * (s * n + at)] : -INFINITY;
+    l[u] = s < p.splits ? p.part_ml[2 * (s * n + at) + 1] : 0.f;
   }
-  float top = m;
+  const float top = wave_largest(fmaxf(m[0], m[1]));
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, wave_shfl_xor(top, x));
-  const float f = m == -INFINITY ? 0.f : fast_exp2((m - top) * p.c);
-  l *= f;
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) l += wave_shfl_xor(l, x);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int u = 0; u < 2; u++) f[u] = m[u] == -INFINITY ? 0.f : fast_exp2((m[u] - top) * p.c);
+  const float sum = lanes_sum(fmaf(l[1], f[1], l[0] * f[0])), inv = sum == 0.f ? 0.f : 1.f / sum;
   const int e = 2 * lane;
   float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int end = p.splits - 64 * u < 64 ? p.splits - 64 * u : 64;
 #pragma unroll 8
-  for (int s = 0; s < p.splits; s++) {
-    const float fs = as_f32(wave_read(as_u32(f), s));
-    if (e < p.d) {
-      const float* po = p.part_o + (s * n + at) * pad + e;
-      a = fmaf(po[0], fs, a);
-      b = fmaf(po[1], fs, b);
+    for (int s = 0; s < end; s++) {
+      const float fs = as_f32(wave_read(as_u32(f[u]), s));
+      if (fs != 0.f && e < p.d) {
+        const float* po = p.part_o + ((s + 64 * u) * n + at) * pad + e;
+        a = fmaf(po[0], fs, a);
+        b = fmaf(po[1], fs, b);
+      }
     }
   }
   const int64_t bh = at / p.S, i = at - bh * p.S, seq = bh / p.H, hd = bh - seq * p.H;

@@ -15,7 +15,7 @@ int launch_attn_fwd_f16(const AttnParams& p, hipStream_t st);
 // rows that share `prefix` and have keys of their own in `own`: parts of both, and all of them joined
 struct AttnShared {
   AttnParams prefix, own, join;
-  int prefix_rw, own_rw;             // waves over the rows of a workgroup; 0: attn_fwd_split_kernel
+  int prefix_rw, own_rw;             // waves over the rows of a workgroup (prefix 4, 2; own 4, then prefix 4 too); 0: attn_split_body
 };
 int launch_attn_shared_f32(const AttnShared& s, hipStream_t st);
 int launch_attn_shared_bf16(const AttnShared& s, hipStream_t st);

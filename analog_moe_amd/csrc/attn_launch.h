@@ -75,49 +75,39 @@ int launch_attn_fwd(const AttnParams& p, hipStream_t st) {
   return rc;
 }
 
-template <typename T, int DP, bool EDGE>
-int launch_attn_parts_of(const AttnParams& p, int rw, hipStream_t st) {
-  const int64_t blocks = ((int64_t)p.copies * p.R * p.S + 32 * rw - 1) / (32 * rw);
-  const dim3 grid((unsigned)((p.B * p.G * blocks * p.splits + 7) / 8 * 8));
-  if constexpr (!EDGE && sizeof(T) == 2) {
-    if (rw == 2) {
-      hipLaunchKernelGGL((&attn_parts_kernel<T, DP, EDGE, 2>), grid, dim3(kAttnThreads), 0, st, p);
-      return launch_rc();
-    }
-  }
-  if (rw != 4) return AMOE_EUNSUPPORTED;
-  hipLaunchKernelGGL((&attn_parts_kernel<T, DP, EDGE, 4>), grid, dim3(kAttnThreads), 0, st, p);
-  return launch_rc();
+inline int64_t attn_parts_groups(const AttnParams& p, int rw) {
+  const int64_t block = rw ? 32 * rw : 32;
+  return (int64_t)p.B * p.G * (((int64_t)p.copies * p.R * p.S + block - 1) / block) * p.splits;
 }
 
-// The parts of one set of keys.
-template <typename T>
-int launch_attn_parts(const AttnParams& p, int rw, hipStream_t st) {
-  int rc = AMOE_OK;
-  if (rw > 0) {
-#define AMOE_LAUNCH(TYPE, DP, EDGE) rc = launch_attn_parts_of<TYPE, DP, EDGE>(p, rw, st)
-    AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
-#undef AMOE_LAUNCH
-    return rc;
+template <typename T, int DP, bool EDGE>
+int launch_attn_shared_of(const AttnShared& s, hipStream_t st) {
+  AttnSharedParams p{s.prefix, s.own, (int)attn_parts_groups(s.prefix, s.prefix_rw), (int)attn_parts_groups(s.own, s.own_rw)};
+  const dim3 grid((unsigned)(8 * ((p.n_prefix + 7) / 8 + (p.n_own + 7) / 8))), block(kAttnThreads);
+  if (s.own_rw == 4) {
+    hipLaunchKernelGGL((&attn_shared_kernel<T, DP, EDGE, 4, 4>), grid, block, 0, st, p);
+  } else if (s.prefix_rw == 4) {
+    hipLaunchKernelGGL((&attn_shared_kernel<T, DP, EDGE, 4, 0>), grid, block, 0, st, p);
+  } else if (s.prefix_rw == 0) {
+    hipLaunchKernelGGL((&attn_shared_kernel<T, DP, EDGE, 0, 0>), grid, block, 0, st, p);
+  } else if constexpr (!EDGE && sizeof(T) == 2) {
+    hipLaunchKernelGGL((&attn_shared_kernel<T, DP, EDGE, 2, 0>), grid, block, 0, st, p);
   }
-  const dim3 grid((unsigned)((int64_t)p.B * p.G * p.splits * (((int64_t)p.copies * p.R * p.S + 31) / 32)));
-#define AMOE_LAUNCH(TYPE, DP, EDGE) hipLaunchKernelGGL((&attn_fwd_split_kernel<TYPE, DP, EDGE>), grid, dim3(kAttnThreads), 0, st, p)
-  AMOE_ATTN_SIZES(AMOE_LAUNCH, T, p);
-#undef AMOE_LAUNCH
   return launch_rc();
 }
 
 template <typename T>
 int launch_attn_shared(const AttnShared& s, hipStream_t st) {
-  if (s.prefix.splits > 0) {
-    if (int rc = launch_attn_parts<T>(s.prefix, s.prefix_rw, st)) return rc;
-  }
-  if (s.own.splits > 0) {
-    if (int rc = launch_attn_parts<T>(s.own, s.own_rw, st)) return rc;
+  if (s.join.splits > 0) {
+    int rc = AMOE_OK;
+#define AMOE_LAUNCH(TYPE, DP, EDGE) rc = launch_attn_shared_of<TYPE, DP, EDGE>(s, st)
+    AMOE_ATTN_SIZES(AMOE_LAUNCH, T, s.own);
+#undef AMOE_LAUNCH
+    if (rc) return rc;
   }
   const int64_t rows = (int64_t)s.join.B * s.join.H * s.join.S;
   const dim3 block(kAttnThreads);
-  if (s.join.splits <= 64) hipLaunchKernelGGL((&attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, s.join);
+  if (s.join.splits <= 128) hipLaunchKernelGGL((&attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, s.join);
   else hipLaunchKernelGGL((&attn_join_kernel<T>), dim3((unsigned)rows), block, 0, st, s.join);
   return launch_rc();
 }

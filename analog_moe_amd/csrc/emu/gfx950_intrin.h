@@ -32,6 +32,15 @@ inline void lds_dma_wait() {
   }
   emu_lds_copies.clear();
 }
+template <int N> inline void lds_dma_wait_but() {
+  const size_t n = emu_lds_copies.size() > N ? emu_lds_copies.size() - N : 0;
+  for (size_t i = 0; i < n; i++) {
+    const EmuLdsCopy& c = emu_lds_copies[i];
+    if (c.from) std::memcpy(c.to, c.from, 16);
+    else std::memset(c.to, 0, 16);
+  }
+  emu_lds_copies.erase(emu_lds_copies.begin(), emu_lds_copies.begin() + n);
+}
 inline uint32_t buffer_load_b32(BufRsrc r, uint32_t lane_off, uint32_t uniform_off = 0) {
   uint32_t v;
   std::memcpy(&v, r.base + (size_t)lane_off + (size_t)uniform_off, 4);

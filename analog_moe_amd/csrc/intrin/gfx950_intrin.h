@@ -84,6 +84,11 @@ __device__ __forceinline__ void buffer_to_lds_b128(BufRsrc r, void* lds, uint32_
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(uintptr_t)to, 16, lane_off, 0, 0, 0);
 }
 __device__ __forceinline__ void lds_dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
+// ... all but the last N that this wave asked for (and no other loads of it are on their way)
+template <int N> __device__ __forceinline__ void lds_dma_wait_but() {
+  static_assert(N >= 0 && N < 16, "four bits of the counter");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
+}
 // Resource over [base, base + bytes): an access at a byte offset >= bytes is out of range; out-of-range stores are
 // dropped by the hardware, which makes a store conditional without a branch around it, and out-of-range loads read zeros.
 __device__ __forceinline__ BufRsrc make_rsrc_sized(void* base, uint32_t bytes) {
