@@ -217,7 +217,10 @@ struct SharedPlan {
   int rw = 0, splits = 0;
 };
 
-// Waves over the rows and parts of the keys, for `rows` rows that share a key head in each of `heads` of them and T keys.
+// Waves over the rows and parts of the keys, for `rows` rows that share a key head in each of `heads` of them and T keys.  Workgroups
+// of many rows: one on a CU, where it leaves room for one of few rows, which waits for memory meanwhile (64 sequences over 30001
+// shared and 1024 own keys, 16 over 4 heads of 128: 46 us, with two on a CU 64; of 64: 36 and 42; four prefixes of 8192, 64 sequences
+// each, 32 over 8 heads: 127 and 147), parts of 256 keys or more.  Of few rows: as attn_splits.
 SharedPlan shared_plan(int64_t rows, int64_t heads, int64_t T, bool whole, size_t es) {
   SharedPlan p;
   if (T == 0) return p;
@@ -228,7 +231,7 @@ SharedPlan shared_plan(int64_t rows, int64_t heads, int64_t T, bool whole, size_
     const int64_t n = (per_cu * cus + groups - 1) / groups, most = (T + keys - 1) / keys;
     return n < most ? n : most;
   };
-  int64_t n = p.rw ? parts(2, 256) : parts(8, 512);
+  int64_t n = p.rw ? parts(1, 256) : parts(8, 512);
   const int64_t few = parts(2, 128);
   if (!p.rw && few > n) n = few;
   p.splits = (int)(n < 1 ? 1 : n > kAttnMaxSplits / 2 ? kAttnMaxSplits / 2 : n);

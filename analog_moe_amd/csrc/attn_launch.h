@@ -107,8 +107,10 @@ int launch_attn_shared(const AttnShared& s, hipStream_t st) {
   }
   const int64_t rows = (int64_t)s.join.B * s.join.H * s.join.S;
   const dim3 block(kAttnThreads);
-  if (s.join.splits <= 128) hipLaunchKernelGGL((&attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, s.join);
-  else hipLaunchKernelGGL((&attn_join_kernel<T>), dim3((unsigned)rows), block, 0, st, s.join);
+  // (all four waves of a workgroup at one row where rows alone would not give every SIMD two waves)
+  if (s.join.splits > 128) hipLaunchKernelGGL((&attn_join_kernel<T>), dim3((unsigned)rows), block, 0, st, s.join);
+  else if (rows < 8 * num_compute_units()) hipLaunchKernelGGL((&attn_join_rows_kernel<T, 4>), dim3((unsigned)rows), block, 0, st, s.join);
+  else hipLaunchKernelGGL((&attn_join_rows_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, s.join);
   return launch_rc();
 }
 
