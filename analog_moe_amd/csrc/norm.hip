@@ -179,30 +179,58 @@ __global__ __launch_bounds__(kNormBwdThreads<NT>) void norm_bwd_kernel(NormParam
   constexpr int BT = kNormBwdThreads<NT>, C = Elem<T>::kChunk, groups = BT / NT, cols = NT * PER * C;
   __shared__ float lds[2][2][16];
   __shared__ __align__(16) float lds_w[groups > 1 ? groups : 1][groups > 1 ? cols : 4];
+  // Rows that all threads work on leave no registers for the weights, which come from the cache every time, and few for what comes
+  // next: their sums are kept in LDS, where there is room, by the thread that has the columns, and the next row is asked for before
+  // the sums of this one (2048 rows of 16384, bf16: 84 us, 3.2 TB/s).
+  constexpr bool kHeld = NT <= 256 && PER <= 2, kInLds = NT == 1024 && 2 * cols * 4 <= 128 << 10, kAhead = NT == 1024 && PER <= 2;
+  __shared__ __align__(16) float lds_sums[kInLds ? 2 : 1][kInLds ? cols : 4];
   const int t = threadIdx.x % NT, g = threadIdx.x / NT;
-  float w[PER][C], dw[PER][C], db[PER][C];
+  float w[kHeld ? PER : 1][C], dw[kInLds ? 1 : PER][C], db[kInLds ? 1 : PER][C];
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    norm_weight<T, VEC>(p.w, p.w_f32, t + j * NT, p.D, 1.f, w[j]);
+    if constexpr (kHeld) norm_weight<T, VEC>(p.w, p.w_f32, t + j * NT, p.D, 1.f, w[j]);
 #pragma unroll
-    for (int e = 0; e < C; e++) dw[j][e] = db[j][e] = 0.f;
+    for (int e = 0; e < C; e++) {
+      dw[kInLds ? 0 : j][e] = db[kInLds ? 0 : j][e] = 0.f;
+      if constexpr (kInLds) lds_sums[0][(t + j * NT) * C + e] = lds_sums[1][(t + j * NT) * C + e] = 0.f;
+    }
   }
+  Raw rx[PER], rg[PER], rs[PER], nx[kAhead ? PER : 1], ng[kAhead ? PER : 1], ns[kAhead ? PER : 1];
+  const auto ask = [&](int64_t r0, Raw (&x)[kAhead ? PER : 1], Raw (&gy)[kAhead ? PER : 1], Raw (&gs)[kAhead ? PER : 1]) __attribute__((always_inline)) {
+    const int64_t row = r0 + g < p.rows ? r0 + g : p.rows - 1;
+#pragma unroll
+    for (int j = 0; j < (kAhead ? PER : 1); j++) {
+      x[j] = norm_load<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx, t + j * NT, p.D);
+      gy[j] = norm_load<T, VEC>(static_cast<const T*>(p.gy) + row * p.ldgy, t + j * NT, p.D);
+      gs[j] = p.gs ? norm_load<T, VEC>(static_cast<const T*>(p.gs) + row * p.ldgs, t + j * NT, p.D) : raw_zero();
+    }
+  };
+  if constexpr (kAhead) ask((int64_t)blockIdx.x * groups, nx, ng, ns);
   const float per_row = 1.f / (float)p.D;
   int turn = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < p.rows; r0 += (int64_t)gridDim.x * groups) {
     const bool ok = r0 + g < p.rows;
     const int64_t row = ok ? r0 + g : p.rows - 1;
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* gy = static_cast<const T*>(p.gy) + row * p.ldgy;
-    Raw rx[PER], rg[PER], rs[PER];
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-      rx[j] = norm_load<T, VEC>(x, t + j * NT, p.D);
-      rg[j] = ok ? norm_load<T, VEC>(gy, t + j * NT, p.D) : raw_zero();
-    }
-    if (p.gs) {
+      for (int j = 0; j < PER; j++) {
+        rx[j] = nx[j];
+        rg[j] = ng[j];
+        rs[j] = ns[j];
+      }
+      if (r0 + (int64_t)gridDim.x * groups < p.rows) ask(r0 + (int64_t)gridDim.x * groups, nx, ng, ns);
+    } else {
+      const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+      const T* gy = static_cast<const T*>(p.gy) + row * p.ldgy;
 #pragma unroll
-      for (int j = 0; j < PER; j++) rs[j] = norm_load<T, VEC>(static_cast<const T*>(p.gs) + row * p.ldgs, t + j * NT, p.D);
+      for (int j = 0; j < PER; j++) {
+        rx[j] = norm_load<T, VEC>(x, t + j * NT, p.D);
+        rg[j] = ok ? norm_load<T, VEC>(gy, t + j * NT, p.D) : raw_zero();
+      }
+      if (p.gs) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) rs[j] = norm_load<T, VEC>(static_cast<const T*>(p.gs) + row * p.ldgs, t + j * NT, p.D);
+      }
     }
     const float mean = p.stats[kNormStats * row], off = p.stats[kNormStats * row + 1], inv = p.stats[kNormStats * row + 2];
     float h[PER][C], a[PER][C], s1 = 0.f, s2 = 0.f;
@@ -210,15 +238,36 @@ __global__ __launch_bounds__(kNormBwdThreads<NT>) void norm_bwd_kernel(NormParam
     for (int j = 0; j < PER; j++) {
       raw_unpack<T>(rx[j], h[j]);
       raw_unpack<T>(rg[j], a[j]);
+      float (&wj)[C] = w[kHeld ? j : 0];
+      if constexpr (!kHeld) norm_weight<T, VEC>(p.w, p.w_f32, t + j * NT, p.D, 1.f, wj);
+      float (&dwj)[C] = dw[kInLds ? 0 : j], (&dbj)[C] = db[kInLds ? 0 : j];
+      if constexpr (kInLds) {
+#pragma unroll
+        for (int e = 0; e < C; e += 4) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&lds_sums[0][(t + j * NT) * C + e]), y = *reinterpret_cast<const f32x4*>(&lds_sums[1][(t + j * NT) * C + e]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            dwj[e + i] = x[i];
+            dbj[e + i] = y[i];
+          }
+        }
+      }
 #pragma unroll
       for (int e = 0; e < C; e++) {
         // (columns past D: their gradients are zeros, and so is what they add)
         h[j][e] = ((h[j][e] - mean) - off) * inv;
-        dw[j][e] = fmaf(a[j][e], h[j][e], dw[j][e]);
-        db[j][e] += a[j][e];
-        a[j][e] *= w[j][e];
+        dwj[e] = fmaf(a[j][e], h[j][e], dwj[e]);
+        dbj[e] += a[j][e];
+        a[j][e] *= wj[e];
         s1 += a[j][e];
         s2 = fmaf(a[j][e], h[j][e], s2);
+      }
+      if constexpr (kInLds) {
+#pragma unroll
+        for (int e = 0; e < C; e += 4) {
+          *reinterpret_cast<f32x4*>(&lds_sums[0][(t + j * NT) * C + e]) = f32x4{dwj[e], dwj[e + 1], dwj[e + 2], dwj[e + 3]};
+          *reinterpret_cast<f32x4*>(&lds_sums[1][(t + j * NT) * C + e]) = f32x4{dbj[e], dbj[e + 1], dbj[e + 2], dbj[e + 3]};
+        }
       }
     }
     norm_sum2<NT>(s1, s2, lds, turn);
@@ -246,7 +295,10 @@ __global__ __launch_bounds__(kNormBwdThreads<NT>) void norm_bwd_kernel(NormParam
       for (int j = 0; j < PER; j++)
 #pragma unroll
         for (int e = 0; e < C; e++)
-          if ((t + j * NT) * C + e < p.D) part[(t + j * NT) * C + e] = which ? db[j][e] : dw[j][e];
+          if ((t + j * NT) * C + e < p.D) {
+            if constexpr (kInLds) part[(t + j * NT) * C + e] = lds_sums[which][(t + j * NT) * C + e];
+            else part[(t + j * NT) * C + e] = which ? db[j][e] : dw[j][e];
+          }
     } else {
       if (which) __syncthreads();
 #pragma unroll
@@ -330,10 +382,11 @@ int launch_norm_fwd(const NormParams& p, bool vec, hipStream_t st) {
   return launch_rc();
 }
 
-// Workgroups of the backward pass: two on a CU, or fewer where a group of threads would not get four rows
+// Workgroups of the backward pass: as many as are on the CUs at once, or fewer, so that a group of threads gets four rows and a
+// workgroup eight: each leaves 8 D bytes of sums, which a row's 8 D (16 bits, with the stream's gradient) are the measure of.
 int64_t norm_bwd_groups(const amoe_norm_args* a) {
   const int nt = norm_row_threads(norm_form(a->D, a->dtype == AMOE_F32 ? 4 : 8)), groups = (nt <= 256 ? 512 : nt) / nt;
-  const int64_t want = (a->rows + 4 * groups - 1) / (4 * groups), most = 2 * num_compute_units();
+  const int64_t rows = groups >= 2 ? 4 * groups : 8, want = (a->rows + rows - 1) / rows, most = (nt == 1024 ? 1 : 2) * num_compute_units();
   return want < most ? want : most;
 }
 
@@ -357,7 +410,10 @@ int norm_check(const amoe_norm_args* a) {
   if (a->dtype != AMOE_F32 && a->dtype != AMOE_BF16 && a->dtype != AMOE_F16) return AMOE_EINVAL;
   if (a->weight_dtype != a->dtype && a->weight_dtype != AMOE_F32) return AMOE_EINVAL;
   if (a->rows < 0 || a->D < 1 || !(a->eps >= 0) || !(a->eps <= 3e38)) return AMOE_EINVAL;
-  return a->D > kNormMaxD || a->rows >= INT64_C(1) << 31 ? AMOE_EUNSUPPORTED : AMOE_OK;
+  // (threads of a launch are counted in 32 bits)
+  if (a->D > kNormMaxD || a->rows >= INT64_C(1) << 31) return AMOE_EUNSUPPORTED;
+  const int64_t nt = norm_row_threads(norm_form(a->D, a->dtype == AMOE_F32 ? 4 : 8));
+  return a->rows * nt >= INT64_C(1) << 32 ? AMOE_EUNSUPPORTED : AMOE_OK;
 }
 
 // A tensor of rows: there, aligned to its elements; whole 16-byte chunks leave vec as it is.

@@ -288,7 +288,7 @@ def test_library_refuses(emu_ops):
     assert call() == 0 and call("bwd") == 0 and call(rows=0, x=0) == 0
     for k in (dict(dtype=3), dict(wdtype=1), dict(rows=-1), dict(D=0), dict(eps=-1.0), dict(eps=float("nan")), dict(ldx=-1)):
         assert call(**k) == -1, k
-    assert call(D=32769) == call(rows=1 << 31) == -6
+    assert call(D=32769) == call(rows=1 << 31) == call(rows=1 << 28) == call(rows=1 << 26, D=512, ldx=512) == call(rows=1 << 22, D=20000, ldx=20000) == -6
     assert call(x=0) == call(y=0) == call(r=p) == call(s=p) == -2 and call("bwd", gy=0) == call("bwd", stats=0) == -2
     assert call(x=p + 2) == call(w=w.data_ptr() + 1) == call(stats=stats.data_ptr() + 2) == -4
     dw = torch.zeros(16)

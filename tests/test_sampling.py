@@ -295,6 +295,21 @@ def test_library_refuses(emu_ops):
     assert lib.amoe_sample(None, None, 0, None) == -2
 
 
+@pytest.mark.gpu
+def test_gpu_library_refuses_a_small_workspace():
+    """(rows in parts: refused on the host, nothing is launched)"""
+    from analog_moe_amd import _abi, ops
+    lib = ops.get_lib()
+    x, u, ids = torch.zeros(2, 50000, device="cuda"), torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    args = _abi.SAMPLE_ARGS.pack(0, 2, 50000, x.data_ptr(), 50000, u.data_ptr(), 0, 0, 0, 0, 0, 0, 1.0, 0.9, 0.0, 0, ids.data_ptr(), 0)
+    need = lib.amoe_sample_workspace(args)
+    ws = torch.empty(need + 8, dtype=torch.uint8, device="cuda")
+    assert need > 0 and need % 8 == 0
+    assert lib.amoe_sample(args, None, 0, None) == -2
+    assert lib.amoe_sample(args, ws.data_ptr(), need - 1, None) == -5
+    assert lib.amoe_sample(args, ws.data_ptr() + 4, need, None) == -4
+
+
 def test_operator_on_meta():
     ids, lp = torch.ops.amoe.sample(torch.empty(3, 5, 16, device="meta"), torch.empty(3, 5, device="meta"), None, None, None, None, 1.0, 0, 1.0, 0.0)
     assert ids.shape == lp.shape == (3, 5) and ids.dtype == torch.int64
