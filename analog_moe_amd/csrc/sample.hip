@@ -9,8 +9,12 @@
 // within 2^-44 of the largest weight.  (In fp32 a row of 10^5 logits would go to a neighbour about once in a thousand draws.)
 // What weighs less than 2^-45 of the largest is never drawn.
 //
-// The cut that top_k and top_p make in the ranking is found without a sort: tokens are counted, or weighed, by their weight's binary
-// logarithm in up to 2047 bins, and only those of the bin with the cut are ranked.
+// The cut that top_k and top_p make in the ranking is found without a sort: tokens are counted, or weighed, by their
+// distance from the largest in up to 2047 bins, and only those of the bin with the cut are ranked.
+//
+// Rows pass three times (their extremes, the bins, the sums), four where both cuts are made, from the caches behind the first.  Bound by
+// the weights' arithmetic (13 operations in 64 bits, at half rate: 256 rows of 130001 fp32 logits 27 us for the largest alone, which is
+// the reading; 56 with one pass of weights; 107 with top_p, 139 with top_k too) and the bins' LDS atomics (2048 rows of 8000: 31 and 68).
 #include <amoe.h>
 
 #include "host_util.h"
@@ -870,13 +874,18 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
 
 namespace {
 
-// Parts that a row is worked on in, 1: all in one launch.
+// Parts that a row is worked on in, 1: all in one launch: as many as there are CUs for, of 4096 elements or more, if they are four.
+// Measured (us, one launch / parts, fp32 or bf16): 8 rows of 130001 with top_p 91 / 40, without a cut 40 / 18, the largest of each
+// 14 / 18; 64 of 50001 54 / 44, 24 / 18, 11 / 18 (what is launched may not depend on what the temperatures are).
 int sample_parts(const amoe_sample_args* a) {
   const int64_t most = num_compute_units() / (a->rows < 1 ? 1 : a->rows), n = a->V / 4096;
   const int64_t parts = n < most ? n : most;
   return (int)(parts < 4 ? 1 : parts > kMaxParts ? kMaxParts : parts);
 }
 
+// 256 threads for short rows, and for longer ones where there are more of them than CUs; not past 32768, where too many tokens would
+// share one of their bins, a quarter as many.  Measured (us, 256 / 1024 threads, top_p 0.95, bf16): 64 rows of 2000 13.6 / 15.3; 1 of 8000 20.1 / 17.8,
+// 100 22.1 / 19.1, 300 25.2 / 34.7, 2048 67 / 145; 512 of 16000 39 / 51; 512 of 32000 67 / 69, 2048 179 / 268.
 template <typename T, bool CUT>
 int launch_sample_cut(const SampleParams& p, bool both, hipStream_t st) {
   const dim3 grid((unsigned)p.rows), parts((unsigned)(p.rows * p.parts)), block(1024);
@@ -888,10 +897,10 @@ int launch_sample_cut(const SampleParams& p, bool both, hipStream_t st) {
     }
     hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kSums>), parts, block, 0, st, p);
     hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kFinish>), grid, block, 0, st, p);
-  } else if (p.V > 16384 || p.rows < 2 * num_compute_units()) {
-    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kAll>), grid, block, 0, st, p);
-  } else {
+  } else if (p.V <= 4096 || (p.rows > num_compute_units() && p.V <= 32768)) {
     hipLaunchKernelGGL((&sample_kernel<T, 256, CUT, kAll>), grid, dim3(256), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((&sample_kernel<T, 1024, CUT, kAll>), grid, block, 0, st, p);
   }
   return launch_rc();
 }

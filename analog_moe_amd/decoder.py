@@ -124,17 +124,21 @@ class DecoderBlock(nn.Module):
         self.ln_ffn = norm(d_model)
         self.ffn = ffn
 
-    def forward(self, x: Tensor, **attn_args) -> Tuple[Tensor, Tensor]:
+    @property
+    def sums(self) -> bool:
+        """Whether its norms form the sums with the residual stream."""
+        return isinstance(self.ln_attn, LayerNorm) and isinstance(self.ln_ffn, LayerNorm)
+
+    def forward(self, x: Tensor, add: Optional[Tensor] = None, split: bool = False, **attn_args):
+        """(stream, regularisation); split, with norms that form the sums: on the stream x + add (None: x), and (stream, what is to be
+        added to it, regularisation)."""
+        if split:
+            n, x = (self.ln_attn(x), x) if add is None else self.ln_attn(add, x)
+            n, x = self.ln_ffn(self.attn(n, **attn_args), x)
+            return x, *self.ffn(n)
         x = x + self.attn(self.ln_attn(x), **attn_args)
         y, reg = self.ffn(self.ln_ffn(x))
         return x + y, reg
-
-    def summed(self, x: Tensor, add: Optional[Tensor], **attn_args) -> Tuple[Tensor, Tensor, Tensor]:
-        """The block on the stream x + add, with norms that form the sums: (stream, what is to be added to it, regularisation)."""
-        n, x = (self.ln_attn(x), x) if add is None else self.ln_attn(add, x)
-        n, x = self.ln_ffn(self.attn(n, **attn_args), x)
-        y, reg = self.ffn(n)
-        return x, y, reg
 
 
 class SigmaMoEDecoder(nn.Module):
@@ -198,12 +202,12 @@ class SigmaMoEDecoder(nn.Module):
                 before = cache.prefix.held.repeat_interleave(B // cache.prefix.held.shape[0], output_size=B)
                 args.update(places=args["positions"], positions=args["positions"] + before[:, None])
         reg = x.new_zeros((), dtype=torch.float32)
-        summed, add = isinstance(self.ln_out, LayerNorm), None
+        split, add = isinstance(self.ln_out, LayerNorm) and all(blk.sums for blk in self.blocks), None
         for i, blk in enumerate(self.blocks):
             if cache is not None:
                 args["layer"] = i
-            if summed:
-                x, add, r = blk.summed(x, add, **args)
+            if split:
+                x, add, r = blk(x, add, True, **args)
             else:
                 x, r = blk(x, **args)
             reg = reg + r.float()

@@ -61,6 +61,22 @@ def test_stock_attention_with_these_norms(emu_ops):
     assert [n for n, _ in m.named_parameters()] == [n for n, _ in like.named_parameters()]
 
 
+def test_norms_of_two_kinds_and_hooks(emu_ops):
+    """A norm that is replaced takes the sums back, and what is hooked onto a block runs."""
+    m, like = same_model(LayerNorm)
+    ids, runs = torch.randint(0, 31, (2, 5), generator=torch.Generator().manual_seed(1)), []
+    for blk in m.blocks:
+        blk.register_forward_hook(lambda *_: runs.append(1))
+    with torch.no_grad():
+        want = like(ids)[0]
+        for name in (None, "ln_out", "ln_attn"):
+            if name is not None:
+                owner = m if name == "ln_out" else m.blocks[1]
+                setattr(owner, name, getattr(like if name == "ln_out" else like.blocks[1], name))
+            assert (m(ids)[0] - want).abs().max() <= 2.0 ** -15 * want.abs().max()
+    assert len(runs) == 6
+
+
 def check_shared(m, ids, prompts, copies, tol, device="cpu"):
     """Prompts [N, S] of the given lengths, then the tokens ids [N * copies, steps] one by one over a cache that shares the prompts:
     the logits of the whole sequences at once.  Then two at once, and the prompts' own cache goes on."""

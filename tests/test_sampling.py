@@ -321,6 +321,8 @@ GPU_CASES = dict(CASES, **{
     "many_p": (700, 3001, "bf16", "normal", "odd", dict(top_p=0.9, temperature=0.8)),
     "many_k": (600, 5003, "f16", "normal", "every", dict(top_k=50)),
     "many_all": (513, 16384, "bf16", "normal", "own", dict(top_k=2000, top_p=0.95, min_p=0.001)),
+    "many_long": (300, 32768, "bf16", "normal", "own", dict(top_k=9000, top_p=0.99)),
+    "many_equal": (257, 30001, "f16", "equal", "own", dict(top_k=20000, top_p=0.9)),
     "large_f32": (9, 130001, "f32", "normal", "own", dict(top_k=60000, top_p=0.95, temperature=1.2)),
     "large_bf16": (5, 50001, "bf16", "normal", "own", dict(top_p=0.99)),
     "large_masked": (5, 50001, "f16", "masked", "odd", dict(top_p=0.9, min_p=0.01)),
