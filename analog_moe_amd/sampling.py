@@ -54,6 +54,8 @@ def draw(logits: Tensor, u: Tensor, temperature: Setting = 1.0, top_k: Union[int
     k, kp, k_all = _setting(top_k, shape, device, "top_k", _INT, 0, 2 ** 63 - 1)
     p, pp, p_all = _setting(top_p, shape, device, "top_p", _F32, 0.0, 1.0)
     m, mp, m_all = _setting(min_p, shape, device, "min_p", _F32, 0.0, 1.0)
+    if not hasattr(k_all, "__index__"):
+        raise TypeError(f"top_k must be an integer, not {k_all}")
     rows = ops._rows2d(logits)
     n = rows.shape[0]
     ids = torch.empty(shape, dtype=torch.int64, device=device)

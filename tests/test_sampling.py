@@ -263,7 +263,7 @@ def test_refusals(emu_ops):
                 dict(top_k=torch.ones((), dtype=torch.int64))):
         with pytest.raises(ValueError):
             S.sample(x, u, **bad)
-    for bad in (dict(temperature=torch.ones(3, dtype=torch.float64)), dict(top_k=torch.ones(3)), dict(min_p=torch.ones(3, dtype=torch.float16))):
+    for bad in (dict(temperature=torch.ones(3, dtype=torch.float64)), dict(top_k=torch.ones(3)), dict(top_k=2.5), dict(min_p=torch.ones(3, dtype=torch.float16))):
         with pytest.raises(TypeError):
             S.sample(x, u, **bad)
     for bad in ((x, u[:2]), (x, u[:, None]), (torch.zeros(3, 0), u), (torch.zeros(1, 1 << 20), u[:1]), (torch.tensor(1.0), u[0])):
