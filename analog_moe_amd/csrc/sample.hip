@@ -311,7 +311,7 @@ __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int coun
   __syncthreads();
 }
 
-// The same for one bin of the row, whatever number of elements (`count`) it has.
+// The same for one bin of the row, whatever number of elements (`count`) it has.  What is ranked is what was listed.
 template <typename T, int NT, class Bin>
 __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, const SampleWeight& weight, Bin bin, int b, int count,
                                               bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked<NT>& r,
@@ -374,7 +374,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
       none);
   if (tid < 64) list_one(row.edge, row.edge_index);
   __syncthreads();
-  sample_sort<NT>(weight, count, by_weight, target, before_n, before_w, r, sh);
+  sample_sort<NT>(weight, sh.listed, by_weight, target, before_n, before_w, r, sh);
 }
 
 // The element at which the sum of weights passes `target`, from the units' sums: weigh(value, index).  True for the thread that has
@@ -647,7 +647,10 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
       float reach = fminf(fmaf(-0.5f, mn, half), 16.25f * temperature);
       if (!by_k) reach = fminf(reach, 0.3466f * temperature * (fast_log2((float)p.V) - fast_log2(1.f - fmaxf(top_p, 0.f)) + 1.f));
       const float step = reach > 0.f ? fminf((kBins<NT> - 2) / reach, 3.402823466e38f) : 0.f;
-      const auto bin = [=](float x) AMOE_INLINE { return (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins<NT> - 1)); };
+      // (What weighs nothing is in the last bin by itself: where the largest is all there is, or the distances are subnormal, its distance
+      // says no such thing, and what a row is padded with would count as tokens.)
+      const float low = weight.low;
+      const auto bin = [=](float x) AMOE_INLINE { return x > low ? (int)fminf(fmaf(-0.5f, x, half) * step, (float)(kBins<NT> - 1)) : kBins<NT> - 1; };
       if (tid == 0) sh.rest = 0;
       if constexpr (STAGE == kAll || STAGE == kHistogram) {
         for (int i = tid; i < kBins<NT>; i += NT) {

@@ -160,6 +160,78 @@ def test_cuts_within_many_equal_logits(emu_ops):
     check(x, torch.tensor([0.999]), top_p=0.97)
 
 
+def fill_lists(dtype, device, V=512):
+    """What the next call finds in the workgroup's memory: lists full of ranks above all of its own."""
+    S.draw(torch.full((1, V), 1e4, dtype=DT[dtype], device=device), torch.zeros(1, device=device), top_k=V - 100, top_p=0.999)
+
+
+def check_equal(dtype, lengths, device="cpu"):
+    """Rows of one value, of lengths that are ranked at once and of a longer one, with numbers missing at either end, and both cuts: what a row is
+    padded with is no token, and what an earlier call left is none either."""
+    u = torch.tensor([0.25, 0.75, 0.96875])
+    for V in lengths:
+        for layout in ("own", "odd"):
+            x = logits(3, V, dtype, "equal", 0, layout).zero_()
+            fill_lists(dtype, device)
+            check(x, u, device, top_k=max(1, V * 3 // 4), top_p=0.9)
+            if V < 8:
+                continue
+            x[0, V - 3:] = -INF                                # fewer numbers than top_k
+            x[1, 0] = float("nan")
+            x[2, 0], x[2, V - 1] = -INF, -INF
+            fill_lists(dtype, device)
+            check(x, u, device, top_k=V - 1, top_p=0.9)
+            if device != "cpu":                                # (the host build takes half a second for each)
+                check(x, u, device, top_k=V - 2)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_of_one_value(emu_ops, dtype):
+    check_equal(dtype, (8, 9, 55, 256))
+
+
+def check_masked_ends(rows, device="cpu", dtypes=tuple(DT), less=(4, 3, 2, 1)):
+    """Rows of one value whose last logits are masked, and more of them asked for than there are: all of them are kept."""
+    n, *lengths = rows
+    for V in lengths:
+        for dtype in dtypes:
+            x = torch.zeros(n, V, dtype=DT[dtype])
+            x[:, V - 3:] = -INF
+            u = numbers(n, V)
+            for n_less in less:
+                check(x, u, device, top_k=V - n_less, top_p=0.9)
+                check(x, u, device, top_k=V - n_less)
+
+
+def test_masked_ends(emu_ops):
+    check_masked_ends((1, 5003, 3003), dtypes=("f32", "bf16"), less=(2,))
+
+
+def check_tiny(lengths, device="cpu"):
+    """Subnormal temperatures and logits: distances of which the bins tell few apart, or none."""
+    g = torch.Generator().manual_seed(3)
+    for V in lengths:
+        for size, temperature in ((1e-40, 1e-40), (1e-38, 3e-40), (1e-43, 1e-45), (1e-40, 1e-38), (0.0, 1e-42), (2e-37, 1e-38)):
+            x = torch.randn(3, V, generator=g) * size
+            x[1, V // 2:] = -INF
+            fill_lists("f32", device)
+            for how in (dict(top_k=V // 3, top_p=0.9), dict(top_k=V - 5, top_p=0.97), dict(top_k=V * 3 // 4), dict(top_p=0.8)):
+                check(x, numbers(3, V), device, temperature=temperature, **how)
+
+
+def test_tiny_temperatures_and_logits(emu_ops):
+    check_tiny((300,))
+
+
+@pytest.mark.gpu
+def test_gpu_rows_of_one_value():
+    for dtype in DT:
+        check_equal(dtype, (1, 7, 8, 9, 55, 63, 65, 256, 300, 511, 512, 600), "cuda")
+    check_masked_ends((1, 5003, 3003, 2049, 20003, 50003), "cuda")
+    check_masked_ends((300, 5003), "cuda", less=(2, 1))
+    check_tiny((40, 300, 700), "cuda")
+
+
 PARTED = {
     # rows worked on in parts: as CASES, and more equal logits at a cut than the parts hand on
     "full": (2, 16500, "f32", "normal", "own", {}),
