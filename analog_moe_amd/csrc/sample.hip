@@ -276,6 +276,10 @@ __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int coun
   int size = 2;
   while (size < count) size *= 2;
   for (int i = count + tid; i < size; i += NT) r.list[i] = 0;
+  if (tid == 0) {
+    sh.cut = 0;
+    sh.found_w = before_w;
+  }
   __syncthreads();
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
@@ -311,7 +315,8 @@ __device__ __forceinline__ void sample_sort(const SampleWeight& weight, int coun
   __syncthreads();
 }
 
-// The same for one bin of the row, whatever number of elements (`count`) it has.  What is ranked is what was listed.
+// The same for one bin of the row, whatever number of elements (`count`) it has.  What is ranked is what was listed, and the digits end
+// with the rank's: a row that is written to meanwhile gives some token of its own.
 template <typename T, int NT, class Bin>
 __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, const SampleWeight& weight, Bin bin, int b, int count,
                                               bool by_weight, u64 target, u64 before_n, u64 before_w, SampleRanked<NT>& r,
@@ -324,7 +329,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
   static_assert(1 << kDigit == kBins<NT>, "a bin for each digit");
   int shift = 32 + kIndexBits;
   u64 prefix = 0;
-  while (count > kBins<NT>) {
+  while (count > kBins<NT> && shift > 0) {
     const int next = shift > kDigit ? shift - kDigit : 0, size = 1 << (shift - next);
     __syncthreads();
     for (int i = tid; i < kBins<NT>; i += NT) {
@@ -350,7 +355,7 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
     if (tid < 64) count_one(row.edge, row.edge_index);
     __syncthreads();
     sample_crossing<NT>(r.digit, size, by_weight, target - (by_weight ? before_w : before_n), sh);
-    const int d = sh.found;
+    const int d = sh.found < 0 ? size - 1 : sh.found;
     count = (int)r.digit.n[d];
     before_n += sh.found_n;
     before_w += sh.found_w;
@@ -363,7 +368,9 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
   const auto list_one = [&](float x, int index) AMOE_INLINE {
     if (bin(x) != b) return;
     const u64 rank = sample_rank(x, index);
-    if (rank >> shift == prefix) r.list[atomicAdd(&sh.listed, 1)] = rank;
+    if (rank >> shift != prefix) return;
+    const int n = atomicAdd(&sh.listed, 1);
+    if (n < kBins<NT>) r.list[n] = rank;
   };
   row.all(
       -INFINITY,
@@ -374,11 +381,17 @@ __device__ __forceinline__ void sample_refine(const SampleRow<T, NT / 64>& row, 
       none);
   if (tid < 64) list_one(row.edge, row.edge_index);
   __syncthreads();
-  sample_sort<NT>(weight, sh.listed, by_weight, target, before_n, before_w, r, sh);
+  sample_sort<NT>(weight, sh.listed < kBins<NT> ? sh.listed : kBins<NT>, by_weight, target, before_n, before_w, r, sh);
+}
+
+// the first lane whose sum passes; the first of all where none does, which only a row that is written to meanwhile can bring about
+__device__ __forceinline__ int sample_first(bool passes) {
+  const uint64_t lanes = wave_ballot(passes);
+  return lanes ? ctz64(lanes) : 0;
 }
 
 // The element at which the sum of weights passes `target`, from the units' sums: weigh(value, index).  True for the thread that has
-// it.  Every thread calls this.
+// it, one of them whatever the sums are, and its index is one of the row.  Every thread calls this.
 template <typename T, int W, class Weigh>
 __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float low, u64 target, Weigh weigh, SampleShared<W>& sh, int& index,
                                             float& value) {
@@ -392,7 +405,7 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float lo
     mine += part[i];
   }
   u64 run = wave_scan(mine);
-  const int at = ctz64(wave_ballot(run > target));
+  const int at = sample_first(run > target);
   run -= mine;
   int in = -1;
 #pragma unroll
@@ -401,7 +414,7 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float lo
     if (in < 0) run += part[i];
   }
   target -= wave_read(run, at);
-  const int unit = P * at + (int)wave_read((uint32_t)in, at);
+  const int unit = P * at + (int)wave_read((uint32_t)(in < 0 ? 0 : in), at);
   const bool edges = unit == 0 || unit == row.last;
   const int g0 = (unit - 1) * row.per, g1 = g0 + row.per < row.groups ? g0 + row.per : row.groups;
   const auto group_sum = [&](int g, u64 (&w)[C], float (&x)[C], int& start) AMOE_INLINE {
@@ -435,17 +448,19 @@ __device__ __forceinline__ bool sample_find(const SampleRow<T, W>& row, float lo
     run = wave_scan((lane == 0) == (unit == 0) && row.edge != -INFINITY ? weigh(row.edge, row.edge_index) : 0);
     index = row.edge_index;
     value = row.edge;
-    return lane == ctz64(wave_ballot(run > target));
+    return lane == sample_first(run > target);
   }
   mine = lane < g1 - g0 ? sh.group[lane] : 0;
   run = wave_scan(mine);
-  const int group = ctz64(wave_ballot(run > target));
+  const int group = sample_first(run > target);
   target -= wave_read(run - mine, group);
   mine = group_sum(g0 + group, w, x, start);
   run = wave_scan(mine);
-  const bool here = lane == ctz64(wave_ballot(run > target));
+  const bool here = lane == sample_first(run > target);
   u64 sum = run - mine;
   bool found = false;
+  index = start;
+  value = x[0];
 #pragma unroll
   for (int e = 0; e < C; e++) {
     sum += w[e];

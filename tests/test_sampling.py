@@ -232,6 +232,35 @@ def test_gpu_rows_of_one_value():
     check_tiny((40, 300, 700), "cuda")
 
 
+def test_rows_written_to_meanwhile(emu_ops):
+    """Passes over a row that see other logits each time: the token may be any, but it is one of the row, and the call ends."""
+    import threading
+    import time
+    from analog_moe_amd import _abi
+    lib, V = emu_ops.get_lib(), 600
+    x = torch.zeros(1, V)
+    now = [torch.zeros(1, V), torch.full((1, V), -INF), torch.full((1, V), 3.0), logits(1, V, "f32") * 5]
+    done = threading.Event()
+
+    def write():
+        while not done.is_set():
+            for t in now:
+                x.copy_(t)
+                time.sleep(2e-3)
+    writer = threading.Thread(target=write)
+    writer.start()
+    try:
+        for i in range(18):
+            ids, u = torch.full((1,), -7), torch.tensor([(0.999, 0.5, 0.0)[i % 3]])
+            k, p = ((300, 0.9), (300, 1.0), (0, 1.0), (0, 0.5))[i % 4]
+            assert lib.amoe_sample(_abi.SAMPLE_ARGS.pack(0, 1, V, x.data_ptr(), V, u.data_ptr(), 0, 0, 0, 0, 0, 0, 1.0, p, 0.0, k,
+                                                         ids.data_ptr(), 0), None, 0, None) == 0
+            assert -1 <= int(ids) < V, i
+    finally:
+        done.set()
+        writer.join()
+
+
 PARTED = {
     # rows worked on in parts: as CASES, and more equal logits at a cut than the parts hand on
     "full": (2, 16500, "f32", "normal", "own", {}),
