@@ -129,7 +129,7 @@ template <typename T, int W> struct SampleRow {
 // terms of its series, which leave 2^-48.
 struct SampleWeight {
   float low;                         // weighs nothing: this and what is smaller
-  bool hot;                          // that is minus infinity alone
+  bool hot;                          // that is minus infinity alone: all numbers are within 66 temperatures of the largest
   double top, scale;                 // 32 log2(e) / temperature
   const double* table;               // the lane's copy of 2^(j / 32)
   __device__ __forceinline__ SampleWeight(float mx, float temperature, const double* tables) : top(mx), table(tables + (threadIdx.x & (kCopies - 1))) {
@@ -138,7 +138,7 @@ struct SampleWeight {
     const float down = fminf(mx - 33.f * temperature, mx);
     const uint32_t b = as_u32(down);
     low = down == 0.f ? -1e-45f : as_f32(down > 0.f ? b - 1 : b + 1);
-    hot = !(down > -3.3e38f);
+    hot = !(down > -3.402823466e38f);
     if (hot) low = -INFINITY;
     scale = kSteps * 1.44269504088896340736 / (double)temperature;
     const double most = 30000.0 / (top - (double)low);

@@ -207,6 +207,30 @@ def test_masked_ends(emu_ops):
     check_masked_ends((1, 5003, 3003), dtypes=("f32", "bf16"), less=(2,))
 
 
+def check_lowest(device="cpu", temperatures=(1e-30, 1.0, 3e29, 2e31, 1e36, 3e38)):
+    """Logits next to the type's lowest value, masks of that value and of another type's among them, and one at minus infinity."""
+    lowest, lower = torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min
+    u = torch.tensor([0.3, 0.9, 0.02, 0.6])
+    f32 = torch.empty(4, 70).uniform_(0.0, 1.0, generator=torch.Generator().manual_seed(4)) * -1e37 - 3.3e38
+    f32[1] = torch.where(f32[1] < -3.35e38, lowest, lower)
+    f32[2, :60], f32[2, 60:] = lowest, -INF
+    f32[3, ::2] = -INF
+    pair = torch.tensor([[-3.35e38, -3.40e38]]).expand(4, 2)
+    for t in temperatures:
+        for x in (f32, pair, f32.clamp_min(lower).bfloat16()):
+            check(x, u, device, temperature=t)
+            check(x, u, device, temperature=t, top_k=max(1, x.shape[1] // 2), top_p=0.9)
+
+
+def test_lowest_logits(emu_ops):
+    check_lowest()
+
+
+@pytest.mark.gpu
+def test_gpu_lowest_logits():
+    check_lowest("cuda", (1e-45, 1e-30, 1e-3, 1.0, 1e20, 1e29, 3e29, 6e29, 1e30, 2e31, 1e33, 1e36, 1e37, 1e38, 3e38))
+
+
 def check_tiny(lengths, device="cpu"):
     """Subnormal temperatures and logits: distances of which the bins tell few apart, or none."""
     g = torch.Generator().manual_seed(3)
