@@ -256,8 +256,8 @@ __global__ __launch_bounds__(kNormBwdThreads<NT>) void norm_bwd_kernel(NormParam
       }
 #pragma unroll
       for (int e = 0; e < C; e++) {
-        // (columns past D: their gradients are zeros, and so is what they add)
-        h[j][e] = ((h[j][e] - mean) - off) * inv;
+        // (columns past D: their gradients are zeros, and so is what they add, as long as h is a number)
+        h[j][e] = (t + j * NT) * C + e < p.D ? ((h[j][e] - mean) - off) * inv : 0.f;
         dwj[e] = fmaf(a[j][e], h[j][e], dwj[e]);
         dbj[e] += a[j][e];
         a[j][e] *= wj[e];

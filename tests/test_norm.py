@@ -118,6 +118,23 @@ def test_rows_of_one_value(emu_ops):
     check(x, None, w, b, gy, None)
 
 
+def check_large_rows(cases, device="cpu"):
+    """Rows of one value of 2e36 (no spread, so nothing overflows), at widths that leave lanes without columns: h is 0, y the bias, and what lanes
+    without columns hold adds nothing."""
+    to = lambda t: t if device == "cpu" else _on_gpu(t)                                   # noqa: E731
+    for D, dtype in cases:
+        x = torch.full((3, D), 2e36).to(DT[dtype])
+        x[1] = -x[1]
+        _, _, w, b, gy, _ = inputs(3, D, dtype, seed=D)
+        _, _, stats = N.layer_norm_forward(to(x), to(w), to(b), want_stats=True)
+        assert torch.equal(stats[:, 0].cpu(), x[:, 0].float()) and not stats[:, 1].any(), (D, dtype)
+        check(x, None, w, b, gy, None, device=device)
+
+
+def test_large_rows_of_one_value(emu_ops):
+    check_large_rows([(9, "f32"), (16, "f32"), (100, "f32"), (9, "bf16"), (12, "bf16"), (16, "bf16"), (100, "bf16")])
+
+
 def test_no_rows(emu_ops):
     x, w = torch.empty(0, 5, 16), torch.ones(16, requires_grad=True)
     assert N.layer_norm(x).shape == (0, 5, 16)
