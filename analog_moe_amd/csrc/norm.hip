@@ -133,15 +133,17 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_fwd_kernel(NormParam
       rx[j] = raw_pack<T>(a);          // (rounded, as it is stored: what the backward pass reads is what was normalised)
     }
   }
+  // (in units of the widest row: the sum of any finite row is finite, and the same bits otherwise)
+  constexpr float kUnit = 1.f / (float)kNormMaxD;
   float sum = 0.f, sq = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; j++) {
     raw_unpack<T>(rx[j], v[j]);
 #pragma unroll
-    for (int e = 0; e < C; e++) sum += v[j][e];
+    for (int e = 0; e < C; e++) sum = fmaf(v[j][e], kUnit, sum);
   }
   norm_sum2<NT>(sum, sq, lds, 0);
-  const float mean = sum / (float)p.D;
+  const float mean = sum / ((float)p.D * kUnit);
   float off = 0.f;
   sq = 0.f;
 #pragma unroll

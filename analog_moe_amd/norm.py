@@ -142,8 +142,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     Float32, bfloat16 or float16, rows of 1 to 32768 elements, any strides with adjacent elements of a row (others are copied);
     weight and bias [D] of x's type or float32, each optional.  Sums are formed in fp32, the mean as if in more (rows far from
-    zero keep their spread); the squares of what differs from the mean have to stay finite in fp32.  Differentiable once in all four;
-    equal inputs give equal bits in both directions."""
+    zero keep their spread); the squares of what differs from the mean, itself as sums in fp32 give it, and their sum have to stay finite in
+    fp32 (elements up to 2^70 that differ by up to 2^55 do).  Differentiable once in all four; equal inputs give equal bits in both
+    directions."""
     if residual is not None and residual.dtype != x.dtype:
         wide = torch.promote_types(x.dtype, residual.dtype)
         x, residual = x.to(wide), residual.to(wide)

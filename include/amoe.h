@@ -535,8 +535,8 @@ size_t amoe_shared_attn_args_bytes(void);
  * `sum` (both NULL: nothing is added).  weight and bias (either may be NULL) are of the rows' type or fp32.  stats: three floats a
  * row for the backward call, NULL: not wanted.  Rows are ld* elements apart (0 too: the same row again), y, sum and dx are contiguous.
  * D <= 32768; fewer than 2^28 rows of up to 128 elements (64 in fp32), 2^26 of up to 2048 (1024), 2^24 of up to 8192 (4096), 2^22 of more
- * (AMOE_EUNSUPPORTED otherwise).  The squares of what differs from the mean, and their sum, have to
- * stay finite in fp32.
+ * (AMOE_EUNSUPPORTED otherwise).  The squares of what differs from the mean, itself as sums in fp32
+ * give it, and their sum have to stay finite in fp32 (elements up to 2^70 that differ by up to 2^55 do).
  * The backward call reads x = s and stats and gives dx = the gradient of s: through y, whose gradient is gy, plus gs, that of s
  * itself (NULL: none), rounded once; dweight and dbias [D] in the weights' type (each may be NULL, as may dx).  Both are sums in a
  * fixed order in fp32, through the workspace: equal inputs give equal bits. */

@@ -123,7 +123,7 @@ def check_large_rows(cases, device="cpu"):
     without columns hold adds nothing."""
     to = lambda t: t if device == "cpu" else _on_gpu(t)                                   # noqa: E731
     for D, dtype in cases:
-        x = torch.full((3, D), 2e36).to(DT[dtype])
+        x = torch.full((3, D), 2e36).bfloat16().to(DT[dtype])        # (8 bits: sums of 2^15 of them are exact in fp32)
         x[1] = -x[1]
         _, _, w, b, gy, _ = inputs(3, D, dtype, seed=D)
         _, _, stats = N.layer_norm_forward(to(x), to(w), to(b), want_stats=True)
@@ -133,6 +133,22 @@ def check_large_rows(cases, device="cpu"):
 
 def test_large_rows_of_one_value(emu_ops):
     check_large_rows([(9, "f32"), (16, "f32"), (100, "f32"), (9, "bf16"), (12, "bf16"), (16, "bf16"), (100, "bf16")])
+
+
+def test_large_sums(emu_ops):
+    """Rows whose sum no float holds, of one value and of small differences."""
+    check_large_rows([(512, "f32"), (1000, "bf16")])
+    x = torch.full((2, 300), -2.0 ** 126)
+    x[1, ::2] = 2.0 ** 126
+    y, _, stats = N.layer_norm_forward(x[:1], want_stats=True)
+    assert not y.any() and stats[0, 0] == -2.0 ** 126
+    # (differences whose squares are past the floats' range, as documented: no spread is too large for the mean)
+    assert N.layer_norm_forward(x, want_stats=True)[2][1, 0] == 0
+
+
+@pytest.mark.gpu
+def test_gpu_large_rows():
+    check_large_rows([(D, t) for D in (9, 16, 100, 412, 1024, 4096, 8192, 16384, 32768) for t in ("f32", "bf16")], "cuda")
 
 
 def test_no_rows(emu_ops):
