@@ -49,24 +49,33 @@ def _ptr(t: Optional[Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _rows(t: Tensor, D: int):
+    """(what has to live until the launch, its address, elements from row to row): views are calls into torch, most tensors need none."""
+    if t.is_contiguous():
+        return t, t.data_ptr(), D
+    t = ops._rows2d(t)
+    return t, t.data_ptr(), t.stride(0)
+
+
 def layer_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
                        residual: Optional[Tensor] = None,
                        want_stats: bool = False) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     """(y, s, stats [rows, 3] fp32): ``amoe_layer_norm_fwd``.  s is None without a residual (it is x), stats without want_stats."""
     weight, bias, code, wcode = _check(x, residual, weight, bias, eps)
-    rows, D = ops._rows2d(x), x.shape[-1]
-    n = rows.shape[0]
-    y = x.new_empty(x.shape)
+    shape = x.shape
+    D = shape[-1]
+    n = x.numel() // D
+    x, xp, xl = _rows(x, D)
+    y = x.new_empty(shape)
     s = stats = None
     rp = rl = 0
     if residual is not None:
-        res = ops._rows2d(residual)
-        rp, rl = res.data_ptr(), res.stride(0)
-        s = x.new_empty(x.shape)
+        residual, rp, rl = _rows(residual, D)
+        s = x.new_empty(shape)
     if want_stats:
         stats = x.new_empty((n, 3), dtype=torch.float32)
     lib = ops.get_lib()
-    args = _abi.NORM_ARGS.pack(code, wcode, n, D, eps, rows.data_ptr(), rows.stride(0), _ptr(weight), _ptr(bias), _ptr(stats), rp, rl,
+    args = _abi.NORM_ARGS.pack(code, wcode, n, D, eps, xp, xl, _ptr(weight), _ptr(bias), _ptr(stats), rp, rl,
                                y.data_ptr(), _ptr(s), 0, 0, 0, 0, 0, 0, 0)
     with ops.device_of(x):
         rc = lib.amoe_layer_norm_fwd(args, ops._stream(x))
@@ -83,25 +92,26 @@ def layer_norm_backward(gy: Tensor, s: Tensor, weight: Optional[Tensor], bias: O
     if gy.shape != s.shape or gy.dtype != s.dtype or gy.device != s.device:
         raise ValueError("the gradient must have s's shape, dtype and device")
     ops._need_gpu(gy, stats)
-    rows, D = ops._rows2d(s), s.shape[-1]
-    n = rows.shape[0]
+    shape = s.shape
+    D = shape[-1]
+    n = s.numel() // D
     if stats.shape != (n, 3) or stats.dtype != torch.float32 or stats.device != s.device:
         raise ValueError(f"stats must be fp32 [{n}, 3] on {s.device}")
     stats = stats if stats.is_contiguous() else stats.contiguous()
-    dx = s.new_empty(s.shape) if want_x else None
+    dx = s.new_empty(shape) if want_x else None
     want_weight, want_bias = want_weight and weight is not None, want_bias and bias is not None
     if n == 0:
         return dx, torch.zeros_like(weight) if want_weight else None, torch.zeros_like(bias) if want_bias else None
     dw = torch.empty_like(weight) if want_weight else None
     db = torch.empty_like(bias) if want_bias else None
-    g = ops._rows2d(gy)
+    s, sp, sl = _rows(s, D)
+    gy, yp, yl = _rows(gy, D)
     gp = gl = 0
     if gs is not None:
-        gs = ops._rows2d(gs)
-        gp, gl = gs.data_ptr(), gs.stride(0)
+        gs, gp, gl = _rows(gs, D)
     lib = ops.get_lib()
-    args = _abi.NORM_ARGS.pack(code, wcode, n, D, 0.0, rows.data_ptr(), rows.stride(0), _ptr(weight), _ptr(bias), stats.data_ptr(), 0, 0, 0, 0,
-                               g.data_ptr(), g.stride(0), gp, gl, _ptr(dx), _ptr(dw), _ptr(db))
+    args = _abi.NORM_ARGS.pack(code, wcode, n, D, 0.0, sp, sl, _ptr(weight), _ptr(bias), stats.data_ptr(), 0, 0, 0, 0,
+                               yp, yl, gp, gl, _ptr(dx), _ptr(dw), _ptr(db))
     with ops.device_of(s):
         need = lib.amoe_layer_norm_bwd_workspace(args)
         ws = s.new_empty(need, dtype=torch.uint8) if need else None
@@ -151,7 +161,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if torch.compiler.is_compiling():
         y, s, _ = torch.ops.amoe.layer_norm_fwd(x, residual, weight, bias, eps)
         return y if residual is None else (y, s)
-    if ops.unwatched() and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias))):
+    if ops.unwatched() and not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)
+                                                             or (weight is not None and weight.requires_grad)
+                                                             or (bias is not None and bias.requires_grad))):
         y, s, _ = layer_norm_forward(x, weight, bias, eps, residual)
         return y if s is None else (y, s)
     return LayerNormFunction.apply(x, residual, weight, bias, eps)
