@@ -5,6 +5,7 @@ read once, and the backward pass leaves one gradient of s for both summands.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -16,33 +17,37 @@ from .attention import once
 MAX_WIDTH = 32768
 
 
-def _vector(t: Optional[Tensor], x: Tensor, name: str) -> Optional[Tensor]:
-    if t is None:
-        return None
-    if t.shape != x.shape[-1:]:
-        raise ValueError(f"{name} must be [{x.shape[-1]}], not {tuple(t.shape)}")
-    if t.dtype != x.dtype and t.dtype != torch.float32:
-        raise TypeError(f"{name} must be {x.dtype} or float32, not {t.dtype}")
-    if t.device != x.device:
-        raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
 def _check(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
-    """(x, weight, bias) as rows and vectors that the library takes, and the types' codes."""
+    """(weight, bias) as vectors that the library takes, the types' codes, rows and their elements."""
     ops._need_gpu(x, residual, weight, bias)
-    code = raw.code_of(x.dtype)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
-        raise ValueError(f"rows have 1 to {MAX_WIDTH} elements, not {tuple(x.shape)[-1:]}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    shape, dtype, device = x.shape, x.dtype, x.device
+    code = wcode = raw.code_of(dtype)
+    if not shape or not 1 <= shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"rows have 1 to {MAX_WIDTH} elements, not {tuple(shape)[-1:]}")
+    D = shape[-1]
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype or residual.device != device):
         raise ValueError("residual must have x's shape, dtype and device")
     if not 0.0 <= eps <= 3e38:
         raise ValueError(f"eps must be a finite number of 0 or more, not {eps}")
-    weight, bias = _vector(weight, x, "weight"), _vector(bias, x, "bias")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight and bias must share one dtype")
-    like = weight if weight is not None else bias
-    return weight, bias, code, code if like is None else raw.code_of(like.dtype)
+    if weight is not None:
+        weight, wcode = _vector(weight, D, dtype, device, "weight"), raw.code_of(weight.dtype)
+    if bias is not None:
+        bias = _vector(bias, D, dtype, device, "bias")
+        if weight is None:
+            wcode = raw.code_of(bias.dtype)
+        elif bias.dtype != weight.dtype:
+            raise TypeError("weight and bias must share one dtype")
+    return weight, bias, code, wcode, x.numel() // D, D
+
+
+def _vector(t: Tensor, D: int, dtype: torch.dtype, device: torch.device, name: str) -> Tensor:
+    if t.shape != (D,):
+        raise ValueError(f"{name} must be [{D}], not {tuple(t.shape)}")
+    if t.dtype != dtype and t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {dtype} or float32, not {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, x on {device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t: Optional[Tensor]) -> int:
@@ -61,10 +66,8 @@ def layer_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optiona
                        residual: Optional[Tensor] = None,
                        want_stats: bool = False) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     """(y, s, stats [rows, 3] fp32): ``amoe_layer_norm_fwd``.  s is None without a residual (it is x), stats without want_stats."""
-    weight, bias, code, wcode = _check(x, residual, weight, bias, eps)
+    weight, bias, code, wcode, n, D = _check(x, residual, weight, bias, eps)
     shape = x.shape
-    D = shape[-1]
-    n = x.numel() // D
     x, xp, xl = _rows(x, D)
     y = x.new_empty(shape)
     s = stats = None
@@ -84,17 +87,20 @@ def layer_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optiona
     return y, s, stats
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace(lib, code: int, n: int, D: int) -> int:
+    """Bytes of ``amoe_layer_norm_bwd_workspace`` with a gradient of the weight or bias: the sizes decide, not where tensors are."""
+    return lib.amoe_layer_norm_bwd_workspace(_abi.NORM_ARGS.pack(code, code, n, D, 0.0, *[0] * 14, 8, 0))
+
+
 def layer_norm_backward(gy: Tensor, s: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, gs: Optional[Tensor] = None,
                         want_x: bool = True, want_weight: bool = True, want_bias: bool = True):
     """(gradient of s, of weight, of bias) from those of y and (gs) of s itself: ``amoe_layer_norm_bwd``; None for what is not
     wanted or not there."""
-    weight, bias, code, wcode = _check(s, gs, weight, bias, 0.0)
-    if gy.shape != s.shape or gy.dtype != s.dtype or gy.device != s.device:
-        raise ValueError("the gradient must have s's shape, dtype and device")
-    ops._need_gpu(gy, stats)
+    weight, bias, code, wcode, n, D = _check(s, gs, weight, bias, 0.0)
     shape = s.shape
-    D = shape[-1]
-    n = s.numel() // D
+    if gy.shape != shape or gy.dtype != s.dtype or gy.device != s.device:
+        raise ValueError("the gradient must have s's shape, dtype and device")
     if stats.shape != (n, 3) or stats.dtype != torch.float32 or stats.device != s.device:
         raise ValueError(f"stats must be fp32 [{n}, 3] on {s.device}")
     stats = stats if stats.is_contiguous() else stats.contiguous()
@@ -112,8 +118,8 @@ def layer_norm_backward(gy: Tensor, s: Tensor, weight: Optional[Tensor], bias: O
     lib = ops.get_lib()
     args = _abi.NORM_ARGS.pack(code, wcode, n, D, 0.0, sp, sl, _ptr(weight), _ptr(bias), stats.data_ptr(), 0, 0, 0, 0,
                                yp, yl, gp, gl, _ptr(dx), _ptr(dw), _ptr(db))
+    need = _workspace(lib, code, int(n), int(D)) if want_weight or want_bias else 0
     with ops.device_of(s):
-        need = lib.amoe_layer_norm_bwd_workspace(args)
         ws = s.new_empty(need, dtype=torch.uint8) if need else None
         rc = lib.amoe_layer_norm_bwd(args, _ptr(ws), need, ops._stream(s))
     if rc:
