@@ -725,7 +725,8 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
       const auto gather = [&](int l, int& count) AMOE_INLINE {
         const int mine = lane < p.parts ? work->part[lane].listed[l] : 0, before = wave_scan(mine) - mine;
         count = (int)wave_read((uint32_t)(before + mine), 63);
-        if (wave_ballot(mine > kPartList) != 0 || count > kBins<NT>) return false;
+        // (as unsigned: a part of a row that is written to meanwhile may have found no bin and left no number)
+        if (wave_ballot((uint32_t)mine > (uint32_t)kPartList) != 0 || count > kBins<NT>) return false;
         for (int j = wave; j < p.parts; j += W) {
           const int m = (int)wave_read((uint32_t)mine, j), to = (int)wave_read((uint32_t)before, j);
           for (int i = lane; i < m; i += 64) ranked.list[to + i] = work->part[j].list[l][i];

@@ -256,12 +256,10 @@ def test_gpu_rows_of_one_value():
     check_tiny((40, 300, 700), "cuda")
 
 
-def test_rows_written_to_meanwhile(emu_ops):
-    """Passes over a row that see other logits each time: the token may be any, but it is one of the row, and the call ends."""
+def check_written_to(lib, V, calls, ks):
     import threading
     import time
     from analog_moe_amd import _abi
-    lib, V = emu_ops.get_lib(), 600
     x = torch.zeros(1, V)
     now = [torch.zeros(1, V), torch.full((1, V), -INF), torch.full((1, V), 3.0), logits(1, V, "f32") * 5]
     done = threading.Event()
@@ -274,15 +272,21 @@ def test_rows_written_to_meanwhile(emu_ops):
     writer = threading.Thread(target=write)
     writer.start()
     try:
-        for i in range(18):
+        for i in range(calls):
             ids, u = torch.full((1,), -7), torch.tensor([(0.999, 0.5, 0.0)[i % 3]])
-            k, p = ((300, 0.9), (300, 1.0), (0, 1.0), (0, 0.5))[i % 4]
-            assert lib.amoe_sample(_abi.SAMPLE_ARGS.pack(0, 1, V, x.data_ptr(), V, u.data_ptr(), 0, 0, 0, 0, 0, 0, 1.0, p, 0.0, k,
-                                                         ids.data_ptr(), 0), None, 0, None) == 0
+            k, p = ks[i % len(ks)]
+            args = _abi.SAMPLE_ARGS.pack(0, 1, V, x.data_ptr(), V, u.data_ptr(), 0, 0, 0, 0, 0, 0, 1.0, p, 0.0, k, ids.data_ptr(), 0)
+            ws = torch.full((lib.amoe_sample_workspace(args) + 8,), 0xf3, dtype=torch.uint8)
+            assert lib.amoe_sample(args, ws.data_ptr(), ws.numel(), None) == 0
             assert -1 <= int(ids) < V, i
     finally:
         done.set()
         writer.join()
+
+
+def test_rows_written_to_meanwhile(emu_ops):
+    """Passes over a row that see other logits each time: the token may be any, but it is one of the row, and the call ends."""
+    check_written_to(emu_ops.get_lib(), 600, 18, ((300, 0.9), (300, 1.0), (0, 1.0), (0, 0.5)))
 
 
 PARTED = {
@@ -321,6 +325,17 @@ def test_rows_in_parts(emu_ops, names):
              "f.check_parted(sys.argv[1:])\nprint('done')\n")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     got = subprocess.run([sys.executable, "-c", child, *names], cwd=root, env={**os.environ, "AMOE_EMU_CUS": "64"}, capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout.endswith("done\n"), got.stderr
+
+
+def test_masked_ends_and_written_rows_in_parts(emu_ops):
+    """Likewise in parts, with a workspace that may hold anything."""
+    child = ("from analog_moe_amd import _abi, ops\nfrom tests import test_emu_kernels as t, test_sampling as f\n"
+             "ops._LIB, ops._stream, ops._need_gpu = _abi.bind(t.EMU_SO), (lambda x: None), (lambda *a: None)\n"
+             "f.check_masked_ends((1, 16403), dtypes=('bf16',), less=(2,))\n"
+             "f.check_written_to(ops._LIB, 16403, 6, ((9000, 0.9), (16390, 0.5)))\nprint('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = subprocess.run([sys.executable, "-c", child], cwd=root, env={**os.environ, "AMOE_EMU_CUS": "64"}, capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.endswith("done\n"), got.stderr
 
 
