@@ -5,8 +5,8 @@
 // A row lies in the registers of NT threads, so that memory sees it once.  Its mean is summed first and the squares of what differs
 // from it then; that sum carries the differences themselves along, whose own mean is what the rounding of the first one left (rows
 // far from zero: their mean is exact only to 2^-24 of itself, which may be as large as the row's spread).  Bound by memory: 4096 rows
-// of 8192 in fp32, with the sum, 94 us forward and 115 + 5 backward for 537 MB each (5.7 and 4.5 TB/s, a large copy reaches 5.1); 16384
-// of 1024 in bf16 23 and 25 + 4 us for 134 MB each, a part of it from the cache behind the L2.
+// of 8192 in fp32, with the sum, 92 us forward and 114 + 5 backward for 537 MB each (5.8 and 4.5 TB/s, a large copy reaches 5.1); 16384
+// of 1024 in bf16 24 and 26 + 4 us for 134 MB each, a part of it from the cache behind the L2.
 #include <amoe.h>
 
 #include "host_util.h"

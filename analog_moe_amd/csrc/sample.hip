@@ -3,18 +3,21 @@
 //   kept: the first top_k; of these the shortest run from the top with at least top_p of their weight; of these weights of min_p
 //   or more.  Drawn: in the order of the indices, the first up to which the kept ones weigh more than u times all of them.
 //
-// Weights are whole multiples of 2^-44 of the largest one (made in 64 bits, by a table of 2^(j / 256) and four terms of the series
+// Weights are whole multiples of 2^-44 of the largest one (made in 64 bits, by a table of 2^(j / 32) and five terms of the series
 // between), so that their sums are exact and the same in any order: what is drawn depends neither on how a row is shared out
-// among threads nor on the order of the atomics that count, and is the definition's wherever u, top_p and the sums do not meet to
-// within 2^-44 of the largest weight.  (In fp32 a row of 10^5 logits would go to a neighbour about once in a thousand draws.)
-// What weighs less than 2^-45 of the largest is never drawn.
+// among threads nor on the order of the atomics that count.  A weight is off by up to 2^-44 of the largest and a row's sum by V times
+// that: what is drawn is the definition's wherever u and top_p come no nearer to a border between tokens than this, and min_p no nearer
+// to a weight than 2^-44.  (In fp32 a row of 10^5 logits would go to a neighbour about once in a thousand draws.)  What weighs less than
+// 2^-45 of the largest is never drawn.
 //
 // The cut that top_k and top_p make in the ranking is found without a sort: tokens are counted, or weighed, by their
 // distance from the largest in up to 2047 bins, and only those of the bin with the cut are ranked.
 //
-// Rows pass three times (their extremes, the bins, the sums), four where both cuts are made, from the caches behind the first.  Bound by
-// the weights' arithmetic (13 operations in 64 bits, at half rate: 256 rows of 130001 fp32 logits 27 us for the largest alone, which is
-// the reading; 56 with one pass of weights; 107 with top_p, 139 with top_k too) and the bins' LDS atomics (2048 rows of 8000: 31 and 68).
+// Rows pass three times (their extremes, the bins, the sums), four where both cuts are made, from the caches behind the first.  Without a cut
+// bound by the vector unit: 52 instructions a logit, 13 of them a weight's in 64 bits, keep it busy for 22 of 31 us (2048 rows of 8000, fp32).
+// With cuts by that, by the bins' LDS atomics, of which many meet on a bank, and by waiting for both: 256 rows of 130001 fp32 logits 27 us
+// for the largest alone, which is the reading, 56 with one pass of weights, 113 with top_p, 143 with top_k too (100 instructions a
+// logit, 85 us, and 15 us of bank conflicts); 2048 rows of 8000 in bf16 31 and, with top_p, 72.
 #include <amoe.h>
 
 #include "host_util.h"
@@ -894,8 +897,8 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(SampleParams p) {
 namespace {
 
 // Parts that a row is worked on in, 1: all in one launch: as many as there are CUs for, of 4096 elements or more, if they are four.
-// Measured (us, one launch / parts, fp32 or bf16): 8 rows of 130001 with top_p 91 / 40, without a cut 40 / 18, the largest of each
-// 14 / 18; 64 of 50001 54 / 44, 24 / 18, 11 / 18 (what is launched may not depend on what the temperatures are).
+// Measured (us, one launch / parts, fp32 or bf16): 8 rows of 130001 with top_p 92 / 41, without a cut 36 / 17, the largest of each
+// 12 / 17; 64 of 50001 51 / 44, 21 / 17, 10 / 17 (what is launched may not depend on what the temperatures are).
 int sample_parts(const amoe_sample_args* a) {
   const int64_t most = num_compute_units() / (a->rows < 1 ? 1 : a->rows), n = a->V / 4096;
   const int64_t parts = n < most ? n : most;
@@ -903,8 +906,8 @@ int sample_parts(const amoe_sample_args* a) {
 }
 
 // 256 threads for short rows, and for longer ones where there are more of them than CUs; not past 32768, where too many tokens would
-// share one of their bins, a quarter as many.  Measured (us, 256 / 1024 threads, top_p 0.95, bf16): 64 rows of 2000 13.6 / 15.3; 1 of 8000 20.1 / 17.8,
-// 100 22.1 / 19.1, 300 25.2 / 34.7, 2048 67 / 145; 512 of 16000 39 / 51; 512 of 32000 67 / 69, 2048 179 / 268.
+// share one of their bins, a quarter as many.  Measured (us, 256 / 1024 threads, top_p 0.95, bf16): 64 rows of 2000 14.5 / 15.0; 1 of 8000 21.9 / 17.7,
+// 100 23.3 / 19.2, 300 26.3 / 35.7, 2048 70 / 141; 512 of 16000 41 / 48; 512 of 32000 72 / 71, 2048 193 / 274.
 template <typename T, bool CUT>
 int launch_sample_cut(const SampleParams& p, bool both, hipStream_t st) {
   const dim3 grid((unsigned)p.rows), parts((unsigned)(p.rows * p.parts)), block(1024);

@@ -177,7 +177,8 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
 class LayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` of the last dimension on these kernels, with its parameters and state dict: ``norm(x)``, or
-    ``norm(x, residual) -> (y, x + residual)``."""
+    ``norm(x, residual) -> (y, x + residual)``.  Autocast changes nothing here: y is of x's type (of the wider one with a residual), where
+    ``nn.LayerNorm`` gives float32.  Parameters are of y's type or float32: those of a 16-bit module are refused with a float32 stream."""
 
     def __init__(self, width: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None, dtype=None):
         if not isinstance(width, int) or not 1 <= width <= MAX_WIDTH:

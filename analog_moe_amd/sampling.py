@@ -84,9 +84,11 @@ def sample(logits: Tensor, u: Tensor, temperature: Setting = 1.0, top_k: Union[i
     kept ones weigh more than u times all of them.  Temperature 0: the largest logit, with logarithm 0.  Settings are numbers, or
     tensors with one for each row (float32; top_k int32 / int64), which are taken as the nearest that is allowed.
 
-    Not-a-numbers count as minus infinity, which is never drawn; a row of nothing else gives -1 and minus infinity.  Sums of weights
-    are exact (whole multiples of 2^-44 of the largest), so that a token is the definition's and the same every time.  Up to 2^20 - 1
-    logits a row.  No gradients."""
+    Not-a-numbers count as minus infinity, which is never drawn; a row of nothing else gives -1 and minus infinity.  Weights are whole
+    multiples of 2^-44 of the largest (what weighs less than half of that is never drawn, and weights that differ by less are equal) and
+    sums of them exact, so that a token is the same every time; it is the definition's unless u or top_p meets a border between tokens to
+    within V times 2^-44 of the largest weight, or min_p a weight to within 2^-44.  Numbers are taken in float32.  Up to 2^20 - 1 logits a
+    row.  No gradients."""
     if want_logprob and torch.is_grad_enabled() and logits.requires_grad:
         raise RuntimeError("the logarithms of sample have no gradient: call it under torch.no_grad(), or on detached logits")
     if torch.compiler.is_compiling() or not ops.unwatched():

@@ -539,7 +539,8 @@ size_t amoe_shared_attn_args_bytes(void);
  * give it, and their sum have to stay finite in fp32 (elements up to 2^70 that differ by up to 2^55 do).
  * The backward call reads x = s and stats and gives dx = the gradient of s: through y, whose gradient is gy, plus gs, that of s
  * itself (NULL: none), rounded once; dweight and dbias [D] in the weights' type (each may be NULL, as may dx).  Both are sums in a
- * fixed order in fp32, through the workspace: equal inputs give equal bits. */
+ * fixed order in fp32, through the workspace: equal inputs give equal bits.  Without rows there is nothing to do, and sums over them
+ * are refused (AMOE_EINVAL): they are the caller's zeros. */
 typedef struct amoe_norm_args {
   int64_t dtype, weight_dtype, rows, D;
   double eps;
@@ -569,7 +570,7 @@ size_t amoe_norm_args_bytes(void);
  * Settings: one pointer each to a number per row, or NULL and the number for all.  A row's own settings are not refused: temperatures
  * that are not above 0 count as 0, negative top_k as 0, top_p and min_p as the nearer end of [0, 1] (not a number: 1 and 0).
  * Weights are multiples of 2^-44 of the largest (what weighs less than half of that is never drawn), sums of them exact: equal inputs
- * give equal bits.  V < 2^20, fewer than 2^22 rows (AMOE_EUNSUPPORTED otherwise); rows ld elements apart, adjacent elements. */
+ * give equal bits.  A row that is written to during the call gives some id of its own or -1.  V < 2^20, fewer than 2^22 rows (AMOE_EUNSUPPORTED otherwise); rows ld elements apart, adjacent elements. */
 typedef struct amoe_sample_args {
   int64_t dtype, rows, V;
   const void* logits;  int64_t ld;

@@ -281,6 +281,19 @@ def test_module(emu_ops):
         N.LayerNorm(0)
 
 
+def test_types_of_the_module(emu_ops):
+    """Autocast changes nothing, and parameters of a 16-bit module do not go with a float32 stream."""
+    x, r, _, _, _, _ = inputs(5, 48, "bf16")
+    m = N.LayerNorm(48)
+    with torch.autocast("cpu", torch.bfloat16):
+        assert m(x).dtype == torch.bfloat16 and m(x.float()).dtype == torch.float32 and m(x, r.float())[0].dtype == torch.float32
+        assert torch.equal(m(x), N.layer_norm(x, m.weight, m.bias))
+    m = m.bfloat16()
+    assert m(x, r)[0].dtype == torch.bfloat16
+    with pytest.raises(TypeError):
+        m(x, r.float())
+
+
 def test_refusals(emu_ops):
     x, r, w, b, gy, _ = inputs(4, 16, "bf16")
     for bad in (dict(weight=w[:8]), dict(bias=b.reshape(1, 16)), dict(residual=r[:2]), dict(eps=-1.0), dict(eps=float("nan")),
